@@ -38,11 +38,13 @@ HIP_FLAGS = [
 ]
 
 
-# Per-source additions. The prefill kernel keeps its MFMA accumulators in
-# ordinary VGPRs: its online softmax rescales them between products, which in
+# Per-source additions. The attention kernels on MFMA keep their accumulators in
+# ordinary VGPRs: the online softmax rescales them between products, which in
 # the accumulator-register form costs a move out and back for every element.
 FILE_FLAGS = {
     "prefill_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv8_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "kv8_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

@@ -27,6 +27,8 @@ CDB_DTYPE_BF16 = 1
 CDB_DECODE_SCRATCH_BYTES = 16 << 20  # include/cdb_amd.h
 CDB_DECODE_STAGE_PLAN = 1
 CDB_DECODE_STAGE_ATTEND = 2
+CDB_LAYOUT_MAX_SEQS = 4000
+CDB_LAYOUT_TOKENS_FULL, CDB_LAYOUT_TILES_FULL, CDB_LAYOUT_NO_BLOCKS, CDB_LAYOUT_BAD_REQUEST = 1, 2, 4, 8
 
 _P = c_void_p
 _I32P = c_void_p
@@ -173,6 +175,48 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _P, c_int64, c_int32, _P, _P, c_int32,  # bank, bank_rows, width, hidden, w_packed, vocab
             _P, _P, c_int64, _P, _P,  # tokens, workspace, workspace_bytes, embed, host_tokens
             _P, _P, _P, c_int64, c_int32, _P,  # cdf, survival, pending, state_capacity, dtype, stream
+        ],
+    ),
+    "cdb_kv8_write": (
+        c_int32,
+        [
+            _P, _P, _P, _P, _P, _P,  # q, k, v, q_out, codes, scales
+            c_int32, c_int64, c_int32, _P, _P,  # num_cache_layers, pool_blocks, layer, rows, positions
+            _P, _P, c_int32, c_int32, _P, _P,  # rope_cos, rope_sin, rope_style, max_positions, q_bias, k_bias
+            c_int64, c_int32, c_int32, c_int32, c_int32,  # tokens, H, Hkv, D, block_size
+            c_int64, c_int64, c_int32, _P,  # q_stride, kv_stride, dtype, stream
+        ],
+    ),
+    "cdb_kv8_decode_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "cdb_kv8_decode_attention": (
+        c_int32,
+        [
+            _P, _P, _P, _P, _P,  # q, k_new, v_new, codes, scales
+            c_int32, c_int64, _P, c_int32,  # num_cache_layers, pool_blocks, cache_layer, cache_layer0
+            _P, _P, c_int32, c_int32, _P,  # block_table, table_row, table_rows, table_width, seqlens
+            _P, _P, c_int32, c_int32, _P, _P,  # rope_cos, rope_sin, rope_style, max_positions, q_bias, k_bias
+            _P, _P, c_int64,  # out, workspace, workspace_bytes
+            c_int32, c_int32, c_int32, c_int32, c_int32,  # rows, H, Hkv, D, block_size
+            c_float, c_int64, c_int64, c_int32, _P,  # scale, q_stride, kv_stride, dtype, stream
+        ],
+    ),
+    "cdb_kv8_prefill_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32]),
+    "cdb_kv8_prefill_attention": (
+        c_int32,
+        [
+            _P, _P, _P, c_int32, c_int64, c_int32,  # q, codes, scales, num_cache_layers, pool_blocks, layer
+            _P, _P, c_int32, c_int32,  # block_table, table_row, table_rows, table_width
+            _P, _P, c_int32, _P, _P, c_int32,  # cu_q, past, num_seqs, tile_seq, tile_q0, num_tiles
+            _P, c_int64, c_int32, _P, c_int64,  # out, tokens, splits, workspace, workspace_bytes
+            c_int32, c_int32, c_int32, c_int32, c_float, c_int32, _P,  # H, Hkv, D, block_size, scale, dtype, stream
+        ],
+    ),
+    "cdb_batch_layout": (
+        c_int32,
+        [
+            _P, _P, c_int32, _P, _P, c_int32, c_int32,  # past, lens, num_seqs, table, table_row, table rows, width
+            _P, c_int32, c_int32, _P, _P, _P, c_int32,  # free, num_free, block_size, cu_q, positions, rows, capacity
+            _P, _P, c_int32, _P, _P,  # tile_seq, tile_q0, tile_capacity, counts, stream
         ],
     ),
 }

@@ -1,0 +1,484 @@
+// Filling the 8-bit KV cache: the rotating, quantising write of a batch of tokens, and the block
+// tables, slot maps and attention tiles of a batch from its requests' lengths.
+#include "cdb_amd.h"
+#include "kv8_common.h"
+#include "kv8_host.h"
+
+namespace cdb {
+
+struct Kv8WriteParams {
+  const void *q, *k, *v;
+  void* q_out;
+  Kv8Cache cache;
+  int64_t layer;
+  const int64_t* rows;
+  int64_t pool_rows;
+  const int32_t* positions;
+  const float *cos, *sin;
+  const void *q_bias, *k_bias;
+  int64_t tokens, q_stride, kv_stride;
+  int32_t num_heads, max_positions, chunk;
+  int64_t chunks, kv_blocks;  // chunks of tokens; workgroups of the cache write, before those that rotate queries
+  bool vec;
+};
+
+// One wave writes the tokens of one KV head that start a run inside its chunk. A run is the tokens of
+// one tile that follow each other in the batch, 16 at most, so a tile's scale is known to the wave
+// that writes it: the maximum over the run, and for a tile that held earlier tokens their scale too.
+// Lane (r, g) = (lane % 16, lane / 16) holds units g, g + 4 of token r of the key tile, and group g of
+// elements 4r.. of the value tile, which are the tile's own 16-byte pieces: each store is contiguous.
+template <typename T, int D, int STYLE>
+CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t token0, int n, int64_t row0, int head) {
+  constexpr int kUnits = D / 16;
+  constexpr int kParts = (kUnits + 3) / 4;
+  const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
+  const int64_t tile = row0 >> 4;
+  const int off = (int)(row0 & 15);
+  const int64_t block = tile >> P.cache.tile_log2;
+  const int sub = (int)(tile & ((1 << P.cache.tile_log2) - 1));
+  const T* k = static_cast<const T*>(P.k) + head * D;
+  const T* v = static_cast<const T*>(P.v) + head * D;
+  const T* k_bias = P.k_bias == nullptr ? nullptr : static_cast<const T*>(P.k_bias) + head * D;
+  const int64_t k_tile = P.cache.tile(P.layer, 0, block, head, sub), v_tile = P.cache.tile(P.layer, 1, block, head, sub);
+  uint8_t* k_codes = P.cache.codes + k_tile * (kTile * D);
+  uint8_t* v_codes = P.cache.codes + v_tile * (kTile * D);
+
+  // Keys: token r of the tile is token r - off of the run.
+  const bool live = r >= off && r < off + n;
+  const int64_t t = token0 + (live ? r - off : 0);
+  const int64_t angle = STYLE == 0 ? 0 : (int64_t)P.positions[t] * (D / 2);
+  float x[kParts][16];
+  float top = 0.f;
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    const int u = g + 4 * j;
+    if (u < kUnits) {
+      load_rotated<T, D, STYLE, 16>(k + t * P.kv_stride, k_bias, P.cos + angle, P.sin + angle, 16 * u, P.vec, x[j]);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, finite_abs(x[j][i]));
+    }
+  }
+  top = wave_max(live ? top : 0.f);
+
+  // Values: elements 64j + 4r.. (the last 32 of a head of 96: 64 + 2r..) of tokens 4g..4g+3.
+  float y[kParts][4][4];
+  float v_top = 0.f;
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    constexpr int kLast = D % 64 == 0 ? 4 : 2;
+    const int w = j + 1 < kParts ? 4 : kLast;
+    const int d = 64 * j + w * r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int slot = 4 * g + i - off;
+      const bool on = slot >= 0 && slot < n;
+      const T* src = v + (token0 + (on ? slot : 0)) * P.kv_stride + d;
+      if (w == 4) load_f32<T, 4>(src, y[j][i], P.vec);
+      else load_f32<T, 2>(src, y[j][i], P.vec);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (e < w && on) v_top = fmaxf(v_top, finite_abs(y[j][i][e]));
+    }
+  }
+  v_top = wave_max(v_top);
+
+  int k_now = scale_byte(top), v_now = scale_byte(v_top);
+  int k_old = 0, v_old = 0;
+  if (off > 0) {
+    k_old = min((int)P.cache.scales[k_tile], 254);
+    v_old = min((int)P.cache.scales[v_tile], 254);
+    k_now = max(k_now, k_old);
+    v_now = max(v_now, v_old);
+  }
+  const float k_inv = inverse_scale_of(k_now), v_inv = inverse_scale_of(v_now);
+  const bool k_grown = off > 0 && k_now != k_old, v_grown = off > 0 && v_now != v_old;
+
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    const int u = g + 4 * j;
+    if (u >= kUnits) continue;
+    u32x4_t* at = reinterpret_cast<u32x4_t*>(k_codes + u * 256 + r * 16);
+    if (live) {
+      u32x4_t w;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        w[i] = codes_of(mul_rn(x[j][4 * i], k_inv), mul_rn(x[j][4 * i + 1], k_inv), mul_rn(x[j][4 * i + 2], k_inv),
+                        mul_rn(x[j][4 * i + 3], k_inv));
+      *at = w;
+    } else if (k_grown && r < off) {
+      const float f = recode_factor(k_old, k_now);
+      u32x4_t w = *at;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = recode(w[i], f);
+      *at = w;
+    }
+  }
+
+  const uint32_t before = tokens_below(off - 4 * g);                      // earlier tokens of the group
+  const uint32_t fresh = tokens_below(off + n - 4 * g) & ~before;         // the run's
+  const bool merge = fresh != ~0u;
+#pragma unroll
+  for (int j = 0; j < kParts; ++j) {
+    constexpr int kLast = D % 64 == 0 ? 4 : 2;
+    const int w = j + 1 < kParts ? 4 : kLast;
+    uint32_t* at = reinterpret_cast<uint32_t*>(v_codes + g * (4 * D) + 256 * j + 4 * w * r);
+    if (fresh == 0u && !(v_grown && before != 0u)) continue;
+    u32x4_t old = {0, 0, 0, 0};
+    if (merge) {
+      if (w == 4) old = *reinterpret_cast<const u32x4_t*>(at);
+      else { const u32x2_t o = *reinterpret_cast<const u32x2_t*>(at); old[0] = o[0]; old[1] = o[1]; }
+    }
+    const float f = recode_factor(v_old, v_now);
+    u32x4_t out;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (e >= w) continue;
+      const uint32_t c = codes_of(mul_rn(y[j][0][e], v_inv), mul_rn(y[j][1][e], v_inv), mul_rn(y[j][2][e], v_inv),
+                                  mul_rn(y[j][3][e], v_inv));
+      uint32_t kept = old[e];
+      if (v_grown) kept = (kept & ~before) | (recode(kept, f) & before);
+      out[e] = (c & fresh) | (kept & ~fresh);
+    }
+    if (w == 4) *reinterpret_cast<u32x4_t*>(at) = out;
+    else *reinterpret_cast<u32x2_t*>(at) = (u32x2_t){out[0], out[1]};
+  }
+  if (lane == 0) {
+    P.cache.scales[k_tile] = (uint8_t)k_now;
+    P.cache.scales[v_tile] = (uint8_t)v_now;
+  }
+}
+
+// The rotated queries, and the keys and values as codes. Both halves are bound by HBM bytes.
+template <typename T, int D, int STYLE>
+__global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteParams P) {
+  const int lane = threadIdx.x & 63;
+  if (blockIdx.x < P.kv_blocks) {
+    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int heads = P.cache.num_kv_heads;
+    const int64_t chunk = item / heads;
+    const int head = (int)(item - chunk * heads);
+    if (chunk >= P.chunks) return;
+    // Lane t holds the slots of token base + t and of the one before it; a run reaches at most 15
+    // tokens past the chunk.
+    const int64_t base = chunk * P.chunk, idx = base + lane;
+    auto slot = [&](int64_t i) -> int64_t {
+      if (i < 0 || i >= P.tokens) return -1;
+      const int64_t row = P.rows[i];
+      if (row < 0 || row >= P.pool_rows) return -1;
+      if (STYLE != 0) {
+        const int p = P.positions[i];
+        if (p < 0 || p >= P.max_positions) return -1;
+      }
+      return row;
+    };
+    const bool near = lane < P.chunk + 16;
+    const int64_t row = near ? slot(idx) : -1;
+    const int64_t prev = near ? slot(idx - 1) : -1;
+    const bool follows = row >= 0 && prev >= 0 && row == prev + 1 && (row & 15) != 0;
+    uint64_t starts = __ballot(row >= 0 && !follows && lane < P.chunk);
+    const uint64_t conts = __ballot(follows);
+    while (starts != 0) {
+      const int s = __builtin_ctzll(starts);
+      starts &= starts - 1;
+      const int n = 1 + __builtin_ctzll(~(conts >> (s + 1)));
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)row, s);
+      const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(row >> 32), s);
+      write_run<T, D, STYLE>(P, base + s, n, (int64_t)(((uint64_t)hi << 32) | lo), head);
+    }
+    return;
+  }
+  // Queries: 16 elements a thread, two pieces of 8 (STYLE 1: one of each half).
+  const int64_t item = (int64_t)(blockIdx.x - P.kv_blocks) * 256 + threadIdx.x;
+  constexpr int kUnits = D / 16;
+  const int u = (int)(item % kUnits);
+  const int64_t th = item / kUnits;
+  const int64_t t = th / P.num_heads;
+  const int h = (int)(th - t * P.num_heads);
+  if (t >= P.tokens) return;
+  const int64_t row = P.rows[t];
+  if (row < 0) return;
+  int64_t angle = 0;
+  bool bad = false;
+  if constexpr (STYLE != 0) {
+    const int p = P.positions[t];
+    bad = p < 0 || p >= P.max_positions;
+    angle = bad ? 0 : (int64_t)p * (D / 2);
+  }
+  const T* q = static_cast<const T*>(P.q) + t * P.q_stride + h * D;
+  const T* bias = P.q_bias == nullptr ? nullptr : static_cast<const T*>(P.q_bias) + h * D;
+  T* out = static_cast<T*>(P.q_out) + (t * P.num_heads + h) * D;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    const int d = STYLE == 1 ? 8 * u + half * (D / 2) : 16 * u + 8 * half;
+    float x[8];
+    load_rotated<T, D, STYLE, 8>(q, bias, P.cos + angle, P.sin + angle, d, P.vec, x);
+    Vec<T, 8> w;
+#pragma unroll
+    for (int i = 0; i < 8; i += 2)
+      w.set_pair(i, bad ? NAN : x[i], bad ? NAN : x[i + 1]);
+    w.store(out + d);
+  }
+}
+
+template <typename T, int D>
+static int write_style(const Kv8WriteParams& P, int style, int64_t blocks, hipStream_t stream) {
+  const dim3 grid((unsigned)blocks), wg(256);
+  if (style == 0) kv8_write_kernel<T, D, 0><<<grid, wg, 0, stream>>>(P);
+  else if (style == 1) kv8_write_kernel<T, D, 1><<<grid, wg, 0, stream>>>(P);
+  else kv8_write_kernel<T, D, 2><<<grid, wg, 0, stream>>>(P);
+  return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;
+}
+
+template <typename T>
+static int write_dim(const Kv8WriteParams& P, int dim, int style, int64_t blocks, hipStream_t stream) {
+  switch (dim) {
+    case 64: return write_style<T, 64>(P, style, blocks, stream);
+    case 96: return write_style<T, 96>(P, style, blocks, stream);
+    case 128: return write_style<T, 128>(P, style, blocks, stream);
+    default: return CDB_ERR_UNSUPPORTED;
+  }
+}
+
+// -- batch layout -------------------------------------------------------------------------------------------------
+
+struct LayoutParams {
+  const int32_t *past, *lens, *table_row, *free_blocks;
+  int32_t* table;
+  int32_t num_seqs, table_rows, table_width, num_free, bs_log2;
+  int32_t *cu_q, *positions, *tile_seq, *tile_q0, *counts;
+  int64_t* rows;
+  int32_t token_capacity, tile_capacity;
+};
+
+constexpr int kLayoutThreads = 1024;
+constexpr int kLayoutWaves = kLayoutThreads / 64;
+constexpr int kTileQueries = 128;
+
+// Inclusive scan over the lanes of a wave.
+CDB_DEVICE int64_t wave_scan(int64_t v) {
+  const int lane = threadIdx.x & 63;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const int64_t up = __shfl_up((long long)v, d);
+    if (lane >= d) v += up;
+  }
+  return v;
+}
+
+// The last i with first[i] <= x, for ascending first[0..n] with first[0] <= x < first[n].
+CDB_DEVICE int last_at_most(const int32_t* first, int n, int x) {
+  int lo = 0, hi = n;
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) >> 1;
+    if (first[mid] <= x) lo = mid;
+    else hi = mid;
+  }
+  return lo;
+}
+
+// Tiles of a sequence whose key range ends past x (tile j's ends at past + min(128 (j + 1), len)).
+CDB_DEVICE int tiles_past(int x, int past, int len) {
+  const int y = x - past;
+  if (y >= len) return 0;
+  const int tiles = (len + kTileQueries - 1) / kTileQueries;
+  return y < 0 ? tiles : tiles - y / kTileQueries;
+}
+
+// Every workgroup scans the requests' lengths into LDS (a few microseconds' work that saves a second
+// launch and any order between workgroups), then takes its share of tokens, new blocks and tiles.
+// A tile's place in the longest-first list is the number of tiles before it in that order: counted per
+// request in closed form, a wave's lanes splitting the requests.
+__global__ void __launch_bounds__(kLayoutThreads) batch_layout_kernel(LayoutParams P) {
+  extern __shared__ int32_t lds[];
+  const int S = P.num_seqs;
+  int32_t* cu = lds;                 // [S + 1] first token
+  int32_t* taken = cu + S + 1;       // [S + 1] first new block
+  int32_t* tiles = taken + S + 1;    // [S + 1] first tile
+  int32_t* begin = tiles + S + 1;    // [S] cached tokens
+  __shared__ int64_t part[kLayoutWaves][3];
+  __shared__ int32_t status;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  if (tid == 0) status = 0;
+  __syncthreads();
+  const int64_t most = (int64_t)P.table_width << P.bs_log2;
+  const int bs_mask = (1 << P.bs_log2) - 1;
+  const int each = (S + kLayoutThreads - 1) / kLayoutThreads;
+  const int s0 = min(tid * each, S), s1 = min(s0 + each, S);
+  auto request = [&](int s, int& past, int& len) {
+    past = P.past[s];
+    len = P.lens[s];
+    const int row = P.table_row == nullptr ? s : P.table_row[s];
+    if (past < 0 || len < 0 || (int64_t)past + len > most || row < 0 || row >= P.table_rows) {
+      past = len = 0;
+      atomicOr(&status, CDB_LAYOUT_BAD_REQUEST);
+    }
+  };
+  int64_t sum[3] = {0, 0, 0};
+  for (int s = s0; s < s1; ++s) {
+    int past, len;
+    request(s, past, len);
+    sum[0] += len;
+    sum[1] += ((past + len + bs_mask) >> P.bs_log2) - ((past + bs_mask) >> P.bs_log2);
+    sum[2] += (len + kTileQueries - 1) / kTileQueries;
+  }
+  int64_t upto[3];
+#pragma unroll
+  for (int c = 0; c < 3; ++c) {
+    upto[c] = wave_scan(sum[c]);
+    if (lane == 63) part[wave][c] = upto[c];
+    upto[c] -= sum[c];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int c = 0; c < 3; ++c)
+    for (int w = 0; w < wave; ++w) upto[c] += part[w][c];
+  auto clip = [](int64_t x) { return (int32_t)(x < 0x7fffffff ? x : 0x7fffffff); };
+  for (int s = s0; s < s1; ++s) {
+    int past, len;
+    request(s, past, len);
+    cu[s] = clip(upto[0]);
+    taken[s] = clip(upto[1]);
+    tiles[s] = clip(upto[2]);
+    begin[s] = past;
+    upto[0] += len;
+    upto[1] += ((past + len + bs_mask) >> P.bs_log2) - ((past + bs_mask) >> P.bs_log2);
+    upto[2] += (len + kTileQueries - 1) / kTileQueries;
+  }
+  if (tid == kLayoutThreads - 1) {
+    cu[S] = clip(upto[0]);
+    taken[S] = clip(upto[1]);
+    tiles[S] = clip(upto[2]);
+  }
+  __syncthreads();
+  const int num_tokens = cu[S], num_taken = taken[S], num_tiles = tiles[S];
+  if (blockIdx.x == 0) {
+    for (int s = tid; s <= S; s += kLayoutThreads) P.cu_q[s] = cu[s];
+    if (tid == 0) {
+      P.counts[0] = num_tokens;
+      P.counts[1] = num_tiles;
+      P.counts[2] = num_taken;
+      P.counts[3] = status | (num_tokens > P.token_capacity ? CDB_LAYOUT_TOKENS_FULL : 0) |
+                    (num_tiles > P.tile_capacity ? CDB_LAYOUT_TILES_FULL : 0) |
+                    (num_taken > P.num_free ? CDB_LAYOUT_NO_BLOCKS : 0);
+    }
+  }
+  const int64_t stride = (int64_t)gridDim.x * kLayoutThreads;
+  const int64_t id = (int64_t)blockIdx.x * kLayoutThreads + tid;
+  auto table_at = [&](int s) { return P.table + (int64_t)(P.table_row == nullptr ? s : P.table_row[s]) * P.table_width; };
+
+  for (int64_t t = id; t < P.token_capacity; t += stride) {
+    int pos = -1;
+    int64_t row = -1;
+    if (t < num_tokens) {
+      const int s = last_at_most(cu, S, (int)t);
+      pos = begin[s] + (int)t - cu[s];
+      const int held = (begin[s] + bs_mask) >> P.bs_log2, column = pos >> P.bs_log2;
+      int block;
+      if (column < held) {
+        block = table_at(s)[column];
+      } else {
+        const int n = taken[s] + column - held;
+        block = n < P.num_free ? P.free_blocks[n] : -1;
+      }
+      if (block >= 0) row = ((int64_t)block << P.bs_log2) + (pos & bs_mask);
+    }
+    P.positions[t] = pos;
+    P.rows[t] = row;
+  }
+  for (int64_t n = id; n < num_taken; n += stride) {
+    const int s = last_at_most(taken, S, (int)n);
+    const int column = ((begin[s] + bs_mask) >> P.bs_log2) + (int)n - taken[s];
+    table_at(s)[column] = n < P.num_free ? P.free_blocks[n] : -1;
+  }
+  for (int64_t n = num_tiles + id; n < P.tile_capacity; n += stride) {
+    P.tile_seq[n] = -1;
+    P.tile_q0[n] = 0;
+  }
+  for (int64_t n = (int64_t)blockIdx.x * kLayoutWaves + wave; n < num_tiles; n += (int64_t)gridDim.x * kLayoutWaves) {
+    const int s = last_at_most(tiles, S, (int)n);
+    const int q0 = ((int)n - tiles[s]) * kTileQueries;
+    const int end = begin[s] + min(q0 + kTileQueries, cu[s + 1] - cu[s]);
+    int before = 0;
+    for (int o = lane; o < S; o += 64) before += tiles_past(o < s ? end - 1 : end, begin[o], cu[o + 1] - cu[o]);
+#pragma unroll
+    for (int m = 32; m >= 1; m >>= 1) before += __shfl_xor(before, m);
+    if (lane == 0 && before < P.tile_capacity) {
+      P.tile_seq[before] = s;
+      P.tile_q0[before] = q0;
+    }
+  }
+}
+
+}  // namespace cdb
+
+extern "C" int cdb_kv8_write(const void* q, const void* k, const void* v, void* q_out, void* codes, void* scales,
+                             int32_t num_cache_layers, int64_t pool_blocks, int32_t layer, const int64_t* rows,
+                             const int32_t* positions, const float* rope_cos, const float* rope_sin,
+                             int32_t rope_style, int32_t max_positions, const void* q_bias, const void* k_bias,
+                             int64_t tokens, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, int64_t q_stride, int64_t kv_stride, int32_t dtype,
+                             hipStream_t stream) {
+  using namespace cdb;
+  if (tokens < 0 || num_heads < 0 || layer < 0 || layer >= num_cache_layers) return CDB_ERR_SHAPE;
+  if (rope_style < 0 || rope_style > 2) return CDB_ERR_UNSUPPORTED;
+  if (tokens == 0) return CDB_OK;
+  if (k == nullptr || v == nullptr || rows == nullptr) return CDB_ERR_NULL;
+  if (num_heads > 0 && (q == nullptr || q_out == nullptr)) return CDB_ERR_NULL;
+  if (rope_style != 0 && (rope_cos == nullptr || rope_sin == nullptr || positions == nullptr)) return CDB_ERR_NULL;
+  if (rope_style != 0 && max_positions <= 0) return CDB_ERR_SHAPE;
+  Kv8WriteParams P{};
+  const int code = kv8_cache_of(&P.cache, codes, scales, num_cache_layers, pool_blocks, num_kv_heads, head_dim, block_size);
+  if (code != CDB_OK) return code;
+  if (dtype != CDB_DTYPE_F32 && dtype != CDB_DTYPE_BF16) return CDB_ERR_UNSUPPORTED;
+  if (q_stride == 0) q_stride = (int64_t)num_heads * head_dim;
+  if (kv_stride == 0) kv_stride = (int64_t)num_kv_heads * head_dim;
+  if ((num_heads > 0 && q_stride < (int64_t)num_heads * head_dim) || kv_stride < (int64_t)num_kv_heads * head_dim)
+    return CDB_ERR_SHAPE;
+  if (q_out != nullptr && reinterpret_cast<uintptr_t>(q_out) % 16 != 0) return CDB_ERR_SHAPE;
+  const int size = dtype == CDB_DTYPE_F32 ? 4 : 2;
+  P.q = q; P.k = k; P.v = v; P.q_out = q_out;
+  P.layer = layer; P.rows = rows; P.pool_rows = pool_blocks * block_size; P.positions = positions;
+  P.cos = rope_cos; P.sin = rope_sin; P.q_bias = q_bias; P.k_bias = k_bias;
+  P.tokens = tokens; P.q_stride = q_stride; P.kv_stride = kv_stride;
+  P.num_heads = num_heads; P.max_positions = max_positions;
+  P.vec = kv8_aligned(size, {q, k, v, q_bias, k_bias, rope_cos, rope_sin}, {q_stride, kv_stride});
+  // A chunk of 16 tokens is one tile's worth of a prompt. Few tokens take one a wave, so that a decode
+  // batch, whose every token is a run of its own, is not written 16 runs one after the other.
+  P.chunk = tokens <= 1024 ? 1 : 16;
+  P.chunks = (tokens + P.chunk - 1) / P.chunk;
+  P.kv_blocks = (P.chunks * num_kv_heads + 3) / 4;
+  const int64_t q_blocks = (tokens * num_heads * (head_dim / 16) + 255) / 256;
+  if (P.kv_blocks + q_blocks > 0x7fffffffll) return CDB_ERR_SHAPE;
+  return dtype == CDB_DTYPE_F32 ? write_dim<float>(P, head_dim, rope_style, P.kv_blocks + q_blocks, stream)
+                                : write_dim<bf16_t>(P, head_dim, rope_style, P.kv_blocks + q_blocks, stream);
+}
+
+extern "C" int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs, int32_t* block_table,
+                                const int32_t* table_row, int32_t table_rows, int32_t table_width,
+                                const int32_t* free_blocks, int32_t num_free, int32_t block_size, int32_t* cu_q,
+                                int32_t* positions, int64_t* rows, int32_t token_capacity, int32_t* tile_seq,
+                                int32_t* tile_q0, int32_t tile_capacity, int32_t* counts, hipStream_t stream) {
+  using namespace cdb;
+  if (num_seqs < 0 || num_seqs > CDB_LAYOUT_MAX_SEQS || table_rows < 0 || table_width <= 0 || num_free < 0 ||
+      token_capacity < 0 || tile_capacity < 0)
+    return CDB_ERR_SHAPE;
+  if (block_size <= 0 || (block_size & (block_size - 1)) != 0) return CDB_ERR_SHAPE;
+  if ((int64_t)table_width * block_size > (1ll << 30)) return CDB_ERR_SHAPE;
+  if (table_row == nullptr && table_rows < num_seqs) return CDB_ERR_SHAPE;
+  if (cu_q == nullptr || counts == nullptr || (num_seqs > 0 && (past == nullptr || lens == nullptr || block_table == nullptr)))
+    return CDB_ERR_NULL;
+  if ((token_capacity > 0 && (positions == nullptr || rows == nullptr)) ||
+      (tile_capacity > 0 && (tile_seq == nullptr || tile_q0 == nullptr)) || (num_free > 0 && free_blocks == nullptr))
+    return CDB_ERR_NULL;
+  LayoutParams P{};
+  P.past = past; P.lens = lens; P.table_row = table_row; P.free_blocks = free_blocks; P.table = block_table;
+  P.num_seqs = num_seqs; P.table_rows = table_rows; P.table_width = table_width; P.num_free = num_free;
+  P.bs_log2 = __builtin_ctz(block_size);
+  P.cu_q = cu_q; P.positions = positions; P.rows = rows; P.tile_seq = tile_seq; P.tile_q0 = tile_q0; P.counts = counts;
+  P.token_capacity = token_capacity; P.tile_capacity = tile_capacity;
+  const size_t lds = sizeof(int32_t) * (4 * (size_t)num_seqs + 3);
+  // A token a thread, a tile a wave, at most one workgroup a CU.
+  const int64_t want = max((int64_t)token_capacity / kLayoutThreads, (int64_t)tile_capacity / kLayoutWaves) + 1;
+  batch_layout_kernel<<<dim3((unsigned)min(want, (int64_t)256)), dim3(kLayoutThreads), lds, stream>>>(P);
+  return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;
+}

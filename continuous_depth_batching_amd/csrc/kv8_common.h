@@ -1,0 +1,163 @@
+// Device helpers of the 8-bit KV cache kernels.
+//
+// The cache holds tiles of 16 tokens of one KV head, keys and values apart: e4m3 codes and one
+// power-of-two scale a tile, kept as its biased exponent (byte b stands for 2^(b - 127)). A scale
+// that is a power of two makes every step but the rounding to e4m3 itself exact: scaling a value
+// down, widening a code to bf16 or fp16, and rescaling a code when a tile's scale grows.
+//
+// Tile t (counted over [layer, plane, block, head, block_size / 16]) has its codes at t * 16 * D and
+// its scale at t. Inside a tile the codes lie as the MFMA kernels read them, 16 bytes a lane:
+//   keys   [D / 16][16 tokens][16]: unit u of token r holds elements 16u..16u+15;
+//   values [4][D][4 tokens]: group g of element d holds tokens 4g..4g+3.
+#pragma once
+
+#include "cdb_common.h"
+
+namespace cdb {
+
+constexpr int kTile = 16;  // tokens of a tile
+
+typedef __bf16 bf16x2_t __attribute__((ext_vector_type(2)));
+typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
+typedef float f32x2_t __attribute__((ext_vector_type(2)));
+typedef float f32x4_t __attribute__((ext_vector_type(4)));
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+
+// 2^(b - 127) of a scale byte, as the conversion instructions take it.
+CDB_DEVICE float scale_of(uint32_t b) { return __uint_as_float(b << 23); }
+// 2^(127 - b): the factor that brings a value to a code. Bytes above 253 give 0.
+CDB_DEVICE float inverse_scale_of(uint32_t b) { return b >= 254u ? 0.f : __uint_as_float((254u - b) << 23); }
+
+// The byte of the smallest power of two s with amax / s <= 448 = 1.75 * 2^8, for a finite amax >= 0:
+// its exponent less 8, one more where the mantissa is above 1.75.
+CDB_DEVICE int scale_byte(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  const int b = (int)(bits >> 23) - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return min(max(b, 1), 254);
+}
+
+// |x| where x is finite, else 0: infinities and NaN take no part in a tile's scale.
+CDB_DEVICE float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+
+// Four values, already divided by the scale, as e4m3 codes in one word, rounded to nearest even.
+// An infinity or NaN becomes the NaN code.
+CDB_DEVICE uint32_t codes_of(float a, float b, float c, float d) {
+  auto clean = [](float x) { return fabsf(x) < INFINITY ? x : __uint_as_float(0x7fc00000u); };
+  int w = __builtin_amdgcn_cvt_pk_fp8_f32(clean(a), clean(b), 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clean(c), clean(d), w, true);
+}
+
+// Codes of one word rounded again for a scale 2^grow times larger (factor = 2^-grow).
+CDB_DEVICE uint32_t recode(uint32_t w, float factor) {
+  const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
+  const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  return codes_of(mul_rn(lo.x, factor), mul_rn(lo.y, factor), mul_rn(hi.x, factor), mul_rn(hi.y, factor));
+}
+
+// 2^(old - now) for old <= now, flushed to 2^-126 beyond the normal range (every code then gives 0).
+CDB_DEVICE float recode_factor(int old, int now) { return __uint_as_float((uint32_t)max(127 + old - now, 1) << 23); }
+
+// Byte mask of a word's tokens below n (n <= 0: none, n >= 4: all).
+CDB_DEVICE uint32_t tokens_below(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
+
+// N storage elements as fp32; vec: p is aligned for 16-byte loads (8-byte ones where N elements are 8 bytes).
+template <typename T, int N> CDB_DEVICE void load_f32(const T* p, float* out, bool vec) {
+  if (vec) {
+    Vec<T, N> x;
+    x.load(p);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = x.get(i);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = Elem<T>::load(p + i);
+  }
+}
+
+// N consecutive elements of a head, from element d on: x + bias, rotated, in fp32 with every product
+// and sum rounded once. STYLE 1 pairs element d with d + D/2, STYLE 2 pairs even and odd elements.
+// Runs of N must not cross D/2 (STYLE 1); cos/sin point at the position's row of D/2 angles.
+template <typename T, int D, int STYLE, int N>
+CDB_DEVICE void load_rotated(const T* head, const T* bias, const float* cos, const float* sin, int d, bool vec,
+                             float* out) {
+  load_f32<T, N>(head + d, out, vec);
+  if (bias != nullptr) {
+    float b[N];
+    load_f32<T, N>(bias + d, b, vec);
+#pragma unroll
+    for (int i = 0; i < N; ++i) out[i] = add_rn(out[i], b[i]);
+  }
+  if constexpr (STYLE == 1) {
+    const bool low = d < D / 2;
+    const int pd = low ? d + D / 2 : d - D / 2;
+    const int a = low ? d : pd;
+    float p[N], c[N], s[N];
+    load_f32<T, N>(head + pd, p, vec);
+    if (bias != nullptr) {
+      float b[N];
+      load_f32<T, N>(bias + pd, b, vec);
+#pragma unroll
+      for (int i = 0; i < N; ++i) p[i] = add_rn(p[i], b[i]);
+    }
+    load_f32<float, N>(cos + a, c, vec);
+    load_f32<float, N>(sin + a, s, vec);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float ps = mul_rn(p[i], s[i]);
+      out[i] = add_rn(mul_rn(out[i], c[i]), low ? -ps : ps);
+    }
+  } else if constexpr (STYLE == 2) {
+    float c[N / 2], s[N / 2];
+    load_f32<float, N / 2>(cos + d / 2, c, vec);
+    load_f32<float, N / 2>(sin + d / 2, s, vec);
+#pragma unroll
+    for (int i = 0; i < N / 2; ++i) {
+      const float e = out[2 * i], o = out[2 * i + 1];
+      out[2 * i] = sub_rn(mul_rn(e, c[i]), mul_rn(o, s[i]));
+      out[2 * i + 1] = add_rn(mul_rn(o, c[i]), mul_rn(e, s[i]));
+    }
+  }
+}
+
+// Max over the four lanes that differ in bits 4 and 5.
+CDB_DEVICE float column_max(float v) {
+  v = fmaxf(v, shfl_xor_f32(v, 16));
+  return fmaxf(v, shfl_xor_f32(v, 32));
+}
+CDB_DEVICE float column_sum(float v) {
+  v += shfl_xor_f32(v, 16);
+  return v + shfl_xor_f32(v, 32);
+}
+
+// 8 codes (two words) widened to bf16 with their scale: exact, e4m3 has 4 significant bits.
+CDB_DEVICE bf16x8_t widen_bf16(uint32_t w0, float s0, uint32_t w1, float s1) {
+  union { bf16x2_t p[4]; bf16x8_t v; } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s0, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w0, s0, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s1, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w1, s1, true);
+  return u.v;
+}
+
+// The cache as a kernel sees it: all strides in tiles.
+struct Kv8Cache {
+  uint8_t* codes;
+  uint8_t* scales;
+  int64_t plane_tiles;  // pool_blocks * num_kv_heads * tiles of a block
+  int64_t pool_blocks;
+  int32_t num_layers;
+  int32_t num_kv_heads;
+  int32_t tile_log2;    // log2 of the tiles of a block
+
+  CDB_DEVICE int64_t tile(int64_t layer, int plane, int64_t block, int head, int sub) const {
+    return (layer * 2 + plane) * plane_tiles + ((block * num_kv_heads + head) << tile_log2) + sub;
+  }
+};
+
+}  // namespace cdb

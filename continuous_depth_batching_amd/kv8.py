@@ -1,0 +1,450 @@
+"""An 8-bit paged KV cache: its write, the attention that reads it, and the layout of a batch.
+
+Keys and values are held in tiles of 16 tokens of one KV head as e4m3 codes with one power-of-two
+scale a tile (``include/cdb_amd.h``, "8-bit KV cache"): half the bytes of a bf16 cache, and half the
+time of a decode step's attention, which reads every cached byte once. The calls mirror those of the
+pool in the model's type (``ops``): ``write`` beside ``rope_kv_write``, ``decode_attention`` beside
+``paged_decode_attention``, ``prefill_attention`` beside ``prefill_attention``; ``batch_layout`` builds
+on the GPU what they take as block tables, slots and attention tiles.
+
+Each ``*_raw`` function checks its arguments on the host and makes one C call on torch's current stream
+without allocating, so it can be captured into a HIP graph; the ``torch.ops.cdb.kv8_*`` ops wrap them.
+Tensors must lie on the current device.
+"""
+
+from __future__ import annotations
+
+from dataclasses import dataclass
+
+import torch
+
+from . import _lib
+from .ops import _ptr, _require_contiguous, _require_int32, _stream, dtype_code
+
+TILE = 16  # tokens of a cache tile
+PREFILL_TILE = 128  # query tokens of an attention tile
+
+LAYOUT_TOKENS_FULL = _lib.CDB_LAYOUT_TOKENS_FULL
+LAYOUT_TILES_FULL = _lib.CDB_LAYOUT_TILES_FULL
+LAYOUT_NO_BLOCKS = _lib.CDB_LAYOUT_NO_BLOCKS
+LAYOUT_BAD_REQUEST = _lib.CDB_LAYOUT_BAD_REQUEST
+
+
+@dataclass(frozen=True)
+class Kv8Pool:
+    """The cache: ``codes`` float8_e4m3fn ``[layers, 2, blocks, Hkv, block_size / 16, 16 * D]`` and
+    ``scales`` uint8 ``[layers, 2, blocks, Hkv, block_size / 16]`` (b stands for 2 ** (b - 127)), keys at
+    index 0 of dim 1 and values at 1."""
+
+    codes: torch.Tensor
+    scales: torch.Tensor
+
+    def __post_init__(self) -> None:
+        c, s = self.codes, self.scales
+        if c.dtype is not torch.float8_e4m3fn or s.dtype is not torch.uint8:
+            raise TypeError("an 8-bit pool holds float8_e4m3fn codes and uint8 scales")
+        if c.dim() != 6 or c.shape[1] != 2 or tuple(s.shape) != tuple(c.shape[:5]) or c.shape[5] % TILE:
+            raise ValueError("codes must be [layers, 2, blocks, Hkv, block_size / 16, 16 * D] and scales match them")
+        if not c.is_contiguous() or not s.is_contiguous() or c.device != s.device:
+            raise ValueError("codes and scales must be contiguous and on one device")
+        # What every call needs of the pool, resolved once.
+        object.__setattr__(self, "_args", (c.data_ptr(), s.data_ptr(), c.shape[0], c.shape[2]))
+        object.__setattr__(self, "_shape", (c.shape[3], c.shape[5] // TILE, c.shape[4] * TILE))
+
+    @classmethod
+    def allocate(cls, num_cache_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
+                 device: torch.device | str) -> "Kv8Pool":
+        """A pool of zeros."""
+
+        if block_size < TILE or block_size & (block_size - 1):
+            raise ValueError(f"block_size must be a power of two of at least {TILE}, got {block_size}")
+        shape = (num_cache_layers, 2, num_blocks, num_kv_heads, block_size // TILE)
+        codes = torch.zeros((*shape, TILE * head_dim), dtype=torch.uint8, device=device).view(torch.float8_e4m3fn)
+        return cls(codes, torch.zeros(shape, dtype=torch.uint8, device=device))
+
+    @property
+    def num_cache_layers(self) -> int:
+        return self.codes.shape[0]
+
+    @property
+    def num_blocks(self) -> int:
+        return self.codes.shape[2]
+
+    @property
+    def num_kv_heads(self) -> int:
+        return self._shape[0]
+
+    @property
+    def head_dim(self) -> int:
+        return self._shape[1]
+
+    @property
+    def block_size(self) -> int:
+        return self._shape[2]
+
+    def dequantize(self, layer: int, blocks: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+        """fp32 keys and values ``[len(blocks) * block_size, Hkv, D]`` of the named blocks of a cache layer, for
+        inspection and tests (torch indexing, not a kernel)."""
+
+        d = self.head_dim
+        raw = self.codes.view(torch.uint8)[layer][:, blocks].view(torch.float8_e4m3fn).float()
+        scale = torch.ldexp(torch.ones((), device=raw.device, dtype=torch.float64),
+                            self.scales[layer][:, blocks].int() - 127).float()
+        raw = raw * scale[..., None]
+        k = raw[0].unflatten(-1, (d // 16, TILE, 16)).transpose(-3, -2).flatten(-2)   # [blocks, Hkv, tiles, 16, D]
+        v = raw[1].unflatten(-1, (4, d, 4)).transpose(-2, -1).flatten(-3, -2)
+        return tuple(x.permute(0, 2, 3, 1, 4).flatten(0, 2) for x in (k, v))
+
+
+def _require_here(*tensors: torch.Tensor | None) -> None:
+    """Every tensor on the current device, whose stream the launch goes to."""
+
+    here = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            raise RuntimeError("CDB kernels run on the GPU only; got a tensor on " + str(t.device))
+        if here is None:
+            here = torch.cuda.current_device()
+        if t.get_device() != here:
+            raise RuntimeError(f"got a tensor on {t.device} while cuda:{here} is the current device")
+
+
+def _check_rope(rope_style: int, cos: torch.Tensor | None, sin: torch.Tensor | None, head_dim: int) -> int:
+    """The tables' positions; raises on tables that do not fit."""
+
+    if rope_style == 0:
+        return 0
+    if rope_style not in (1, 2):
+        raise ValueError(f"rope_style must be 0, 1 or 2, got {rope_style}")
+    if cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
+            or cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != head_dim // 2:
+        raise ValueError("rope tables must be float32 [max_positions, D/2]")
+    _require_contiguous(rope_cos=cos, rope_sin=sin)
+    return cos.shape[0]
+
+
+def _check_bias(name: str, bias: torch.Tensor | None, heads: int, dim: int, dtype: torch.dtype) -> None:
+    if bias is None:
+        return
+    if bias.shape != (heads, dim) or bias.dtype is not dtype or not bias.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous [{heads}, {dim}] tensor of q's dtype")
+
+
+def _row_stride(name: str, t: torch.Tensor, head_dim: int) -> int:
+    """Elements between rows of a [rows, heads, D] tensor whose heads are dense; a single row's is its own size."""
+
+    rows, heads, _ = t.shape
+    s = t.stride()
+    if s[2] != 1 or (s[1] != head_dim and heads > 1):
+        raise ValueError(f"{name} must have contiguous heads and head dimension (the row stride may differ)")
+    if rows <= 1:
+        return heads * head_dim
+    if s[0] < heads * head_dim:
+        raise ValueError(f"{name}'s rows overlap")
+    return s[0]
+
+
+def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor | None, pool: Kv8Pool,
+              layer: int, rows: torch.Tensor, positions: torch.Tensor, rope_cos: torch.Tensor | None,
+              rope_sin: torch.Tensor | None, rope_style: int, q_bias: torch.Tensor | None,
+              k_bias: torch.Tensor | None) -> None:
+    """Launch ``cdb_kv8_write``: code T tokens' rotated keys and their values into slots ``rows`` of cache layer
+    ``layer`` and put the rotated queries into ``q_out`` (q and q_out None: keys and values alone). q, k and v
+    may be token-strided views. The tokens of one tile follow each other at consecutive slots; a negative slot
+    is padding, whose q_out is left as it was."""
+
+    heads_kv, dim, block = pool._shape
+    if k.dim() != 3 or k.shape[1:] != (heads_kv, dim) or v.shape != k.shape or v.dtype is not k.dtype:
+        raise ValueError(f"k and v must be [T, {heads_kv}, {dim}] of one dtype")
+    tokens = k.shape[0]
+    heads = 0
+    if (q is None) != (q_out is None):
+        raise ValueError("q and q_out come together")
+    if q is not None:
+        heads = q.shape[1]
+        if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim or q.dtype is not k.dtype:
+            raise ValueError(f"q must be [{tokens}, H, {dim}] of k's dtype")
+        if q_out.shape != q.shape or q_out.dtype is not q.dtype or not q_out.is_contiguous():
+            raise ValueError("q_out must be contiguous and match q")
+    if rows.dtype is not torch.int64 or positions.dtype is not torch.int32:
+        raise TypeError("rows must be int64 and positions int32")
+    if rows.numel() < tokens or positions.numel() < tokens:
+        raise ValueError("rows and positions need an entry per token")
+    if not 0 <= layer < pool._args[2]:
+        raise ValueError("layer out of range")
+    max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
+    _check_bias("q_bias", q_bias, heads, dim, k.dtype)
+    _check_bias("k_bias", k_bias, heads_kv, dim, k.dtype)
+    _require_contiguous(rows=rows, positions=positions)
+    _require_here(q, k, v, q_out, pool.codes, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
+    kv_stride = _row_stride("k", k, dim)
+    if _row_stride("v", v, dim) != kv_stride:
+        raise ValueError("k and v must share one token stride")
+    codes, scales, layers, blocks = pool._args
+    code = _lib.lib().cdb_kv8_write(
+        _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), codes, scales, layers, blocks, layer, rows.data_ptr(),
+        positions.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
+        tokens, heads, heads_kv, dim, block, 0 if q is None else _row_stride("q", q, dim), kv_stride,
+        dtype_code(k.dtype), _stream())
+    if code:
+        _lib.check(code, "cdb_kv8_write")
+
+
+@torch.library.custom_op("cdb::kv8_write", mutates_args=("codes", "scales"), device_types="cuda")
+def write(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, layer: int,
+          rows: torch.Tensor, positions: torch.Tensor, rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None,
+          rope_style: int, q_bias: torch.Tensor | None, k_bias: torch.Tensor | None) -> torch.Tensor:
+    """Rotate and append T tokens to the 8-bit cache; returns the rotated queries [T, H, D] (zeros for padding
+    tokens, whose slot is negative)."""
+
+    q_rot = q.new_zeros(q.shape)
+    write_raw(q, k, v, q_rot, Kv8Pool(codes, scales), layer, rows, positions, rope_cos, rope_sin, rope_style, q_bias,
+              k_bias)
+    return q_rot
+
+
+@write.register_fake
+def _(q, k, v, codes, scales, layer, rows, positions, rope_cos, rope_sin, rope_style, q_bias, k_bias):
+    return q.new_empty(q.shape)
+
+
+def decode_workspace_bytes(num_rows: int, num_heads: int, num_kv_heads: int, head_dim: int, max_seqlen: int) -> int:
+    """Workspace of decode launches of up to ``num_rows`` rows whose positions are below ``max_seqlen``. Rows with
+    longer contexts are served too, in fewer and longer chunks."""
+
+    n = int(_lib.lib().cdb_kv8_decode_workspace_bytes(num_rows, num_heads, num_kv_heads, head_dim, max_seqlen))
+    if n < 0:
+        raise ValueError("invalid arguments for the decode workspace size")
+    return n
+
+
+def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, pool: Kv8Pool,
+                         cache_layer: torch.Tensor | None, cache_layer0: int, block_table: torch.Tensor,
+                         table_row: torch.Tensor | None, seqlens: torch.Tensor, rope_cos: torch.Tensor | None,
+                         rope_sin: torch.Tensor | None, rope_style: int, q_bias: torch.Tensor | None,
+                         k_bias: torch.Tensor | None, out: torch.Tensor, workspace: torch.Tensor,
+                         scale: float) -> torch.Tensor:
+    """Launch ``cdb_kv8_decode_attention``: append each row's new token at position ``seqlens[b]`` and attend over
+    positions 0..seqlens[b] (negative: a padding row, zero output). Arguments as ``ops.paged_decode_attention_raw``
+    without its chunking; ``workspace`` is any dense tensor of ``decode_workspace_bytes`` bytes. Calls that may
+    overlap need a workspace each."""
+
+    heads_kv, dim, block = pool._shape
+    if q.dim() != 3 or q.shape[2] != dim:
+        raise ValueError(f"q must be [rows, H, {dim}]")
+    num_rows, num_heads, _ = q.shape
+    dt = q.dtype
+    if k_new.shape != (num_rows, heads_kv, dim) or v_new.shape != k_new.shape:
+        raise ValueError(f"k_new and v_new must be [{num_rows}, {heads_kv}, {dim}]")
+    if k_new.dtype is not dt or v_new.dtype is not dt:
+        raise TypeError("q, k_new and v_new must share a dtype")
+    if num_heads == 0 or num_heads % heads_kv:
+        raise ValueError(f"{num_heads} query heads cannot share {heads_kv} KV heads evenly")
+    if out.shape != q.shape or out.dtype is not dt or not out.is_contiguous():
+        raise ValueError("out must be contiguous and match q")
+    if block_table.dim() != 2 or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous [rows, width]")
+    for name, t in (("seqlens", seqlens), ("table_row", table_row), ("cache_layer", cache_layer)):
+        if t is not None and (t.shape != (num_rows,) or not t.is_contiguous()):
+            raise ValueError(f"{name} must have one entry per row")
+    if table_row is None and block_table.shape[0] < num_rows:
+        raise ValueError("block_table needs a row per batch row when table_row is not given")
+    _require_int32(cache_layer=cache_layer, block_table=block_table, table_row=table_row, seqlens=seqlens)
+    max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
+    _check_bias("q_bias", q_bias, num_heads, dim, dt)
+    _check_bias("k_bias", k_bias, heads_kv, dim, dt)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    _require_here(q, k_new, v_new, pool.codes, cache_layer, block_table, table_row, seqlens, rope_cos, rope_sin,
+                  q_bias, k_bias, out, workspace)
+    kv_stride = _row_stride("k_new", k_new, dim)
+    if _row_stride("v_new", v_new, dim) != kv_stride:
+        raise ValueError("k_new and v_new must share a row stride")
+    codes, scales, layers, blocks = pool._args
+    code = _lib.lib().cdb_kv8_decode_attention(
+        q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), codes, scales, layers, blocks, _ptr(cache_layer),
+        cache_layer0, block_table.data_ptr(), _ptr(table_row), block_table.shape[0], block_table.shape[1],
+        seqlens.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
+        out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), num_rows, num_heads,
+        heads_kv, dim, block, scale, _row_stride("q", q, dim), kv_stride, dtype_code(dt), _stream())
+    if code:
+        _lib.check(code, "cdb_kv8_decode_attention")
+    return out
+
+
+@torch.library.custom_op("cdb::kv8_decode_attention", mutates_args=("codes", "scales", "workspace"),
+                         device_types="cuda")
+def decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, codes: torch.Tensor,
+                     scales: torch.Tensor, cache_layer: torch.Tensor | None, cache_layer0: int,
+                     block_table: torch.Tensor, table_row: torch.Tensor | None, seqlens: torch.Tensor,
+                     rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, rope_style: int,
+                     q_bias: torch.Tensor | None, k_bias: torch.Tensor | None, workspace: torch.Tensor,
+                     scale: float) -> torch.Tensor:
+    """Paged decode attention over the 8-bit cache with fused rotation and append; see ``decode_attention_raw``."""
+
+    out = q.new_empty(q.shape)
+    return decode_attention_raw(q, k_new, v_new, Kv8Pool(codes, scales), cache_layer, cache_layer0, block_table,
+                                table_row, seqlens, rope_cos, rope_sin, rope_style, q_bias, k_bias, out, workspace,
+                                scale)
+
+
+@decode_attention.register_fake
+def _(q, k_new, v_new, codes, scales, cache_layer, cache_layer0, block_table, table_row, seqlens, rope_cos, rope_sin,
+      rope_style, q_bias, k_bias, workspace, scale):
+    return q.new_empty(q.shape)
+
+
+def prefill_splits(num_tiles: int, num_heads: int, num_kv_heads: int, longest: int, num_cus: int = 256) -> int:
+    """Parts that a prefill launch cuts each tile's key range into: enough to give every CU two workgroups, while
+    a part keeps at least 512 keys of the longest range ``longest`` (cached and new tokens of a sequence)."""
+
+    del num_kv_heads
+    want = -(-2 * num_cus // max(1, num_tiles * num_heads))
+    return max(1, min(want, longest // 512))
+
+
+def prefill_workspace_bytes(num_tiles: int, splits: int, num_heads: int, head_dim: int) -> int:
+    n = int(_lib.lib().cdb_kv8_prefill_workspace_bytes(num_tiles, splits, num_heads, head_dim))
+    if n < 0:
+        raise ValueError("invalid arguments for the prefill workspace size")
+    return n
+
+
+def prefill_attention_raw(q: torch.Tensor, pool: Kv8Pool, layer: int, block_table: torch.Tensor,
+                          table_row: torch.Tensor, cu_q: torch.Tensor, past: torch.Tensor, tile_seq: torch.Tensor,
+                          tile_q0: torch.Tensor, out: torch.Tensor, scale: float, splits: int = 1,
+                          workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Launch ``cdb_kv8_prefill_attention``: causal attention of rotated queries q [T, H, D] over cache layer
+    ``layer``, whose keys and values hold the chunk's own tokens already. Sequences, block table and tiles as
+    ``ops.prefill_attention_raw`` (``tile_seq[n] < 0``: no tile); ``splits`` from ``prefill_splits`` with a
+    workspace of ``prefill_workspace_bytes`` bytes when above 1. Calls that may overlap need a workspace each."""
+
+    heads_kv, dim, block = pool._shape
+    if q.dim() != 3 or q.shape[2] != dim or not q.is_contiguous():
+        raise ValueError(f"q must be a contiguous [T, H, {dim}]")
+    tokens, num_heads, _ = q.shape
+    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
+        raise ValueError("out must be contiguous and match q")
+    if num_heads == 0 or num_heads % heads_kv:
+        raise ValueError(f"{num_heads} query heads cannot share {heads_kv} KV heads evenly")
+    num_seqs = past.numel()
+    if cu_q.numel() != num_seqs + 1 or table_row.numel() < num_seqs or tile_seq.numel() != tile_q0.numel():
+        raise ValueError("inconsistent prefill metadata")
+    if not 0 <= layer < pool._args[2]:
+        raise ValueError("layer out of range")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [rows, width]")
+    if splits > 1 and workspace is None:
+        raise ValueError("split launches need a workspace")
+    _require_int32(block_table=block_table, table_row=table_row, cu_q=cu_q, past=past, tile_seq=tile_seq,
+                   tile_q0=tile_q0)
+    _require_contiguous(block_table=block_table, table_row=table_row, cu_q=cu_q, past=past, tile_seq=tile_seq,
+                        tile_q0=tile_q0, workspace=workspace)
+    _require_here(q, pool.codes, block_table, table_row, cu_q, past, tile_seq, tile_q0, out, workspace)
+    codes, scales, layers, blocks = pool._args
+    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
+    code = _lib.lib().cdb_kv8_prefill_attention(
+        q.data_ptr(), codes, scales, layers, blocks, layer, block_table.data_ptr(), table_row.data_ptr(),
+        block_table.shape[0], block_table.shape[1], cu_q.data_ptr(), past.data_ptr(), num_seqs, tile_seq.data_ptr(),
+        tile_q0.data_ptr(), tile_seq.numel(), out.data_ptr(), tokens, splits, _ptr(workspace), nbytes, num_heads,
+        heads_kv, dim, block, scale, dtype_code(q.dtype), _stream())
+    if code:
+        _lib.check(code, "cdb_kv8_prefill_attention")
+    return out
+
+
+@torch.library.custom_op("cdb::kv8_prefill_attention", mutates_args=("workspace",), device_types="cuda")
+def prefill_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor, layer: int,
+                      block_table: torch.Tensor, table_row: torch.Tensor, cu_q: torch.Tensor, past: torch.Tensor,
+                      tile_seq: torch.Tensor, tile_q0: torch.Tensor, scale: float, splits: int,
+                      workspace: torch.Tensor | None) -> torch.Tensor:
+    """Varlen causal prefill attention over the 8-bit cache; see ``prefill_attention_raw``."""
+
+    out = q.new_empty(q.shape)
+    return prefill_attention_raw(q, Kv8Pool(codes, scales), layer, block_table, table_row, cu_q, past, tile_seq,
+                                 tile_q0, out, scale, splits, workspace)
+
+
+@prefill_attention.register_fake
+def _(q, codes, scales, layer, block_table, table_row, cu_q, past, tile_seq, tile_q0, scale, splits, workspace):
+    return q.new_empty(q.shape)
+
+
+@dataclass(frozen=True)
+class BatchLayout:
+    """What ``batch_layout`` writes: ``cu_q`` [S + 1], ``positions`` int32 and ``rows`` int64 [tokens] (-1 behind
+    the last token), ``tile_seq`` and ``tile_q0`` [tiles] ((-1, 0) behind the last), ``counts`` [tokens, tiles,
+    blocks taken, LAYOUT_* bits]."""
+
+    cu_q: torch.Tensor
+    positions: torch.Tensor
+    rows: torch.Tensor
+    tile_seq: torch.Tensor
+    tile_q0: torch.Tensor
+    counts: torch.Tensor
+
+    @classmethod
+    def allocate(cls, num_seqs: int, token_capacity: int, tile_capacity: int,
+                 device: torch.device | str) -> "BatchLayout":
+        def ints(n: int) -> torch.Tensor:
+            return torch.empty(n, dtype=torch.int32, device=device)
+
+        return cls(ints(num_seqs + 1), ints(token_capacity),
+                   torch.empty(token_capacity, dtype=torch.int64, device=device), ints(tile_capacity),
+                   ints(tile_capacity), ints(4))
+
+
+def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor,
+                     table_row: torch.Tensor | None, free_blocks: torch.Tensor, block_size: int,
+                     layout: BatchLayout) -> None:
+    """Launch ``cdb_batch_layout``: block tables, slots and attention tiles of a batch whose request s holds
+    ``past[s]`` tokens and brings ``lens[s]`` more. New blocks come from the front of ``free_blocks`` in request
+    order and go to the requests' rows of ``block_table``; ``layout`` receives the rest. The caller drops
+    ``counts[2]`` ids from its free list and looks at the bits of ``counts[3]``."""
+
+    num_seqs = past.numel()
+    if lens.numel() != num_seqs or (table_row is not None and table_row.numel() != num_seqs):
+        raise ValueError("past, lens and table_row need an entry per request")
+    if num_seqs > _lib.CDB_LAYOUT_MAX_SEQS:
+        raise ValueError(f"a layout takes up to {_lib.CDB_LAYOUT_MAX_SEQS} requests, got {num_seqs}")
+    if block_table.dim() != 2:
+        raise ValueError("block_table must be [rows, width]")
+    if table_row is None and block_table.shape[0] < num_seqs:
+        raise ValueError("block_table needs a row per request when table_row is not given")
+    a = layout
+    if a.cu_q.numel() != num_seqs + 1 or a.rows.numel() != a.positions.numel() or a.counts.numel() < 4 \
+            or a.tile_seq.numel() != a.tile_q0.numel():
+        raise ValueError("the layout's buffers do not fit the batch")
+    if a.rows.dtype is not torch.int64:
+        raise TypeError("rows must be int64")
+    named = dict(past=past, lens=lens, block_table=block_table, table_row=table_row, free_blocks=free_blocks,
+                 cu_q=a.cu_q, positions=a.positions, tile_seq=a.tile_seq, tile_q0=a.tile_q0, counts=a.counts)
+    _require_int32(**named)
+    _require_contiguous(rows=a.rows, **named)
+    _require_here(*named.values(), a.rows)
+    code = _lib.lib().cdb_batch_layout(
+        past.data_ptr(), lens.data_ptr(), num_seqs, block_table.data_ptr(), _ptr(table_row), block_table.shape[0],
+        block_table.shape[1], free_blocks.data_ptr(), free_blocks.numel(), block_size, a.cu_q.data_ptr(),
+        a.positions.data_ptr(), a.rows.data_ptr(), a.positions.numel(), a.tile_seq.data_ptr(), a.tile_q0.data_ptr(),
+        a.tile_seq.numel(), a.counts.data_ptr(), _stream())
+    if code:
+        _lib.check(code, "cdb_batch_layout")
+
+
+@torch.library.custom_op("cdb::batch_layout", mutates_args=("block_table",), device_types="cuda")
+def batch_layout(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor, table_row: torch.Tensor | None,
+                 free_blocks: torch.Tensor, block_size: int, token_capacity: int, tile_capacity: int
+                 ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
+    """(cu_q, positions, rows, tile_seq, tile_q0, counts) of a batch; see ``batch_layout_raw``."""
+
+    a = BatchLayout.allocate(past.numel(), token_capacity, tile_capacity, past.device)
+    batch_layout_raw(past, lens, block_table, table_row, free_blocks, block_size, a)
+    return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts
+
+
+@batch_layout.register_fake
+def _(past, lens, block_table, table_row, free_blocks, block_size, token_capacity, tile_capacity):
+    a = BatchLayout.allocate(past.numel(), token_capacity, tile_capacity, past.device)
+    return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts

@@ -1223,3 +1223,6 @@ def prefill_attention_raw(q: torch.Tensor, view: KVPoolView, layer: int, block_t
         num_seqs, tile_seq.data_ptr(), tile_q0.data_ptr(), tile_seq.numel(), out.data_ptr(), num_heads,
         pool.shape[3], head_dim, view.block_size, scale, dtype_code(q.dtype), _stream())
     _lib.check(code, "cdb_prefill_attention")
+
+
+from . import kv8  # noqa: E402,F401  (registers torch.ops.cdb.kv8_* and cdb::batch_layout)

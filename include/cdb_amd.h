@@ -380,6 +380,101 @@ int cdb_coda_greedy(const int64_t* host_upload, int64_t* dev_upload, int32_t row
                     int64_t* host_tokens, double* cdf, double* survival, float* pending, int64_t state_capacity,
                     int32_t dtype, hipStream_t stream);
 
+/* ---- 8-bit KV cache ------------------------------------------------------------------------------------------
+ * No counterpart in the reference, whose cache holds the model's type. Keys and values are held in tiles of
+ * 16 tokens of one KV head, as e4m3 codes with one power-of-two scale a tile, keys and values apart:
+ *   codes  [num_cache_layers, 2, pool_blocks, Hkv, block_size / 16, 16 * D] bytes, 16-byte aligned;
+ *   scales [num_cache_layers, 2, pool_blocks, Hkv, block_size / 16] bytes b, the scale being 2^(b - 127).
+ * A key tile lies as [D / 16][16 tokens][16], a value tile as [4][D][4 tokens]. block_size is a power of two
+ * of at least 16; D is 64, 96 or 128; the codes need no address below 2^63 bytes, and offsets are 64-bit.
+ * Position t of a sequence is token t % 16 of tile t % block_size / 16 of block block_table[t / block_size].
+ *
+ * Writing: a tile's scale is the smallest power of two s with |x| <= 448 s for the finite values written
+ * (2^-126 at least). Tokens that join a tile behind earlier ones keep the larger of its scale and theirs, and
+ * where it grows the earlier codes are rounded again. A tile written from its first token starts anew. Codes
+ * behind the last token written stay as they are, and count for nothing. An infinity or NaN is held as NaN.
+ * Rotations are computed in fp32, each product and sum rounded once, and not rounded to the storage type
+ * before they are coded. */
+
+/* Rotate and append a batch of tokens: q_out = rotate(q [+ q_bias]); rotate(k [+ k_bias]) and v are coded into
+ * cache layer `layer` at slots rows[t] = block * block_size + offset. The 8-bit counterpart of
+ * cdb_rope_kv_write, with its q/k/v views, strides, rotation styles and biases. The tokens of one tile follow
+ * each other in the call at consecutive slots, as a sequence's tokens do; a slot is written once in a call. Tokens
+ * with a negative slot are padding: nothing of theirs is read or written, q_out included. A slot past the pool
+ * or a position outside the angle tables writes no key or value (and NaN to q_out for such a position).
+ * num_heads 0 (q and q_out null) writes keys and values alone. q_out is dense and 16-byte aligned. */
+int cdb_kv8_write(const void* q, const void* k, const void* v, void* q_out, void* codes, void* scales,
+                  int32_t num_cache_layers, int64_t pool_blocks, int32_t layer, const int64_t* rows,
+                  const int32_t* positions, const float* rope_cos, const float* rope_sin, int32_t rope_style,
+                  int32_t max_positions, const void* q_bias, const void* k_bias, int64_t tokens, int32_t num_heads,
+                  int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t q_stride, int64_t kv_stride,
+                  int32_t dtype, hipStream_t stream);
+
+/* Workspace bytes of cdb_kv8_decode_attention for positions below max_seqlen (-1 for invalid arguments): per row,
+ * query head and 256-token chunk an fp32 partial of head_dim + 2 values. A smaller workspace is legal down to one
+ * chunk a row: the chunks then grow until the table's whole width fits. */
+int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                       int32_t max_seqlen);
+
+/* Mixed-depth paged decode attention over the 8-bit cache, with fused rotation and append: the counterpart of
+ * cdb_paged_decode_attention, with its rows, positions (seqlens), per-row cache layers, block table, biases and
+ * padding rows. Row b's new key and value are coded into its cache first, and it attends over the codes of
+ * positions 0..seqlens[b], its own included. Rows whose position, table row or cache layer is out of range get a
+ * NaN output and no write, and so does a row whose blocks in use are not all inside the pool. num_heads is a
+ * multiple of num_kv_heads. Two rows of a call never append to the same tile. A row's context is cut into
+ * chunks of 256 tokens, merged in order, so its output does not depend on the other rows. */
+int cdb_kv8_decode_attention(const void* q, const void* k_new, const void* v_new, void* codes, void* scales,
+                             int32_t num_cache_layers, int64_t pool_blocks, const int32_t* cache_layer,
+                             int32_t cache_layer0, const int32_t* block_table, const int32_t* table_row,
+                             int32_t table_rows, int32_t table_width, const int32_t* seqlens, const float* rope_cos,
+                             const float* rope_sin, int32_t rope_style, int32_t max_positions, const void* q_bias,
+                             const void* k_bias, void* out, void* workspace, int64_t workspace_bytes,
+                             int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                             int32_t block_size, float scale, int64_t q_stride, int64_t kv_stride, int32_t dtype,
+                             hipStream_t stream);
+
+/* Workspace bytes of cdb_kv8_prefill_attention (0 for splits == 1; -1 for invalid arguments): per tile, split and
+ * head an fp32 partial of 128 * (head_dim + 2) values. */
+int64_t cdb_kv8_prefill_workspace_bytes(int32_t num_tiles, int32_t splits, int32_t num_heads, int32_t head_dim);
+
+/* Varlen causal prefill attention over the 8-bit cache: the counterpart of cdb_prefill_attention, with its
+ * sequences, block table and tiles of 128 query tokens (tile_seq[n] < 0: no tile). q [T, H, D] is rotated; the
+ * chunk's own keys and values are already in the cache. splits > 1 cuts every tile's key range into that many
+ * parts, merged in order by a second launch: for few tiles with long histories. Queries of a sequence whose
+ * table row is out of range or whose blocks in use are not all inside the pool get NaN. q and out are dense. */
+int cdb_kv8_prefill_attention(const void* q, const void* codes, const void* scales, int32_t num_cache_layers,
+                              int64_t pool_blocks, int32_t layer, const int32_t* block_table,
+                              const int32_t* table_row, int32_t table_rows, int32_t table_width, const int32_t* cu_q,
+                              const int32_t* past, int32_t num_seqs, const int32_t* tile_seq, const int32_t* tile_q0,
+                              int32_t num_tiles, void* out, int64_t tokens, int32_t splits, void* workspace,
+                              int64_t workspace_bytes, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                              int32_t block_size, float scale, int32_t dtype, hipStream_t stream);
+
+enum {
+  CDB_LAYOUT_MAX_SEQS = 4000,  /* requests of one call: their four prefixes fill 64 KB of LDS */
+  /* bits of counts[3] */
+  CDB_LAYOUT_TOKENS_FULL = 1,  /* more tokens than token_capacity: the rest is left out */
+  CDB_LAYOUT_TILES_FULL = 2,   /* more tiles than tile_capacity: the last of the list are left out */
+  CDB_LAYOUT_NO_BLOCKS = 4,    /* more new blocks than free ones: -1 in the table, slot -1 for their tokens */
+  CDB_LAYOUT_BAD_REQUEST = 8   /* a negative length, one past the table's width, or a table row out of range:
+                                  the request counts as one without tokens */
+};
+
+/* Block tables, slot map and attention tiles of a batch, on the device, from its requests' lengths: what the
+ * engine otherwise assembles on the host for a prefill launch (continuous_batching/cache_manager.py:72-90,
+ * :190-213; prefill_tiles). Request s holds past[s] tokens and brings lens[s] >= 0 more. Its
+ * blocks ceil(past / block_size).. ceil((past + lens) / block_size) are taken from the front of free_blocks, in
+ * request order, and written to row table_row[s] (s when null) of block_table; each request has a row of its own.
+ *   cu_q [num_seqs + 1]; positions, rows [token_capacity]: position and slot of each token, -1 behind the last;
+ *   tile_seq, tile_q0 [tile_capacity]: tiles of 128 query tokens, longest key range first and in request order
+ *   among equals, (-1, 0) behind the last;
+ *   counts [4]: tokens, tiles, blocks taken, CDB_LAYOUT_* bits. The caller drops counts[2] ids from its free list. */
+int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs, int32_t* block_table,
+                     const int32_t* table_row, int32_t table_rows, int32_t table_width, const int32_t* free_blocks,
+                     int32_t num_free, int32_t block_size, int32_t* cu_q, int32_t* positions, int64_t* rows,
+                     int32_t token_capacity, int32_t* tile_seq, int32_t* tile_q0, int32_t tile_capacity,
+                     int32_t* counts, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
