@@ -24,6 +24,7 @@ typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef float f32x2_t __attribute__((ext_vector_type(2)));
 typedef float f32x4_t __attribute__((ext_vector_type(4)));
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
@@ -125,14 +126,27 @@ CDB_DEVICE void load_rotated(const T* head, const T* bias, const float* cos, con
   }
 }
 
-// Max over the four lanes that differ in bits 4 and 5.
+// A value and the one of the lane that differs in bit 4 (or 5), in either order: two vector
+// instructions, against the LDS round trip of a permute.
+CDB_DEVICE f32x2_t pair16(float v) {
+  const auto x = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return (f32x2_t){__uint_as_float(x[0]), __uint_as_float(x[1])};
+}
+CDB_DEVICE f32x2_t pair32(float v) {
+  const auto x = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return (f32x2_t){__uint_as_float(x[0]), __uint_as_float(x[1])};
+}
+
+// Max, and sum, over the four lanes that differ in bits 4 and 5.
 CDB_DEVICE float column_max(float v) {
-  v = fmaxf(v, shfl_xor_f32(v, 16));
-  return fmaxf(v, shfl_xor_f32(v, 32));
+  f32x2_t x = pair16(v);
+  x = pair32(fmaxf(x[0], x[1]));
+  return fmaxf(x[0], x[1]);
 }
 CDB_DEVICE float column_sum(float v) {
-  v += shfl_xor_f32(v, 16);
-  return v + shfl_xor_f32(v, 32);
+  f32x2_t x = pair16(v);
+  x = pair32(x[0] + x[1]);
+  return x[0] + x[1];
 }
 
 // 8 codes (two words) widened to bf16 with their scale: exact, e4m3 has 4 significant bits.

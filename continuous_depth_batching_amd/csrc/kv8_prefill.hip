@@ -64,7 +64,10 @@ CDB_DEVICE f16x8_t widen_f16(uint32_t w0, uint32_t w1, float s) {
   return u.v;
 }
 
-CDB_DEVICE float half_max(float v) { return fmaxf(v, shfl_xor_f32(v, 32)); }
+CDB_DEVICE float half_max(float v) {
+  const f32x2_t x = pair32(v);
+  return fmaxf(x[0], x[1]);
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P) {

@@ -19,7 +19,7 @@ from dataclasses import dataclass
 import torch
 
 from . import _lib
-from .ops import _ptr, _require_contiguous, _require_int32, _stream, dtype_code
+from .ops import _ptr, _stream, dtype_code
 
 TILE = 16  # tokens of a cache tile
 PREFILL_TILE = 128  # query tokens of an attention tile
@@ -96,6 +96,9 @@ class Kv8Pool:
         return tuple(x.permute(0, 2, 3, 1, 4).flatten(0, 2) for x in (k, v))
 
 
+# A decode step's call takes about as long as its kernel, so the checks below touch each tensor property once.
+
+
 def _require_here(*tensors: torch.Tensor | None) -> None:
     """Every tensor on the current device, whose stream the launch goes to."""
 
@@ -103,12 +106,28 @@ def _require_here(*tensors: torch.Tensor | None) -> None:
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()
+        if at < 0:
             raise RuntimeError("CDB kernels run on the GPU only; got a tensor on " + str(t.device))
         if here is None:
-            here = torch.cuda.current_device()
-        if t.get_device() != here:
+            here = torch._C._cuda_getDevice()
+        if at != here:
             raise RuntimeError(f"got a tensor on {t.device} while cuda:{here} is the current device")
+
+
+def _check_ints(name: str, t: torch.Tensor, n: int) -> None:
+    if t.dtype is not torch.int32:
+        raise TypeError(f"{name} must be int32, got {t.dtype}")
+    if t.numel() != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be contiguous with {n} entries")
+
+
+def _check_table(block_table: torch.Tensor) -> tuple[int, int]:
+    if block_table.dtype is not torch.int32:
+        raise TypeError(f"block_table must be int32, got {block_table.dtype}")
+    if block_table.dim() != 2 or not block_table.is_contiguous():
+        raise ValueError("block_table must be a contiguous [rows, width]")
+    return tuple(block_table.shape)
 
 
 def _check_rope(rope_style: int, cos: torch.Tensor | None, sin: torch.Tensor | None, head_dim: int) -> int:
@@ -118,11 +137,13 @@ def _check_rope(rope_style: int, cos: torch.Tensor | None, sin: torch.Tensor | N
         return 0
     if rope_style not in (1, 2):
         raise ValueError(f"rope_style must be 0, 1 or 2, got {rope_style}")
-    if cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32 \
-            or cos.dim() != 2 or cos.shape != sin.shape or cos.shape[1] != head_dim // 2:
+    if cos is None or sin is None or cos.dtype is not torch.float32 or sin.dtype is not torch.float32:
         raise ValueError("rope tables must be float32 [max_positions, D/2]")
-    _require_contiguous(rope_cos=cos, rope_sin=sin)
-    return cos.shape[0]
+    shape = cos.shape
+    if len(shape) != 2 or shape[1] != head_dim // 2 or sin.shape != shape or not cos.is_contiguous() \
+            or not sin.is_contiguous():
+        raise ValueError("rope tables must be contiguous float32 [max_positions, D/2]")
+    return shape[0]
 
 
 def _check_bias(name: str, bias: torch.Tensor | None, heads: int, dim: int, dtype: torch.dtype) -> None:
@@ -132,18 +153,17 @@ def _check_bias(name: str, bias: torch.Tensor | None, heads: int, dim: int, dtyp
         raise ValueError(f"{name} must be a contiguous [{heads}, {dim}] tensor of q's dtype")
 
 
-def _row_stride(name: str, t: torch.Tensor, head_dim: int) -> int:
+def _row_stride(name: str, t: torch.Tensor, rows: int, heads: int, head_dim: int) -> int:
     """Elements between rows of a [rows, heads, D] tensor whose heads are dense; a single row's is its own size."""
 
-    rows, heads, _ = t.shape
-    s = t.stride()
-    if s[2] != 1 or (s[1] != head_dim and heads > 1):
+    row, head, element = t.stride()
+    if element != 1 or (head != head_dim and heads > 1):
         raise ValueError(f"{name} must have contiguous heads and head dimension (the row stride may differ)")
     if rows <= 1:
         return heads * head_dim
-    if s[0] < heads * head_dim:
+    if row < heads * head_dim:
         raise ValueError(f"{name}'s rows overlap")
-    return s[0]
+    return row
 
 
 def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: torch.Tensor | None, pool: Kv8Pool,
@@ -156,38 +176,41 @@ def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: t
     is padding, whose q_out is left as it was."""
 
     heads_kv, dim, block = pool._shape
-    if k.dim() != 3 or k.shape[1:] != (heads_kv, dim) or v.shape != k.shape or v.dtype is not k.dtype:
+    codes, scales, layers, blocks = pool._args
+    shape, dt = k.shape, k.dtype
+    if len(shape) != 3 or shape[1] != heads_kv or shape[2] != dim or v.shape != shape or v.dtype is not dt:
         raise ValueError(f"k and v must be [T, {heads_kv}, {dim}] of one dtype")
-    tokens = k.shape[0]
-    heads = 0
+    tokens = shape[0]
+    heads = q_ptr = out_ptr = q_stride = 0
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out come together")
     if q is not None:
-        heads = q.shape[1]
-        if q.dim() != 3 or q.shape[0] != tokens or q.shape[2] != dim or q.dtype is not k.dtype:
+        shape = q.shape
+        if len(shape) != 3 or shape[0] != tokens or shape[2] != dim or q.dtype is not dt:
             raise ValueError(f"q must be [{tokens}, H, {dim}] of k's dtype")
-        if q_out.shape != q.shape or q_out.dtype is not q.dtype or not q_out.is_contiguous():
+        heads = shape[1]
+        if q_out.shape != shape or q_out.dtype is not dt or not q_out.is_contiguous():
             raise ValueError("q_out must be contiguous and match q")
+        q_ptr, out_ptr, q_stride = q.data_ptr(), q_out.data_ptr(), _row_stride("q", q, tokens, heads, dim)
     if rows.dtype is not torch.int64 or positions.dtype is not torch.int32:
         raise TypeError("rows must be int64 and positions int32")
-    if rows.numel() < tokens or positions.numel() < tokens:
-        raise ValueError("rows and positions need an entry per token")
-    if not 0 <= layer < pool._args[2]:
+    if rows.numel() < tokens or positions.numel() < tokens or not rows.is_contiguous() \
+            or not positions.is_contiguous():
+        raise ValueError("rows and positions must be contiguous with an entry per token")
+    if not 0 <= layer < layers:
         raise ValueError("layer out of range")
     max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
-    _check_bias("q_bias", q_bias, heads, dim, k.dtype)
-    _check_bias("k_bias", k_bias, heads_kv, dim, k.dtype)
-    _require_contiguous(rows=rows, positions=positions)
+    _check_bias("q_bias", q_bias, heads, dim, dt)
+    _check_bias("k_bias", k_bias, heads_kv, dim, dt)
     _require_here(q, k, v, q_out, pool.codes, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
-    kv_stride = _row_stride("k", k, dim)
-    if _row_stride("v", v, dim) != kv_stride:
+    kv_stride = _row_stride("k", k, tokens, heads_kv, dim)
+    if _row_stride("v", v, tokens, heads_kv, dim) != kv_stride:
         raise ValueError("k and v must share one token stride")
-    codes, scales, layers, blocks = pool._args
     code = _lib.lib().cdb_kv8_write(
-        _ptr(q), k.data_ptr(), v.data_ptr(), _ptr(q_out), codes, scales, layers, blocks, layer, rows.data_ptr(),
-        positions.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
-        tokens, heads, heads_kv, dim, block, 0 if q is None else _row_stride("q", q, dim), kv_stride,
-        dtype_code(k.dtype), _stream())
+        q_ptr or None, k.data_ptr(), v.data_ptr(), out_ptr or None, codes, scales, layers, blocks, layer,
+        rows.data_ptr(), positions.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions,
+        _ptr(q_bias), _ptr(k_bias), tokens, heads, heads_kv, dim, block, q_stride, kv_stride, dtype_code(dt),
+        _stream())
     if code:
         _lib.check(code, "cdb_kv8_write")
 
@@ -232,26 +255,28 @@ def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
     overlap need a workspace each."""
 
     heads_kv, dim, block = pool._shape
-    if q.dim() != 3 or q.shape[2] != dim:
+    codes, scales, layers, blocks = pool._args
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != dim:
         raise ValueError(f"q must be [rows, H, {dim}]")
-    num_rows, num_heads, _ = q.shape
-    dt = q.dtype
-    if k_new.shape != (num_rows, heads_kv, dim) or v_new.shape != k_new.shape:
+    num_rows, num_heads = shape[0], shape[1]
+    kv_shape = k_new.shape
+    if kv_shape != (num_rows, heads_kv, dim) or v_new.shape != kv_shape:
         raise ValueError(f"k_new and v_new must be [{num_rows}, {heads_kv}, {dim}]")
     if k_new.dtype is not dt or v_new.dtype is not dt:
         raise TypeError("q, k_new and v_new must share a dtype")
     if num_heads == 0 or num_heads % heads_kv:
         raise ValueError(f"{num_heads} query heads cannot share {heads_kv} KV heads evenly")
-    if out.shape != q.shape or out.dtype is not dt or not out.is_contiguous():
+    if out.shape != shape or out.dtype is not dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and match q")
-    if block_table.dim() != 2 or not block_table.is_contiguous():
-        raise ValueError("block_table must be a contiguous [rows, width]")
-    for name, t in (("seqlens", seqlens), ("table_row", table_row), ("cache_layer", cache_layer)):
-        if t is not None and (t.shape != (num_rows,) or not t.is_contiguous()):
-            raise ValueError(f"{name} must have one entry per row")
-    if table_row is None and block_table.shape[0] < num_rows:
+    table_rows, width = _check_table(block_table)
+    _check_ints("seqlens", seqlens, num_rows)
+    if table_row is not None:
+        _check_ints("table_row", table_row, num_rows)
+    elif table_rows < num_rows:
         raise ValueError("block_table needs a row per batch row when table_row is not given")
-    _require_int32(cache_layer=cache_layer, block_table=block_table, table_row=table_row, seqlens=seqlens)
+    if cache_layer is not None:
+        _check_ints("cache_layer", cache_layer, num_rows)
     max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
     _check_bias("q_bias", q_bias, num_heads, dim, dt)
     _check_bias("k_bias", k_bias, heads_kv, dim, dt)
@@ -259,16 +284,15 @@ def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
         raise ValueError("workspace must be contiguous")
     _require_here(q, k_new, v_new, pool.codes, cache_layer, block_table, table_row, seqlens, rope_cos, rope_sin,
                   q_bias, k_bias, out, workspace)
-    kv_stride = _row_stride("k_new", k_new, dim)
-    if _row_stride("v_new", v_new, dim) != kv_stride:
+    kv_stride = _row_stride("k_new", k_new, num_rows, heads_kv, dim)
+    if _row_stride("v_new", v_new, num_rows, heads_kv, dim) != kv_stride:
         raise ValueError("k_new and v_new must share a row stride")
-    codes, scales, layers, blocks = pool._args
     code = _lib.lib().cdb_kv8_decode_attention(
         q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), codes, scales, layers, blocks, _ptr(cache_layer),
-        cache_layer0, block_table.data_ptr(), _ptr(table_row), block_table.shape[0], block_table.shape[1],
-        seqlens.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
-        out.data_ptr(), workspace.data_ptr(), workspace.numel() * workspace.element_size(), num_rows, num_heads,
-        heads_kv, dim, block, scale, _row_stride("q", q, dim), kv_stride, dtype_code(dt), _stream())
+        cache_layer0, block_table.data_ptr(), _ptr(table_row), table_rows, width, seqlens.data_ptr(),
+        _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias), out.data_ptr(),
+        workspace.data_ptr(), workspace.nbytes, num_rows, num_heads, heads_kv, dim, block, scale,
+        _row_stride("q", q, num_rows, num_heads, dim), kv_stride, dtype_code(dt), _stream())
     if code:
         _lib.check(code, "cdb_kv8_decode_attention")
     return out
@@ -322,34 +346,32 @@ def prefill_attention_raw(q: torch.Tensor, pool: Kv8Pool, layer: int, block_tabl
     workspace of ``prefill_workspace_bytes`` bytes when above 1. Calls that may overlap need a workspace each."""
 
     heads_kv, dim, block = pool._shape
-    if q.dim() != 3 or q.shape[2] != dim or not q.is_contiguous():
+    codes, scales, layers, blocks = pool._args
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != dim or not q.is_contiguous():
         raise ValueError(f"q must be a contiguous [T, H, {dim}]")
-    tokens, num_heads, _ = q.shape
-    if out.shape != q.shape or out.dtype is not q.dtype or not out.is_contiguous():
+    num_heads = shape[1]
+    if out.shape != shape or out.dtype is not dt or not out.is_contiguous():
         raise ValueError("out must be contiguous and match q")
     if num_heads == 0 or num_heads % heads_kv:
         raise ValueError(f"{num_heads} query heads cannot share {heads_kv} KV heads evenly")
-    num_seqs = past.numel()
-    if cu_q.numel() != num_seqs + 1 or table_row.numel() < num_seqs or tile_seq.numel() != tile_q0.numel():
-        raise ValueError("inconsistent prefill metadata")
-    if not 0 <= layer < pool._args[2]:
+    num_seqs, num_tiles = past.numel(), tile_seq.numel()
+    table_rows, width = _check_table(block_table)
+    for name, t, n in (("past", past, num_seqs), ("cu_q", cu_q, num_seqs + 1), ("table_row", table_row, num_seqs),
+                       ("tile_seq", tile_seq, num_tiles), ("tile_q0", tile_q0, num_tiles)):
+        _check_ints(name, t, n)
+    if not 0 <= layer < layers:
         raise ValueError("layer out of range")
-    if block_table.dim() != 2:
-        raise ValueError("block_table must be [rows, width]")
     if splits > 1 and workspace is None:
         raise ValueError("split launches need a workspace")
-    _require_int32(block_table=block_table, table_row=table_row, cu_q=cu_q, past=past, tile_seq=tile_seq,
-                   tile_q0=tile_q0)
-    _require_contiguous(block_table=block_table, table_row=table_row, cu_q=cu_q, past=past, tile_seq=tile_seq,
-                        tile_q0=tile_q0, workspace=workspace)
+    if workspace is not None and not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
     _require_here(q, pool.codes, block_table, table_row, cu_q, past, tile_seq, tile_q0, out, workspace)
-    codes, scales, layers, blocks = pool._args
-    nbytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     code = _lib.lib().cdb_kv8_prefill_attention(
-        q.data_ptr(), codes, scales, layers, blocks, layer, block_table.data_ptr(), table_row.data_ptr(),
-        block_table.shape[0], block_table.shape[1], cu_q.data_ptr(), past.data_ptr(), num_seqs, tile_seq.data_ptr(),
-        tile_q0.data_ptr(), tile_seq.numel(), out.data_ptr(), tokens, splits, _ptr(workspace), nbytes, num_heads,
-        heads_kv, dim, block, scale, dtype_code(q.dtype), _stream())
+        q.data_ptr(), codes, scales, layers, blocks, layer, block_table.data_ptr(), table_row.data_ptr(), table_rows,
+        width, cu_q.data_ptr(), past.data_ptr(), num_seqs, tile_seq.data_ptr(), tile_q0.data_ptr(), num_tiles,
+        out.data_ptr(), shape[0], splits, _ptr(workspace), 0 if workspace is None else workspace.nbytes, num_heads,
+        heads_kv, dim, block, scale, dtype_code(dt), _stream())
     if code:
         _lib.check(code, "cdb_kv8_prefill_attention")
     return out
@@ -388,12 +410,12 @@ class BatchLayout:
     @classmethod
     def allocate(cls, num_seqs: int, token_capacity: int, tile_capacity: int,
                  device: torch.device | str) -> "BatchLayout":
-        def ints(n: int) -> torch.Tensor:
-            return torch.empty(n, dtype=torch.int32, device=device)
+        """Buffers for up to ``token_capacity`` tokens and ``tile_capacity`` tiles, parts of one allocation."""
 
-        return cls(ints(num_seqs + 1), ints(token_capacity),
-                   torch.empty(token_capacity, dtype=torch.int64, device=device), ints(tile_capacity),
-                   ints(tile_capacity), ints(4))
+        sizes = (2 * token_capacity, token_capacity, tile_capacity, tile_capacity, num_seqs + 1, 4)
+        rows, positions, tile_seq, tile_q0, cu_q, counts = torch.empty(
+            sum(sizes), dtype=torch.int32, device=device).split(sizes)
+        return cls(cu_q, positions, rows.view(torch.int64), tile_seq, tile_q0, counts)
 
 
 def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor,
@@ -405,32 +427,41 @@ def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.
     ``counts[2]`` ids from its free list and looks at the bits of ``counts[3]``."""
 
     num_seqs = past.numel()
-    if lens.numel() != num_seqs or (table_row is not None and table_row.numel() != num_seqs):
-        raise ValueError("past, lens and table_row need an entry per request")
     if num_seqs > _lib.CDB_LAYOUT_MAX_SEQS:
         raise ValueError(f"a layout takes up to {_lib.CDB_LAYOUT_MAX_SEQS} requests, got {num_seqs}")
-    if block_table.dim() != 2:
-        raise ValueError("block_table must be [rows, width]")
-    if table_row is None and block_table.shape[0] < num_seqs:
-        raise ValueError("block_table needs a row per request when table_row is not given")
+    table_rows, width = _check_table(block_table)
     a = layout
-    if a.cu_q.numel() != num_seqs + 1 or a.rows.numel() != a.positions.numel() or a.counts.numel() < 4 \
-            or a.tile_seq.numel() != a.tile_q0.numel():
-        raise ValueError("the layout's buffers do not fit the batch")
+    tokens, tiles, num_free = a.positions.numel(), a.tile_seq.numel(), free_blocks.numel()
+    for name, t, n in (("past", past, num_seqs), ("lens", lens, num_seqs), ("free_blocks", free_blocks, num_free),
+                       ("cu_q", a.cu_q, num_seqs + 1), ("positions", a.positions, tokens),
+                       ("tile_seq", a.tile_seq, tiles), ("tile_q0", a.tile_q0, tiles), ("counts", a.counts, 4)):
+        _check_ints(name, t, n)
+    if table_row is not None:
+        _check_ints("table_row", table_row, num_seqs)
+    elif table_rows < num_seqs:
+        raise ValueError("block_table needs a row per request when table_row is not given")
     if a.rows.dtype is not torch.int64:
         raise TypeError("rows must be int64")
-    named = dict(past=past, lens=lens, block_table=block_table, table_row=table_row, free_blocks=free_blocks,
-                 cu_q=a.cu_q, positions=a.positions, tile_seq=a.tile_seq, tile_q0=a.tile_q0, counts=a.counts)
-    _require_int32(**named)
-    _require_contiguous(rows=a.rows, **named)
-    _require_here(*named.values(), a.rows)
+    if a.rows.numel() != tokens or not a.rows.is_contiguous():
+        raise ValueError("rows must be contiguous with an entry per position")
+    _require_here(past, lens, block_table, table_row, free_blocks, a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0,
+                  a.counts)
     code = _lib.lib().cdb_batch_layout(
-        past.data_ptr(), lens.data_ptr(), num_seqs, block_table.data_ptr(), _ptr(table_row), block_table.shape[0],
-        block_table.shape[1], free_blocks.data_ptr(), free_blocks.numel(), block_size, a.cu_q.data_ptr(),
-        a.positions.data_ptr(), a.rows.data_ptr(), a.positions.numel(), a.tile_seq.data_ptr(), a.tile_q0.data_ptr(),
-        a.tile_seq.numel(), a.counts.data_ptr(), _stream())
+        past.data_ptr(), lens.data_ptr(), num_seqs, block_table.data_ptr(), _ptr(table_row), table_rows, width,
+        free_blocks.data_ptr(), num_free, block_size, a.cu_q.data_ptr(), a.positions.data_ptr(), a.rows.data_ptr(),
+        tokens, a.tile_seq.data_ptr(), a.tile_q0.data_ptr(), tiles, a.counts.data_ptr(), _stream())
     if code:
         _lib.check(code, "cdb_batch_layout")
+
+
+def _apart(num_seqs: int, tokens: int, tiles: int, device: torch.device) -> BatchLayout:
+    """A layout whose buffers are tensors of their own, as an op's results have to be."""
+
+    def ints(n: int) -> torch.Tensor:
+        return torch.empty(n, dtype=torch.int32, device=device)
+
+    return BatchLayout(ints(num_seqs + 1), ints(tokens), torch.empty(tokens, dtype=torch.int64, device=device),
+                       ints(tiles), ints(tiles), ints(4))
 
 
 @torch.library.custom_op("cdb::batch_layout", mutates_args=("block_table",), device_types="cuda")
@@ -439,12 +470,12 @@ def batch_layout(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tens
                  ) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor, torch.Tensor]:
     """(cu_q, positions, rows, tile_seq, tile_q0, counts) of a batch; see ``batch_layout_raw``."""
 
-    a = BatchLayout.allocate(past.numel(), token_capacity, tile_capacity, past.device)
+    a = _apart(past.numel(), token_capacity, tile_capacity, past.device)
     batch_layout_raw(past, lens, block_table, table_row, free_blocks, block_size, a)
     return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts
 
 
 @batch_layout.register_fake
 def _(past, lens, block_table, table_row, free_blocks, block_size, token_capacity, tile_capacity):
-    a = BatchLayout.allocate(past.numel(), token_capacity, tile_capacity, past.device)
+    a = _apart(past.numel(), token_capacity, tile_capacity, past.device)
     return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts

@@ -410,9 +410,10 @@ int cdb_kv8_write(const void* q, const void* k, const void* v, void* q_out, void
                   int32_t num_kv_heads, int32_t head_dim, int32_t block_size, int64_t q_stride, int64_t kv_stride,
                   int32_t dtype, hipStream_t stream);
 
-/* Workspace bytes of cdb_kv8_decode_attention for positions below max_seqlen (-1 for invalid arguments): per row,
- * query head and 256-token chunk an fp32 partial of head_dim + 2 values. A smaller workspace is legal down to one
- * chunk a row: the chunks then grow until the table's whole width fits. */
+/* Workspace bytes of cdb_kv8_decode_attention for positions below max_seqlen (-1 for invalid arguments): per row
+ * and chunk of 1024 tokens (64 chunks at most) an fp32 partial of head_dim + 2 values a query head and 8 bytes a
+ * KV head. A smaller workspace is legal down to one chunk a row: rows with more take longer chunks. Nothing in
+ * it need be set before a call; calls that may overlap need one each. */
 int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                        int32_t max_seqlen);
 
@@ -422,7 +423,7 @@ int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int3
  * positions 0..seqlens[b], its own included. Rows whose position, table row or cache layer is out of range get a
  * NaN output and no write, and so does a row whose blocks in use are not all inside the pool. num_heads is a
  * multiple of num_kv_heads. Two rows of a call never append to the same tile. A row's context is cut into
- * chunks of 256 tokens, merged in order, so its output does not depend on the other rows. */
+ * chunks of 1024 tokens, merged in order, so its output does not depend on the other rows. */
 int cdb_kv8_decode_attention(const void* q, const void* k_new, const void* v_new, void* codes, void* scales,
                              int32_t num_cache_layers, int64_t pool_blocks, const int32_t* cache_layer,
                              int32_t cache_layer0, const int32_t* block_table, const int32_t* table_row,

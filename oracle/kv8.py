@@ -99,16 +99,17 @@ class Cache:
         return np.ldexp(self.codes[layer, plane][tile, :, off], e[..., None])
 
 
-def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, end: np.ndarray, scale: float,
-           round_off: float, score_off: float, prob_off: float, floor: float = 0.0) -> tuple[np.ndarray, np.ndarray]:
+def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, end: np.ndarray, scale: float, round_off: float,
+           score_off: float, prob_off: float, floor: float = 0.0, top_off: float = 0.0
+           ) -> tuple[np.ndarray, np.ndarray]:
     """Attention of q [n, H, D] over k, v [tokens, Hkv, D] in 64 bits, query i over keys 0..end[i], and a bound on
-    what a computation may be off by whose scores are off by at most ``score_off`` times sum_d |q_d k_d| * scale,
+    what a computation may be off by whose scores are off by at most
+    d = scale * sum_d (score_off |q_d| + top_off max|q|) |k_d|,
     whose probabilities and sums are off by the relative ``prob_off`` besides, and whose results are rounded by
     the relative ``round_off``; ``floor`` is what each probability may be off by at any size, the largest being 1.
 
     Scores off by at most d move each p_i / sum(p) by a factor within exp(+-2 d); so
-    |error| <= round_off |o| + (1 + round_off) (exp(2 d + prob_off) - 1) sum_i p_i |v_i|
-    + floor sum_i |v_i|.
+    |error| <= round_off |o| + (1 + round_off) (exp(2 d + prob_off) - 1) sum_i p_i |v_i| + floor sum_i |v_i|.
     """
 
     n, heads, dim = q.shape
@@ -117,14 +118,15 @@ def attend(q: np.ndarray, k: np.ndarray, v: np.ndarray, end: np.ndarray, scale: 
     for h in range(heads):
         kh, vh = k[:, h // group], v[:, h // group]
         s = q[:, h] @ kh.T * scale
-        mass = np.abs(q[:, h]) @ np.abs(kh).T * scale
+        size = np.abs(q[:, h])
+        mass = (score_off * size + top_off * size.max(1, keepdims=True)) @ np.abs(kh).T * scale
         seen = np.arange(len(kh))[None, :] <= end[:, None]
         for i in range(n):
             ks = seen[i]
             p = np.exp(s[i, ks] - s[i, ks].max())
             p /= p.sum()
             o = p @ vh[ks]
-            d = score_off * mass[i, ks].max()
+            d = mass[i, ks].max()
             out[i, h] = o
             bound[i, h] = round_off * np.abs(o) + (1 + round_off) * np.expm1(2 * d + prob_off) * (p @ np.abs(vh[ks]))
             bound[i, h] += floor * np.abs(vh[ks]).sum(0)

@@ -19,18 +19,23 @@ TINY = 2.0 ** -24  # half a step of fp32
 def bounds(kind: str, dtype: str, dim: int, tokens: int) -> dict[str, float]:
     """What a computation rounds, relative (oracle.kv8.attend).
 
-    Scores: dim products summed in fp32 once for each bf16 part the query is taken in (decode 2, fp32 models 3,
-    a bf16 prefill query is its own single part), what the parts leave (2^-16 after two, 2^-24 after three), and a
-    few roundings of scaling. Probabilities: the exponential and its argument, the parts they are taken in (decode
-    bf16: 2^-16 after two, fp32 2^-24; prefill fp16: 2^-11 after one, 2^-22 after two, and 2^-25 at any size),
-    and the fp32 sums over tokens. The result: a half step of its type, and a division and a merge in fp32."""
+    Scores: dim products summed in fp32 once for each part the query is taken in, and a few roundings of scaling.
+    A prefill query in bf16 is its own single part; in fp32 both take three bf16 parts (2^-24 left of each element).
+    A bf16 decode query is 3 e4m3 parts, the first with the head's largest element in (224, 448], each next one 16
+    times finer: parts of at most 448, 256 and 128 leave at most half their step, 16, 8 and 4, times 16^-(part - 1);
+    so 4 / 16^2 of 224, 2^-13.8 of the largest element, after three. Its products sum in fewer bits than fp32: some
+    2^-16 of the largest term each, 3 products.
+    Probabilities: the exponential and its argument, the fp16 parts they are taken in (2^-11 after one, 2^-22 after
+    two for fp32, and 2^-25 at any size), and the fp32 sums over tokens. The result: a half step of its type, and a
+    division and a merge in fp32."""
     out = 2.0 ** -8 if dtype == "bf16" else 8 * TINY
+    prob = 2.0 ** -11 if dtype == "bf16" else 2.0 ** -22
     if kind == "decode":
-        parts, left, prob, floor = (2, 2.0 ** -16, 2.0 ** -16, 0.0) if dtype == "bf16" else (3, TINY, TINY, 0.0)
+        parts, left, top = (3, 0.0, 2.0 ** -13.8 + 3 * 2.0 ** -16) if dtype == "bf16" else (3, TINY, 0.0)
     else:
-        parts, left, prob, floor = (1, 0.0, 2.0 ** -11, 2.0 ** -25) if dtype == "bf16" else (3, TINY, 2.0 ** -22, 2.0 ** -25)
-    return dict(round_off=out + 8 * TINY, score_off=(parts * dim + 8) * TINY + left,
-                prob_off=prob + (2 * tokens + 16) * TINY, floor=floor)
+        parts, left, top = (1, 0.0, 0.0) if dtype == "bf16" else (3, TINY, 0.0)
+    return dict(round_off=out + 8 * TINY, score_off=(parts * dim + 8) * TINY + left, top_off=top,
+                prob_off=prob + (2 * tokens + 16) * TINY, floor=2.0 ** -25)
 
 
 def dev(a, dtype=None) -> torch.Tensor:
@@ -277,13 +282,20 @@ def test_decode_scales_grow_and_hold(std) -> None:
     DecodeCase(13, "bf16", 2, 2, 64, 1, False, 16, [1, 2, 5, 16, 17, 18, 31, 270, 272, 273], std=std).check()
 
 
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 4, 2, 128), ("f32", 1, 1, 64), ("bf16", 20, 1, 96)])
+def test_decode_chunk_edges(dtype, heads, kv, dim) -> None:
+    """Contexts around the length of a chunk and of two, and rows of several chunks beside rows of one."""
+    contexts = [1009, 1023, 1024, 1025, 1040, 1041, 2047, 2048, 2049, 5, 4000]
+    DecodeCase(26, dtype, heads, kv, dim, 1, False, 16, contexts, nan=True).check()
+
+
 def test_decode_over_permuted_table_rows() -> None:
     DecodeCase(14, "bf16", 4, 2, 128, 1, False, 32, [1, 70, 0, 300, 17], by_row=True, nan=True).check()
 
 
 def test_decode_long_context_and_short_workspace() -> None:
     """Partials for fewer chunks than the context has: the chunks lengthen, past one look-up window too."""
-    for longest in (300, 1024, 5000):
+    for longest in (300, 2048, 5000):
         DecodeCase(15, "bf16", 2, 1, 64, 1, False, 16, [5000, 100, 4097], longest=longest, nan=True).check()
 
 
@@ -601,6 +613,18 @@ def test_layout_without_requests_or_tokens() -> None:
         assert out.counts.tolist() == [0, 0, 0, 0] and out.cu_q.tolist() == [0] * (len(past) + 1)
         assert out.rows.tolist() == [-1] * 4 and out.tile_seq.tolist() == [-1] * 2
         np.testing.assert_array_equal(got, table)
+
+
+def test_layout_op() -> None:
+    past, lens, table = np.array([0, 20]), np.array([40, 150]), np.full((2, 12), 99, np.int32)
+    free = np.arange(20, dtype=np.int32)
+    t = dev(table)
+    cu, pos, slot, seq, q0, counts = torch.ops.cdb.batch_layout(dev(past, torch.int32), dev(lens, torch.int32), t, None,
+                                                                dev(free), 16, 190, 3)
+    want = plain_layout(past, lens, table, [0, 1], free, 16)
+    assert (cu.tolist(), pos.tolist(), slot.tolist()) == want[:3]
+    assert list(zip(seq.tolist(), q0.tolist())) == want[3] and counts.tolist() == [190, 3, want[4], 0]
+    np.testing.assert_array_equal(t.cpu().numpy(), want[5])
 
 
 def test_layout_reports_what_does_not_fit() -> None:

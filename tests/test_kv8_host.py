@@ -106,8 +106,8 @@ def test_oracle_attention_of_one_key_and_of_equal_keys() -> None:
 
 
 def test_workspace_sizes() -> None:
-    assert kv8.decode_workspace_bytes(3, 8, 2, 128, 257) >= 3 * 8 * 2 * 130 * 4
-    assert kv8.decode_workspace_bytes(3, 8, 2, 128, 256) < kv8.decode_workspace_bytes(3, 8, 2, 128, 257)
+    assert kv8.decode_workspace_bytes(3, 8, 2, 128, 1025) >= 3 * 8 * 2 * 130 * 4
+    assert kv8.decode_workspace_bytes(3, 8, 2, 128, 1024) < kv8.decode_workspace_bytes(3, 8, 2, 128, 1025)
     for bad in ((-1, 8, 2, 128, 1), (1, 0, 2, 128, 1), (1, 8, 2, 128, 0)):
         with pytest.raises(ValueError):
             kv8.decode_workspace_bytes(*bad)
