@@ -47,26 +47,50 @@ CDB_DEVICE float finite_abs(float x) {
   return a < INFINITY ? a : 0.f;
 }
 
-// Four values, already divided by the scale, as e4m3 codes in one word, rounded to nearest even.
-// An infinity or NaN becomes the NaN code.
+// |x| as bits, which order as the sizes do; from kNotFinite on, x is an infinity or NaN.
+constexpr uint32_t kNotFinite = 0x7f800000u;
+CDB_DEVICE uint32_t size_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Four values as e4m3 codes in one word: divided by a scale, rounded to nearest even. The conversion makes an
+// infinity or NaN the NaN code by itself (both forms checked over every code, every midpoint and its neighbours).
+typedef short s16x2_t __attribute__((ext_vector_type(2)));
+CDB_DEVICE uint32_t codes_of(float a, float b, float c, float d, float scale) {
+  s16x2_t w = {0, 0};
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, a, b, scale, false);
+  w = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(w, c, d, scale, true);
+  return __builtin_bit_cast(uint32_t, w);
+}
 CDB_DEVICE uint32_t codes_of(float a, float b, float c, float d) {
-  auto clean = [](float x) { return fabsf(x) < INFINITY ? x : __uint_as_float(0x7fc00000u); };
-  int w = __builtin_amdgcn_cvt_pk_fp8_f32(clean(a), clean(b), 0, false);
-  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(clean(c), clean(d), w, true);
+  const int w = __builtin_amdgcn_cvt_pk_fp8_f32(a, b, 0, false);
+  return (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(c, d, w, true);
 }
 
-// Codes of one word rounded again for a scale 2^grow times larger (factor = 2^-grow).
-CDB_DEVICE uint32_t recode(uint32_t w, float factor) {
+// Codes of one word rounded again for a scale `growth` times larger.
+CDB_DEVICE uint32_t recode(uint32_t w, float growth) {
   const f32x2_t lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false);
   const f32x2_t hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
-  return codes_of(mul_rn(lo.x, factor), mul_rn(lo.y, factor), mul_rn(hi.x, factor), mul_rn(hi.y, factor));
+  return codes_of(lo.x, lo.y, hi.x, hi.y, growth);
 }
+// 2^(now - old) for old <= now; where it leaves the normal range every code rounds to 0 all the same.
+CDB_DEVICE float growth_of(int old, int now) { return scale_of((uint32_t)min(127 + now - old, 254)); }
 
-// 2^(old - now) for old <= now, flushed to 2^-126 beyond the normal range (every code then gives 0).
-CDB_DEVICE float recode_factor(int old, int now) { return __uint_as_float((uint32_t)max(127 + old - now, 1) << 23); }
+// 2^(old - now) for old <= now, flushed to 2^-126 beyond the normal range.
+CDB_DEVICE float shrink_of(int old, int now) { return scale_of((uint32_t)max(127 + old - now, 1)); }
 
 // Byte mask of a word's tokens below n (n <= 0: none, n >= 4: all).
 CDB_DEVICE uint32_t tokens_below(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
+
+// N storage elements as they lie; vec as for load_f32.
+template <typename T, int N> CDB_DEVICE Vec<T, N> load_raw(const T* p, bool vec) {
+  Vec<T, N> x;
+  if (vec) {
+    x.load(p);
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i += 2) x.set_pair(i, Elem<T>::load(p + i), Elem<T>::load(p + i + 1));
+  }
+  return x;
+}
 
 // N storage elements as fp32; vec: p is aligned for 16-byte loads (8-byte ones where N elements are 8 bytes).
 template <typename T, int N> CDB_DEVICE void load_f32(const T* p, float* out, bool vec) {
@@ -126,6 +150,38 @@ CDB_DEVICE void load_rotated(const T* head, const T* bias, const float* cos, con
   }
 }
 
+// Two runs of N elements of a head, x + bias, rotated: STYLE 1 the elements from d on, in its first half, and
+// those from d + D/2 on, which share their angles; otherwise the elements from d on and from d + N on.
+template <typename T, int D, int STYLE, int N>
+CDB_DEVICE void load_rotated_pair(const T* head, const T* bias, const float* cos, const float* sin, int d, bool vec,
+                                  float* a, float* b) {
+  if constexpr (STYLE == 1) {
+    float c[N], s[N];
+    load_f32<T, N>(head + d, a, vec);
+    load_f32<T, N>(head + d + D / 2, b, vec);
+    load_f32<float, N>(cos + d, c, vec);
+    load_f32<float, N>(sin + d, s, vec);
+    if (bias != nullptr) {
+      float e[N];
+      load_f32<T, N>(bias + d, e, vec);
+#pragma unroll
+      for (int i = 0; i < N; ++i) a[i] = add_rn(a[i], e[i]);
+      load_f32<T, N>(bias + d + D / 2, e, vec);
+#pragma unroll
+      for (int i = 0; i < N; ++i) b[i] = add_rn(b[i], e[i]);
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const float x = a[i], y = b[i];
+      a[i] = sub_rn(mul_rn(x, c[i]), mul_rn(y, s[i]));
+      b[i] = add_rn(mul_rn(y, c[i]), mul_rn(x, s[i]));
+    }
+  } else {
+    load_rotated<T, D, STYLE, N>(head, bias, cos, sin, d, vec, a);
+    load_rotated<T, D, STYLE, N>(head, bias, cos, sin, d + N, vec, b);
+  }
+}
+
 // A value and the one of the lane that differs in bit 4 (or 5), in either order: two vector
 // instructions, against the LDS round trip of a permute.
 CDB_DEVICE f32x2_t pair16(float v) {
@@ -143,6 +199,7 @@ CDB_DEVICE float column_max(float v) {
   x = pair32(fmaxf(x[0], x[1]));
   return fmaxf(x[0], x[1]);
 }
+CDB_DEVICE float all_max(float v) { return column_max(row16_max(v)); }  // over the wave
 CDB_DEVICE float column_sum(float v) {
   f32x2_t x = pair16(v);
   x = pair32(x[0] + x[1]);

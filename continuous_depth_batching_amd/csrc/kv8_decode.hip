@@ -295,10 +295,10 @@ template <int D, bool kWide> struct Attention {
   CDB_DEVICE void values(const ValueRegs<D>& v0, const ValueRegs<D>& v1, int e0, int e1, const f16x8_t* parts) {
     const int now = max(max(e0, e1), ref);
     if (now > ref) {
-      scale_acc(recode_factor(ref, now));
+      scale_acc(shrink_of(ref, now));
       ref = now;
     }
-    const float s0 = recode_factor(e0, ref), s1 = recode_factor(e1, ref);
+    const float s0 = shrink_of(e0, ref), s1 = shrink_of(e1, ref);
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
       union { f16x2_t h[4]; f16x8_t x; } v;
@@ -328,7 +328,7 @@ CDB_DEVICE void append_token(const Kv8Cache& cache, const Fresh<D>& fresh, int64
   const bool k_grown = __builtin_amdgcn_readfirstlane(off != 0 && k_now != k_old);
   const bool v_grown = __builtin_amdgcn_readfirstlane(off != 0 && v_now != v_old);
   if (k_grown && r < off) {
-    const float f = recode_factor(k_old, k_now);
+    const float f = growth_of(k_old, k_now);
 #pragma unroll
     for (int j = 0; j < K::kFull; ++j)
 #pragma unroll
@@ -350,7 +350,7 @@ CDB_DEVICE void append_token(const Kv8Cache& cache, const Fresh<D>& fresh, int64
   }
   const uint32_t before = tokens_below(off - 4 * g), here = tokens_below(off + 1 - 4 * g) & ~before;
   if (v_grown) {
-    const float f = recode_factor(v_old, v_now);
+    const float f = growth_of(v_old, v_now);
 #pragma unroll
     for (int m = 0; m < V::kWords; ++m) v.w[m] = (v.w[m] & ~before) | (recode(v.w[m], f) & before);
   }
@@ -495,7 +495,7 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
                                      P.sin + angle, d, P.vec, x);
         x[0] *= P.scale_log2;
         x[1] *= P.scale_log2;
-        const float most = column_max(row16_max(fmaxf(finite_abs(x[0]), finite_abs(x[1]))));
+        const float most = all_max(fmaxf(finite_abs(x[0]), finite_abs(x[1])));
         Query::store(q_codes, q_bytes, c, 2 * lane, real ? x[0] : 0.f, real ? x[1] : 0.f, most);
       }
     }
@@ -508,18 +508,18 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
       load_f32<T, 2>(static_cast<const T*>(P.v_new) + row + d, y, P.vec);
       load_rotated<T, D, STYLE, 2>(static_cast<const T*>(P.k_new) + row, bias == nullptr ? nullptr : bias + kvh * D,
                                    P.cos + angle, P.sin + angle, d, P.vec, x);
-      const int k_new = scale_byte(column_max(row16_max(fmaxf(finite_abs(x[0]), finite_abs(x[1])))));
-      const int v_new = scale_byte(column_max(row16_max(fmaxf(finite_abs(y[0]), finite_abs(y[1])))));
+      const int k_new = scale_byte(all_max(fmaxf(finite_abs(x[0]), finite_abs(x[1]))));
+      const int v_new = scale_byte(all_max(fmaxf(finite_abs(y[0]), finite_abs(y[1]))));
       const int k_old = min((int)end_k, 254), v_old = min((int)end_v, 254);
       end_k = off != 0 ? max(k_new, k_old) : k_new;
       end_v = off != 0 ? max(v_new, v_old) : v_new;
-      const float k_inv = inverse_scale_of(end_k), v_inv = inverse_scale_of(end_v);
+      const float k_scale = scale_of(end_k), v_scale = scale_of(end_v);
       if (real) {
         const int at = KeyRegs<D>::place(d, 0);
         *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(fresh.key) + (at >> 9) * 32 + (at & 31)) =
-            (uint16_t)codes_of(mul_rn(x[0], k_inv), mul_rn(x[1], k_inv), 0.f, 0.f);
+            (uint16_t)codes_of(x[0], x[1], 0.f, 0.f, k_scale);
         *reinterpret_cast<uint16_t*>(reinterpret_cast<uint8_t*>(fresh.value) + d) =
-            (uint16_t)codes_of(mul_rn(y[0], v_inv), mul_rn(y[1], v_inv), 0.f, 0.f);
+            (uint16_t)codes_of(y[0], y[1], 0.f, 0.f, v_scale);
       }
       __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       if (!lost_end) append_token<D>(P.cache, fresh, end_tile, off, r, g, k_old, end_k, v_old, end_v, k[0], v[0]);

@@ -205,12 +205,12 @@ __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P)
         if (t >= total) continue;
         const int v_exp = max((int)__builtin_amdgcn_readlane((int)v_byte, 2 * i + a), 1);
         if (v_exp > ref) {
-          const float f = recode_factor(ref, v_exp);
+          const float f = shrink_of(ref, v_exp);
 #pragma unroll
           for (int m = 0; m < kTiles; ++m) acc[m] *= f;
           ref = v_exp;
         }
-        const float v_scale = recode_factor(v_exp, ref);
+        const float v_scale = shrink_of(v_exp, ref);
         if (t + kTile > total) {  // codes behind the sequence count for nothing, NaN among them
 #pragma unroll
           for (int g = 0; g < 2; ++g)
