@@ -1,4 +1,24 @@
 // Varlen causal prefill attention over the 8-bit paged KV cache.
+//
+// One workgroup of 4 waves takes 128 query tokens of a sequence and one query head, a wave 32 of them, and walks
+// the keys in blocks of 32, two tiles, with a running maximum and sum (the maximum moves only when a score outgrows
+// it by 2^8). Codes go from memory to registers; each wave loads the next block's keys and values as soon as this
+// block's are used up, so nothing waits on LDS or on another wave.
+//   S^T = K Q^T in bf16: a code times a power of two is exact there, so scores are the products' fp32 sums.
+//   O^T = V^T P^T in fp16, which holds a code exactly and P to 2^-11; values widen with their scale relative to the
+//   largest met. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-22).
+// A lane's 16 scores are those of the 16 tokens whose values it holds, so P never moves; queries are the columns of
+// both products, so maximum and sum are a lane's own and its neighbour's, 32 lanes away.
+//
+// Bound: instruction issue. A wave's block takes 16 matrix instructions of 32 cycles and some 180 vector ones of 4
+// (64 widen codes, 32 are fma and exponential), 770 cycles of a SIMD against 512 of its matrix core; two waves a
+// SIMD overlap them to 1270. Measured (a launch from a graph): two sequences of 6000..8190 tokens, 32 heads on
+// 8 x 128, 873 us (935 TFLOP/s; a large bf16 product reaches 1199); 24 fresh prompts of 24..1300 tokens, 16 heads,
+// 47 us, where the longest tile's chain of blocks is most of it; four chunks of some 110 tokens after 16000, cut in
+// 8 parts, 113 us. Slower or no faster: the scores on the codes themselves with queries of 3 e4m3 parts (876, 52 and
+// 116 us); blocks staged in LDS, 5 ahead, at 3 waves a SIMD (845, 52 and 124); waves of one workgroup parting the
+// keys of the same queries (927, 57 and 118); 64 queries a wave, which widens each code once for twice the queries
+// but leaves one wave a SIMD (1024, 80 and 131); the longest tiles first (957, 61 and 119).
 #include "cdb_amd.h"
 #include "kv8_common.h"
 #include "kv8_host.h"
@@ -6,6 +26,7 @@
 namespace cdb {
 
 constexpr int kQueries = 128;  // query tokens of a tile: 32 a wave
+constexpr int kMaxSplits = 64;  // parts of a tile's keys: a lane each in the merge
 
 struct Kv8PrefillParams {
   const void* q;
@@ -19,38 +40,82 @@ struct Kv8PrefillParams {
   float scale_log2;
 };
 
-// What one lane holds of a block of 32 keys (two tiles): of the keys, 16-byte units 2j + h of token
-// lane % 32; of the values, the words of groups h and h + 2 of each tile for the lane's elements.
+// What a lane (c, h) = (lane % 32, lane / 32) holds of a block of 32 keys, two tiles: of the keys, 16-byte
+// units 2j + h of token c; of the values, the words of groups h and h + 2 of each tile for its elements.
 template <int D> struct BlockRegs {
   static constexpr int kUnits = D / 32, kWords = D / 32;
   u32x4_t k[kUnits];
   uint32_t v[2][2][kWords];  // [tile][group half][element]
 
-  CDB_DEVICE void load_keys(const uint8_t* k0, const uint8_t* k1, int c, int h) {
-    const uint8_t* p = (c & 16 ? k1 : k0) + (c & 15) * 16 + h * 256;
+  CDB_DEVICE void load_keys(const uint8_t* p) {
 #pragma unroll
     for (int j = 0; j < kUnits; ++j) k[j] = *reinterpret_cast<const u32x4_t*>(p + j * 512);
   }
-  CDB_DEVICE void load_values(int a, const uint8_t* vp, int c, int h) {
+  CDB_DEVICE void load_values(int a, const uint8_t* tile, int c, int h) {
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      const uint8_t* p = vp + (h + 2 * s) * (4 * D);
       if constexpr (D == 128) {
-        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(p + c * 16);
+        const u32x4_t w = *reinterpret_cast<const u32x4_t*>(tile + 2 * s * (4 * D) + (h * (4 * D) + c * 16));
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[a][s][i] = w[i];
       } else {
-        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(p + c * 8);
+        const u32x2_t w = *reinterpret_cast<const u32x2_t*>(tile + 2 * s * (4 * D) + (h * (4 * D) + c * 8));
         v[a][s][0] = w[0];
         v[a][s][1] = w[1];
-        if constexpr (D == 96) v[a][s][2] = *reinterpret_cast<const uint32_t*>(p + 256 + c * 4);
+        if constexpr (D == 96)
+          v[a][s][2] = *reinterpret_cast<const uint32_t*>(tile + 2 * s * (4 * D) + 256 + (h * (4 * D) + c * 4));
       }
     }
   }
-  // Head element of accumulator row `row` of value product i.
+  // Head element of row `row` of value product i.
   static CDB_DEVICE int value_element(int i, int row) {
     if constexpr (D == 128) return 4 * row + i;
     return i < 2 ? 2 * row + i : 64 + row;
+  }
+};
+
+CDB_DEVICE float half_max(float v) {
+  const f32x2_t x = pair32(v);
+  return fmaxf(x[0], x[1]);
+}
+
+// A lane's share of 32 queries as the operand of the products with the keys: bf16 as it is, fp32 as 3 bf16 parts.
+template <typename T, int D> struct BlockQuery {
+  static constexpr int kParts = sizeof(T) == 4 ? 3 : 1, kSteps = D / 16;
+  bf16x8_t w[kSteps][kParts];
+
+  CDB_DEVICE void load(const T* q, int h) {
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) {
+      const T* at = q + 32 * (m >> 1) + 16 * h + 8 * (m & 1);
+      if constexpr (kParts == 1) {
+        w[m][0] = *reinterpret_cast<const bf16x8_t*>(at);
+      } else {
+        float x[8];
+        load_f32<T, 8>(at, x, true);
+#pragma unroll
+        for (int p = 0; p < kParts; ++p)
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const __bf16 y = (__bf16)x[i];
+            w[m][p][i] = y;
+            x[i] -= (float)y;
+          }
+      }
+    }
+  }
+  CDB_DEVICE f32x16_t scores(const BlockRegs<D>& x, int k_byte) const {
+    const float f = scale_of(k_byte);
+    f32x16_t s;
+#pragma unroll
+    for (int e = 0; e < 16; ++e) s[e] = 0.f;
+#pragma unroll
+    for (int m = 0; m < kSteps; ++m) {
+      const bf16x8_t k = widen_bf16(x.k[m >> 1][2 * (m & 1)], f, x.k[m >> 1][2 * (m & 1) + 1], f);
+#pragma unroll
+      for (int p = kParts - 1; p >= 0; --p) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, w[m][p], s, 0, 0, 0);
+    }
+    return s;
   }
 };
 
@@ -64,17 +129,18 @@ CDB_DEVICE f16x8_t widen_f16(uint32_t w0, uint32_t w1, float s) {
   return u.v;
 }
 
-CDB_DEVICE float half_max(float v) {
-  const f32x2_t x = pair32(v);
-  return fmaxf(x[0], x[1]);
-}
+// 0x80 in each byte of w that holds the NaN code.
+CDB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
+// How far scores may outgrow the maximum that the sums are counted from before they are counted anew: P stays
+// below 2^8, far inside fp16, and most blocks move nothing.
+constexpr float kSlack = 8.f;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P) {
   using Regs = BlockRegs<D>;
-  constexpr bool kWide = sizeof(T) == 4;
-  constexpr int kQParts = kWide ? 3 : 1, kPParts = kWide ? 2 : 1;
-  constexpr int kSteps = D / 16, kTiles = D / 32;
+  constexpr int kPParts = sizeof(T) == 4 ? 2 : 1;
+  constexpr int kTiles = D / 32;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int heads = P.cache.num_kv_heads;
@@ -86,97 +152,81 @@ __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P)
   if (s < 0 || s >= P.num_seqs) return;
   const int64_t token0 = P.cu_q[s];
   const int num = P.cu_q[s + 1] - (int)token0, past = P.past[s];
-  const int w0 = P.tile_q0[n] + 32 * wave;
-  if (token0 < 0 || num < 0 || token0 + num > P.tokens || past < 0 || w0 < 0 || w0 >= num) return;
+  const int q0 = P.tile_q0[n], w0 = q0 + 32 * wave;
+  if (token0 < 0 || num < 0 || token0 + num > P.tokens || past < 0 || q0 < 0 || q0 >= num || w0 >= num) return;
   const int query = w0 + c, pos = past + query;
   const int64_t total = (int64_t)past + num;
   const int trow = P.table_row[s];
   const bool bad = total > ((int64_t)P.table_width << P.bs_log2) || trow < 0 || trow >= P.table_rows;
 
-  const int tile_end = past + min(P.tile_q0[n] + kQueries, num), wave_end = past + min(w0 + 32, num);
-  const int blocks = (tile_end + 31) / 32;
-  const int part = blockIdx.y;
-  const int from = (int)((int64_t)blocks * part / P.splits);
-  const int to = bad ? 0 : min((int)((int64_t)blocks * (part + 1) / P.splits), (wave_end + 31) / 32);
+  // Blocks of 32 keys: the tile's, this part's of them, and of those the ones that the wave's queries see.
+  const int blocks = (past + min(q0 + kQueries, num) + 31) / 32;
+  const int part = blockIdx.y, parts = P.splits;
+  const int from = parts == 1 ? 0 : (uint32_t)blocks * part / parts;
+  const int end = parts == 1 ? blocks : (int)((uint32_t)blocks * (part + 1) / parts);
+  const int to = bad ? 0 : min(end, (past + min(w0 + 32, num) + 31) / 32);
 
-  bf16x8_t q[kSteps][kQParts];
-  {
-    const T* src = static_cast<const T*>(P.q) + ((token0 + min(query, num - 1)) * P.num_heads + head) * D;
-#pragma unroll
-    for (int m = 0; m < kSteps; ++m) {
-      const T* at = src + 32 * (m >> 1) + 16 * h + 8 * (m & 1);
-      if constexpr (kWide) {
-        float x[8];
-        load_f32<T, 8>(at, x, true);
-#pragma unroll
-        for (int p = 0; p < kQParts; ++p)
-#pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const __bf16 y = (__bf16)x[i];
-            q[m][p][i] = y;
-            x[i] -= (float)y;
-          }
-      } else {
-        q[m][0] = *reinterpret_cast<const bf16x8_t*>(at);
-      }
-    }
-  }
+  BlockQuery<T, D> q;
+  q.load(static_cast<const T*>(P.q) + ((token0 + min(query, num - 1)) * P.num_heads + head) * D, h);
   f32x16_t acc[kTiles];
 #pragma unroll
   for (int i = 0; i < kTiles; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-  float top = -INFINITY, sum = 0.f;
+  // Scores are counted, in units of log2, from `base`, anew once they pass `limit`.
+  float base = 0.f, limit = -INFINITY, sum = 0.f;
   int ref = 1;  // biased exponent that the accumulators are counted in
   bool missing = bad;
   const int32_t* table = P.block_table + (int64_t)(bad ? 0 : trow) * P.table_width;
   const int bs_mask = (1 << P.bs_log2) - 1;
+  const int64_t plane = P.cache.plane_tiles * (kTile * D);
 
   for (int window = from; window < to; window += 32) {
     const int count = min(32, to - window);
+    // Lane j looks up tile j of the window; one past the sequence is any tile, and masked.
     int64_t where = 0;
-    uint32_t k_byte = 0, v_byte = 0;
+    uint32_t bytes = 0x0101u;
     bool lost = false;
     if (lane < 2 * count) {
       const int t = window * 32 + lane * kTile;
       if (t < total) {
         const int block = table[t >> P.bs_log2];
         lost = block < 0 || block >= P.cache.pool_blocks;
-        where = P.cache.tile(P.layer, 0, lost ? 0 : block, kvh, (t & bs_mask) >> 4);
-        k_byte = P.cache.scales[where];
-        v_byte = P.cache.scales[where + P.cache.plane_tiles];
+        const int64_t tile = P.cache.tile(P.layer, 0, lost ? 0 : block, kvh, (t & bs_mask) >> 4);
+        bytes = P.cache.scales[tile] | (uint32_t)P.cache.scales[tile + P.cache.plane_tiles] << 8;
+        where = tile * (kTile * D);
       }
     }
     missing = missing || __ballot(lost) != 0;
-    auto codes_at = [&](int j) -> const uint8_t* {
+    auto codes_at = [&](int j) __attribute__((always_inline)) -> const uint8_t* {
       const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)where, j);
       const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(where >> 32), j);
-      return P.cache.codes + (int64_t)(((uint64_t)hi << 32) | lo) * (kTile * D);
+      return P.cache.codes + (((uint64_t)hi << 32) | lo);
     };
-    const int64_t plane = P.cache.plane_tiles * (kTile * D);
-    auto load = [&](Regs& x, int i) {
+    Regs x;
+    auto load_keys = [&](int i) __attribute__((always_inline)) {
       const uint8_t *t0 = codes_at(2 * i), *t1 = codes_at(2 * i + 1);
-      x.load_keys(t0, t1, c, h);
-      x.load_values(0, t0 + plane, c, h);
-      x.load_values(1, t1 + plane, c, h);
+      x.load_keys((c & 16 ? t1 : t0) + ((c & 15) * 16 + h * 256));
     };
-    Regs cur, next;
-    load(cur, 0);
+    auto load_values = [&](int i) __attribute__((always_inline)) {
+      x.load_values(0, codes_at(2 * i) + plane, c, h);
+      x.load_values(1, codes_at(2 * i + 1) + plane, c, h);
+    };
+    load_keys(0);
+    __builtin_amdgcn_sched_barrier(0);
+    load_values(0);
     for (int i = 0; i < count; ++i) {
-      if (i + 1 < count) load(next, i + 1);
+      // The loads ahead repeat the last block at the end: a branch around them would make the wait for this
+      // block's values one for the next block's keys too.
+      const int ahead = min(i + 1, count - 1);
       const int key0 = (window + i) * 32;
-      const float k_scale = scale_of(c & 16 ? __builtin_amdgcn_readlane((int)k_byte, 2 * i + 1)
-                                            : __builtin_amdgcn_readlane((int)k_byte, 2 * i));
-      f32x16_t sc;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = 0.f;
-#pragma unroll
-      for (int m = 0; m < kSteps; ++m) {
-        const bf16x8_t k = widen_bf16(cur.k[m >> 1][2 * (m & 1)], k_scale, cur.k[m >> 1][2 * (m & 1) + 1], k_scale);
-#pragma unroll
-        for (int p = kQParts - 1; p >= 0; --p) sc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(k, q[m][p], sc, 0, 0, 0);
-      }
-      if (key0 + 31 > past + w0) {  // some query of the wave does not see some key of the block
+      const uint32_t b0 = __builtin_amdgcn_readlane((int)bytes, 2 * i);
+      const uint32_t b1 = __builtin_amdgcn_readlane((int)bytes, 2 * i + 1);
+      f32x16_t sc = q.scores(x, (int)((c & 16 ? b1 : b0) & 255));
+      load_keys(ahead);
+      const bool diagonal = key0 + 31 > past + w0;  // some query of the wave does not see some key of the block
+      if (diagonal) {
+        __asm__ volatile("");  // keeps this a branch: most blocks have nothing to mask
 #pragma unroll
         for (int e = 0; e < 16; ++e)
           if (key0 + (e >> 2) * 8 + 4 * h + (e & 3) > pos) sc[e] = -INFINITY;
@@ -184,26 +234,22 @@ __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P)
       float most = sc[0];
 #pragma unroll
       for (int e = 1; e < 16; ++e) most = fmaxf(most, sc[e]);
-      most = fmaxf(top, half_max(most) * P.scale_log2);
-      const float base = most == -INFINITY ? 0.f : most;  // a query that has seen no key yet
-      if (__any(most > top)) {
-        const float keep = __builtin_amdgcn_exp2f(top - base);
-        sum *= keep;
+      if (__any(most * P.scale_log2 > limit)) {
+        most = half_max(most) * P.scale_log2;
+        const bool more = most > limit;
+        const float keep = more && limit != -INFINITY ? __builtin_amdgcn_exp2f(base - most) : 1.f;
+        sum *= keep;  // the first count finds zeros
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) acc[m] *= keep;
-        top = most;
+        base = more ? most : base;
+        limit = more ? most + kSlack : limit;
       }
-      float prob[16];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        prob[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, -base));
-        sum += prob[e];
-      }
+      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, -base));
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int t = key0 + kTile * a;
-        if (t >= total) continue;
-        const int v_exp = max((int)__builtin_amdgcn_readlane((int)v_byte, 2 * i + a), 1);
+        const int v_exp = max((int)((a ? b1 : b0) >> 8), 1);
         if (v_exp > ref) {
           const float f = shrink_of(ref, v_exp);
 #pragma unroll
@@ -211,41 +257,73 @@ __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P)
           ref = v_exp;
         }
         const float v_scale = shrink_of(v_exp, ref);
-        if (t + kTile > total) {  // codes behind the sequence count for nothing, NaN among them
+        f16x8_t pp[kPParts];
+#pragma unroll
+        for (int p = 0; p < kPParts; ++p)
+#pragma unroll
+          for (int e = 0; e < 8; e += 2) {
+            const f16x2_t y = __builtin_convertvector((f32x2_t){sc[8 * a + e], sc[8 * a + e + 1]}, f16x2_t);
+            pp[p][e] = y[0];
+            pp[p][e + 1] = y[1];
+            sum = __builtin_amdgcn_fdot2(y, (f16x2_t){(_Float16)1.f, (_Float16)1.f}, sum, false);
+            if (p + 1 < kPParts) {
+              sc[8 * a + e] -= (float)y[0];
+              sc[8 * a + e + 1] -= (float)y[1];
+            }
+          }
+        if (diagonal) {
+          // A value counts only for the queries that see its token: codes behind the sequence are taken out,
+          // and so are NaN codes, which a probability of zero would not keep from the other queries; those that
+          // do see one get it by a product of where NaN is with what is seen.
+          uint32_t any_nan = 0;
 #pragma unroll
           for (int g = 0; g < 2; ++g)
 #pragma unroll
-            for (int m = 0; m < Regs::kWords; ++m) cur.v[a][g][m] &= tokens_below((int)(total - t) - 4 * (h + 2 * g));
-        }
-        f16x8_t pp[kPParts];
-        {
-          float left[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) left[e] = prob[8 * a + e];
-#pragma unroll
-          for (int p = 0; p < kPParts; ++p)
-#pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-              const f16x2_t y = __builtin_convertvector((f32x2_t){left[e], left[e + 1]}, f16x2_t);
-              pp[p][e] = y[0];
-              pp[p][e + 1] = y[1];
-              left[e] -= (float)y[0];
-              left[e + 1] -= (float)y[1];
+            for (int m = 0; m < Regs::kWords; ++m) {
+              uint32_t& w = x.v[a][g][m];
+              w &= tokens_below((int)(total - t) - 4 * (h + 2 * g));
+              any_nan |= nan_bytes(w);
             }
+          if (__any(any_nan != 0)) {
+            f16x8_t seen;
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              seen[e] = t + (e >> 2) * 8 + 4 * h + (e & 3) <= pos ? (_Float16)1.f : (_Float16)0.f;
+#pragma unroll
+            for (int m = 0; m < kTiles; ++m) {
+              uint32_t where_nan[2];
+#pragma unroll
+              for (int g = 0; g < 2; ++g) {
+                const uint32_t hit = nan_bytes(x.v[a][g][m]) >> 7;  // 1 in each such byte
+                where_nan[g] = hit * 0x38u;                         // the code of 1
+                x.v[a][g][m] &= ~(hit * 0xffu);
+              }
+              f32x16_t met;
+#pragma unroll
+              for (int e = 0; e < 16; ++e) met[e] = 0.f;
+              met = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen_f16(where_nan[0], where_nan[1], 1.f), seen, met, 0, 0,
+                                                           0);
+#pragma unroll
+              for (int e = 0; e < 16; ++e) acc[m][e] = met[e] != 0.f ? NAN : acc[m][e];
+            }
+          }
         }
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
-          const f16x8_t v = widen_f16(cur.v[a][0][m], cur.v[a][1][m], v_scale);
+          const f16x8_t v = widen_f16(x.v[a][0][m], x.v[a][1][m], v_scale);
 #pragma unroll
           for (int p = kPParts - 1; p >= 0; --p)
             acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pp[p], acc[m], 0, 0, 0);
         }
       }
-      cur = next;
+      __builtin_amdgcn_sched_barrier(0);
+      load_values(ahead);
+      __builtin_amdgcn_sched_barrier(0);
     }
   }
 
   sum += shfl_xor_f32(sum, 32);
+  const float top = sum == 0.f ? -INFINITY : base;  // a query that has seen no key
   if (missing) sum = NAN;
   const float back = scale_of(ref);
   if (query >= num) return;
@@ -260,7 +338,7 @@ __global__ void __launch_bounds__(256, 2) kv8_prefill_kernel(Kv8PrefillParams P)
     return;
   }
   float* to_part = P.partials +
-                   ((((int64_t)n * P.splits + part) * P.num_heads + head) * kQueries + (32 * wave + c)) * (D + 2);
+                   ((((int64_t)n * P.splits + part) * P.num_heads + head) * kQueries + (query - q0)) * (D + 2);
 #pragma unroll
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
@@ -284,22 +362,32 @@ __global__ void __launch_bounds__(256) kv8_prefill_merge_kernel(Kv8PrefillParams
   if (s < 0 || s >= P.num_seqs) return;
   const int64_t token0 = P.cu_q[s];
   const int num = P.cu_q[s + 1] - (int)token0, query = P.tile_q0[n] + i;
-  if (token0 < 0 || num < 0 || token0 + num > P.tokens || P.past[s] < 0 || P.tile_q0[n] < 0 || query >= num) return;
+  if (token0 < 0 || num < 0 || token0 + num > P.tokens || P.past[s] < 0 || P.tile_q0[n] < 0 || P.tile_q0[n] >= num ||
+      query >= num)
+    return;
   const int64_t stride = (int64_t)P.num_heads * kQueries * (D + 2);
   const float* x = P.partials + (((int64_t)n * P.splits * P.num_heads + head) * kQueries + i) * (D + 2);
-  float most = -INFINITY;
-  for (int p = 0; p < P.splits; ++p) most = fmaxf(most, x[p * stride + D]);
-  float o[2] = {0.f, 0.f}, l = 0.f;
-  for (int p = 0; p < P.splits; ++p) {
-    const float* y = x + p * stride;
-    const float f = __builtin_amdgcn_exp2f(y[D] - most);
-    l = fmaf(f, y[D + 1], l);
-    o[0] = fmaf(f, y[lane], o[0]);
-    if (lane + 64 < D) o[1] = fmaf(f, y[lane + 64], o[1]);
+  // Lane p weighs part p; every lane then joins two elements.
+  float top = -INFINITY, l = 0.f;
+  if (lane < P.splits) {
+    const f32x2_t y = *reinterpret_cast<const f32x2_t*>(x + lane * stride + D);
+    top = y[0];
+    l = y[1];
   }
-  T* out = static_cast<T*>(P.out) + ((token0 + query) * P.num_heads + head) * D;
-  Elem<T>::store(out + lane, o[0] / l);
-  if (lane + 64 < D) Elem<T>::store(out + lane + 64, o[1] / l);
+  const float f = __builtin_amdgcn_exp2f(top - wave_max(top));
+  l = wave_sum(f * l);
+  if (2 * lane >= D) return;
+  f32x2_t o = {0.f, 0.f};
+#pragma unroll 4
+  for (int p = 0; p < P.splits; ++p) {
+    const f32x2_t y = *reinterpret_cast<const f32x2_t*>(x + p * stride + 2 * lane);
+    const float g = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(f), p));
+    o[0] = fmaf(g, y[0], o[0]);
+    o[1] = fmaf(g, y[1], o[1]);
+  }
+  T* out = static_cast<T*>(P.out) + ((token0 + query) * P.num_heads + head) * D + 2 * lane;
+  Elem<T>::store(out, o[0] / l);
+  Elem<T>::store(out + 1, o[1] / l);
 }
 
 template <typename T, int D> static int prefill_dim(const Kv8PrefillParams& P, hipStream_t stream) {
@@ -324,7 +412,7 @@ template <typename T> static int prefill_type(const Kv8PrefillParams& P, int dim
 
 extern "C" int64_t cdb_kv8_prefill_workspace_bytes(int32_t num_tiles, int32_t splits, int32_t num_heads,
                                                    int32_t head_dim) {
-  if (num_tiles < 0 || splits <= 0 || num_heads <= 0 || head_dim <= 0) return -1;
+  if (num_tiles < 0 || splits <= 0 || splits > cdb::kMaxSplits || num_heads <= 0 || head_dim <= 0) return -1;
   return splits == 1 ? 0 : (int64_t)num_tiles * splits * num_heads * cdb::kQueries * (head_dim + 2) * 4;
 }
 
@@ -340,7 +428,7 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, const void* codes, const
   using namespace cdb;
   if (dtype != CDB_DTYPE_F32 && dtype != CDB_DTYPE_BF16) return CDB_ERR_UNSUPPORTED;
   if (num_seqs < 0 || num_tiles < 0 || tokens < 0 || num_heads <= 0 || table_rows <= 0 || table_width <= 0 ||
-      layer < 0 || layer >= num_cache_layers || splits <= 0 || splits > 65535)
+      layer < 0 || layer >= num_cache_layers || splits <= 0 || splits > kMaxSplits || tokens > 0x7fffff00ll)
     return CDB_ERR_SHAPE;
   if (num_seqs == 0 || num_tiles == 0 || tokens == 0) return CDB_OK;
   if (q == nullptr || out == nullptr || block_table == nullptr || table_row == nullptr || cu_q == nullptr ||
@@ -357,7 +445,8 @@ extern "C" int cdb_kv8_prefill_attention(const void* q, const void* codes, const
   if (reinterpret_cast<uintptr_t>(q) % 16 != 0 || reinterpret_cast<uintptr_t>(out) % 16 != 0 ||
       reinterpret_cast<uintptr_t>(workspace) % 16 != 0)
     return CDB_ERR_SHAPE;
-  if (workspace_bytes < cdb_kv8_prefill_workspace_bytes(num_tiles, splits, num_heads, head_dim)) return CDB_ERR_CAPACITY;
+  if (workspace_bytes < cdb_kv8_prefill_workspace_bytes(num_tiles, splits, num_heads, head_dim))
+    return CDB_ERR_CAPACITY;
   P.q = q; P.layer = layer;
   P.block_table = block_table; P.table_row = table_row; P.cu_q = cu_q; P.past = past;
   P.tile_seq = tile_seq; P.tile_q0 = tile_q0;

@@ -441,8 +441,9 @@ int64_t cdb_kv8_prefill_workspace_bytes(int32_t num_tiles, int32_t splits, int32
 /* Varlen causal prefill attention over the 8-bit cache: the counterpart of cdb_prefill_attention, with its
  * sequences, block table and tiles of 128 query tokens (tile_seq[n] < 0: no tile). q [T, H, D] is rotated; the
  * chunk's own keys and values are already in the cache. splits > 1 cuts every tile's key range into that many
- * parts, merged in order by a second launch: for few tiles with long histories. Queries of a sequence whose
- * table row is out of range or whose blocks in use are not all inside the pool get NaN. q and out are dense. */
+ * parts (at most 64), merged in order by a second launch: for few tiles with long histories. Queries of a sequence
+ * whose table row is out of range or too short get NaN, and so do those that see a block outside the pool, with
+ * the rest of their 32 in a tile. q and out are dense. */
 int cdb_kv8_prefill_attention(const void* q, const void* codes, const void* scales, int32_t num_cache_layers,
                               int64_t pool_blocks, int32_t layer, const int32_t* block_table,
                               const int32_t* table_row, int32_t table_rows, int32_t table_width, const int32_t* cu_q,

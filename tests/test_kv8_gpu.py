@@ -74,7 +74,8 @@ class WriteCase:
         a = dict(q=self.q, k=self.k, v=self.v, rows=dev(self.rows), pos=dev(self.pos, torch.int32)) | over
         q_out = torch.full(self.q.shape, 7.0, dtype=self.q.dtype, device=DEV) if q_out is None else q_out
         kv8.write_raw(a["q"], a["k"], a["v"], q_out if a["q"] is not None else None, self.pool, self.layer, a["rows"],
-                      a["pos"], None if self.cos is None else dev(self.cos), None if self.sin is None else dev(self.sin),
+                      a["pos"], None if self.cos is None else dev(self.cos),
+                      None if self.sin is None else dev(self.sin),
                       self.style, self.q_bias if a["q"] is not None else None, self.k_bias)
         return q_out
 
@@ -399,7 +400,8 @@ def test_decode_graph_replays_and_streams() -> None:
 def test_decode_op() -> None:
     c = DecodeCase(23, "bf16", 4, 2, 128, 1, False, 16, [700, 3, 0])
     a = c.args()
-    got = torch.ops.cdb.kv8_decode_attention(c.q, c.k, c.v, c.pool.codes, c.pool.scales, a["layer"], 0, a["table"], None,
+    got = torch.ops.cdb.kv8_decode_attention(c.q, c.k, c.v, c.pool.codes, c.pool.scales, a["layer"], 0, a["table"],
+                                             None,
                                              a["pos"], a["cos"], a["sin"], 1, None, None, c.workspace, c.scale)
     helpers.close(got, *c.expect())
     assert (got[2] == 0).all()
@@ -445,9 +447,11 @@ class PrefillCase:
 
     def run(self, splits=1, extra_tiles=0, **over):
         seq, q0 = ops.prefill_tiles(self.new, self.past)
-        seq, q0 = np.concatenate([seq, np.full(extra_tiles, -1, np.int32)]), np.concatenate([q0, np.zeros(extra_tiles, np.int32)])
+        seq = np.concatenate([seq, np.full(extra_tiles, -1, np.int32)])
+        q0 = np.concatenate([q0, np.zeros(extra_tiles, np.int32)])
         heads = self.q.shape[1]
-        ws = torch.full((kv8.prefill_workspace_bytes(len(seq), splits, heads, self.dim),), 255, dtype=torch.uint8, device=DEV)
+        ws = torch.full((kv8.prefill_workspace_bytes(len(seq), splits, heads, self.dim),), 255, dtype=torch.uint8,
+                        device=DEV)
         a = dict(q=self.q, pool=self.pool, layer=self.layer, table=dev(self.table),
                  table_row=dev(np.arange(len(self.past), dtype=np.int32)), cu=dev(self.cu),
                  past=dev(self.past.astype(np.int32)), seq=dev(seq), q0=dev(q0),
@@ -525,6 +529,30 @@ def test_prefill_sequence_out_of_range_gives_nan() -> None:
         helpers.close(got[40:80], want[40:80], bound[40:80])
 
 
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("bf16", 96), ("f32", 64)])
+def test_prefill_nan_values_reach_only_queries_that_see_them(dtype, dim) -> None:
+    """NaN codes of keys and values inside the chunk and in its history: earlier queries are untouched, later ones
+    have NaN (a key: everywhere; a value: in its element)."""
+    c = PrefillCase(39, dtype, 2, 2, dim, 16, [(40, 90), (0, 70)])
+    for s, at, plane, head, d in ((0, 60, 1, 0, 5), (0, 61, 1, 0, 6), (0, 100, 1, 1, dim - 1), (1, 33, 0, 0, 3),
+                                  (1, 3, 1, 1, 9)):
+        slot = int(helpers.slots(c.table[s], np.array([at]), 16)[0])
+        c.cache.codes[c.layer, plane, slot // 16, head, slot % 16, d] = np.nan
+    c.upload()
+    for splits in (1, 3):
+        got = c.run(splits=splits).float().cpu().numpy()
+        hit = np.zeros(got.shape, bool)
+        hit[60 - 40:90, 0, 5] = hit[61 - 40:90, 0, 6] = hit[100 - 40:90, 1, dim - 1] = True
+        hit[90 + 33:, 0, :] = True
+        hit[90 + 3:, 1, 9] = True
+        np.testing.assert_array_equal(np.isnan(got), hit)
+        c.cache.codes, keep = np.nan_to_num(c.cache.codes), c.cache.codes
+        want, bound = c.expect()
+        c.cache.codes = keep
+        ok = np.abs(got - want) <= bound
+        assert ok[:60 - 40].all() and ok[90:90 + 3].all() and ok[90:90 + 33, 0].all()
+
+
 def test_prefill_graph_replays() -> None:
     c = PrefillCase(37, "bf16", 2, 1, 128, 16, [(700, 60), (0, 200)])
     seq, q0 = ops.prefill_tiles(c.new, c.past)
@@ -549,8 +577,9 @@ def test_prefill_graph_replays() -> None:
 def test_prefill_op() -> None:
     c = PrefillCase(38, "bf16", 4, 2, 64, 16, [(20, 60)])
     seq, q0 = ops.prefill_tiles(c.new, c.past)
-    got = torch.ops.cdb.kv8_prefill_attention(c.q, c.pool.codes, c.pool.scales, c.layer, dev(c.table), dev([0], torch.int32),
-                                              dev(c.cu), dev(c.past.astype(np.int32)), dev(seq), dev(q0), c.scale, 1, None)
+    got = torch.ops.cdb.kv8_prefill_attention(c.q, c.pool.codes, c.pool.scales, c.layer, dev(c.table),
+                                              dev([0], torch.int32), dev(c.cu), dev(c.past.astype(np.int32)),
+                                              dev(seq), dev(q0), c.scale, 1, None)
     helpers.close(got, *c.expect())
 
 
@@ -578,7 +607,8 @@ def plain_layout(past, lens, table, rows, free, block):
 def run_layout(past, lens, table, rows, free, block, tokens, tiles):
     out = kv8.BatchLayout.allocate(len(past), tokens, tiles, DEV)
     t = dev(table)
-    kv8.batch_layout_raw(dev(past, torch.int32), dev(lens, torch.int32), t, None if rows is None else dev(rows, torch.int32),
+    kv8.batch_layout_raw(dev(past, torch.int32), dev(lens, torch.int32), t,
+                         None if rows is None else dev(rows, torch.int32),
                          dev(free, torch.int32), block, out)
     return out, t.cpu().numpy()
 
@@ -608,7 +638,8 @@ def test_layout_matches_the_requests_one_by_one(block, seqs, hi, past_hi) -> Non
 def test_layout_without_requests_or_tokens() -> None:
     table = np.zeros((2, 3), np.int32)
     for past, lens in (([], []), ([5, 0], [0, 0])):
-        out, got = run_layout(np.array(past, np.int32), np.array(lens, np.int32), table, None, np.zeros(0, np.int32), 16,
+        out, got = run_layout(np.array(past, np.int32), np.array(lens, np.int32), table, None, np.zeros(0, np.int32),
+                              16,
                               4, 2)
         assert out.counts.tolist() == [0, 0, 0, 0] and out.cu_q.tolist() == [0] * (len(past) + 1)
         assert out.rows.tolist() == [-1] * 4 and out.tile_seq.tolist() == [-1] * 2
@@ -681,7 +712,8 @@ def test_layout_write_prefill_and_decode_together() -> None:
         k_rot = oracle.rotate(f32(k), None, cos, sin, pos, 1)
         cache.write(0, slot, k_rot, f32(v))
         if decode:
-            out = kv8.decode_attention_raw(q, k, v, pool, None, 0, table, None, plan.positions, dev(cos), dev(sin), 1, None,
+            out = kv8.decode_attention_raw(q, k, v, pool, None, 0, table, None, plan.positions, dev(cos), dev(sin), 1,
+                                           None,
                                            None, torch.empty_like(q), ws, 0.125)
             turned = oracle.rotate(f32(q), None, cos, sin, pos, 1).astype(np.float64)
         else:

@@ -258,7 +258,8 @@ def test_python_write_checks() -> None:
 
     with pytest.raises(RuntimeError, match="GPU only"):
         call()
-    for bad in (dict(q=None), dict(q=q[:2]), dict(q_out=q[:, :2]), dict(k=k[:, :1]), dict(v=k.bfloat16()), dict(layer=1),
+    for bad in (dict(q=None), dict(q=q[:2]), dict(q_out=q[:, :2]), dict(k=k[:, :1]), dict(v=k.bfloat16()),
+                dict(layer=1),
                 dict(rows=rows[:2]), dict(cos=cos[:, :16]), dict(style=3), dict(qb=torch.zeros(4, 32)),
                 dict(kb=torch.zeros(2, 64).bfloat16())):
         with pytest.raises(ValueError):
