@@ -470,7 +470,9 @@ enum {
  *   cu_q [num_seqs + 1]; positions, rows [token_capacity]: position and slot of each token, -1 behind the last;
  *   tile_seq, tile_q0 [tile_capacity]: tiles of 128 query tokens, longest key range first and in request order
  *   among equals, (-1, 0) behind the last;
- *   counts [4]: tokens, tiles, blocks taken, CDB_LAYOUT_* bits. The caller drops counts[2] ids from its free list. */
+ *   counts [4]: tokens, tiles, blocks taken, CDB_LAYOUT_* bits. The caller drops counts[2] ids from its free list.
+ * A batch of 2^31 - 1 tokens or more is counted as that many, flagged CDB_LAYOUT_TOKENS_FULL, and not laid out: the
+ * table stays, and every entry is that behind the last. */
 int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs, int32_t* block_table,
                      const int32_t* table_row, int32_t table_rows, int32_t table_width, const int32_t* free_blocks,
                      int32_t num_free, int32_t block_size, int32_t* cu_q, int32_t* positions, int64_t* rows,

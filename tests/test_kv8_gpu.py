@@ -670,6 +670,33 @@ def test_layout_reports_what_does_not_fit() -> None:
     np.testing.assert_array_equal(got, want)
 
 
+@pytest.mark.parametrize("seqs", [255, 256, 257, 1000, 1024, 1025])
+def test_layout_at_the_sizes_where_its_scan_changes(seqs) -> None:
+    rng = np.random.default_rng(42)
+    lens, past = rng.integers(0, 300, size=seqs), rng.integers(0, 200, size=seqs)
+    lens[[0, seqs // 2, -1]] = 0, 129, 300
+    table = rng.integers(0, 1000, size=(seqs, 32)).astype(np.int32)
+    free = rng.permutation(seqs * 32).astype(np.int32)
+    total, tiles = int(lens.sum()), int((-(-lens // 128)).sum())
+    out, got_table = run_layout(past, lens, table, None, free, 16, total, tiles)
+    cu, pos, slot, order, taken, want_table = plain_layout(past, lens, table, np.arange(seqs), free, 16)
+    assert out.counts.tolist() == [total, tiles, taken, 0]
+    assert out.cu_q.tolist() == cu and out.positions.tolist() == pos and out.rows.tolist() == slot
+    assert list(zip(out.tile_seq.tolist(), out.tile_q0.tolist())) == order
+    np.testing.assert_array_equal(got_table, want_table)
+
+
+def test_layout_of_too_many_tokens_to_count_is_left_out() -> None:
+    lens = np.full(3, 1 << 30)
+    table = np.full((3, 1 << 14), 7, np.int32)
+    out, got_table = run_layout(np.zeros(3), lens, table, None, np.arange(5), 1 << 16, 40, 9)
+    assert out.counts.tolist() == [2 ** 31 - 1, 3 << 23, 3 << 14, kv8.LAYOUT_TOKENS_FULL | kv8.LAYOUT_TILES_FULL |
+                                   kv8.LAYOUT_NO_BLOCKS]
+    assert out.positions.tolist() == [-1] * 40 and out.rows.tolist() == [-1] * 40
+    assert out.tile_seq.tolist() == [-1] * 9 and out.tile_q0.tolist() == [0] * 9
+    np.testing.assert_array_equal(got_table, table)
+
+
 def test_layout_leaves_out_bad_requests() -> None:
     past, lens = np.array([3, -1, 0, 5, 0, 100]), np.array([4, 5, -2, 6, 7, 93])
     rows = np.array([0, 1, 2, 9, 3, 4])
