@@ -19,7 +19,7 @@
 // 116 us); blocks staged in LDS, 5 ahead, at 3 waves a SIMD (845, 52 and 124); waves of one workgroup parting the
 // keys of the same queries (927, 57 and 118); 64 queries a wave, which widens each code once for twice the queries
 // but leaves one wave a SIMD (1024, 80 and 131); products and vector instructions interleaved by hand (957, 76 and
-// 135); the tile list, longest first, from its end (957, 61 and 119); the long tiles of fresh prompts in two parts (64).
+// 135); the tile list, longest first, from its end (957, 61 and 119); long tiles of fresh prompts in two parts (64).
 #include "cdb_amd.h"
 #include "kv8_common.h"
 #include "kv8_host.h"
