@@ -408,15 +408,42 @@ class BatchLayout:
     tile_q0: torch.Tensor
     counts: torch.Tensor
 
+    def __post_init__(self) -> None:
+        tokens, tiles = self.positions.numel(), self.tile_seq.numel()
+        for name, n in (("cu_q", max(1, self.cu_q.numel())), ("positions", tokens), ("tile_seq", tiles),
+                        ("tile_q0", tiles), ("counts", 4)):
+            _check_ints(name, getattr(self, name), n)
+        if self.rows.dtype is not torch.int64:
+            raise TypeError("rows must be int64")
+        if self.rows.numel() != tokens or not self.rows.is_contiguous():
+            raise ValueError("rows must be contiguous with an entry per position")
+        if len({t.device for t in (self.cu_q, self.positions, self.rows, self.tile_seq, self.tile_q0,
+                                   self.counts)}) > 1:
+            raise ValueError("a layout's buffers lie on one device")
+        # What every call needs of the buffers, resolved once.
+        self.__dict__["_args"] = (self.cu_q.data_ptr(), self.positions.data_ptr(), self.rows.data_ptr(), tokens,
+                                  self.tile_seq.data_ptr(), self.tile_q0.data_ptr(), tiles, self.counts.data_ptr())
+        self.__dict__["_num_seqs"] = self.cu_q.numel() - 1
+
     @classmethod
     def allocate(cls, num_seqs: int, token_capacity: int, tile_capacity: int,
                  device: torch.device | str) -> "BatchLayout":
         """Buffers for up to ``token_capacity`` tokens and ``tile_capacity`` tiles, parts of one allocation."""
 
-        sizes = (2 * token_capacity, token_capacity, tile_capacity, tile_capacity, num_seqs + 1, 4)
-        rows, positions, tile_seq, tile_q0, cu_q, counts = torch.empty(
-            sum(sizes), dtype=torch.int32, device=device).split(sizes)
-        return cls(cu_q, positions, rows.view(torch.int64), tile_seq, tile_q0, counts)
+        ends = (2 * token_capacity, 3 * token_capacity, 3 * token_capacity + tile_capacity,
+                3 * token_capacity + 2 * tile_capacity, 3 * token_capacity + 2 * tile_capacity + num_seqs + 1)
+        buffer = torch.empty(ends[4] + 4, dtype=torch.int32, device=device)
+        # Outputs of a step, like those of an op: parts that need no tracking as views of each other.
+        rows, positions, tile_seq, tile_q0, cu_q, counts = torch.unsafe_split_with_sizes(
+            buffer, (ends[0], token_capacity, tile_capacity, tile_capacity, num_seqs + 1, 4))
+        at = buffer.data_ptr()
+        self = object.__new__(cls)  # its buffers are right by construction: no checks
+        self.__dict__.update(
+            cu_q=cu_q, positions=positions, rows=rows.view(torch.int64), tile_seq=tile_seq, tile_q0=tile_q0,
+            counts=counts, _num_seqs=num_seqs,
+            _args=(at + 4 * ends[3], at + 4 * ends[0], at, token_capacity, at + 4 * ends[1], at + 4 * ends[2],
+                   tile_capacity, at + 4 * ends[4]))
+        return self
 
 
 def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tensor,
@@ -431,38 +458,32 @@ def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.
     if num_seqs > _lib.CDB_LAYOUT_MAX_SEQS:
         raise ValueError(f"a layout takes up to {_lib.CDB_LAYOUT_MAX_SEQS} requests, got {num_seqs}")
     table_rows, width = _check_table(block_table)
-    a = layout
-    tokens, tiles, num_free = a.positions.numel(), a.tile_seq.numel(), free_blocks.numel()
-    for name, t, n in (("past", past, num_seqs), ("lens", lens, num_seqs), ("free_blocks", free_blocks, num_free),
-                       ("cu_q", a.cu_q, num_seqs + 1), ("positions", a.positions, tokens),
-                       ("tile_seq", a.tile_seq, tiles), ("tile_q0", a.tile_q0, tiles), ("counts", a.counts, 4)):
-        _check_ints(name, t, n)
+    num_free = free_blocks.numel()
+    _check_ints("past", past, num_seqs)
+    _check_ints("lens", lens, num_seqs)
+    _check_ints("free_blocks", free_blocks, num_free)
+    if layout._num_seqs != num_seqs:
+        raise ValueError(f"the layout holds {layout._num_seqs} requests, got {num_seqs}")
     if table_row is not None:
         _check_ints("table_row", table_row, num_seqs)
     elif table_rows < num_seqs:
         raise ValueError("block_table needs a row per request when table_row is not given")
-    if a.rows.dtype is not torch.int64:
-        raise TypeError("rows must be int64")
-    if a.rows.numel() != tokens or not a.rows.is_contiguous():
-        raise ValueError("rows must be contiguous with an entry per position")
-    _require_here(past, lens, block_table, table_row, free_blocks, a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0,
-                  a.counts)
+    _require_here(past, lens, block_table, table_row, free_blocks, layout.counts)
     code = _lib.lib().cdb_batch_layout(
         past.data_ptr(), lens.data_ptr(), num_seqs, block_table.data_ptr(), _ptr(table_row), table_rows, width,
-        free_blocks.data_ptr(), num_free, block_size, a.cu_q.data_ptr(), a.positions.data_ptr(), a.rows.data_ptr(),
-        tokens, a.tile_seq.data_ptr(), a.tile_q0.data_ptr(), tiles, a.counts.data_ptr(), _stream())
+        free_blocks.data_ptr(), num_free, block_size, *layout._args, _stream())
     if code:
         _lib.check(code, "cdb_batch_layout")
 
 
-def _apart(num_seqs: int, tokens: int, tiles: int, device: torch.device) -> BatchLayout:
-    """A layout whose buffers are tensors of their own, as an op's results have to be."""
+def _apart(num_seqs: int, tokens: int, tiles: int, device: torch.device) -> tuple[torch.Tensor, ...]:
+    """A layout's buffers as tensors of their own, as an op's results have to be."""
 
     def ints(n: int) -> torch.Tensor:
         return torch.empty(n, dtype=torch.int32, device=device)
 
-    return BatchLayout(ints(num_seqs + 1), ints(tokens), torch.empty(tokens, dtype=torch.int64, device=device),
-                       ints(tiles), ints(tiles), ints(4))
+    return (ints(num_seqs + 1), ints(tokens), torch.empty(tokens, dtype=torch.int64, device=device), ints(tiles),
+            ints(tiles), ints(4))
 
 
 @torch.library.custom_op("cdb::batch_layout", mutates_args=("block_table",), device_types="cuda")
@@ -472,11 +493,10 @@ def batch_layout(past: torch.Tensor, lens: torch.Tensor, block_table: torch.Tens
     """(cu_q, positions, rows, tile_seq, tile_q0, counts) of a batch; see ``batch_layout_raw``."""
 
     a = _apart(past.numel(), token_capacity, tile_capacity, past.device)
-    batch_layout_raw(past, lens, block_table, table_row, free_blocks, block_size, a)
-    return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts
+    batch_layout_raw(past, lens, block_table, table_row, free_blocks, block_size, BatchLayout(*a))
+    return a
 
 
 @batch_layout.register_fake
 def _(past, lens, block_table, table_row, free_blocks, block_size, token_capacity, tile_capacity):
-    a = _apart(past.numel(), token_capacity, tile_capacity, past.device)
-    return a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts
+    return _apart(past.numel(), token_capacity, tile_capacity, past.device)
