@@ -323,7 +323,7 @@ def _(q, k_new, v_new, codes, scales, cache_layer, cache_layer0, block_table, ta
 def prefill_splits(num_tiles: int, num_heads: int, num_kv_heads: int, longest: int, num_cus: int = 256) -> int:
     """Parts that a prefill launch cuts each tile's key range into: enough to give every CU two workgroups, while
     a part keeps at least 512 keys of the longest range ``longest`` (cached and new tokens of a sequence), and at
-    most 64."""
+    most 64. Heads that share keys take a workgroup each all the same, so ``num_kv_heads`` makes no difference."""
 
     del num_kv_heads
     want = -(-2 * num_cus // max(1, num_tiles * num_heads))

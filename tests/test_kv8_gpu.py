@@ -760,3 +760,112 @@ def test_layout_write_prefill_and_decode_together() -> None:
             helpers.close(out[at:at + n], want, bound)
             at += n
         past = past + np.array(lens, np.int32)
+
+
+def test_two_captured_decodes_share_a_workspace() -> None:
+    """Graphs of different batches replayed in turn over one workspace, with an eager call between them."""
+    cases = [DecodeCase(61, "bf16", 4, 2, 128, 1, False, 16, [2100, 5, 1300]),
+             DecodeCase(62, "bf16", 4, 2, 128, 1, False, 16, [1025, 3000, 1024, 0, 2048])]
+    ws = torch.full((max(c.workspace.nbytes for c in cases),), 255, dtype=torch.uint8, device=DEV)
+    args = [c.args(ws=ws) for c in cases]
+    want = [kv8.decode_attention_raw(*a.values()).clone() for a in args]  # appends; the same again changes nothing
+    graphs = []
+    for a in args:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            kv8.decode_attention_raw(*a.values())
+    for turn in (0, 1, 0, 0, 1, 1, 0):
+        args[turn]["out"].fill_(3.0)
+        graphs[turn].replay()
+        assert torch.equal(args[turn]["out"], want[turn])
+        assert torch.equal(cases[1 - turn].run(ws=ws), want[1 - turn])
+
+
+def test_layout_write_and_prefill_captured_together() -> None:
+    """One graph lays out, writes and attends batches of other lengths than those it was captured with, padded to
+    its capacity; what lies behind the last token stays as it was."""
+    rng = np.random.default_rng(63)
+    heads, kv, dim, block, blocks, tokens, tiles = 4, 2, 128, 16, 400, 500, 8
+    pools = [kv8.Kv8Pool.allocate(2, blocks, block, kv, dim, DEV) for _ in range(2)]
+    seed = torch.from_numpy(rng.integers(0, 120, size=pools[0].codes.shape).astype(np.uint8)).to(DEV)
+    for p in pools:
+        p.codes.view(torch.uint8).copy_(seed)
+        p.scales.fill_(120)
+    cos, sin = (dev(x) for x in helpers.rope_tables(dim, 2000))
+    q, k, v = (helpers.values(rng, "bf16", tokens, n, dim).to(DEV) for n in (heads, kv, kv))
+    fixed = rng.permutation(blocks).astype(np.int32)
+    past, lens = dev([0, 0, 0], torch.int32), dev([1, 1, 1], torch.int32)
+    free = dev(fixed[300:])
+    start = np.full((3, 125), -1, np.int32)
+    start[:, :100] = fixed[:300].reshape(3, 100)
+    ws = torch.empty(kv8.prefill_workspace_bytes(tiles, 3, heads, dim), dtype=torch.uint8, device=DEV)
+
+    def step(pool, table, plan, q_rot, out):
+        kv8.batch_layout_raw(past, lens, table, None, free, block, plan)
+        kv8.write_raw(q, k, v, q_rot, pool, 1, plan.rows, plan.positions, cos, sin, 1, None, None)
+        kv8.prefill_attention_raw(q_rot, pool, 1, table, dev_rows, plan.cu_q, past, plan.tile_seq, plan.tile_q0, out,
+                                  0.09, 3, ws)
+
+    dev_rows = dev([0, 1, 2], torch.int32)
+    sides = [(p, dev(start), kv8.BatchLayout.allocate(3, tokens, tiles, DEV), torch.empty_like(q), torch.empty_like(q))
+             for p in pools]
+    step(*sides[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step(*sides[0])
+    pools[0].codes.view(torch.uint8).copy_(seed)
+    pools[0].scales.fill_(120)
+    for p, n in (([0, 1500, 31], [300, 1, 130]), ([16, 0, 1599], [0, 257, 200]), ([700, 700, 700], [0, 0, 0])):
+        past.copy_(dev(p, torch.int32))
+        lens.copy_(dev(n, torch.int32))
+        for side in sides:
+            side[1].copy_(dev(start))
+            side[3].fill_(5.0)
+            side[4].fill_(5.0)
+        graph.replay()
+        step(*sides[1])
+        torch.cuda.synchronize()
+        total = sum(n)
+        for a, b in zip(*sides):
+            if isinstance(a, torch.Tensor):
+                assert torch.equal(a, b)
+        for name in ("cu_q", "positions", "rows", "tile_seq", "tile_q0", "counts"):
+            assert torch.equal(getattr(sides[0][2], name), getattr(sides[1][2], name))
+        assert sides[0][2].counts.tolist()[0] == total and sides[0][2].counts.tolist()[3] == 0
+        assert torch.equal(pools[0].codes.view(torch.uint8), pools[1].codes.view(torch.uint8))
+        assert torch.equal(pools[0].scales, pools[1].scales)
+        for t in sides[0][3:]:
+            assert (t[total:] == 5.0).all() and torch.isfinite(t[:total]).all()
+
+
+def test_blocks_past_4_gib_give_the_same_bits() -> None:
+    """Write, prefill and decode through blocks whose codes lie past 2^32 bytes, against the same in a small pool."""
+    rng = np.random.default_rng(64)
+    heads, kv, dim, block, few, many = 16, 16, 128, 16, 130, 70_000
+    lens, width = [1100, 700], 70
+    assert (2 * many - 1) * kv * 16 * dim > 2 ** 32
+    small = rng.permutation(few)[:sum(-(-(n + 1) // block) for n in lens)]
+    q, k, v = (helpers.values(rng, "bf16", sum(lens) + 2, n, dim).to(DEV) for n in (heads, kv, kv))
+    cos, sin = (dev(x) for x in helpers.rope_tables(dim, 1200))
+    results = []
+    for blocks, ids in ((few, small), (many, many - 1 - small)):
+        pool = kv8.Kv8Pool.allocate(1, blocks, block, kv, dim, DEV)
+        table = np.full((2, width), -1, np.int32)
+        table[0, :69], table[1, :44] = ids[:69], ids[69:113]
+        pos = np.concatenate([np.arange(n) for n in lens])
+        rows = np.concatenate([helpers.slots(table[s], np.arange(n), block) for s, n in enumerate(lens)])
+        q_rot, out = torch.empty_like(q[:-2]), torch.empty_like(q[:-2])
+        kv8.write_raw(q[:-2], k[:-2], v[:-2], q_rot, pool, 0, dev(rows, torch.int64), dev(pos, torch.int32), cos, sin, 1,
+                      None, None)
+        seq, q0 = ops.prefill_tiles(np.array(lens), np.zeros(2, np.int64))
+        kv8.prefill_attention_raw(q_rot, pool, 0, dev(table), dev([0, 1], torch.int32),
+                                  dev([0, lens[0], sum(lens)], torch.int32), dev([0, 0], torch.int32), dev(seq), dev(q0),
+                                  out, 0.09)
+        ws = torch.empty(kv8.decode_workspace_bytes(2, heads, kv, dim, 1200), dtype=torch.uint8, device=DEV)
+        step = kv8.decode_attention_raw(q[-2:], k[-2:], v[-2:], pool, None, 0, dev(table), None, dev(lens, torch.int32),
+                                        cos, sin, 1, None, None, torch.empty_like(q[-2:]), ws, 0.09)
+        at = torch.from_numpy(ids.astype(np.int64)).to(DEV)
+        results.append((out, step, pool.codes.view(torch.uint8)[:, :, at], pool.scales[:, :, at]))
+        del pool
+    assert all(torch.equal(a, b) for a, b in zip(*results))
+    assert torch.isfinite(results[0][0]).all() and torch.isfinite(results[0][1]).all()
