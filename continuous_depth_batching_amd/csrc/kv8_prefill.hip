@@ -142,7 +142,7 @@ constexpr float kSlack = 8.f;
 template <typename T, int D> constexpr int kPrefillWaves = sizeof(T) == 2 && D <= 96 ? 3 : 2;
 
 template <typename T, int D>
-__global__ void __launch_bounds__(256, kPrefillWaves<T, D>) kv8_prefill_kernel(Kv8PrefillParams P) {
+__global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel(Kv8PrefillParams P) {
   using Regs = BlockRegs<D>;
   constexpr int kPParts = sizeof(T) == 4 ? 2 : 1;
   constexpr int kTiles = D / 32;

@@ -855,12 +855,12 @@ def test_blocks_past_4_gib_give_the_same_bits() -> None:
         pos = np.concatenate([np.arange(n) for n in lens])
         rows = np.concatenate([helpers.slots(table[s], np.arange(n), block) for s, n in enumerate(lens)])
         q_rot, out = torch.empty_like(q[:-2]), torch.empty_like(q[:-2])
-        kv8.write_raw(q[:-2], k[:-2], v[:-2], q_rot, pool, 0, dev(rows, torch.int64), dev(pos, torch.int32), cos, sin, 1,
-                      None, None)
+        kv8.write_raw(q[:-2], k[:-2], v[:-2], q_rot, pool, 0, dev(rows, torch.int64), dev(pos, torch.int32), cos, sin,
+                      1, None, None)
         seq, q0 = ops.prefill_tiles(np.array(lens), np.zeros(2, np.int64))
         kv8.prefill_attention_raw(q_rot, pool, 0, dev(table), dev([0, 1], torch.int32),
-                                  dev([0, lens[0], sum(lens)], torch.int32), dev([0, 0], torch.int32), dev(seq), dev(q0),
-                                  out, 0.09)
+                                  dev([0, lens[0], sum(lens)], torch.int32), dev([0, 0], torch.int32), dev(seq),
+                                  dev(q0), out, 0.09)
         ws = torch.empty(kv8.decode_workspace_bytes(2, heads, kv, dim, 1200), dtype=torch.uint8, device=DEV)
         step = kv8.decode_attention_raw(q[-2:], k[-2:], v[-2:], pool, None, 0, dev(table), None, dev(lens, torch.int32),
                                         cos, sin, 1, None, None, torch.empty_like(q[-2:]), ws, 0.09)
