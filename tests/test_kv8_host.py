@@ -2,6 +2,7 @@
 
 from __future__ import annotations
 
+import dataclasses
 import ctypes
 
 import numpy as np
@@ -317,3 +318,36 @@ def test_python_prefill_and_layout_checks() -> None:
             kv8.batch_layout_raw(*args, free, 16, a)
     with pytest.raises(TypeError):
         kv8.batch_layout_raw(pos, pos, tables.long(), None, free, 16, a)
+
+
+@pytest.mark.parametrize("seqs,tokens,tiles", [(3, 8, 4), (0, 0, 0), (1, 7, 1), (4000, 1, 0)])
+def test_a_layouts_buffers_are_where_its_tensors_say(seqs, tokens, tiles) -> None:
+    a = kv8.BatchLayout.allocate(seqs, tokens, tiles, "cpu")
+    parts = (a.cu_q, a.positions, a.rows, a.tile_seq, a.tile_q0, a.counts)
+    assert [t.numel() for t in parts] == [seqs + 1, tokens, tokens, tiles, tiles, 4]
+    assert a.rows.dtype is torch.int64 and all(t.dtype is torch.int32 for t in parts if t is not a.rows)
+    b = kv8.BatchLayout(*parts)
+    assert a._num_seqs == b._num_seqs == seqs
+
+    def pointers(x):  # an empty tensor's is null
+        p = x._args
+        return (p[0], p[1] if tokens else 0, p[2] if tokens else 0, p[3], p[4] if tiles else 0, p[5] if tiles else 0,
+                p[6], p[7])
+
+    assert pointers(a) == pointers(b)
+
+
+def test_layout_refuses_buffers_that_do_not_fit() -> None:
+    a = kv8.BatchLayout.allocate(3, 8, 4, "cpu")
+    for bad in (dict(rows=a.positions), dict(positions=a.rows), dict(counts=a.counts.long())):
+        with pytest.raises(TypeError):
+            dataclasses.replace(a, **bad)
+    wide = torch.zeros(16, dtype=torch.int32)
+    for bad in (dict(rows=a.rows[:7]), dict(positions=a.positions[:7]), dict(tile_q0=a.tile_q0[:3]),
+                dict(counts=a.counts[:3]), dict(positions=wide[::2]), dict(tile_seq=wide[::4]),
+                dict(cu_q=torch.zeros(0, dtype=torch.int32)), dict(cu_q=torch.zeros(4, dtype=torch.int32, device="meta"))):
+        with pytest.raises(ValueError):
+            dataclasses.replace(a, **bad)
+    with pytest.raises(ValueError, match="3 requests"):
+        pos = torch.zeros(2, dtype=torch.int32)
+        kv8.batch_layout_raw(pos, pos, torch.zeros(2, 2, dtype=torch.int32), None, pos, 16, a)
