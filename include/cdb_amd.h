@@ -421,9 +421,10 @@ int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int3
  * cdb_paged_decode_attention, with its rows, positions (seqlens), per-row cache layers, block table, biases and
  * padding rows. Row b's new key and value are coded into its cache first, and it attends over the codes of
  * positions 0..seqlens[b], its own included. Rows whose position, table row or cache layer is out of range get a
- * NaN output and no write, and so does a row whose blocks in use are not all inside the pool. num_heads is a
- * multiple of num_kv_heads. Two rows of a call never append to the same tile. A row's context is cut into
- * chunks of 1024 tokens, merged in order, so its output does not depend on the other rows. */
+ * NaN output and no write; a row with a block in use outside the pool gets NaN, and writes its token where the
+ * token's own block is inside. num_heads is a multiple of num_kv_heads. Two rows of a call never append to the same
+ * tile, and none reads a tile that another appends to. A row's context is cut into chunks of 1024 tokens, merged in
+ * order, so its output does not depend on the other rows. */
 int cdb_kv8_decode_attention(const void* q, const void* k_new, const void* v_new, void* codes, void* scales,
                              int32_t num_cache_layers, int64_t pool_blocks, const int32_t* cache_layer,
                              int32_t cache_layer0, const int32_t* block_table, const int32_t* table_row,

@@ -2,8 +2,8 @@
 
 from __future__ import annotations
 
-import dataclasses
 import ctypes
+import dataclasses
 
 import numpy as np
 import pytest
@@ -345,7 +345,8 @@ def test_layout_refuses_buffers_that_do_not_fit() -> None:
     wide = torch.zeros(16, dtype=torch.int32)
     for bad in (dict(rows=a.rows[:7]), dict(positions=a.positions[:7]), dict(tile_q0=a.tile_q0[:3]),
                 dict(counts=a.counts[:3]), dict(positions=wide[::2]), dict(tile_seq=wide[::4]),
-                dict(cu_q=torch.zeros(0, dtype=torch.int32)), dict(cu_q=torch.zeros(4, dtype=torch.int32, device="meta"))):
+                dict(cu_q=torch.zeros(0, dtype=torch.int32)),
+                dict(cu_q=torch.zeros(4, dtype=torch.int32, device="meta"))):
         with pytest.raises(ValueError):
             dataclasses.replace(a, **bad)
     with pytest.raises(ValueError, match="3 requests"):
