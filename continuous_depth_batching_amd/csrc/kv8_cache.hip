@@ -32,6 +32,12 @@ template <int D> struct ValuePieces {
   static CDB_DEVICE int element(int j, int r) { return j == 0 ? kMost * r : 64 + 2 * r; }
 };
 
+// Whether keys and values are read past the caches. That pays for prompts with bf16 heads of 128, whole lines of 256
+// bytes (7700 tokens of 16 heads: 39.0 us against 41.7), and costs elsewhere (bf16 heads of 96: 117 against 111; fp32
+// heads of 128: 70 against 62, of 64: 41 against 36). Over 1024 single tokens, which a wave of such heads reads over
+// and over, take 97 us against 82 for 1500; a choice at run time took the registers of a third wave a SIMD (42.6).
+template <typename T, int D> constexpr bool kHeadOnce = sizeof(T) == 2 && D == 128;
+
 // The angles of a lane's units of a key: kept while the wave goes through its heads.
 template <int D, int STYLE> struct KeyAngles {
   static constexpr int kUnits = D / 16, kParts = (kUnits + 3) / 4;
@@ -52,7 +58,7 @@ template <int D, int STYLE> struct KeyAngles {
   template <typename T>
   CDB_DEVICE void key(const T* head, const T* bias, int g, bool vec, float x[kParts][16]) const {
     auto unit = [&](int u, float* to) __attribute__((always_inline)) {
-      load_f32<T, 16>(head + 16 * u, to, vec);
+      load_f32<T, 16, kHeadOnce<T, D>>(head + 16 * u, to, vec);
       if (bias != nullptr) {
         float b[16];
         load_f32<T, 16>(bias + 16 * u, b, vec);
@@ -133,7 +139,7 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, i
   for (int i = 0; i < 4; ++i) {
     const int slot = 4 * g + i - off;
     const T* src = v + (base + s + (slot >= 0 && slot < n ? slot : 0)) * P.kv_stride;
-    y0[i] = load_raw<T, V::kMost>(src + V::element(0, r), P.vec);
+    y0[i] = load_raw<T, V::kMost, kHeadOnce<T, D>>(src + V::element(0, r), P.vec);
     if constexpr (V::kPieces == 2) y1[i] = load_raw<T, 2>(src + V::element(1, r), P.vec);
   }
 
@@ -241,7 +247,7 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, i
 }
 
 // The rotated queries, and the keys and values as codes, bound by HBM bytes: 7700 tokens of 16 heads x 128 in
-// 41.8 us (158 MB, 3.8 TB/s), the queries alone 15 us. 61 single tokens take 5.1 us, two dependent loads and a store.
+// 39.0 us (158 MB, 4.0 TB/s), the queries alone 15 us. 61 single tokens take 5.1 us, two dependent loads and a store.
 template <typename T, int D, int STYLE>
 __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteParams P) {
   const int lane = threadIdx.x & 63;
@@ -571,8 +577,9 @@ extern "C" int cdb_kv8_write(const void* q, const void* k, const void* v, void* 
   // batch, whose every token is a run of its own, is not written 16 runs one after the other.
   P.chunk = tokens <= 1024 ? 1 : 16;
   P.chunks = (tokens + P.chunk - 1) / P.chunk;
-  // Two heads a wave share the angles, which are twice a bf16 head's bytes: 7700 tokens of 16 x 128 41.8 us
-  // against 44.1 with one. In fp32 they are not, and the larger waves cost more: 2300 of 55 x 96 37.6 against 35.1.
+  // Two heads a wave share the angles, which are twice a bf16 head's bytes: 7700 tokens of 16 x 128 take 41.8 us
+  // against 44.1 with one (both before keys and values were read past the caches). In fp32 they are not, and the
+  // larger waves cost more: 2300 of 55 x 96 37.6 against 35.1.
   P.heads_each = tokens <= 1024 || size == 4 ? 1 : 2;
   P.kv_blocks = (P.chunks * ((num_kv_heads + P.heads_each - 1) / P.heads_each) + 3) / 4;
   const int64_t q_blocks = (tokens * num_heads * (head_dim / 16) + 255) / 256;

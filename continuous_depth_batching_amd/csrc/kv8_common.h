@@ -80,11 +80,12 @@ CDB_DEVICE float shrink_of(int old, int now) { return scale_of((uint32_t)max(127
 // Byte mask of a word's tokens below n (n <= 0: none, n >= 4: all).
 CDB_DEVICE uint32_t tokens_below(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
-// N storage elements as they lie; vec as for load_f32.
-template <typename T, int N> CDB_DEVICE Vec<T, N> load_raw(const T* p, bool vec) {
+// N storage elements as they lie; vec as for load_f32, kOnce: they are read once and need no place in the caches.
+template <typename T, int N, bool kOnce = false> CDB_DEVICE Vec<T, N> load_raw(const T* p, bool vec) {
   Vec<T, N> x;
   if (vec) {
-    x.load(p);
+    if constexpr (kOnce) x.load_nt(p);
+    else x.load(p);
   } else {
 #pragma unroll
     for (int i = 0; i < N; i += 2) x.set_pair(i, Elem<T>::load(p + i), Elem<T>::load(p + i + 1));
@@ -93,10 +94,11 @@ template <typename T, int N> CDB_DEVICE Vec<T, N> load_raw(const T* p, bool vec)
 }
 
 // N storage elements as fp32; vec: p is aligned for 16-byte loads (8-byte ones where N elements are 8 bytes).
-template <typename T, int N> CDB_DEVICE void load_f32(const T* p, float* out, bool vec) {
+template <typename T, int N, bool kOnce = false> CDB_DEVICE void load_f32(const T* p, float* out, bool vec) {
   if (vec) {
     Vec<T, N> x;
-    x.load(p);
+    if constexpr (kOnce) x.load_nt(p);
+    else x.load(p);
 #pragma unroll
     for (int i = 0; i < N; ++i) out[i] = x.get(i);
   } else {
