@@ -300,6 +300,12 @@ def test_decode_long_context_and_short_workspace() -> None:
         DecodeCase(15, "bf16", 2, 1, 64, 1, False, 16, [5000, 100, 4097], longest=longest, nan=True).check()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_decode_context_of_more_chunks_than_a_row_has(dtype) -> None:
+    """Past 64 chunks of 1024 tokens a row takes longer ones, with a workspace of any size."""
+    DecodeCase(18, dtype, 2, 1, 64, 1, False, 64, [70_000, 3, 65_537], layers=1).check()
+
+
 def test_decode_marks_rows_out_of_range() -> None:
     c = DecodeCase(16, "bf16", 2, 2, 64, 1, False, 16, [20, 300, 40, 50, 60, 300, 33], by_row=True)
     c.table[c.table_row[1], 3] = c.pool.num_blocks     # a block past the pool inside the context
