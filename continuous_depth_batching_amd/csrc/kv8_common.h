@@ -218,6 +218,22 @@ CDB_DEVICE bf16x8_t widen_bf16(uint32_t w0, float s0, uint32_t w1, float s1) {
   return u.v;
 }
 
+// 8 codes (two words) widened to fp16 by powers of two.
+CDB_DEVICE f16x8_t widen_f16(uint32_t w0, float s0, uint32_t w1, float s1) {
+  union { f16x2_t p[4]; f16x8_t v; } u;
+  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s0, false);
+  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s0, true);
+  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s1, false);
+  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s1, true);
+  return u.v;
+}
+
+// fp32 models take probabilities as two fp16 parts. The second, what the first leaves, is raised by 2^11 and meets
+// values lowered by as much: it is then as large as the first, as far above fp16's smallest step. Values are raised by
+// 2^7 (448 * 2^7 is within fp16), which keeps the lowered ones exact down to scales of 2^-11 of the largest.
+constexpr float kSecondRaise = 2048.f;
+template <typename T> constexpr int kValueRaise = sizeof(T) == 4 ? 7 : 0;
+
 // The cache as a kernel sees it: all strides in tiles.
 struct Kv8Cache {
   uint8_t* codes;

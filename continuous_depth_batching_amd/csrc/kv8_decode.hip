@@ -8,8 +8,10 @@
 //   as the operand's: a key costs no vector instruction. The query is taken as 3 e4m3 parts, each 16
 //   times finer than the one before; what they leave of it is 2^-13.8 of the head's largest element.
 //   fp32 models take 3 bf16 parts, 2^-24, and widen the codes to bf16, which is exact.
-//   O^T = V^T P^T runs in fp16, which holds a code exactly and P to 2^-11 (fp32 models: two parts,
-//   2^-22): codes widen with their scale, relative to the largest scale met, one instruction a pair.
+//   O^T = V^T P^T runs in fp16, which holds a code exactly and P to 2^-11: it is raised by 2^15, so that
+//   keys down to 2^-29 of the row's largest keep that, and none is off by more than 2^-40 of it. fp32 models
+//   take P as 2 fp16 parts (2^-23, and 2^-51 of the largest). Codes widen with their scale, relative to the largest scale
+//   met, one instruction a pair.
 //   Both products are 16 query heads wide (columns without a head repeat the last). A lane's four scores
 //   are those of the four tokens it holds of V, so P never moves.
 //
@@ -236,7 +238,10 @@ template <int D> struct QueryRegs<D, true> {
 // One wave's share of a chunk: a running maximum and sum (of the lane's query head r, over its own
 // tokens), and O^T with element rows and head columns, counted in units of 2^(ref - 127).
 template <int D, bool kWide> struct Attention {
-  static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1;
+  static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1, kUp = kWide ? kValueRaise<float> : 0;
+  // Probabilities are counted in units of 2^-15, the largest then being 2^15, within fp16: its smallest step, 2^-24,
+  // stands for 2^-39.
+  static constexpr int kRaise = 15;
   float top, sum;
   int ref;
   f32x4_t acc[kTiles];
@@ -261,7 +266,7 @@ template <int D, bool kWide> struct Attention {
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) acc[m] *= f;
   }
-  // Probabilities of two tiles' scores, as fp16 parts in the order of the value products' tokens.
+  // Probabilities of two tiles' scores, in the order of the value products' tokens.
   CDB_DEVICE void softmax(const f32x4_t* s, f16x8_t* parts) {
     float most = top;
 #pragma unroll
@@ -273,24 +278,25 @@ template <int D, bool kWide> struct Attention {
       scale_acc(keep);
       top = most;
     }
-    float left[8];
+    const float lowered = top - (float)kRaise;
+    float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      left[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - top);
-      sum += left[i];
+      p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - lowered);
+      sum += p[i];
     }
 #pragma unroll
-    for (int p = 0; p < kPParts; ++p)
-#pragma unroll
-      for (int i = 0; i < 8; i += 2) {
-        const f16x2_t y = __builtin_convertvector((f32x2_t){left[i], left[i + 1]}, f16x2_t);
-        parts[p][i] = y[0];
-        parts[p][i + 1] = y[1];
-        if (p + 1 < kPParts) {
-          left[i] -= (float)y[0];
-          left[i + 1] -= (float)y[1];
-        }
+    for (int i = 0; i < 8; i += 2) {
+      const f16x2_t y = __builtin_convertvector((f32x2_t){p[i], p[i + 1]}, f16x2_t);
+      parts[0][i] = y[0];
+      parts[0][i + 1] = y[1];
+      if constexpr (kWide) {
+        const f16x2_t z = __builtin_convertvector(
+            (f32x2_t){(p[i] - (float)y[0]) * kSecondRaise, (p[i + 1] - (float)y[1]) * kSecondRaise}, f16x2_t);
+        parts[kPParts - 1][i] = z[0];
+        parts[kPParts - 1][i + 1] = z[1];
       }
+    }
   }
   CDB_DEVICE void values(const ValueRegs<D>& v0, const ValueRegs<D>& v1, int e0, int e1, const f16x8_t* parts) {
     const int now = max(max(e0, e1), ref);
@@ -298,17 +304,14 @@ template <int D, bool kWide> struct Attention {
       scale_acc(shrink_of(ref, now));
       ref = now;
     }
-    const float s0 = shrink_of(e0, ref), s1 = shrink_of(e1, ref);
+    const float s0 = shrink_of(e0 + kUp, ref), s1 = shrink_of(e1 + kUp, ref);
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
-      union { f16x2_t h[4]; f16x8_t x; } v;
-      v.h[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v0.w[m], s0, false);
-      v.h[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v0.w[m], s0, true);
-      v.h[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v1.w[m], s1, false);
-      v.h[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(v1.w[m], s1, true);
-#pragma unroll
-      for (int p = kPParts - 1; p >= 0; --p)
-        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v.x, parts[p], acc[m], 0, 0, 0);
+      if constexpr (kWide) {
+        const f16x8_t v = widen_f16(v0.w[m], s0 / kSecondRaise, v1.w[m], s1 / kSecondRaise);
+        acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(v, parts[kPParts - 1], acc[m], 0, 0, 0);
+      }
+      acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_f16(widen_f16(v0.w[m], s0, v1.w[m], s1), parts[0], acc[m], 0, 0, 0);
     }
   }
 };
@@ -567,17 +570,17 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
     }
 
     // Join the waves: [wave][column][D + 2] holds O, the maximum and the sum.
-    float sum = column_sum(state.sum);
+    float sum = ldexpf(column_sum(state.sum), -state.kRaise);
     if (missing) sum = NAN;
     if (r < cols) {
       float* mine = join + (wave * cols + r) * kJoin;
-      const float back = scale_of(state.ref);
+      const int back = state.ref - 127 - state.kUp - state.kRaise;
 #pragma unroll
       for (int m = 0; m < D / 16; m += 2)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
           *reinterpret_cast<f32x2_t*>(mine + ValueRegs<D>::element(m, 4 * g + i)) =
-              (f32x2_t){state.acc[m][i] * back, state.acc[m + 1][i] * back};
+              (f32x2_t){ldexpf(state.acc[m][i], back), ldexpf(state.acc[m + 1][i], back)};
       if (g == 0) {
         mine[D] = state.top;
         mine[D + 1] = sum;

@@ -2,11 +2,13 @@
 //
 // One workgroup of 4 waves takes 128 query tokens of a sequence and one query head, a wave 32 of them, and walks
 // the keys in blocks of 32, two tiles, with a running maximum and sum (the maximum moves only when a score outgrows
-// it by 2^8). Codes go from memory to registers; each wave loads the next block's keys and values as soon as this
+// it by 2^6). Codes go from memory to registers; each wave loads the next block's keys and values as soon as this
 // block's are used up, so nothing waits on LDS or on another wave.
 //   S^T = K Q^T in bf16: a code times a power of two is exact there, so scores are the products' fp32 sums.
-//   O^T = V^T P^T in fp16, which holds a code exactly and P to 2^-11; values widen with their scale relative to the
-//   largest met. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-22).
+//   O^T = V^T P^T in fp16, which holds a code exactly and P to 2^-11: it is raised by 2^9, so that keys down to 2^-23
+//   of the query's largest keep that, and none is off by more than 2^-34 of it. Values widen with their scale relative
+//   to the largest met. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-23, and 2^-45 of the
+//   largest).
 // A lane's 16 scores are those of the 16 tokens whose values it holds, so P never moves; queries are the columns of
 // both products, so maximum and sum are a lane's own and its neighbour's, 32 lanes away.
 //
@@ -120,22 +122,13 @@ template <typename T, int D> struct BlockQuery {
   }
 };
 
-// Eight codes (two words) as fp16, scaled by a power of two.
-CDB_DEVICE f16x8_t widen_f16(uint32_t w0, uint32_t w1, float s) {
-  union { f16x2_t p[4]; f16x8_t v; } u;
-  u.p[0] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s, false);
-  u.p[1] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w0, s, true);
-  u.p[2] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s, false);
-  u.p[3] = __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w1, s, true);
-  return u.v;
-}
-
 // 0x80 in each byte of w that holds the NaN code.
 CDB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// How far scores may outgrow the maximum that the sums are counted from before they are counted anew: P stays
-// below 2^8, far inside fp16, and most blocks move nothing.
-constexpr float kSlack = 8.f;
+// How far scores may outgrow the maximum that the sums are counted from before they are counted anew, and what
+// probabilities are raised by: 2^15 is then the largest, within fp16, and its smallest step, 2^-24, stands for 2^-33.
+// Less slack moves more blocks (two sequences of 6000..8190 tokens: 908 us with 4, 900 with 6, 898 with 8).
+constexpr float kSlack = 6.f, kRaise = 9.f;
 
 // Waves a SIMD: three where the registers allow it without spills (5000 tokens of 55 heads x 96, 360 us against 380);
 // for bf16 heads of 128 they would spill 27, and take 904 and 125 us for 900 and 113.
@@ -144,7 +137,8 @@ template <typename T, int D> constexpr int kPrefillWaves = sizeof(T) == 2 && D <
 template <typename T, int D>
 __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel(Kv8PrefillParams P) {
   using Regs = BlockRegs<D>;
-  constexpr int kPParts = sizeof(T) == 4 ? 2 : 1;
+  constexpr bool kWide = sizeof(T) == 4;
+  constexpr int kPParts = kWide ? 2 : 1;
   constexpr int kTiles = D / 32;
   const int lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -178,8 +172,8 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
   for (int i = 0; i < kTiles; ++i)
 #pragma unroll
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
-  // Scores are counted, in units of log2, from `base`, anew once they pass `limit`.
-  float base = 0.f, limit = -INFINITY, sum = 0.f;
+  // Scores are counted, in units of log2, from -`shift`, anew once they pass `limit`.
+  float shift = 0.f, limit = -INFINITY, sum = 0.f;
   int ref = 1;  // biased exponent that the accumulators are counted in
   bool missing = bad;
   const int32_t* table = P.block_table + (int64_t)(bad ? 0 : trow) * P.table_width;
@@ -242,15 +236,16 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
       if (__any(most * P.scale_log2 > limit)) {
         most = half_max(most) * P.scale_log2;
         const bool more = most > limit;
-        const float keep = more && limit != -INFINITY ? __builtin_amdgcn_exp2f(base - most) : 1.f;
+        const float moved = kRaise - most;
+        const float keep = more && limit != -INFINITY ? __builtin_amdgcn_exp2f(moved - shift) : 1.f;
         sum *= keep;  // the first count finds zeros
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) acc[m] *= keep;
-        base = more ? most : base;
+        shift = more ? moved : shift;
         limit = more ? most + kSlack : limit;
       }
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, -base));
+      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, shift));
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int t = key0 + kTile * a;
@@ -261,21 +256,25 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
           for (int m = 0; m < kTiles; ++m) acc[m] *= f;
           ref = v_exp;
         }
-        const float v_scale = shrink_of(v_exp, ref);
+        const float v_scale = shrink_of(v_exp + kValueRaise<T>, ref);
         f16x8_t pp[kPParts];
 #pragma unroll
-        for (int p = 0; p < kPParts; ++p)
-#pragma unroll
-          for (int e = 0; e < 8; e += 2) {
-            const f16x2_t y = __builtin_convertvector((f32x2_t){sc[8 * a + e], sc[8 * a + e + 1]}, f16x2_t);
-            pp[p][e] = y[0];
-            pp[p][e + 1] = y[1];
+        for (int e = 0; e < 8; e += 2) {
+          const f32x2_t x2 = {sc[8 * a + e], sc[8 * a + e + 1]};
+          const f16x2_t y = __builtin_convertvector(x2, f16x2_t);
+          pp[0][e] = y[0];
+          pp[0][e + 1] = y[1];
+          if constexpr (kWide) {
+            sum += x2[0];
+            sum += x2[1];
+            const f16x2_t z = __builtin_convertvector(
+                (f32x2_t){(x2[0] - (float)y[0]) * kSecondRaise, (x2[1] - (float)y[1]) * kSecondRaise}, f16x2_t);
+            pp[kPParts - 1][e] = z[0];
+            pp[kPParts - 1][e + 1] = z[1];
+          } else {
             sum = __builtin_amdgcn_fdot2(y, (f16x2_t){(_Float16)1.f, (_Float16)1.f}, sum, false);
-            if (p + 1 < kPParts) {
-              sc[8 * a + e] -= (float)y[0];
-              sc[8 * a + e + 1] -= (float)y[1];
-            }
           }
+        }
         if (diagonal) {
           // A value counts only for the queries that see its token: codes behind the sequence are taken out,
           // and so are NaN codes, which a probability of zero would not keep from the other queries; those that
@@ -306,7 +305,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
               f32x16_t met;
 #pragma unroll
               for (int e = 0; e < 16; ++e) met[e] = 0.f;
-              met = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen_f16(where_nan[0], where_nan[1], 1.f), seen, met, 0, 0,
+              met = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen_f16(where_nan[0], 1.f, where_nan[1], 1.f), seen, met, 0, 0,
                                                            0);
 #pragma unroll
               for (int e = 0; e < 16; ++e) acc[m][e] = met[e] != 0.f ? NAN : acc[m][e];
@@ -315,10 +314,13 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
         }
 #pragma unroll
         for (int m = 0; m < kTiles; ++m) {
-          const f16x8_t v = widen_f16(x.v[a][0][m], x.v[a][1][m], v_scale);
-#pragma unroll
-          for (int p = kPParts - 1; p >= 0; --p)
-            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pp[p], acc[m], 0, 0, 0);
+          if constexpr (kWide) {
+            const float s2 = v_scale / kSecondRaise;
+            const f16x8_t v2 = widen_f16(x.v[a][0][m], s2, x.v[a][1][m], s2);
+            acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v2, pp[kPParts - 1], acc[m], 0, 0, 0);
+          }
+          const f16x8_t v = widen_f16(x.v[a][0][m], v_scale, x.v[a][1][m], v_scale);
+          acc[m] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pp[0], acc[m], 0, 0, 0);
         }
       }
       __builtin_amdgcn_sched_barrier(0);
@@ -328,18 +330,17 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
   }
 
   sum += shfl_xor_f32(sum, 32);
-  const float top = sum == 0.f ? -INFINITY : base;  // a query that has seen no key
+  const float top = sum == 0.f ? -INFINITY : -shift;  // a query that has seen no key
   if (missing) sum = NAN;
-  const float back = scale_of(ref);
   if (query >= num) return;
   if (P.splits == 1) {
     T* out = static_cast<T*>(P.out) + ((token0 + query) * P.num_heads + head) * D;
-    const float inv = back / sum;
+    const float inv = 1.f / sum;
 #pragma unroll
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)), acc[m][e] * inv);
+        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)), ldexpf(acc[m][e] * inv, ref - 127 - kValueRaise<T>));
     return;
   }
   float* to_part = P.partials +
@@ -347,10 +348,11 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
 #pragma unroll
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
-    for (int e = 0; e < 16; ++e) to_part[Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3))] = acc[m][e] * back;
+    for (int e = 0; e < 16; ++e) to_part[Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3))] =
+        ldexpf(acc[m][e], ref - 127 - kValueRaise<T> - (int)kRaise);
   if (h == 0) {
     to_part[D] = top;
-    to_part[D + 1] = sum;
+    to_part[D + 1] = ldexpf(sum, -(int)kRaise);
   }
 }
 

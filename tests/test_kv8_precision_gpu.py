@@ -1,0 +1,145 @@
+"""The 8-bit attention kernels where single keys or tiles dwarf the rest, against the definition in 64 bits with
+bounds that the small ones' share alone has to meet."""
+
+from __future__ import annotations
+
+import numpy as np
+import pytest
+import torch
+
+from continuous_depth_batching_amd import kv8, ops
+from oracle import kv8 as oracle
+from tests import kv8_helpers as helpers
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+TINY = 2.0 ** -24  # half a step of fp32
+KINDS = ["decode", "prefill", "split"]
+
+
+def numerics(kind: str, dtype: str, dim: int, tokens: int) -> dict[str, float]:
+    """What a computation rounds, relative (``expect``).
+
+    Scores: dim products summed in fp32 for each part of the query, and a few roundings of scaling. A prefill query in
+    bf16 is its own single part; fp32 queries are three bf16 parts (2^-24 left of each element); a bf16 decode query
+    is 3 e4m3 parts, 2^-13.8 of the head's largest element, whose products keep some 2^-16 of their largest term.
+    Probabilities: an fp16 part leaves 2^-12 of them (2^-11 is counted) and half of fp16's smallest step, 2^-25. They
+    are raised by 2^15 in decode, whose largest probability is 1, and by 2^9 in prefill, where it may be 2^6. fp32
+    models take what is left as a second part that is 2^11 larger: 2^-23, and the step 2^-11 of the first's. The
+    exponential, its argument and the fp32 sums over tokens besides. The result: half a step of its type, divisions
+    and joins."""
+    wide = dtype == "f32"
+    if kind == "decode":
+        parts, left, top = (3, TINY, 0.0) if wide else (3, 0.0, 2.0 ** -13.8 + 3 * 2.0 ** -16)
+    else:
+        parts, left, top = (3, TINY, 0.0) if wide else (1, 0.0, 0.0)
+    return dict(round_off=(16 * TINY if wide else 2.0 ** -8 + 8 * TINY), score_off=(parts * dim + 8) * TINY + left,
+                top_off=top, prob_off=(2.0 ** -23 if wide else 2.0 ** -11) + (2 * tokens + 16) * TINY,
+                floor=(2.0 ** -40 if kind == "decode" else 2.0 ** -34) * (2.0 ** -11 if wide else 1.0))
+
+
+def expect(q, k, v, end, scale, round_off, score_off, top_off, prob_off, floor):
+    """Attention of q [n, H, D] over k, v [tokens, Hkv, D] in 64 bits, query i over keys 0..end[i], and the bound of
+    ``oracle.kv8.attend`` with each probability's floor counted for no more than the probability itself (a smaller
+    one is at worst left out)."""
+    out, bound = np.zeros(q.shape), np.zeros(q.shape)
+    group = q.shape[1] // k.shape[1]
+    for h in range(q.shape[1]):
+        kh, vh = k[:, h // group], v[:, h // group]
+        s = q[:, h] @ kh.T * scale
+        size = np.abs(q[:, h])
+        mass = (score_off * size + top_off * size.max(1, keepdims=True)) @ np.abs(kh).T * scale
+        for i in range(len(q)):
+            n = end[i] + 1
+            p = np.exp(s[i, :n] - s[i, :n].max())
+            p /= p.sum()
+            a = np.abs(vh[:n])
+            out[i, h] = p @ vh[:n]
+            grown = (1 + round_off) * np.expm1(2 * mass[i, :n].max() + prob_off)
+            bound[i, h] = round_off * np.abs(out[i, h]) + grown * (p @ a) + np.minimum(p, floor) @ a
+    return out, bound
+
+
+class Sequence:
+    """One sequence of n tokens of a kind's call: a decode step's last token, or a prefill chunk of the last ``new``.
+    ``keys`` and ``values`` [n, Hkv, D] are codes, ``k_exp`` and ``v_exp`` the exponents of its tiles."""
+
+    def __init__(self, kind, dtype, heads, kv, dim, keys, values, k_exp, v_exp, q, new=40):
+        n, tiles = keys.shape[0], -(-keys.shape[0] // 16)
+        rng = np.random.default_rng(3)
+        self.kind, self.dtype, self.dim, self.n = kind, dtype, dim, n
+        self.new = 1 if kind == "decode" else new
+        perm = rng.permutation(tiles + 1).astype(np.int32)
+        self.table = perm[None, :tiles].copy()
+        codes = np.zeros((1, 2, tiles + 1, kv, 16, dim))
+        exps = np.full((1, 2, tiles + 1, kv), -6)
+        at = helpers.slots(self.table[0], np.arange(n), 16)
+        for plane, (c, e) in enumerate(((keys, k_exp), (values, v_exp))):
+            codes[0, plane, at // 16, :, at % 16] = c
+            exps[0, plane, self.table[0]] = e[:, None]
+        self.cache = oracle.Cache(codes, exps)
+        scales = torch.from_numpy((exps + 127).astype(np.uint8))[:, :, :, None].transpose(3, 4).contiguous()
+        self.pool = kv8.Kv8Pool(helpers.pack(codes, 16).to(DEV), scales.to(DEV))
+        self.q = torch.from_numpy(q).to(helpers.TYPES[dtype]).to(DEV)
+        self.scale, self.at = dim ** -0.5, at
+
+    def run(self, k_new=None, v_new=None):
+        t = lambda a: torch.from_numpy(np.ascontiguousarray(a, dtype=np.int32)).to(DEV)
+        out = torch.empty_like(self.q)
+        heads, kv = self.q.shape[1], self.pool.num_kv_heads
+        if self.kind == "decode":
+            ws = torch.empty(kv8.decode_workspace_bytes(1, heads, kv, self.dim, self.n), dtype=torch.uint8, device=DEV)
+            self.cache.append(0, int(self.at[-1]), k_new.float().cpu().numpy(), v_new.float().cpu().numpy())
+            return kv8.decode_attention_raw(self.q, k_new, v_new, self.pool, None, 0, t(self.table), None,
+                                            t([self.n - 1]), None, None, 0, None, None, out, ws, self.scale)
+        past = self.n - self.new
+        seq, q0 = ops.prefill_tiles(np.array([self.new]), np.array([past]))
+        splits = 3 if self.kind == "split" else 1
+        ws = torch.empty(kv8.prefill_workspace_bytes(len(seq), splits, heads, self.dim), dtype=torch.uint8, device=DEV)
+        return kv8.prefill_attention_raw(self.q, self.pool, 0, t(self.table), t([0]), t([0, self.new]), t([past]),
+                                         t(seq), t(q0), out, self.scale, splits, ws)
+
+    def expect(self):
+        k, v = (self.cache.values(0, plane, self.at) for plane in (0, 1))
+        end = np.arange(self.n - self.new, self.n)
+        return expect(self.q.double().cpu().numpy(), k, v, end, self.scale,
+                      **numerics(self.kind, self.dtype, self.dim, self.n))
+
+    def new_token(self, rng, key=0.0):
+        """A decode step's key (all ``key`` in element 0) and value."""
+        kv = self.pool.num_kv_heads
+        k = torch.zeros(1, kv, self.dim)
+        k[..., 0] = key
+        v = helpers.values(rng, self.dtype, 1, kv, self.dim)
+        return k.to(self.q.dtype).to(DEV), v.to(DEV)
+
+    def check(self, rng, **token):
+        got = self.run(*self.new_token(rng, **token)) if self.kind == "decode" else self.run()
+        want, bound = self.expect()
+        helpers.close(got, want, bound)
+        # The bound says something: a result of zeros is four times past it. (Relative to sum(p |v|) it is some
+        # 2^-8; values of random signs leave sum(p v) up to sqrt(tokens) = 39 times smaller than that.)
+        assert (np.linalg.norm(bound, axis=-1) < np.linalg.norm(want, axis=-1) / 4).all()
+
+
+def line(rng, n, kv, dim, first):
+    """Codes of keys that score ``first`` (by their element 0 alone), and of values over most of their range."""
+    keys = np.zeros((n, kv, dim))
+    keys[:, :, 0] = oracle.round_e4m3(first)[:, None]
+    return keys, oracle.round_e4m3(np.clip(rng.standard_normal((n, kv, dim)) * 90, -448, 448))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 4, 2, 128), ("f32", 2, 2, 64), ("f32", 2, 1, 128),
+                                                ("bf16", 3, 3, 96), ("bf16", 2, 2, 64), ("f32", 1, 1, 96)])
+def test_keys_far_below_a_sink_keep_their_share(kind, dtype, heads, kv, dim) -> None:
+    """A first key that outscores all others by 2^27..2^21 and whose value is zero: what is left is theirs."""
+    rng = np.random.default_rng(71)
+    n = 1500
+    keys, values = line(rng, n, kv, dim, np.concatenate([[448.0], rng.uniform(0.0, 96.0, n - 1)]))
+    values[0] = 0.0
+    tiles = -(-n // 16)
+    k_exp, v_exp = np.full(tiles, -4), rng.integers(-7, -4, tiles)
+    q = np.zeros((1 if kind == "decode" else 40, heads, dim))
+    q[:, :, 0] = 27 * np.log(2.0) / 28 * dim ** 0.5  # the sink's key is 448 / 16
+    Sequence(kind, dtype, heads, kv, dim, keys, values, k_exp, v_exp, q).check(rng)
