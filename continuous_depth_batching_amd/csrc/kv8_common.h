@@ -74,9 +74,6 @@ CDB_DEVICE uint32_t recode(uint32_t w, float growth) {
 // 2^(now - old) for old <= now; where it leaves the normal range every code rounds to 0 all the same.
 CDB_DEVICE float growth_of(int old, int now) { return scale_of((uint32_t)min(127 + now - old, 254)); }
 
-// 2^(old - now) for old <= now, flushed to 2^-126 beyond the normal range.
-CDB_DEVICE float shrink_of(int old, int now) { return scale_of((uint32_t)max(127 + old - now, 1)); }
-
 // Byte mask of a word's tokens below n (n <= 0: none, n >= 4: all).
 CDB_DEVICE uint32_t tokens_below(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
@@ -230,9 +227,33 @@ CDB_DEVICE f16x8_t widen_f16(uint32_t w0, float s0, uint32_t w1, float s1) {
 
 // fp32 models take probabilities as two fp16 parts. The second, what the first leaves, is raised by 2^11 and meets
 // values lowered by as much: it is then as large as the first, as far above fp16's smallest step. Values are raised by
-// 2^7 (448 * 2^7 is within fp16), which keeps the lowered ones exact down to scales of 2^-11 of the largest.
+// 2^7 (448 * 2^7 is within fp16), which keeps the lowered ones exact down to scales 2^11 below the unit.
 constexpr float kSecondRaise = 2048.f;
 template <typename T> constexpr int kValueRaise = sizeof(T) == 4 ? 7 : 0;
+
+// The unit that values are widened in and products with them counted in: 2^(ref - 127). fp16 holds the values of a
+// tile exactly if its scale is at most the unit and no more than 2^kExact below it, so the unit moves where a tile's
+// is not, and the accumulators, fp32, move with it: up with a larger scale, and down for a smaller one, but never
+// more than 2^60 below the largest scale met, so that 2^30 products of 2^31 at most stay within fp32. Values that
+// are 2^(60 + kExact) and more below the largest met lose bits, and vanish 2^9 below that.
+template <typename T> struct ValueUnit {
+  static constexpr int kExact = sizeof(T) == 4 ? 11 : 15, kDeep = 60;
+  int ref = 1, met = 1;
+
+  // Whether a tile of this scale needs another unit.
+  CDB_DEVICE bool moves(int b) const { return (uint32_t)(ref - b) > (uint32_t)kExact; }
+  // Takes it; returns the power of two that the accumulators move by.
+  CDB_DEVICE int move(int b) {
+    met = max(met, b);
+    const int to = max(b, met - kDeep), by = ref - to;
+    ref = to;
+    return by;
+  }
+  // A scale in the unit, as the conversions take it.
+  CDB_DEVICE float scale(int b) const { return scale_of((uint32_t)max(127 + b + kValueRaise<T> - ref, 1)); }
+  // The exponent that brings an accumulator back.
+  CDB_DEVICE int back() const { return ref - 127 - kValueRaise<T>; }
+};
 
 // The cache as a kernel sees it: all strides in tiles.
 struct Kv8Cache {

@@ -10,8 +10,8 @@
 //   fp32 models take 3 bf16 parts, 2^-24, and widen the codes to bf16, which is exact.
 //   O^T = V^T P^T runs in fp16, which holds a code exactly and P to 2^-11: it is raised by 2^15, so that
 //   keys down to 2^-29 of the row's largest keep that, and none is off by more than 2^-40 of it. fp32 models
-//   take P as 2 fp16 parts (2^-23, and 2^-51 of the largest). Codes widen with their scale, relative to the largest scale
-//   met, one instruction a pair.
+//   take P as 2 fp16 parts (2^-23, and 2^-51 of the largest). Codes widen with their scale, in a unit that follows
+//   the tiles' scales, one instruction a pair.
 //   Both products are 16 query heads wide (columns without a head repeat the last). A lane's four scores
 //   are those of the four tokens it holds of V, so P never moves.
 //
@@ -21,6 +21,7 @@
 // tiles and query, 7 pairs a wave, the join. The same loads without arithmetic take 85 and 104 us.
 #include <atomic>
 #include <chrono>
+#include <type_traits>
 
 #include "cdb_amd.h"
 #include "kv8_common.h"
@@ -35,7 +36,8 @@ constexpr int kWaves = 4;
 constexpr int kChunk = 1024;
 constexpr int kMaxChunks = 64;           // of a row; longer contexts take longer chunks
 constexpr int kSkew = 2 * (kWaves - 1);  // pairs that the wave that appends leaves to the others first
-template <typename T> constexpr int kDecodeWaves = sizeof(T) == 4 ? 2 : 4;  // waves a SIMD, which the registers allow
+// Waves a SIMD, as many as the registers allow.
+template <typename T, int D> constexpr int kDecodeWaves = sizeof(T) == 4 ? (D == 64 ? 4 : 3) : (D == 64 ? 5 : 4);
 
 struct Kv8DecodeParams {
   const void *q, *k_new, *v_new;
@@ -236,20 +238,21 @@ template <int D> struct QueryRegs<D, true> {
 };
 
 // One wave's share of a chunk: a running maximum and sum (of the lane's query head r, over its own
-// tokens), and O^T with element rows and head columns, counted in units of 2^(ref - 127).
+// tokens), and O^T with element rows and head columns, in the values' unit.
 template <int D, bool kWide> struct Attention {
-  static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1, kUp = kWide ? kValueRaise<float> : 0;
+  static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1;
   // Probabilities are counted in units of 2^-15, the largest then being 2^15, within fp16: its smallest step, 2^-24,
   // stands for 2^-39.
   static constexpr int kRaise = 15;
+  using Unit = ValueUnit<std::conditional_t<kWide, float, bf16_t>>;
   float top, sum;
-  int ref;
+  Unit unit;
   f32x4_t acc[kTiles];
 
   CDB_DEVICE void start() {
     top = -INFINITY;
     sum = 0.f;
-    ref = 1;
+    unit = Unit();
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) acc[m] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
   }
@@ -265,6 +268,12 @@ template <int D, bool kWide> struct Attention {
   CDB_DEVICE void scale_acc(float f) {
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) acc[m] *= f;
+  }
+  CDB_DEVICE void move_acc(int by) {
+#pragma unroll
+    for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) acc[m][i] = ldexpf(acc[m][i], by);
   }
   // Probabilities of two tiles' scores, in the order of the value products' tokens.
   CDB_DEVICE void softmax(const f32x4_t* s, f16x8_t* parts) {
@@ -299,12 +308,20 @@ template <int D, bool kWide> struct Attention {
     }
   }
   CDB_DEVICE void values(const ValueRegs<D>& v0, const ValueRegs<D>& v1, int e0, int e1, const f16x8_t* parts) {
-    const int now = max(max(e0, e1), ref);
-    if (now > ref) {
-      scale_acc(shrink_of(ref, now));
-      ref = now;
+    if (abs(e0 - e1) > Unit::kExact) {
+      // No unit holds both tiles: the smaller one by itself first, the other one's values flushed.
+      const int low = min(e0, e1);
+      if (unit.moves(low)) move_acc(unit.move(low));
+      products(v0, v1, unit.scale(e0 == low ? e0 : kNothing), unit.scale(e1 == low ? e1 : kNothing), parts);
+      e0 = e0 == low ? kNothing : e0;
+      e1 = e1 == low ? kNothing : e1;
     }
-    const float s0 = shrink_of(e0 + kUp, ref), s1 = shrink_of(e1 + kUp, ref);
+    if (unit.moves(e0) || unit.moves(e1)) move_acc(unit.move(max(e0, e1)));
+    products(v0, v1, unit.scale(e0), unit.scale(e1), parts);
+  }
+  // Values that widen to nothing (NaN to NaN all the same: the row has it anyhow).
+  static constexpr int kNothing = -1000;
+  CDB_DEVICE void products(const ValueRegs<D>& v0, const ValueRegs<D>& v1, float s0, float s1, const f16x8_t* parts) {
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) {
       if constexpr (kWide) {
@@ -373,7 +390,7 @@ CDB_DEVICE void append_token(const Kv8Cache& cache, const Fresh<D>& fresh, int64
 }
 
 template <typename T, int D, int STYLE>
-__global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kernel(Kv8DecodeParams P) {
+__global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_kernel(Kv8DecodeParams P) {
   constexpr bool kWide = sizeof(T) == 4;
   using Query = QueryRegs<D, kWide>;
   __shared__ __align__(32) uint32_t q_codes[Query::kWords];
@@ -535,6 +552,7 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
     f16x8_t parts[Attention<D, kWide>::kPParts];
     f32x4_t s[2];
     if (owner) {
+      end_v = __builtin_amdgcn_readfirstlane(end_v);  // arrived by now; the unit stays in scalar registers
       const uint32_t seen = tokens_below(off + 1 - 4 * g);  // what lies behind counts for nothing, NaN among it
 #pragma unroll
       for (int m = 0; m < ValueRegs<D>::kWords; ++m) v[0].w[m] &= seen;
@@ -542,7 +560,7 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
       s[0] = state.scores(k[0], end_k, q, off + 1, g);
       s[1] = (f32x4_t){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       state.softmax(s, parts);
-      state.values(v[0], v[1], max((int)end_v, 1), 1, parts);
+      state.values(v[0], v[1], max((int)end_v, 1), max((int)end_v, 1), parts);
       load_first();
     }
     // The loads ahead are not left out at the end but read a line each: a branch around them would make the
@@ -574,7 +592,7 @@ __global__ void __launch_bounds__(64 * kWaves, kDecodeWaves<T>) kv8_decode_kerne
     if (missing) sum = NAN;
     if (r < cols) {
       float* mine = join + (wave * cols + r) * kJoin;
-      const int back = state.ref - 127 - state.kUp - state.kRaise;
+      const int back = state.unit.back() - state.kRaise;
 #pragma unroll
       for (int m = 0; m < D / 16; m += 2)
 #pragma unroll

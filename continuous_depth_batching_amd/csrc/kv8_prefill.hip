@@ -6,8 +6,8 @@
 // block's are used up, so nothing waits on LDS or on another wave.
 //   S^T = K Q^T in bf16: a code times a power of two is exact there, so scores are the products' fp32 sums.
 //   O^T = V^T P^T in fp16, which holds a code exactly and P to 2^-11: it is raised by 2^9, so that keys down to 2^-23
-//   of the query's largest keep that, and none is off by more than 2^-34 of it. Values widen with their scale relative
-//   to the largest met. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-23, and 2^-45 of the
+//   of the query's largest keep that, and none is off by more than 2^-34 of it. Values widen with their scale, in a
+//   unit that follows the tiles' scales. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-23, and 2^-45 of the
 //   largest).
 // A lane's 16 scores are those of the 16 tokens whose values it holds, so P never moves; queries are the columns of
 // both products, so maximum and sum are a lane's own and its neighbour's, 32 lanes away.
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
     for (int e = 0; e < 16; ++e) acc[i][e] = 0.f;
   // Scores are counted, in units of log2, from -`shift`, anew once they pass `limit`.
   float shift = 0.f, limit = -INFINITY, sum = 0.f;
-  int ref = 1;  // biased exponent that the accumulators are counted in
+  ValueUnit<T> unit;  // that the accumulators are counted in
   bool missing = bad;
   const int32_t* table = P.block_table + (int64_t)(bad ? 0 : trow) * P.table_width;
   const int bs_mask = (1 << P.bs_log2) - 1;
@@ -182,19 +182,17 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
 
   for (int window = from; window < to; window += 32) {
     const int count = min(32, to - window);
-    // Lane j looks up tile j of the window; one past the sequence is any tile, and masked.
+    // Lane j looks up tile j of the window; for one past the sequence its last, masked.
     int64_t where = 0;
     uint32_t bytes = 0x0101u;
     bool lost = false;
     if (lane < 2 * count) {
-      const int t = window * 32 + lane * kTile;
-      if (t < total) {
-        const int block = table[t >> P.bs_log2];
-        lost = block < 0 || block >= P.cache.pool_blocks;
-        const int64_t tile = P.cache.tile(P.layer, 0, lost ? 0 : block, kvh, (t & bs_mask) >> 4);
-        bytes = P.cache.scales[tile] | (uint32_t)P.cache.scales[tile + P.cache.plane_tiles] << 8;
-        where = tile * (kTile * D);
-      }
+      const int t = min(window * 32 + lane * kTile, (int)total - 1);
+      const int block = table[t >> P.bs_log2];
+      lost = block < 0 || block >= P.cache.pool_blocks;
+      const int64_t tile = P.cache.tile(P.layer, 0, lost ? 0 : block, kvh, (t & bs_mask) >> 4);
+      bytes = P.cache.scales[tile] | (uint32_t)P.cache.scales[tile + P.cache.plane_tiles] << 8;
+      where = tile * (kTile * D);
     }
     missing = missing || __ballot(lost) != 0;
     auto codes_at = [&](int j) __attribute__((always_inline)) -> const uint8_t* {
@@ -250,13 +248,14 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
       for (int a = 0; a < 2; ++a) {
         const int t = key0 + kTile * a;
         const int v_exp = max((int)((a ? b1 : b0) >> 8), 1);
-        if (v_exp > ref) {
-          const float f = shrink_of(ref, v_exp);
+        if (unit.moves(v_exp)) {
+          const int by = unit.move(v_exp);
 #pragma unroll
-          for (int m = 0; m < kTiles; ++m) acc[m] *= f;
-          ref = v_exp;
+          for (int m = 0; m < kTiles; ++m)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[m][e] = ldexpf(acc[m][e], by);
         }
-        const float v_scale = shrink_of(v_exp + kValueRaise<T>, ref);
+        const float v_scale = unit.scale(v_exp);
         f16x8_t pp[kPParts];
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -340,7 +339,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)), ldexpf(acc[m][e] * inv, ref - 127 - kValueRaise<T>));
+        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)), ldexpf(acc[m][e] * inv, unit.back()));
     return;
   }
   float* to_part = P.partials +
@@ -349,7 +348,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
   for (int m = 0; m < kTiles; ++m)
 #pragma unroll
     for (int e = 0; e < 16; ++e) to_part[Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3))] =
-        ldexpf(acc[m][e], ref - 127 - kValueRaise<T> - (int)kRaise);
+        ldexpf(acc[m][e], unit.back() - (int)kRaise);
   if (h == 0) {
     to_part[D] = top;
     to_part[D + 1] = ldexpf(sum, -(int)kRaise);

@@ -143,3 +143,57 @@ def test_keys_far_below_a_sink_keep_their_share(kind, dtype, heads, kv, dim) -> 
     q = np.zeros((1 if kind == "decode" else 40, heads, dim))
     q[:, :, 0] = 27 * np.log(2.0) / 28 * dim ** 0.5  # the sink's key is 448 / 16
     Sequence(kind, dtype, heads, kv, dim, keys, values, k_exp, v_exp, q).check(rng)
+
+
+def spread_values(rng, tiles, pattern, apart):
+    """Exponents of the value tiles: ``pattern`` says which are 2^apart larger."""
+    big = {"first": np.arange(tiles) < 2, "last": np.arange(tiles) >= tiles - 2, "middle": np.arange(tiles) == 50,
+           "every other": np.arange(tiles) % 2 == 1, "every other pair": np.arange(tiles) // 2 % 2 == 0}[pattern]
+    return big, np.where(big, apart - 5, rng.integers(-7, -4, tiles))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("apart", [14, 24, 55])
+@pytest.mark.parametrize("pattern", ["first", "last", "middle", "every other", "every other pair"])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f32", 64), ("bf16", 96)])
+def test_values_far_below_others_keep_their_share(kind, apart, pattern, dtype, dim) -> None:
+    """Tiles of values 2^apart larger, that keys of next to no probability keep out of the result."""
+    rng = np.random.default_rng(72)
+    n = 1497
+    tiles = -(-n // 16)
+    big, v_exp = spread_values(rng, tiles, pattern, apart)
+    far = np.repeat(big, 16)[:n]
+    if kind == "decode":
+        far[-1] = False  # the new token is one of the others, in a tile of large values or not
+        if pattern == "last":
+            v_exp[-1], big[-1] = -6, False
+    # Scores: 0..2 in units of log2 for the small ones, -112 for the large ones (a code of -448 over a key's of 8).
+    first = np.where(far, -448.0, rng.uniform(0.0, 8.0, n))
+    keys, values = line(rng, n, 2, dim, first)
+    values = np.abs(values)  # sums that do not cancel: the bound stays small beside them
+    if kind != "decode" and big[-1]:
+        keys[-40:, :, 0] = 0.0  # the queries' own tokens: see the next test
+        far[-40:] = False
+        v_exp[-3:] = -6
+    q = np.zeros((1 if kind == "decode" else 40, 2, dim))
+    q[:, :, 0] = 112 * np.log(2.0) / 28 * dim ** 0.5
+    Sequence(kind, dtype, 2, 2, dim, keys, values, np.full(tiles, -4), v_exp, q).check(rng)
+
+
+@pytest.mark.parametrize("kind", ["prefill", "split"])
+@pytest.mark.parametrize("apart", [20, 50])
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f32", 64), ("bf16", 96)])
+def test_values_of_later_tokens_leave_earlier_queries_alone(kind, apart, dtype, dim) -> None:
+    """A chunk whose every other tile holds values 2^apart larger: queries before the first of them see none."""
+    rng = np.random.default_rng(73)
+    n, new = 70, 70
+    tiles = -(-n // 16)
+    v_exp = np.where(np.arange(tiles) % 2 == 1, apart - 5, -5)
+    keys = oracle.round_e4m3(np.clip(rng.standard_normal((n, 2, dim)) * 40, -448, 448))
+    values = oracle.round_e4m3(np.clip(rng.standard_normal((n, 2, dim)) * 90, -448, 448))
+    q = rng.standard_normal((new, 2, dim)) * 0.5
+    s = Sequence(kind, dtype, 2, 2, dim, keys, values, np.full(tiles, -5), v_exp, q, new=new)
+    got = s.run()
+    want, bound = s.expect()
+    helpers.close(got, want, bound)
+    assert (np.linalg.norm(bound[:16], axis=-1) < np.linalg.norm(want[:16], axis=-1) / 4).all()
