@@ -128,8 +128,8 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, i
   uint8_t* v_codes = P.cache.codes + v_tile * (kTile * D);
   int k_old = 0, v_old = 0;
   if (off > 0) {
-    k_old = min((int)P.cache.scales[k_tile], 254);
-    v_old = min((int)P.cache.scales[v_tile], 254);
+    k_old = (int)scale_byte_read(P.cache.scales[k_tile]);
+    v_old = (int)scale_byte_read(P.cache.scales[v_tile]);
   }
 
   // Values: tokens 4g..4g+3 of the lane's elements, on their way while the keys are worked on.

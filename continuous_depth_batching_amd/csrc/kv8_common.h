@@ -28,6 +28,9 @@ typedef int i32x8_t __attribute__((ext_vector_type(8)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 
+// A tile's scale byte as every reader takes it, 1 to 254: 0, of a tile that was never written, is read as 1, and 255,
+// which no write leaves, as 254.
+CDB_DEVICE uint32_t scale_byte_read(uint32_t b) { return min(max(b, 1u), 254u); }
 // 2^(b - 127) of a scale byte, as the conversion instructions take it.
 CDB_DEVICE float scale_of(uint32_t b) { return __uint_as_float(b << 23); }
 // 2^(127 - b): the factor that brings a value to a code. Bytes above 253 give 0.

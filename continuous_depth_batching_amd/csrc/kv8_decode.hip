@@ -520,6 +520,10 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
       }
     }
     lds_barrier();
+    if (owner) {  // they have arrived by now
+      end_k = scale_byte_read(end_k);
+      end_v = scale_byte_read(end_v);
+    }
     if (owner && slice == 0) {
       // The row's new key and value, as codes at the scale that their tile will have: this wave's alone.
       const T* bias = static_cast<const T*>(P.k_bias);
@@ -530,7 +534,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
                                    P.cos + angle, P.sin + angle, d, P.vec, x);
       const int k_new = scale_byte(all_max(fmaxf(finite_abs(x[0]), finite_abs(x[1]))));
       const int v_new = scale_byte(all_max(fmaxf(finite_abs(y[0]), finite_abs(y[1]))));
-      const int k_old = min((int)end_k, 254), v_old = min((int)end_v, 254);
+      const int k_old = (int)end_k, v_old = (int)end_v;
       end_k = off != 0 ? max(k_new, k_old) : k_new;
       end_v = off != 0 ? max(v_new, v_old) : v_new;
       const float k_scale = scale_of(end_k), v_scale = scale_of(end_v);
@@ -552,7 +556,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
     f16x8_t parts[Attention<D, kWide>::kPParts];
     f32x4_t s[2];
     if (owner) {
-      end_v = __builtin_amdgcn_readfirstlane(end_v);  // arrived by now; the unit stays in scalar registers
+      end_v = __builtin_amdgcn_readfirstlane(end_v);  // the unit stays in scalar registers
       const uint32_t seen = tokens_below(off + 1 - 4 * g);  // what lies behind counts for nothing, NaN among it
 #pragma unroll
       for (int m = 0; m < ValueRegs<D>::kWords; ++m) v[0].w[m] &= seen;
@@ -560,7 +564,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
       s[0] = state.scores(k[0], end_k, q, off + 1, g);
       s[1] = (f32x4_t){-INFINITY, -INFINITY, -INFINITY, -INFINITY};
       state.softmax(s, parts);
-      state.values(v[0], v[1], max((int)end_v, 1), max((int)end_v, 1), parts);
+      state.values(v[0], v[1], (int)end_v, (int)end_v, parts);
       load_first();
     }
     // The loads ahead are not left out at the end but read a line each: a branch around them would make the
@@ -575,11 +579,11 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
         const int on = 2 * next < count ? -1 : 0, ahead = on ? next : pair;
         const uint32_t b0 = __builtin_amdgcn_readlane((int)bytes, 2 * pair);
         const uint32_t b1 = __builtin_amdgcn_readlane((int)bytes, min(2 * pair + 1, count - 1));
-        s[0] = state.scores(k[0], b0 & 255, q, kTile, g);
-        s[1] = state.scores(k[1], b1 & 255, q, 2 * pair + 1 < count ? kTile : 0, g);
+        s[0] = state.scores(k[0], scale_byte_read(b0 & 255), q, kTile, g);
+        s[1] = state.scores(k[1], scale_byte_read(b1 & 255), q, 2 * pair + 1 < count ? kTile : 0, g);
         load_keys(ahead, on);
         state.softmax(s, parts);
-        state.values(v[0], v[1], max((int)(b0 >> 8), 1), max((int)(b1 >> 8), 1), parts);
+        state.values(v[0], v[1], (int)scale_byte_read(b0 >> 8), (int)scale_byte_read(b1 >> 8), parts);
         __builtin_amdgcn_sched_barrier(0);
         load_values(ahead, on);
         __builtin_amdgcn_sched_barrier(0);

@@ -7,8 +7,8 @@
 //   S^T = K Q^T in bf16: a code times a power of two is exact there, so scores are the products' fp32 sums.
 //   O^T = V^T P^T in fp16, which holds a code exactly and P to 2^-11: it is raised by 2^9, so that keys down to 2^-23
 //   of the query's largest keep that, and none is off by more than 2^-34 of it. Values widen with their scale, in a
-//   unit that follows the tiles' scales. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-23, and 2^-45 of the
-//   largest).
+//   unit that follows the tiles' scales. fp32 models: queries as 3 bf16 parts (2^-24), P as 2 fp16 parts (2^-23, and
+//   2^-45 of the largest).
 // A lane's 16 scores are those of the 16 tokens whose values it holds, so P never moves; queries are the columns of
 // both products, so maximum and sum are a lane's own and its neighbour's, 32 lanes away.
 //
@@ -132,7 +132,7 @@ constexpr float kSlack = 6.f, kRaise = 9.f;
 
 // Waves a SIMD: three where the registers allow it without spills (5000 tokens of 55 heads x 96, 360 us against 380);
 // for bf16 heads of 128 they would spill 27, and take 904 and 125 us for 900 and 113.
-template <typename T, int D> constexpr int kPrefillWaves = sizeof(T) == 2 && D <= 96 ? 3 : 2;
+template <typename T, int D> constexpr int kPrefillWaves = D == 64 || (sizeof(T) == 2 && D == 96) ? 3 : 2;
 
 template <typename T, int D>
 __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel(Kv8PrefillParams P) {
@@ -191,7 +191,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
       const int block = table[t >> P.bs_log2];
       lost = block < 0 || block >= P.cache.pool_blocks;
       const int64_t tile = P.cache.tile(P.layer, 0, lost ? 0 : block, kvh, (t & bs_mask) >> 4);
-      bytes = P.cache.scales[tile] | (uint32_t)P.cache.scales[tile + P.cache.plane_tiles] << 8;
+      bytes = scale_byte_read(P.cache.scales[tile]) | scale_byte_read(P.cache.scales[tile + P.cache.plane_tiles]) << 8;
       where = tile * (kTile * D);
     }
     missing = missing || __ballot(lost) != 0;
@@ -247,7 +247,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int t = key0 + kTile * a;
-        const int v_exp = max((int)((a ? b1 : b0) >> 8), 1);
+        const int v_exp = (int)((a ? b1 : b0) >> 8);
         if (unit.moves(v_exp)) {
           const int by = unit.move(v_exp);
 #pragma unroll
@@ -304,8 +304,8 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
               f32x16_t met;
 #pragma unroll
               for (int e = 0; e < 16; ++e) met[e] = 0.f;
-              met = __builtin_amdgcn_mfma_f32_32x32x16_f16(widen_f16(where_nan[0], 1.f, where_nan[1], 1.f), seen, met, 0, 0,
-                                                           0);
+              const f16x8_t ones = widen_f16(where_nan[0], 1.f, where_nan[1], 1.f);
+              met = __builtin_amdgcn_mfma_f32_32x32x16_f16(ones, seen, met, 0, 0, 0);
 #pragma unroll
               for (int e = 0; e < 16; ++e) acc[m][e] = met[e] != 0.f ? NAN : acc[m][e];
             }
@@ -339,7 +339,8 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
     for (int m = 0; m < kTiles; ++m)
 #pragma unroll
       for (int e = 0; e < 16; ++e)
-        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)), ldexpf(acc[m][e] * inv, unit.back()));
+        Elem<T>::store(out + Regs::value_element(m, (e >> 2) * 8 + 4 * h + (e & 3)),
+                       ldexpf(acc[m][e] * inv, unit.back()));
     return;
   }
   float* to_part = P.partials +

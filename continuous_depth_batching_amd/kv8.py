@@ -33,8 +33,8 @@ LAYOUT_BAD_REQUEST = _lib.CDB_LAYOUT_BAD_REQUEST
 @dataclass(frozen=True)
 class Kv8Pool:
     """The cache: ``codes`` float8_e4m3fn ``[layers, 2, blocks, Hkv, block_size / 16, 16 * D]`` and
-    ``scales`` uint8 ``[layers, 2, blocks, Hkv, block_size / 16]`` (b stands for 2 ** (b - 127)), keys at
-    index 0 of dim 1 and values at 1."""
+    ``scales`` uint8 ``[layers, 2, blocks, Hkv, block_size / 16]`` (b, from 1 to 254, stands for
+    2 ** (b - 127); 0 is read as 1 and 255 as 254), keys at index 0 of dim 1 and values at 1."""
 
     codes: torch.Tensor
     scales: torch.Tensor
@@ -89,7 +89,7 @@ class Kv8Pool:
         d = self.head_dim
         raw = self.codes.view(torch.uint8)[layer][:, blocks].view(torch.float8_e4m3fn).float()
         scale = torch.ldexp(torch.ones((), device=raw.device, dtype=torch.float64),
-                            self.scales[layer][:, blocks].int() - 127).float()
+                            self.scales[layer][:, blocks].int().clamp(1, 254) - 127).float()
         raw = raw * scale[..., None]
         k = raw[0].unflatten(-1, (d // 16, TILE, 16)).transpose(-3, -2).flatten(-2)   # [blocks, Hkv, tiles, 16, D]
         v = raw[1].unflatten(-1, (4, d, 4)).transpose(-2, -1).flatten(-3, -2)

@@ -384,7 +384,8 @@ int cdb_coda_greedy(const int64_t* host_upload, int64_t* dev_upload, int32_t row
  * No counterpart in the reference, whose cache holds the model's type. Keys and values are held in tiles of
  * 16 tokens of one KV head, as e4m3 codes with one power-of-two scale a tile, keys and values apart:
  *   codes  [num_cache_layers, 2, pool_blocks, Hkv, block_size / 16, 16 * D] bytes, 16-byte aligned;
- *   scales [num_cache_layers, 2, pool_blocks, Hkv, block_size / 16] bytes b, the scale being 2^(b - 127).
+ *   scales [num_cache_layers, 2, pool_blocks, Hkv, block_size / 16] bytes b, the scale being 2^(b - 127); written ones
+ *          are 1 to 254. A byte of 0, as in a pool of zeros, is read as 1 and one of 255 as 254.
  * A key tile lies as [D / 16][16 tokens][16], a value tile as [4][D][4 tokens]. block_size is a power of two
  * of at least 16; D is 64, 96 or 128; the codes need no address below 2^63 bytes, and offsets are 64-bit.
  * Position t of a sequence is token t % 16 of tile t % block_size / 16 of block block_table[t / block_size].

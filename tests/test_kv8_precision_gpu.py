@@ -197,3 +197,46 @@ def test_values_of_later_tokens_leave_earlier_queries_alone(kind, apart, dtype, 
     want, bound = s.expect()
     helpers.close(got, want, bound)
     assert (np.linalg.norm(bound[:16], axis=-1) < np.linalg.norm(want[:16], axis=-1) / 4).all()
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 128), ("bf16", 96)])
+@pytest.mark.parametrize("plane,byte", [(0, 0), (0, 255), (1, 0), (1, 255)])
+def test_scale_bytes_outside_their_range_are_read_as_its_ends(kind, dtype, dim, plane, byte) -> None:
+    """0 as 1 and 255 as 254, by every call and by ``dequantize``, with queries that make such keys matter."""
+    rng = np.random.default_rng(74)
+    n, end = 300, -126 if byte == 0 else 127
+    tiles = -(-n // 16)
+    keys, values = line(rng, n, 2, dim, rng.uniform(0.0, 96.0, n))
+    values = np.abs(values)
+    k_exp, v_exp = np.full(tiles, -4), np.full(tiles, -6)
+    (k_exp, v_exp)[plane][:] = end
+    if byte == 255:  # within fp32: codes of up to 2^-6
+        (keys, values)[plane][:] = oracle.round_e4m3((keys, values)[plane] * 2.0 ** -14)
+    unit = np.abs(keys).max() * 2.0 ** float(k_exp[0])
+    q = np.zeros((1 if kind == "decode" else 40, 2, dim))
+    q[:, :, 0] = 2.0 ** np.floor(np.log2(5.0 / unit * dim ** 0.5))  # scores of up to 5
+    s = Sequence(kind, dtype, 2, 2, dim, keys, values, k_exp, v_exp, q)
+    other = s.pool.scales[:, 1 - plane].clone()
+    s.pool.scales[s.pool.scales == (1 if byte == 0 else 254)] = byte
+    assert (s.pool.scales[:, plane] == byte).sum() >= 2 * tiles and torch.equal(s.pool.scales[:, 1 - plane], other)
+    got = s.pool.dequantize(0, torch.from_numpy(s.table[0]).long().to(DEV))[plane][:n].double().cpu().numpy()
+    np.testing.assert_array_equal(got, s.cache.values(0, plane, s.at))
+    s.check(rng)
+
+
+@pytest.mark.parametrize("byte", [0, 255])
+def test_write_joins_a_tile_whose_scale_byte_is_outside_its_range(byte) -> None:
+    rng = np.random.default_rng(75)
+    n, new = 5, 6
+    codes = np.zeros((1, 2, 1, 2, 16, 64))
+    codes[:, :, :, :, :n] = oracle.round_e4m3(np.clip(rng.standard_normal((n, 64)) * 90, -448, 448))
+    cache = oracle.Cache(codes, np.full((1, 2, 1, 2), -126 if byte == 0 else 127))
+    pool = kv8.Kv8Pool(helpers.pack(codes, 16).to(DEV), torch.full((1, 2, 1, 2, 1), byte, dtype=torch.uint8, device=DEV))
+    k, v = (helpers.values(rng, "f32", new, 2, 64) for _ in range(2))
+    if byte == 0:  # far below the range of normal tiles: what was there still counts
+        k, v = k * 2.0 ** -120, v * 2.0 ** -120
+    at = torch.arange(n, n + new)
+    kv8.write_raw(None, k.to(DEV), v.to(DEV), None, pool, 0, at.to(DEV), at.int().to(DEV), None, None, 0, None, None)
+    cache.write(0, at.numpy(), k.numpy(), v.numpy())
+    helpers.same_cache(pool, cache)
