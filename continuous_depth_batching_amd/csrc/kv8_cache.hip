@@ -103,20 +103,22 @@ template <int D, int STYLE> struct KeyAngles {
   }
 };
 
-// One wave writes the tokens of one KV head that start a run inside its chunk. A run is the tokens of
-// one tile that follow each other in the batch, 16 at most, so a tile's scale is known to the wave
-// that writes it: the maximum over the run, and for a tile that held earlier tokens their scale too.
+// One wave writes the tokens of one KV head that start a run inside its chunk. A run is the tokens that a batch
+// brings for one tile, 16 at most, each as far from the first in the batch as in the tile, so a tile's scale is known
+// to the wave that writes it: the maximum over the run, and for a tile that held earlier tokens their scale too.
+// Tokens in between that are left out (padding, a slot or position out of range) do not end a run: two waves would
+// meet in the tile.
 // Lane (r, g) = (lane % 16, lane / 16) holds units g, g + 4 of token r of the key tile, and group g of
 // some elements of the value tile, which are the tile's own pieces of 16 bytes.
+// first: the run's first token; run: a bit for each token of the tile that it writes, the first token's the lowest.
 template <typename T, int D, int STYLE>
-CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, int64_t row0, int head,
+CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t first, uint32_t run, int64_t tile, int head,
                           const KeyAngles<D, STYLE>& angles) {
   using V = ValuePieces<D>;
   constexpr int kUnits = D / 16;
   constexpr int kParts = (kUnits + 3) / 4;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-  const int64_t tile = row0 >> 4;
-  const int off = (int)(row0 & 15);
+  const int off = __builtin_ctz(run);
   const int64_t block = tile >> P.cache.tile_log2;
   const int sub = (int)(tile & ((1 << P.cache.tile_log2) - 1));
   const T* k = static_cast<const T*>(P.k) + head * D;
@@ -137,16 +139,16 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, i
   Vec<T, 2> y1[4];  // of heads of 96
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int slot = 4 * g + i - off;
-    const T* src = v + (base + s + (slot >= 0 && slot < n ? slot : 0)) * P.kv_stride;
+    const int slot = 4 * g + i;
+    const T* src = v + (first + (run >> slot & 1 ? slot - off : 0)) * P.kv_stride;
     y0[i] = load_raw<T, V::kMost, kHeadOnce<T, D>>(src + V::element(0, r), P.vec);
     if constexpr (V::kPieces == 2) y1[i] = load_raw<T, 2>(src + V::element(1, r), P.vec);
   }
 
-  // Keys: token r of the tile is token r - off of the run.
-  const bool live = r >= off && r < off + n;
+  // Keys: token r of the tile is the (r - off)th from the run's first.
+  const bool live = (run >> r & 1) != 0;
   float x[kParts][16];
-  angles.template key<T>(k + (base + s + (live ? r - off : 0)) * P.kv_stride, k_bias, g, P.vec, x);
+  angles.template key<T>(k + (first + (live ? r - off : 0)) * P.kv_stride, k_bias, g, P.vec, x);
   // The largest size among them, infinities and NaN left out: those are looked for, and almost never found.
   auto size = [](float z, bool finite) {
     const uint32_t bits = size_bits(z);
@@ -189,8 +191,8 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t base, int s, int n, i
     }
   }
 
-  const uint32_t before = tokens_below(off - 4 * g);               // earlier tokens of the group
-  const uint32_t fresh = tokens_below(off + n - 4 * g) & ~before;  // the run's
+  const uint32_t before = tokens_below(off - 4 * g);  // earlier tokens of the group
+  const uint32_t fresh = tokens_in(run >> (4 * g));   // the run's
   auto v_size = [&](bool finite) __attribute__((always_inline)) {
     uint32_t top = 0;
 #pragma unroll
@@ -252,7 +254,7 @@ template <typename T, int D, int STYLE>
 __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteParams P) {
   const int lane = threadIdx.x & 63;
   if (blockIdx.x < P.kv_blocks) {
-    const int64_t item = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int64_t item = (int64_t)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int heads = P.cache.num_kv_heads;
     const int groups = (heads + P.heads_each - 1) / P.heads_each;
     const int64_t chunk = item / groups;
@@ -273,24 +275,35 @@ __global__ void __launch_bounds__(256) kv8_write_kernel(Kv8WriteParams P) {
     int position, unused;
     const int64_t row = slot(idx, position);
     const int64_t prev = slot(idx - 1, unused);
-    const bool follows = row >= 0 && prev >= 0 && row == prev + 1 && (row & 15) != 0;
+    bool follows = row >= 0 && prev >= 0 && row == prev + 1 && (row & 15) != 0;
+    // Behind a token left out, the last one before it that is not decides.
+    const int64_t reach = min(idx, row & 15);
+    bool open = row >= 0 && prev < 0 && reach > 1;
+    for (int d = 2; __any(open); ++d) {
+      const int64_t before = open ? slot(idx - d, unused) : -1;
+      if (open && before >= 0) follows = row == before + d;
+      open = open && before < 0 && d < reach;
+    }
     uint64_t starts = __ballot(row >= 0 && !follows && lane < P.chunk);
-    const uint64_t conts = __ballot(follows);
     while (starts != 0) {
       const int s = __builtin_ctzll(starts);
       starts &= starts - 1;
-      const int n = 1 + __builtin_ctzll(~(conts >> (s + 1)));
       const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)row, s);
       const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(row >> 32), s);
       const int64_t row0 = (int64_t)(((uint64_t)hi << 32) | lo);
+      // The tokens from s on that go with it, up to the first that does not.
+      const bool same = row >= 0 && row - row0 == lane - s && (row >> 4) == (row0 >> 4);
+      const uint64_t others = __ballot(row >= 0 && !same) >> s;
+      const uint64_t with = (__ballot(same) >> s) & (others == 0 ? ~0ull : (others & -others) - 1);
       const int slot0 = (int)(lo & 15), r = lane & 15;
+      const uint32_t run = (uint32_t)with << slot0;
       KeyAngles<D, STYLE> angles;
       if constexpr (STYLE != 0) {
-        const int p = __shfl(position, s + (r >= slot0 && r < slot0 + n ? r - slot0 : 0));
+        const int p = __shfl(position, s + (run >> r & 1 ? r - slot0 : 0));
         angles.load(P.cos + (int64_t)p * (D / 2), P.sin + (int64_t)p * (D / 2), lane >> 4, P.vec);
       }
       for (int h = head; h < min(head + P.heads_each, heads); ++h)
-        write_run<T, D, STYLE>(P, base, s, n, row0, h, angles);
+        write_run<T, D, STYLE>(P, base + s, run, row0 >> 4, h, angles);
     }
     return;
   }

@@ -80,6 +80,9 @@ CDB_DEVICE float growth_of(int old, int now) { return scale_of((uint32_t)min(127
 // Byte mask of a word's tokens below n (n <= 0: none, n >= 4: all).
 CDB_DEVICE uint32_t tokens_below(int n) { return n <= 0 ? 0u : n >= 4 ? ~0u : (1u << (8 * n)) - 1u; }
 
+// Byte mask of the low four bits of m.
+CDB_DEVICE uint32_t tokens_in(uint32_t m) { return (((m & 15u) * 0x00204081u) & 0x01010101u) * 255u; }
+
 // N storage elements as they lie; vec as for load_f32, kOnce: they are read once and need no place in the caches.
 template <typename T, int N, bool kOnce = false> CDB_DEVICE Vec<T, N> load_raw(const T* p, bool vec) {
   Vec<T, N> x;

@@ -173,7 +173,8 @@ def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: t
     """Launch ``cdb_kv8_write``: code T tokens' rotated keys and their values into slots ``rows`` of cache layer
     ``layer`` and put the rotated queries into ``q_out`` (q and q_out None: keys and values alone). q, k and v
     may be token-strided views. The tokens of one tile follow each other at consecutive slots; a negative slot
-    is padding, whose q_out is left as it was."""
+    is padding, whose q_out is left as it was. A token left out between others of its tile (padding, a slot or
+    position out of range) keeps its place in the call."""
 
     heads_kv, dim, block = pool._shape
     codes, scales, layers, blocks = pool._args

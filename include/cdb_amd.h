@@ -402,7 +402,9 @@ int cdb_coda_greedy(const int64_t* host_upload, int64_t* dev_upload, int32_t row
  * cdb_rope_kv_write, with its q/k/v views, strides, rotation styles and biases. The tokens of one tile follow
  * each other in the call at consecutive slots, as a sequence's tokens do; a slot is written once in a call. Tokens
  * with a negative slot are padding: nothing of theirs is read or written, q_out included. A slot past the pool
- * or a position outside the angle tables writes no key or value (and NaN to q_out for such a position).
+ * or a position outside the angle tables writes no key or value (and NaN to q_out for such a position). A token left
+ * out in one of these ways between others of its tile keeps its place in the call, the next one's slot being two
+ * further: its codes stay as they were, and the others share one scale as if they followed each other.
  * num_heads 0 (q and q_out null) writes keys and values alone. q_out is dense and 16-byte aligned. */
 int cdb_kv8_write(const void* q, const void* k, const void* v, void* q_out, void* codes, void* scales,
                   int32_t num_cache_layers, int64_t pool_blocks, int32_t layer, const int64_t* rows,

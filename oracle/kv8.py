@@ -60,35 +60,38 @@ class Cache:
     def __init__(self, codes: np.ndarray, exponents: np.ndarray) -> None:
         self.codes, self.exponents = codes.astype(np.float64), exponents.astype(np.int64)
 
-    def append(self, layer: int, slot: int, k: np.ndarray, v: np.ndarray) -> None:
-        """Tokens k, v [n, Hkv, D] (fp32) at ``slot``.. of one tile, slots consecutive."""
+    def append(self, layer: int, slot: int, k: np.ndarray, v: np.ndarray, steps: np.ndarray | None = None) -> None:
+        """Tokens k, v [n, Hkv, D] (fp32) of one tile, the first at ``slot`` and the others ``steps`` (0, ..) behind
+        it; consecutive without."""
 
         tile, off = slot // TILE, slot % TILE
+        at = off + (np.arange(len(k)) if steps is None else steps)
+        assert at[0] == off and at[-1] < TILE
         for plane, x in enumerate((k, v)):
-            n, heads, _ = x.shape
-            assert off + n <= TILE
-            for h in range(heads):
+            for h in range(x.shape[1]):
                 code, old = self.codes[layer, plane, tile, h], self.exponents[layer, plane, tile, h]
                 new = tile_exponent(x[:, h])
                 if off:
                     new = max(new, old)
                     if new != old:
                         code[:off] = round_e4m3(np.ldexp(code[:off], old - new))
-                code[off:off + n] = round_e4m3(np.ldexp(x[:, h].astype(np.float64), -new))
+                code[at] = round_e4m3(np.ldexp(x[:, h].astype(np.float64), -new))
                 self.exponents[layer, plane, tile, h] = new
 
     def write(self, layer: int, rows: np.ndarray, k: np.ndarray, v: np.ndarray) -> None:
-        """A batch of tokens at slots ``rows`` (negative: padding), a tile's tokens next to each other."""
+        """A batch of tokens at slots ``rows`` (negative: left out), a tile's tokens next to each other."""
 
         t = 0
         while t < len(rows):
             if rows[t] < 0:
                 t += 1
                 continue
-            n = 1
-            while t + n < len(rows) and rows[t + n] == rows[t] + n and rows[t + n] % TILE:
+            run, n = [0], 1
+            while t + n < len(rows) and rows[t] % TILE + n < TILE and rows[t + n] in (rows[t] + n, -1):
+                run += [n] if rows[t + n] >= 0 else []
                 n += 1
-            self.append(layer, int(rows[t]), k[t:t + n], v[t:t + n])
+            steps = np.array(run)
+            self.append(layer, int(rows[t]), k[t + steps], v[t + steps], steps)
             t += n
 
     def values(self, layer: int, plane: int, slots: np.ndarray) -> np.ndarray:

@@ -875,3 +875,40 @@ def test_blocks_past_4_gib_give_the_same_bits() -> None:
         del pool
     assert all(torch.equal(a, b) for a, b in zip(*results))
     assert torch.isfinite(results[0][0]).all() and torch.isfinite(results[0][1]).all()
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("how", ["slot", "position", "padding"])
+@pytest.mark.parametrize("dtype,heads,kv,dim,style,block", [("bf16", 3, 3, 128, 1, 16), ("f32", 2, 1, 96, 2, 32),
+                                                            ("bf16", 2, 2, 64, 0, 16)])
+def test_write_leaves_tokens_out_inside_a_tile(dtype, heads, kv, dim, style, block, how, many) -> None:
+    """Tokens left out between others of their tile, in batches of which a wave takes one token or sixteen: the others
+    are coded as one run, and the codes at their places stay as they were."""
+    if how == "position" and style == 0:
+        how = "slot"
+    seqs = [(0, 40), (5, 30), (9, 3), (14, 20), (0, 16), (2, 13)] + ([(3, 1200), (0, 77)] if many else [])
+    c = WriteCase(65, dtype, heads, kv, dim, style, False, block, seqs)
+    rng = np.random.default_rng(66)
+    out = rng.random(c.rows.size) < 0.3
+    start = np.cumsum([0] + [n for _, n in seqs])
+    out[start[0]:start[0] + 16] = [False] + [True] * 14 + [False]      # a tile's first and last token alone
+    out[start[4]:start[4] + 16] = [True] * 3 + [False] + [True] * 11 + [False]  # not its first
+    rows, pos = c.rows.copy(), c.pos.copy()
+    if how == "padding":
+        rows[out] = -1
+    elif how == "slot":
+        rows[out] = c.pool.num_blocks * block + c.rows[out]
+    else:
+        pos[out] = np.where(rng.random(out.sum()) < 0.5, -1, c.pos.max() + 1)
+    got = c.run(rows=dev(rows), pos=dev(pos, torch.int32)).cpu()
+    c.rows[out] = -1
+    want = c.expect()
+    left = torch.from_numpy(out)
+    assert torch.equal(got[~left], want[~left])
+    if how == "padding":
+        assert (got[left] == 7.0).all()
+    elif how == "position":
+        assert got[left].isnan().all()
+    else:
+        assert torch.equal(got[left], want[left])
+    helpers.same_cache(c.pool, c.cache)

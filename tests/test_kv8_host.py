@@ -352,3 +352,18 @@ def test_layout_refuses_buffers_that_do_not_fit() -> None:
     with pytest.raises(ValueError, match="3 requests"):
         pos = torch.zeros(2, dtype=torch.int32)
         kv8.batch_layout_raw(pos, pos, torch.zeros(2, 2, dtype=torch.int32), None, pos, 16, a)
+
+
+def test_oracle_codes_a_run_over_tokens_left_out() -> None:
+    rng = np.random.default_rng(2)
+    codes, exps = np.full((1, 2, 2, 1, 16, 4), 3.0), np.full((1, 2, 2, 1), -7)
+    k = rng.standard_normal((6, 1, 4)).astype(np.float32) * np.float32(2.0) ** np.arange(6)[:, None, None]
+    cache = oracle.Cache(codes.copy(), exps)
+    cache.write(0, np.array([16 + 2, -1, 16 + 4, 16 + 5, -1, 0]), k, k)
+    top = oracle.tile_exponent(k[[0, 2, 3]])
+    assert (cache.exponents[0, :, 1, 0] == max(top, -7)).all()
+    got = cache.codes[0, 0, 1, 0]
+    for slot, t in ((2, 0), (4, 2), (5, 3)):
+        np.testing.assert_array_equal(got[slot], oracle.round_e4m3(k[t, 0] * 2.0 ** -float(top)))
+    assert (got[[3] + list(range(6, 16))] == 3.0).all() and (got[:2] == oracle.round_e4m3(3.0 * 2.0 ** (-7.0 - top))).all()
+    assert cache.exponents[0, 0, 0, 0] == oracle.tile_exponent(k[5])
