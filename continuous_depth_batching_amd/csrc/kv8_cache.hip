@@ -32,10 +32,10 @@ template <int D> struct ValuePieces {
   static CDB_DEVICE int element(int j, int r) { return j == 0 ? kMost * r : 64 + 2 * r; }
 };
 
-// Whether keys and values are read past the caches. That pays for prompts with bf16 heads of 128, whole lines of 256
-// bytes (7700 tokens of 16 heads: 39.0 us against 41.7), and costs elsewhere (bf16 heads of 96: 117 against 111; fp32
-// heads of 128: 70 against 62, of 64: 41 against 36). Over 1024 single tokens, which a wave of such heads reads over
-// and over, take 97 us against 82 for 1500; a choice at run time took the registers of a third wave a SIMD (42.6).
+// Whether a whole tile's keys and values are read past the caches. For bf16 heads of 128 that pays where q, k and v are
+// not in a cache (7700 tokens of 16 heads: 38.5 us against 41.7) and is as good where they have just been written (33.2
+// both); it costs elsewhere (bf16 heads of 96: 117 against 111; fp32 heads of 128: 70 against 62, of 64: 41 against
+// 36). Shorter runs never are: 1500 single tokens take 97 us with it and 87 so (82 in a kernel without the choice).
 template <typename T, int D> constexpr bool kHeadOnce = sizeof(T) == 2 && D == 128;
 
 // The angles of a lane's units of a key: kept while the wave goes through its heads.
@@ -56,9 +56,10 @@ template <int D, int STYLE> struct KeyAngles {
   }
   // Units g + 4j of a head, x + bias, rotated, in fp32 with every product and sum rounded once.
   template <typename T>
-  CDB_DEVICE void key(const T* head, const T* bias, int g, bool vec, float x[kParts][16]) const {
+  CDB_DEVICE void key(const T* head, const T* bias, int g, bool vec, bool once, float x[kParts][16]) const {
     auto unit = [&](int u, float* to) __attribute__((always_inline)) {
-      load_f32<T, 16, kHeadOnce<T, D>>(head + 16 * u, to, vec);
+      if (kHeadOnce<T, D> && once) load_f32<T, 16, true>(head + 16 * u, to, vec);
+      else load_f32<T, 16>(head + 16 * u, to, vec);
       if (bias != nullptr) {
         float b[16];
         load_f32<T, 16>(bias + 16 * u, b, vec);
@@ -119,6 +120,7 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t first, uint32_t run, 
   constexpr int kParts = (kUnits + 3) / 4;
   const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
   const int off = __builtin_ctz(run);
+  const bool once = run == 0xffffu;
   const int64_t block = tile >> P.cache.tile_log2;
   const int sub = (int)(tile & ((1 << P.cache.tile_log2) - 1));
   const T* k = static_cast<const T*>(P.k) + head * D;
@@ -141,14 +143,15 @@ CDB_DEVICE void write_run(const Kv8WriteParams& P, int64_t first, uint32_t run, 
   for (int i = 0; i < 4; ++i) {
     const int slot = 4 * g + i;
     const T* src = v + (first + (run >> slot & 1 ? slot - off : 0)) * P.kv_stride;
-    y0[i] = load_raw<T, V::kMost, kHeadOnce<T, D>>(src + V::element(0, r), P.vec);
+    if (kHeadOnce<T, D> && once) y0[i] = load_raw<T, V::kMost, true>(src + V::element(0, r), P.vec);
+    else y0[i] = load_raw<T, V::kMost>(src + V::element(0, r), P.vec);
     if constexpr (V::kPieces == 2) y1[i] = load_raw<T, 2>(src + V::element(1, r), P.vec);
   }
 
   // Keys: token r of the tile is the (r - off)th from the run's first.
   const bool live = (run >> r & 1) != 0;
   float x[kParts][16];
-  angles.template key<T>(k + (first + (live ? r - off : 0)) * P.kv_stride, k_bias, g, P.vec, x);
+  angles.template key<T>(k + (first + (live ? r - off : 0)) * P.kv_stride, k_bias, g, P.vec, once, x);
   // The largest size among them, infinities and NaN left out: those are looked for, and almost never found.
   auto size = [](float z, bool finite) {
     const uint32_t bits = size_bits(z);
