@@ -2,9 +2,9 @@
 
 Keys and values are held in tiles of 16 tokens of one KV head as e4m3 codes with one power-of-two
 scale a tile (``include/cdb_amd.h``, "8-bit KV cache"): half the bytes of a bf16 cache, and three fifths
-of the time of a decode step's attention (256 rows, 16 heads x 128: 107 us a layer against 178). The calls mirror those of the
-pool in the model's type (``ops``): ``write`` beside ``rope_kv_write``, ``decode_attention`` beside
-``paged_decode_attention``, ``prefill_attention`` beside ``prefill_attention``; ``batch_layout`` builds
+of the time of a decode step's attention (256 rows, 16 heads x 128: 107 us a layer against 178). The calls
+mirror those of the pool in the model's type (``ops``): ``write`` beside ``rope_kv_write``, ``decode_attention``
+beside ``paged_decode_attention``, ``prefill_attention`` beside ``prefill_attention``; ``batch_layout`` builds
 on the GPU what they take as block tables, slots and attention tiles.
 
 Each ``*_raw`` function checks its arguments on the host and makes one C call on torch's current stream
@@ -22,6 +22,7 @@ from . import _lib
 from .ops import _ptr, _stream, dtype_code
 
 TILE = 16  # tokens of a cache tile
+_E4M3, _U8, _I32, _I64 = torch.float8_e4m3fn, torch.uint8, torch.int32, torch.int64
 PREFILL_TILE = 128  # query tokens of an attention tile
 
 LAYOUT_TOKENS_FULL = _lib.CDB_LAYOUT_TOKENS_FULL
@@ -40,16 +41,31 @@ class Kv8Pool:
     scales: torch.Tensor
 
     def __post_init__(self) -> None:
+        self._check()
+
+    def _check(self) -> tuple[torch.Size, torch.Size, tuple[int, int, int, int, int]]:
         c, s = self.codes, self.scales
         if c.dtype is not torch.float8_e4m3fn or s.dtype is not torch.uint8:
             raise TypeError("an 8-bit pool holds float8_e4m3fn codes and uint8 scales")
-        if c.dim() != 6 or c.shape[1] != 2 or tuple(s.shape) != tuple(c.shape[:5]) or c.shape[5] % TILE:
+        shape = c.shape
+        if len(shape) != 6 or shape[1] != 2 or s.shape != shape[:5] or shape[5] % TILE:
             raise ValueError("codes must be [layers, 2, blocks, Hkv, block_size / 16, 16 * D] and scales match them")
         if not c.is_contiguous() or not s.is_contiguous() or c.device != s.device:
             raise ValueError("codes and scales must be contiguous and on one device")
-        # What every call needs of the pool, resolved once.
-        object.__setattr__(self, "_args", (c.data_ptr(), s.data_ptr(), c.shape[0], c.shape[2]))
-        object.__setattr__(self, "_shape", (c.shape[3], c.shape[5] // TILE, c.shape[4] * TILE))
+        layers, _, blocks, heads, tiles, tile = shape
+        facts = (shape, s.shape, (layers, blocks, heads, tile // TILE, tiles * TILE))
+        object.__setattr__(self, "_facts", facts)
+        return facts
+
+    def _resolve(self) -> tuple[int, int, tuple[int, int, int, int, int]]:
+        """(codes, scales, (layers, blocks, Hkv, D, block_size)) of the tensors as they are now. Every call asks: a
+        pool may be a copy, or its tensors may have been given other memory."""
+
+        c, s, facts = self.codes, self.scales, self._facts
+        if c.shape != facts[0] or s.shape != facts[1] or c.dtype is not _E4M3 or s.dtype is not _U8 \
+                or not c.is_contiguous() or not s.is_contiguous():
+            facts = self._check()
+        return c.data_ptr(), s.data_ptr(), facts[2]
 
     @classmethod
     def allocate(cls, num_cache_layers: int, num_blocks: int, block_size: int, num_kv_heads: int, head_dim: int,
@@ -72,15 +88,15 @@ class Kv8Pool:
 
     @property
     def num_kv_heads(self) -> int:
-        return self._shape[0]
+        return self.codes.shape[3]
 
     @property
     def head_dim(self) -> int:
-        return self._shape[1]
+        return self.codes.shape[5] // TILE
 
     @property
     def block_size(self) -> int:
-        return self._shape[2]
+        return self.codes.shape[4] * TILE
 
     def dequantize(self, layer: int, blocks: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
         """fp32 keys and values ``[len(blocks) * block_size, Hkv, D]`` of the named blocks of a cache layer, for
@@ -102,21 +118,20 @@ class Kv8Pool:
 def _require_here(*tensors: torch.Tensor | None) -> None:
     """Every tensor on the current device, whose stream the launch goes to."""
 
-    here = None
+    devices = {t.get_device() for t in tensors if t is not None}
+    if len(devices) == 1 and -1 not in devices and torch._C._cuda_getDevice() in devices:
+        return
     for t in tensors:
-        if t is None:
-            continue
-        at = t.get_device()
-        if at < 0:
+        if t is not None and t.get_device() < 0:
             raise RuntimeError("CDB kernels run on the GPU only; got a tensor on " + str(t.device))
-        if here is None:
-            here = torch._C._cuda_getDevice()
-        if at != here:
+    here = torch._C._cuda_getDevice()
+    for t in tensors:
+        if t is not None and t.get_device() != here:
             raise RuntimeError(f"got a tensor on {t.device} while cuda:{here} is the current device")
 
 
 def _check_ints(name: str, t: torch.Tensor, n: int) -> None:
-    if t.dtype is not torch.int32:
+    if t.dtype is not _I32:
         raise TypeError(f"{name} must be int32, got {t.dtype}")
     if t.numel() != n or not t.is_contiguous():
         raise ValueError(f"{name} must be contiguous with {n} entries")
@@ -176,8 +191,7 @@ def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: t
     is padding, whose q_out is left as it was. A token left out between others of its tile (padding, a slot or
     position out of range) keeps its place in the call."""
 
-    heads_kv, dim, block = pool._shape
-    codes, scales, layers, blocks = pool._args
+    codes, scales, (layers, blocks, heads_kv, dim, block) = pool._resolve()
     shape, dt = k.shape, k.dtype
     if len(shape) != 3 or shape[1] != heads_kv or shape[2] != dim or v.shape != shape or v.dtype is not dt:
         raise ValueError(f"k and v must be [T, {heads_kv}, {dim}] of one dtype")
@@ -203,7 +217,7 @@ def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: t
     max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
     _check_bias("q_bias", q_bias, heads, dim, dt)
     _check_bias("k_bias", k_bias, heads_kv, dim, dt)
-    _require_here(q, k, v, q_out, pool.codes, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
+    _require_here(q, k, v, q_out, pool.codes, pool.scales, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
     kv_stride = _row_stride("k", k, tokens, heads_kv, dim)
     if _row_stride("v", v, tokens, heads_kv, dim) != kv_stride:
         raise ValueError("k and v must share one token stride")
@@ -255,8 +269,7 @@ def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
     without its chunking; ``workspace`` is any dense tensor of ``decode_workspace_bytes`` bytes. Calls that may
     overlap need a workspace each."""
 
-    heads_kv, dim, block = pool._shape
-    codes, scales, layers, blocks = pool._args
+    codes, scales, (layers, blocks, heads_kv, dim, block) = pool._resolve()
     shape, dt = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != dim:
         raise ValueError(f"q must be [rows, H, {dim}]")
@@ -283,8 +296,8 @@ def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
     _check_bias("k_bias", k_bias, heads_kv, dim, dt)
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _require_here(q, k_new, v_new, pool.codes, cache_layer, block_table, table_row, seqlens, rope_cos, rope_sin,
-                  q_bias, k_bias, out, workspace)
+    _require_here(q, k_new, v_new, pool.codes, pool.scales, cache_layer, block_table, table_row, seqlens, rope_cos,
+                  rope_sin, q_bias, k_bias, out, workspace)
     kv_stride = _row_stride("k_new", k_new, num_rows, heads_kv, dim)
     if _row_stride("v_new", v_new, num_rows, heads_kv, dim) != kv_stride:
         raise ValueError("k_new and v_new must share a row stride")
@@ -347,8 +360,7 @@ def prefill_attention_raw(q: torch.Tensor, pool: Kv8Pool, layer: int, block_tabl
     ``ops.prefill_attention_raw`` (``tile_seq[n] < 0``: no tile); ``splits`` from ``prefill_splits`` with a
     workspace of ``prefill_workspace_bytes`` bytes when above 1. Calls that may overlap need a workspace each."""
 
-    heads_kv, dim, block = pool._shape
-    codes, scales, layers, blocks = pool._args
+    codes, scales, (layers, blocks, heads_kv, dim, block) = pool._resolve()
     shape, dt = q.shape, q.dtype
     if len(shape) != 3 or shape[2] != dim or not q.is_contiguous():
         raise ValueError(f"q must be a contiguous [T, H, {dim}]")
@@ -368,7 +380,7 @@ def prefill_attention_raw(q: torch.Tensor, pool: Kv8Pool, layer: int, block_tabl
         raise ValueError("split launches need a workspace")
     if workspace is not None and not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _require_here(q, pool.codes, block_table, table_row, cu_q, past, tile_seq, tile_q0, out, workspace)
+    _require_here(q, pool.codes, pool.scales, block_table, table_row, cu_q, past, tile_seq, tile_q0, out, workspace)
     code = _lib.lib().cdb_kv8_prefill_attention(
         q.data_ptr(), codes, scales, layers, blocks, layer, block_table.data_ptr(), table_row.data_ptr(), table_rows,
         width, cu_q.data_ptr(), past.data_ptr(), num_seqs, tile_seq.data_ptr(), tile_q0.data_ptr(), num_tiles,
@@ -410,6 +422,9 @@ class BatchLayout:
     counts: torch.Tensor
 
     def __post_init__(self) -> None:
+        self._check()
+
+    def _check(self) -> None:
         tokens, tiles = self.positions.numel(), self.tile_seq.numel()
         for name, n in (("cu_q", max(1, self.cu_q.numel())), ("positions", tokens), ("tile_seq", tiles),
                         ("tile_q0", tiles), ("counts", 4)):
@@ -421,10 +436,27 @@ class BatchLayout:
         if len({t.device for t in (self.cu_q, self.positions, self.rows, self.tile_seq, self.tile_q0,
                                    self.counts)}) > 1:
             raise ValueError("a layout's buffers lie on one device")
-        # What every call needs of the buffers, resolved once.
-        self.__dict__["_args"] = (self.cu_q.data_ptr(), self.positions.data_ptr(), self.rows.data_ptr(), tokens,
-                                  self.tile_seq.data_ptr(), self.tile_q0.data_ptr(), tiles, self.counts.data_ptr())
-        self.__dict__["_num_seqs"] = self.cu_q.numel() - 1
+
+    @property
+    def _num_seqs(self) -> int:
+        return self.cu_q.numel() - 1
+
+    @property
+    def _args(self) -> tuple[int, int, int, int, int, int, int, int]:
+        """The C call's arguments, of the tensors as they are now. Every call asks: a layout may be a copy, or its
+        tensors may have been given other memory."""
+
+        cu_q, positions, rows, tile_seq, tile_q0, counts = (self.cu_q, self.positions, self.rows, self.tile_seq,
+                                                            self.tile_q0, self.counts)
+        tokens, tiles = positions.numel(), tile_seq.numel()
+        if rows.numel() != tokens or tile_q0.numel() != tiles or counts.numel() != 4 or cu_q.dtype is not _I32 \
+                or positions.dtype is not _I32 or rows.dtype is not _I64 or tile_seq.dtype is not _I32 \
+                or tile_q0.dtype is not _I32 or counts.dtype is not _I32 or not cu_q.is_contiguous() \
+                or not positions.is_contiguous() or not rows.is_contiguous() or not tile_seq.is_contiguous() \
+                or not tile_q0.is_contiguous() or not counts.is_contiguous():
+            self._check()
+        return (cu_q.data_ptr(), positions.data_ptr(), rows.data_ptr(), tokens, tile_seq.data_ptr(),
+                tile_q0.data_ptr(), tiles, counts.data_ptr())
 
     @classmethod
     def allocate(cls, num_seqs: int, token_capacity: int, tile_capacity: int,
@@ -437,13 +469,9 @@ class BatchLayout:
         # Outputs of a step, like those of an op: parts that need no tracking as views of each other.
         rows, positions, tile_seq, tile_q0, cu_q, counts = torch.unsafe_split_with_sizes(
             buffer, (ends[0], token_capacity, tile_capacity, tile_capacity, num_seqs + 1, 4))
-        at = buffer.data_ptr()
-        self = object.__new__(cls)  # its buffers are right by construction: no checks
-        self.__dict__.update(
-            cu_q=cu_q, positions=positions, rows=rows.view(torch.int64), tile_seq=tile_seq, tile_q0=tile_q0,
-            counts=counts, _num_seqs=num_seqs,
-            _args=(at + 4 * ends[3], at + 4 * ends[0], at, token_capacity, at + 4 * ends[1], at + 4 * ends[2],
-                   tile_capacity, at + 4 * ends[4]))
+        self = object.__new__(cls)  # its buffers are right by construction: checked by the call that uses them
+        self.__dict__.update(cu_q=cu_q, positions=positions, rows=rows.view(torch.int64), tile_seq=tile_seq,
+                             tile_q0=tile_q0, counts=counts)
         return self
 
 
@@ -469,7 +497,8 @@ def batch_layout_raw(past: torch.Tensor, lens: torch.Tensor, block_table: torch.
         _check_ints("table_row", table_row, num_seqs)
     elif table_rows < num_seqs:
         raise ValueError("block_table needs a row per request when table_row is not given")
-    _require_here(past, lens, block_table, table_row, free_blocks, layout.counts)
+    _require_here(past, lens, block_table, table_row, free_blocks, layout.cu_q, layout.positions, layout.rows,
+                  layout.tile_seq, layout.tile_q0, layout.counts)
     code = _lib.lib().cdb_batch_layout(
         past.data_ptr(), lens.data_ptr(), num_seqs, block_table.data_ptr(), _ptr(table_row), table_rows, width,
         free_blocks.data_ptr(), num_free, block_size, *layout._args, _stream())

@@ -2,8 +2,10 @@
 
 from __future__ import annotations
 
+import copy
 import ctypes
 import dataclasses
+import io
 
 import numpy as np
 import pytest
@@ -367,3 +369,97 @@ def test_oracle_codes_a_run_over_tokens_left_out() -> None:
         np.testing.assert_array_equal(got[slot], oracle.round_e4m3(k[t, 0] * 2.0 ** -float(top)))
     assert (got[[3] + list(range(6, 16))] == 3.0).all() and (got[:2] == oracle.round_e4m3(3.0 * 2.0 ** (-7.0 - top))).all()
     assert cache.exponents[0, 0, 0, 0] == oracle.tile_exponent(k[5])
+
+
+# -- a call reaches the memory that its tensors have when it is made ----------------------------------------------
+
+
+class _Recorder:
+    """Stands in for the library: keeps the last call's arguments and answers that all is well."""
+
+    def __getattr__(self, name):
+        def call(*args):
+            self.name, self.args = name, args
+            return 0
+        return call
+
+
+@pytest.fixture
+def recorder(monkeypatch):
+    r = _Recorder()
+    monkeypatch.setattr(kv8._lib, "lib", lambda: r)
+    monkeypatch.setattr(kv8, "_require_here", lambda *tensors: None)
+    monkeypatch.setattr(kv8, "_stream", lambda: 0)
+    return r
+
+
+def _deep(x):
+    return copy.deepcopy(x)
+
+
+def _saved(x):
+    buffer = io.BytesIO()
+    torch.save(x, buffer)
+    buffer.seek(0)
+    return torch.load(buffer, weights_only=False)
+
+
+def _moved(x):
+    """The same object, its tensors moved to other storages in place."""
+    for f in dataclasses.fields(x):
+        t = getattr(x, f.name)
+        t.data = t.detach().clone()
+    return x
+
+
+def _set(x):
+    for f in dataclasses.fields(x):
+        t = getattr(x, f.name)
+        t.set_(t.detach().clone())
+    return x
+
+
+ANOTHER = [_deep, _saved, _moved, _set, copy.copy]
+
+
+@pytest.mark.parametrize("another", ANOTHER)
+def test_calls_on_another_pool_reach_its_own_memory(recorder, another) -> None:
+    pool, q, k, rows, pos, cos = _python_args()
+    pool = another(pool)
+    own = (pool.codes.data_ptr(), pool.scales.data_ptr(), 1, 4)
+    kv8.write_raw(q, k, k, q, pool, 0, rows, pos, cos, cos, 1, None, None)
+    assert recorder.name == "cdb_kv8_write" and recorder.args[4:8] == own
+    table, ws = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8)
+    kv8.decode_attention_raw(q, k, k, pool, None, 0, table, None, pos, cos, cos, 1, None, None, q, ws, 0.1)
+    assert recorder.name == "cdb_kv8_decode_attention" and recorder.args[3:7] == own
+    cu, one = torch.tensor([0, 3], dtype=torch.int32), pos[:1]
+    kv8.prefill_attention_raw(q, pool, 0, table, one, cu, one, one, one, q, 0.1)
+    assert recorder.name == "cdb_kv8_prefill_attention" and recorder.args[1:5] == own
+
+
+@pytest.mark.parametrize("made,another", [(m, a) for m in ("allocated", "given") for a in ANOTHER
+                                          if (m, a) != ("allocated", _saved)])  # torch does not save such views
+def test_calls_on_another_layout_reach_its_own_memory(recorder, another, made) -> None:
+    a = kv8.BatchLayout.allocate(3, 8, 4, "cpu")
+    if made == "given":
+        a = kv8.BatchLayout(*(getattr(a, f.name).clone() for f in dataclasses.fields(a)))
+    a = another(a)
+    pos, free = torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    kv8.batch_layout_raw(pos, pos, torch.zeros(3, 2, dtype=torch.int32), None, free, 16, a)
+    assert recorder.args[-9:-1] == (a.cu_q.data_ptr(), a.positions.data_ptr(), a.rows.data_ptr(), 8,
+                                    a.tile_seq.data_ptr(), a.tile_q0.data_ptr(), 4, a.counts.data_ptr())
+
+
+def test_buffers_changed_after_they_were_checked_are_checked_again(recorder) -> None:
+    pool, q, k, rows, pos, cos = _python_args()
+    pool.codes.resize_(1, 2, 9, 2, 1, 1024)
+    with pytest.raises(ValueError, match="scales match"):
+        kv8.write_raw(q, k, k, q, pool, 0, rows, pos, cos, cos, 1, None, None)
+    free = torch.zeros(4, dtype=torch.int32)
+    for change in (lambda a: a.positions.resize_(9), lambda a: a.tile_q0.resize_(3), lambda a: a.counts.resize_(3),
+                   lambda a: a.cu_q.resize_(9), lambda a: a.rows.resize_(7)):
+        a = kv8.BatchLayout(*(getattr(x, f.name).clone() for x in [kv8.BatchLayout.allocate(3, 8, 4, "cpu")]
+                              for f in dataclasses.fields(x)))
+        change(a)
+        with pytest.raises(ValueError):
+            kv8.batch_layout_raw(pos, pos, torch.zeros(3, 2, dtype=torch.int32), None, free, 16, a)
