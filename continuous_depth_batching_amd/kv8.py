@@ -217,10 +217,10 @@ def write_raw(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, q_out: t
     max_positions = _check_rope(rope_style, rope_cos, rope_sin, dim)
     _check_bias("q_bias", q_bias, heads, dim, dt)
     _check_bias("k_bias", k_bias, heads_kv, dim, dt)
-    _require_here(q, k, v, q_out, pool.codes, pool.scales, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
     kv_stride = _row_stride("k", k, tokens, heads_kv, dim)
     if _row_stride("v", v, tokens, heads_kv, dim) != kv_stride:
         raise ValueError("k and v must share one token stride")
+    _require_here(q, k, v, q_out, pool.codes, pool.scales, rows, positions, rope_cos, rope_sin, q_bias, k_bias)
     code = _lib.lib().cdb_kv8_write(
         q_ptr or None, k.data_ptr(), v.data_ptr(), out_ptr or None, codes, scales, layers, blocks, layer,
         rows.data_ptr(), positions.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions,
@@ -296,17 +296,18 @@ def decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tens
     _check_bias("k_bias", k_bias, heads_kv, dim, dt)
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
-    _require_here(q, k_new, v_new, pool.codes, pool.scales, cache_layer, block_table, table_row, seqlens, rope_cos,
-                  rope_sin, q_bias, k_bias, out, workspace)
+    q_stride = _row_stride("q", q, num_rows, num_heads, dim)
     kv_stride = _row_stride("k_new", k_new, num_rows, heads_kv, dim)
     if _row_stride("v_new", v_new, num_rows, heads_kv, dim) != kv_stride:
         raise ValueError("k_new and v_new must share a row stride")
+    _require_here(q, k_new, v_new, pool.codes, pool.scales, cache_layer, block_table, table_row, seqlens, rope_cos,
+                  rope_sin, q_bias, k_bias, out, workspace)
     code = _lib.lib().cdb_kv8_decode_attention(
         q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), codes, scales, layers, blocks, _ptr(cache_layer),
         cache_layer0, block_table.data_ptr(), _ptr(table_row), table_rows, width, seqlens.data_ptr(),
         _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias), out.data_ptr(),
         workspace.data_ptr(), workspace.nbytes, num_rows, num_heads, heads_kv, dim, block, scale,
-        _row_stride("q", q, num_rows, num_heads, dim), kv_stride, dtype_code(dt), _stream())
+        q_stride, kv_stride, dtype_code(dt), _stream())
     if code:
         _lib.check(code, "cdb_kv8_decode_attention")
     return out

@@ -463,3 +463,46 @@ def test_buffers_changed_after_they_were_checked_are_checked_again(recorder) -> 
         change(a)
         with pytest.raises(ValueError):
             kv8.batch_layout_raw(pos, pos, torch.zeros(3, 2, dtype=torch.int32), None, free, 16, a)
+
+
+def _views(rows: int, heads: int, dim: int) -> dict[str, torch.Tensor]:
+    """Views that no call can read by a row stride and dense heads, with a word of what is said of each."""
+
+    whole = torch.zeros(rows, heads, 2 * dim)
+    return {
+        "contiguous heads": whole[..., ::2],
+        "contiguous heads ": whole[..., :dim],
+        "rows overlap": torch.zeros(1, heads, dim).expand(rows, heads, dim),
+        "rows overlap ": torch.zeros((rows + 1) * heads * dim).as_strided((rows, heads, dim), (dim, dim, 1)),
+    }
+
+
+@pytest.mark.parametrize("which", ["q", "k", "v"])
+@pytest.mark.parametrize("view", sorted(_views(3, 2, 64)))
+def test_write_and_decode_refuse_views_they_cannot_read(which, view) -> None:
+    pool, q, k, rows, pos, cos = _python_args()
+    given = dict(q=q, k=k, v=k) | {which: _views(3, 4 if which == "q" else 2, 64)[view]}
+    with pytest.raises(ValueError, match=view.strip()):
+        kv8.write_raw(*given.values(), q, pool, 0, rows, pos, cos, cos, 1, None, None)
+    table, ws = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8)
+    with pytest.raises(ValueError, match=view.strip()):
+        kv8.decode_attention_raw(*given.values(), pool, None, 0, table, None, pos, cos, cos, 1, None, None, q, ws, 0.1)
+
+
+def test_write_and_decode_refuse_keys_and_values_of_different_strides() -> None:
+    pool, q, k, rows, pos, cos = _python_args()
+    wide = torch.zeros(3, 5, 64)[:, :2]
+    for key, value in ((k, wide), (wide, k)):
+        with pytest.raises(ValueError, match="stride"):
+            kv8.write_raw(q, key, value, q, pool, 0, rows, pos, cos, cos, 1, None, None)
+        table, ws = torch.zeros(3, 2, dtype=torch.int32), torch.zeros(1 << 16, dtype=torch.uint8)
+        with pytest.raises(ValueError, match="stride"):
+            kv8.decode_attention_raw(q, key, value, pool, None, 0, table, None, pos, cos, cos, 1, None, None, q, ws,
+                                     0.1)
+
+
+def test_row_strides_that_calls_take() -> None:
+    assert kv8._row_stride("x", torch.zeros(3, 5, 64)[:, 1:3], 3, 2, 64) == 5 * 64
+    assert kv8._row_stride("x", torch.zeros(3, 2, 64), 3, 2, 64) == 2 * 64
+    assert kv8._row_stride("x", torch.zeros(3, 9, 64)[:, ::9], 3, 1, 64) == 9 * 64      # one head: its stride is free
+    assert kv8._row_stride("x", torch.zeros(1, 2, 64).expand(1, 2, 64), 1, 2, 64) == 2 * 64
