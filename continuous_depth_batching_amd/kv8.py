@@ -250,7 +250,8 @@ def _(q, k, v, codes, scales, layer, rows, positions, rope_cos, rope_sin, rope_s
 
 def decode_workspace_bytes(num_rows: int, num_heads: int, num_kv_heads: int, head_dim: int, max_seqlen: int) -> int:
     """Workspace of decode launches of up to ``num_rows`` rows whose positions are below ``max_seqlen``. Rows with
-    longer contexts are served too, in fewer and longer chunks."""
+    longer contexts are served too, in fewer and longer chunks, whose number (and with it the rounding of such a row)
+    depends on how many rows share the workspace; with this size, a row's bits do not depend on its batch."""
 
     n = int(_lib.lib().cdb_kv8_decode_workspace_bytes(num_rows, num_heads, num_kv_heads, head_dim, max_seqlen))
     if n < 0:
@@ -338,7 +339,8 @@ def _(q, k_new, v_new, codes, scales, cache_layer, cache_layer0, block_table, ta
 def prefill_splits(num_tiles: int, num_heads: int, num_kv_heads: int, longest: int, num_cus: int = 256) -> int:
     """Parts that a prefill launch cuts each tile's key range into: enough to give every CU two workgroups, while
     a part keeps at least 512 keys of the longest range ``longest`` (cached and new tokens of a sequence), and at
-    most 64. Heads that share keys take a workgroup each all the same, so ``num_kv_heads`` makes no difference."""
+    most 64. A sequence's rounding depends on the number of parts: pass a fixed one where that must not follow from
+    the batch. Heads that share keys take a workgroup each all the same, so ``num_kv_heads`` makes no difference."""
 
     del num_kv_heads
     want = -(-2 * num_cus // max(1, num_tiles * num_heads))

@@ -415,8 +415,9 @@ int cdb_kv8_write(const void* q, const void* k, const void* v, void* q_out, void
 
 /* Workspace bytes of cdb_kv8_decode_attention for positions below max_seqlen (-1 for invalid arguments): per row
  * and chunk of 1024 tokens (64 chunks at most) an fp32 partial of head_dim + 2 values a query head and 8 bytes a
- * KV head. A smaller workspace is legal down to one chunk a row: rows with more take longer chunks. Nothing in
- * it need be set before a call; calls that may overlap need one each. */
+ * KV head. A smaller workspace is legal down to one chunk a row: it has partials for workspace_bytes / num_rows, and
+ * rows with more chunks take longer ones. Nothing in it need be set before a call; calls that may overlap need one
+ * each. */
 int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
                                        int32_t max_seqlen);
 
@@ -426,8 +427,10 @@ int64_t cdb_kv8_decode_workspace_bytes(int32_t num_rows, int32_t num_heads, int3
  * positions 0..seqlens[b], its own included. Rows whose position, table row or cache layer is out of range get a
  * NaN output and no write; a row with a block in use outside the pool gets NaN, and writes its token where the
  * token's own block is inside. num_heads is a multiple of num_kv_heads. Two rows of a call never append to the same
- * tile, and none reads a tile that another appends to. A row's context is cut into chunks of 1024 tokens, merged in
- * order, so its output does not depend on the other rows. */
+ * tile, and none reads a tile that another appends to. A row's context is cut into chunks of 1024 tokens (64 at most,
+ * longer ones past that), merged in order, so its output does not depend on the other rows: with a workspace that the
+ * function above gives for at least the call's rows and positions. With a smaller one the chunks of rows that it is
+ * short for, and so their rounding, depend on num_rows too. */
 int cdb_kv8_decode_attention(const void* q, const void* k_new, const void* v_new, void* codes, void* scales,
                              int32_t num_cache_layers, int64_t pool_blocks, const int32_t* cache_layer,
                              int32_t cache_layer0, const int32_t* block_table, const int32_t* table_row,
@@ -445,7 +448,8 @@ int64_t cdb_kv8_prefill_workspace_bytes(int32_t num_tiles, int32_t splits, int32
 /* Varlen causal prefill attention over the 8-bit cache: the counterpart of cdb_prefill_attention, with its
  * sequences, block table and tiles of 128 query tokens (tile_seq[n] < 0: no tile). q [T, H, D] is rotated; the
  * chunk's own keys and values are already in the cache. splits > 1 cuts every tile's key range into that many
- * parts (at most 64), merged in order by a second launch: for few tiles with long histories. Queries of a sequence
+ * parts (at most 64), merged in order by a second launch: for few tiles with long histories. The rounding of a
+ * sequence's output depends on splits, and on nothing else of the other sequences. Queries of a sequence
  * whose table row is out of range or too short get NaN, and so do those that see a block outside the pool, with
  * the rest of their 32 in a tile. q and out are dense. */
 int cdb_kv8_prefill_attention(const void* q, const void* codes, const void* scales, int32_t num_cache_layers,

@@ -912,3 +912,33 @@ def test_write_leaves_tokens_out_inside_a_tile(dtype, heads, kv, dim, style, blo
     else:
         assert torch.equal(got[left], want[left])
     helpers.same_cache(c.pool, c.cache)
+
+
+@pytest.mark.parametrize("dtype,heads,kv", [("bf16", 4, 2), ("f32", 2, 1)])
+def test_decode_rows_keep_their_bits_over_a_workspace_that_is_large_enough(dtype, heads, kv) -> None:
+    """One workspace, sized for all rows and the longest context, past 64 chunks too: rows alone, in any order and in
+    any company give the same bits."""
+    contexts = [70_000, 5000, 1025, 3, 0, 2048, 66_000]
+    c = DecodeCase(67, dtype, heads, kv, 64, 1, False, 64, contexts, layers=1)
+    whole = c.run()
+    for rows in ([0], [1], [6, 0], [2, 1, 5], [5, 4, 3, 2, 1]):
+        r = torch.tensor(rows, device=DEV)
+        a = c.args()
+        part = c.run(q=c.q[r], k=c.k[r], v=c.v[r], layer=a["layer"][r], table=a["table"][r], pos=a["pos"][r],
+                     out=torch.empty_like(whole[r]))
+        assert torch.equal(part, whole[r])
+
+
+def test_prefill_sequences_keep_their_bits_in_any_batch() -> None:
+    """With the same number of parts."""
+    c = PrefillCase(68, "bf16", 4, 2, 128, 16, [(700, 60), (0, 200), (300, 1), (1500, 129)])
+    for splits in (1, 5):
+        whole = c.run(splits=splits)
+        for s in range(4):
+            mine = slice(c.cu[s], c.cu[s + 1])
+            seq, q0 = ops.prefill_tiles(c.new[s:s + 1], c.past[s:s + 1])
+            ws = torch.empty(kv8.prefill_workspace_bytes(len(seq), splits, 4, 128), dtype=torch.uint8, device=DEV)
+            part = kv8.prefill_attention_raw(c.q[mine], c.pool, c.layer, dev(c.table[s:s + 1]), dev([0], torch.int32),
+                                             dev([0, int(c.new[s])], torch.int32), dev(c.past[s:s + 1], torch.int32),
+                                             dev(seq), dev(q0), torch.empty_like(c.q[mine]), c.scale, splits, ws)
+            assert torch.equal(part, whole[mine])
