@@ -942,3 +942,28 @@ def test_prefill_sequences_keep_their_bits_in_any_batch() -> None:
                                              dev([0, int(c.new[s])], torch.int32), dev(c.past[s:s + 1], torch.int32),
                                              dev(seq), dev(q0), torch.empty_like(c.q[mine]), c.scale, splits, ws)
             assert torch.equal(part, whole[mine])
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 4, 2, 128), ("f32", 2, 2, 64)])
+def test_decode_rewrites_a_position_at_each_loop_step(dtype, heads, kv, dim) -> None:
+    """The same positions again with other keys and values, smaller and larger ones, as a looped model that keeps one
+    slot a position does: a tile keeps the larger scale, and starts anew at its first token."""
+    c = DecodeCase(69, dtype, heads, kv, dim, 1, False, 16, [1, 2, 16, 17, 40, 300, 0, 1030], nan=True)
+    rng = np.random.default_rng(70)
+    for std in (1.0, 0.05, 3.0, 0.3):
+        for t in (c.q, c.k, c.v):
+            t.copy_(helpers.values(rng, dtype, *t.shape, std=1.0 if t is c.q else std))
+        c.check()
+
+
+@pytest.mark.parametrize("dtype,heads,kv,dim", [("bf16", 4, 2, 64), ("f32", 2, 2, 96), ("bf16", 2, 1, 128)])
+@pytest.mark.parametrize("std,q_std", [(3.0, 1.5), (30.0, 0.05), (300.0, 0.006), (1e-4, 1.5)])
+def test_decode_peaked_scores_and_growing_scales(dtype, heads, kv, dim, std, q_std) -> None:
+    """New tokens that dwarf their tile's scale or vanish beside it, with queries of a size at which scores peak and a
+    computation's error stays small: the bound is at most a quarter of each result."""
+    c = DecodeCase(71, dtype, heads, kv, dim, 1, False, 16, [1, 2, 5, 16, 17, 18, 31, 270, 272, 273, 1500], std=std)
+    c.q.copy_(helpers.values(np.random.default_rng(72), dtype, *c.q.shape, std=q_std))
+    want, bound = c.expect()
+    assert (np.linalg.norm(bound, axis=-1) < np.linalg.norm(want, axis=-1) / 4).all()
+    helpers.close(c.run(), want, bound)
+    helpers.same_cache(c.pool, c.cache)
