@@ -231,6 +231,9 @@ CDB_DEVICE f16x8_t widen_f16(uint32_t w0, float s0, uint32_t w1, float s1) {
   return u.v;
 }
 
+// Scores of this size and more are spaced too widely for a raise: a sum with it would round by more than fp16 has room.
+constexpr float kWideScore = 0x1p22f;
+
 // fp32 models take probabilities as two fp16 parts. The second, what the first leaves, is raised by 2^11 and meets
 // values lowered by as much: it is then as large as the first, as far above fp16's smallest step. Values are raised by
 // 2^7 (448 * 2^7 is within fp16), which keeps the lowered ones exact down to scales 2^11 below the unit.

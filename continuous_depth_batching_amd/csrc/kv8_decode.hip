@@ -242,16 +242,17 @@ template <int D> struct QueryRegs<D, true> {
 template <int D, bool kWide> struct Attention {
   static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1;
   // Probabilities are counted in units of 2^-15, the largest then being 2^15, within fp16: its smallest step, 2^-24,
-  // stands for 2^-39.
+  // stands for 2^-39. That is, scores are counted from `low`, 15 below the maximum (0 below a very large one, where
+  // 15 would round to 16 or nothing, and keys that far below are gone in fp32 all the same).
   static constexpr int kRaise = 15;
   using Unit = ValueUnit<std::conditional_t<kWide, float, bf16_t>>;
-  float top, sum;
+  float top, low, sum;
   Unit unit;
   f32x4_t acc[kTiles];
 
   CDB_DEVICE void start() {
     top = -INFINITY;
-    sum = 0.f;
+    low = sum = 0.f;
     unit = Unit();
 #pragma unroll
     for (int m = 0; m < kTiles; ++m) acc[m] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
@@ -282,16 +283,17 @@ template <int D, bool kWide> struct Attention {
     for (int i = 0; i < 4; ++i) most = fmaxf(fmaxf(most, s[0][i]), s[1][i]);
     most = column_max(most);
     if (__any(most > top)) {
-      const float keep = __builtin_amdgcn_exp2f(top - most);
+      const float now = most - (fabsf(most) < kWideScore ? (float)kRaise : 0.f);
+      const float keep = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(low - now);  // the first count finds zeros
       sum *= keep;
       scale_acc(keep);
       top = most;
+      low = most == -INFINITY ? 0.f : now;
     }
-    const float lowered = top - (float)kRaise;
     float p[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - lowered);
+      p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - low);
       sum += p[i];
     }
 #pragma unroll
@@ -604,7 +606,7 @@ __global__ void __launch_bounds__(64 * kWaves, (kDecodeWaves<T, D>)) kv8_decode_
           *reinterpret_cast<f32x2_t*>(mine + ValueRegs<D>::element(m, 4 * g + i)) =
               (f32x2_t){ldexpf(state.acc[m][i], back), ldexpf(state.acc[m + 1][i], back)};
       if (g == 0) {
-        mine[D] = state.top;
+        mine[D] = sum == 0.f ? -INFINITY : state.low;  // no key yet, or none above -infinity
         mine[D + 1] = sum;
       }
     }

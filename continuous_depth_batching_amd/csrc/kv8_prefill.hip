@@ -234,7 +234,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
       if (__any(most * P.scale_log2 > limit)) {
         most = half_max(most) * P.scale_log2;
         const bool more = most > limit;
-        const float moved = kRaise - most;
+        const float moved = (fabsf(most) < kWideScore ? kRaise : 0.f) - most;
         const float keep = more && limit != -INFINITY ? __builtin_amdgcn_exp2f(moved - shift) : 1.f;
         sum *= keep;  // the first count finds zeros
 #pragma unroll
@@ -242,8 +242,14 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
         shift = more ? moved : shift;
         limit = more ? most + kSlack : limit;
       }
+      if (__any(fabsf(shift) >= kWideScore)) {
+        // Rounded as the maximum was, so that the difference is exact: a fused product keeps what here is many units.
 #pragma unroll
-      for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, shift));
+        for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(add_rn(mul_rn(sc[e], P.scale_log2), shift));
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[e] = __builtin_amdgcn_exp2f(fmaf(sc[e], P.scale_log2, shift));
+      }
 #pragma unroll
       for (int a = 0; a < 2; ++a) {
         const int t = key0 + kTile * a;

@@ -395,7 +395,7 @@ int cdb_coda_greedy(const int64_t* host_upload, int64_t* dev_upload, int32_t row
  * where it grows the earlier codes are rounded again. A tile written from its first token starts anew. Codes
  * behind the last token written stay as they are, and count for nothing. An infinity or NaN is held as NaN.
  * Rotations are computed in fp32, each product and sum rounded once, and not rounded to the storage type
- * before they are coded. */
+ * before they are coded. Scores past fp32's range are infinities, or NaN from 2^132 on. */
 
 /* Rotate and append a batch of tokens: q_out = rotate(q [+ q_bias]); rotate(k [+ k_bias]) and v are coded into
  * cache layer `layer` at slots rows[t] = block * block_size + offset. The 8-bit counterpart of

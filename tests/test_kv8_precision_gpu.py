@@ -240,3 +240,52 @@ def test_write_joins_a_tile_whose_scale_byte_is_outside_its_range(byte) -> None:
     kv8.write_raw(None, k.to(DEV), v.to(DEV), None, pool, 0, at.to(DEV), at.int().to(DEV), None, None, 0, None, None)
     cache.write(0, at.numpy(), k.numpy(), v.numpy())
     helpers.same_cache(pool, cache)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 128), ("bf16", 96)])
+@pytest.mark.parametrize("size", [21.7, 22.3, 23.4, 24.6, 25.5, 26.2, 27.8, 28.5, 31.1, 60.0, 110.0])
+@pytest.mark.parametrize("sign", [1.0, -1.0])
+def test_scores_of_any_size_pick_the_largest(kind, dtype, dim, size, sign) -> None:
+    """Scores of up to +-2^size, whose gaps are far past what any computation is off by: the result is the value of the
+    largest, and the mean of both where two are the same."""
+    rng = np.random.default_rng(76)
+    n, tiles = 600, 38
+    first = np.where(sign > 0, rng.uniform(0.0, 200.0, n), rng.uniform(-448.0, -300.0, n))
+    best, last = (448.0, 0.0) if sign > 0 else (-200.0, -440.0)
+    first[37] = first[520] = best
+    first[-40:] = np.minimum(first[-40:], last if sign < 0 else 200.0)
+    keys, values = line(rng, n, 2, dim, first)
+    q = np.zeros((1 if kind == "decode" else 40, 2, dim))
+    q[:, :, 0] = 2.0 ** (size - 8.8) * dim ** 0.5 * 16 * np.log(2.0)  # a key's code is 2^8.8 at most, over 16
+    s = Sequence(kind, dtype, 2, 2, dim, keys, values, np.full(tiles, -4), np.full(tiles, -6), q)
+    got = (s.run(*s.new_token(rng, key=-28.0 if sign < 0 else 0.0)) if kind == "decode" else s.run()).double().cpu()
+    v = s.cache.values(0, 1, s.at)
+    want, size = (v[37] + v[520]) / 2, (np.abs(v[37]) + np.abs(v[520])) / 2
+    # Probabilities leave 2^-11 (fp32 models 2^-23) of each term, which may cancel; products, sum, division and result
+    # round once each.
+    bound = (2.0 ** -8 * np.abs(want) + 2.0 ** -11 * size if dtype == "bf16" else (2.0 ** -23 + 4 * TINY) * size)
+    helpers.close(got, np.broadcast_to(want, got.shape), np.broadcast_to(bound, got.shape) + 2.0 ** -100)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("f32", 128)])
+def test_scores_of_minus_infinity_count_for_nothing(kind, dtype, dim) -> None:
+    """Keys whose scores overflow to minus infinity before others that do not.
+
+    They are some -2^128.4 (decode takes a query in parts, the second up to 2^-4 of the first and of either sign: from
+    2^132 on both overflow, and minus and plus infinity make NaN; no score exists in fp32 there)."""
+    rng = np.random.default_rng(77)
+    n, tiles = 600, 38
+    first = np.full(n, -448.0)
+    first[300:] = 0.0
+    keys, values = line(rng, n, 1, dim, first)
+    k_exp = np.where(np.arange(tiles) < 18, 60, -4)
+    q = np.zeros((1 if kind == "decode" else 40, 1, dim))
+    q[:, :, 0] = 2.0 ** 128.4 / (2.0 ** 68.8 * np.log2(np.e) * dim ** -0.5)
+    s = Sequence(kind, dtype, 1, 1, dim, keys, values, k_exp, np.full(tiles, -6), q)
+    got = (s.run(*s.new_token(rng)) if kind == "decode" else s.run()).double().cpu()
+    v = s.cache.values(0, 1, s.at)
+    end = np.arange(n - s.new, n)
+    want = np.stack([v[300:e + 1].mean(0) for e in end])
+    np.testing.assert_allclose(got.numpy(), want, rtol=0, atol=2.0 ** -8 * np.abs(want).max() + 2.0 ** -11 * np.abs(v).mean())
