@@ -79,11 +79,6 @@ template <int D> struct KeyRegs {
     for (int j = 0; j < kFull; ++j) *reinterpret_cast<u32x4_t*>(p + at(j, r, g)) = w[j];
     if constexpr (kTail) *reinterpret_cast<u32x2_t*>(p + kFull * 1024 + tail_lane(r, g)) = t;
   }
-  CDB_DEVICE void clear() {
-#pragma unroll
-    for (int j = 0; j < kFull; ++j) w[j] = (u32x4_t){0, 0, 0, 0};
-    if constexpr (kTail) t = (u32x2_t){0, 0};
-  }
   // Operand of the 128-deep product: the lane's D / 4 codes, and zeros up to 32.
   CDB_DEVICE i32x8_t operand() const {
     i32x8_t x = {0, 0, 0, 0, 0, 0, 0, 0};
