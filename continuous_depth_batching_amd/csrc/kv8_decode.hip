@@ -15,9 +15,9 @@
 //   Both products are 16 query heads wide (columns without a head repeat the last). A lane's four scores
 //   are those of the four tokens it holds of V, so P never moves.
 //
-// Measured (a launch from a graph): 256 rows of 32..2048 tokens, 16 heads x 128, 108 us (4.8 TB/s of cached
+// Measured (a launch from a graph): 256 rows of 32..2048 tokens, 16 heads x 128, 107-110 us (4.8 TB/s of cached
 // codes; 118 with chunks of 512 tokens, 128 with a merge launch of its own); 21 rows of 4k..32k tokens, 32 heads
-// on 8 x 128, 112 us (5.3 TB/s); one row of 900 tokens 9.3 us, a chain of latencies: position, block ids,
+// on 8 x 128, 113 us (5.2 TB/s); one row of 900 tokens 9.6-10.5 us, a chain of latencies: position, block ids,
 // tiles and query, 7 pairs a wave, the join. The same loads without arithmetic take 85 and 104 us.
 #include <atomic>
 #include <chrono>

@@ -13,15 +13,17 @@
 // both products, so maximum and sum are a lane's own and its neighbour's, 32 lanes away.
 //
 // Bound: instruction issue. A wave's block takes 16 matrix instructions of 32 cycles and some 180 vector ones of 4
-// (64 widen codes, 32 are fma and exponential), 770 cycles of a SIMD against 512 of its matrix core; two waves a
-// SIMD overlap them to 1270. Measured (a launch from a graph): two sequences of 6000..8190 tokens, 32 heads on
-// 8 x 128, 873 us (935 TFLOP/s; a large bf16 product reaches 1199); 24 fresh prompts of 24..1300 tokens, 16 heads,
-// 47 us, where the longest tile's chain of blocks is most of it; four chunks of some 110 tokens after 16000, cut in
-// 8 parts, 113 us. Slower or no faster: the scores on the codes themselves with queries of 3 e4m3 parts (876, 52 and
-// 116 us); blocks staged in LDS, 5 ahead, at 3 waves a SIMD (845, 52 and 124); waves of one workgroup parting the
-// keys of the same queries (927, 57 and 118); 64 queries a wave, which widens each code once for twice the queries
-// but leaves one wave a SIMD (1024, 80 and 131); products and vector instructions interleaved by hand (957, 76 and
-// 135); the tile list, longest first, from its end (957, 61 and 119); long tiles of fresh prompts in two parts (64).
+// (64 widen codes, 32 are fma and exponential): 512 cycles of a SIMD's matrix core and 770 of its issue, which the two
+// waves of a SIMD hardly overlap (1270 a block). Measured (a launch from a graph, on cards whose clocks differ; the
+// first launches after idling take up to 1060): two sequences of 6000..8190 tokens, 32 heads on 8 x 128, 870-950 us
+// (860-940 TFLOP/s; a large bf16 product reaches 1199); 24 fresh prompts of 24..1300 tokens, 16 heads, 43-48 us, where
+// the longest tile's chain of blocks is most of it; four chunks of some 110 tokens after 16000, cut in 8 parts,
+// 107-117 us; one of 8000 in fp32, 1070-1205. Tried on one card, where these took 873, 47 and 113, and were slower or
+// no faster: the scores on the codes themselves with queries of 3 e4m3 parts (876, 52 and 116 us); blocks staged in
+// LDS, 5 ahead, at 3 waves a SIMD (845, 52 and 124); waves of one workgroup parting the keys of the same queries (927,
+// 57 and 118); 64 queries a wave, which widens each code once for twice the queries but leaves one wave a SIMD (1024,
+// 80 and 131); products and vector instructions interleaved by hand (957, 76 and 135); the tile list, longest first,
+// from its end (957, 61 and 119); long tiles of fresh prompts in two parts (64).
 #include "cdb_amd.h"
 #include "kv8_common.h"
 #include "kv8_host.h"

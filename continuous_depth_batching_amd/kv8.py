@@ -2,7 +2,7 @@
 
 Keys and values are held in tiles of 16 tokens of one KV head as e4m3 codes with one power-of-two
 scale a tile (``include/cdb_amd.h``, "8-bit KV cache"): half the bytes of a bf16 cache, and three fifths
-of the time of a decode step's attention (256 rows, 16 heads x 128: 107 us a layer against 178). The calls
+of the time of a decode step's attention (256 rows, 16 heads x 128: 107-110 us a layer against 178). The calls
 mirror those of the pool in the model's type (``ops``): ``write`` beside ``rope_kv_write``, ``decode_attention``
 beside ``paged_decode_attention``, ``prefill_attention`` beside ``prefill_attention``; ``batch_layout`` builds
 on the GPU what they take as block tables, slots and attention tiles.
