@@ -238,8 +238,10 @@ template <int D, bool kWide> struct Attention {
   static constexpr int kTiles = D / 16, kPParts = kWide ? 2 : 1;
   // Probabilities are counted in units of 2^-15, the largest then being 2^15, within fp16: its smallest step, 2^-24,
   // stands for 2^-39. That is, scores are counted from `low`, 15 below the maximum (0 below a very large one, where
-  // 15 would round to 16 or nothing, and keys that far below are gone in fp32 all the same).
+  // 15 would round to 16 or nothing, and keys that far below are gone in fp32 all the same). fp32 models count from
+  // the maximum and raise by a product, which is exact: the 15 would cost an exponent near 0 three of its bits.
   static constexpr int kRaise = 15;
+  static constexpr float kFrom = kWide ? 0.f : (float)kRaise, kTimes = kWide ? 0x1p15f : 1.f;
   using Unit = ValueUnit<std::conditional_t<kWide, float, bf16_t>>;
   float top, low, sum;
   Unit unit;
@@ -278,7 +280,7 @@ template <int D, bool kWide> struct Attention {
     for (int i = 0; i < 4; ++i) most = fmaxf(fmaxf(most, s[0][i]), s[1][i]);
     most = column_max(most);
     if (__any(most > top)) {
-      const float now = most - (fabsf(most) < kWideScore ? (float)kRaise : 0.f);
+      const float now = most - (fabsf(most) < kWideScore ? kFrom : 0.f);
       const float keep = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(low - now);  // the first count finds zeros
       sum *= keep;
       scale_acc(keep);
@@ -289,6 +291,7 @@ template <int D, bool kWide> struct Attention {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       p[i] = __builtin_amdgcn_exp2f(s[i >> 2][i & 3] - low);
+      if constexpr (kWide) p[i] *= kTimes;
       sum += p[i];
     }
 #pragma unroll

@@ -130,6 +130,7 @@ CDB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x010101
 // How far scores may outgrow the maximum that the sums are counted from before they are counted anew, and what
 // probabilities are raised by: 2^15 is then the largest, within fp16, and its smallest step, 2^-24, stands for 2^-33.
 // Less slack moves more blocks (two sequences of 6000..8190 tokens: 908 us with 4, 900 with 6, 898 with 8).
+// fp32 models raise by a product, which is exact: in the exponent it would cost one near 0 some of its bits.
 constexpr float kSlack = 6.f, kRaise = 9.f;
 
 // Waves a SIMD: three where the registers allow it without spills (5000 tokens of 55 heads x 96, 360 us against 380);
@@ -236,7 +237,7 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
       if (__any(most * P.scale_log2 > limit)) {
         most = half_max(most) * P.scale_log2;
         const bool more = most > limit;
-        const float moved = (fabsf(most) < kWideScore ? kRaise : 0.f) - most;
+        const float moved = (!kWide && fabsf(most) < kWideScore ? kRaise : 0.f) - most;
         const float keep = more && limit != -INFINITY ? __builtin_amdgcn_exp2f(moved - shift) : 1.f;
         sum *= keep;  // the first count finds zeros
 #pragma unroll
@@ -267,7 +268,8 @@ __global__ void __launch_bounds__(256, (kPrefillWaves<T, D>)) kv8_prefill_kernel
         f16x8_t pp[kPParts];
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
-          const f32x2_t x2 = {sc[8 * a + e], sc[8 * a + e + 1]};
+          constexpr float kTimes = kWide ? 0x1p9f : 1.f;
+          const f32x2_t x2 = {sc[8 * a + e] * kTimes, sc[8 * a + e + 1] * kTimes};
           const f16x2_t y = __builtin_convertvector(x2, f16x2_t);
           pp[0][e] = y[0];
           pp[0][e + 1] = y[1];

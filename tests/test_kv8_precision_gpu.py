@@ -289,3 +289,35 @@ def test_scores_of_minus_infinity_count_for_nothing(kind, dtype, dim) -> None:
     end = np.arange(n - s.new, n)
     want = np.stack([v[300:e + 1].mean(0) for e in end])
     np.testing.assert_allclose(got.numpy(), want, rtol=0, atol=2.0 ** -8 * np.abs(want).max() + 2.0 ** -11 * np.abs(v).mean())
+
+
+@pytest.mark.parametrize("kind", ["decode", "prefill"])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_fp32_probabilities_are_as_exact_as_their_scores(kind, dim) -> None:
+    """Few keys whose scores are exact: what is left is the exponential and a few roundings.
+
+    Scores below the largest lie within 2 of it (in log2), so the exponential's argument rounds by 2^-24 at most (2^-21
+    and more if something were added to it first), which moves a probability by ln 2 of that; the scale's own
+    rounding and the product by it move the argument by 2^-23 of 4, all the same way; the exponential is within an
+    ulp, 2^-23. Parts leave 2^-23; six more roundings of sums, products and the division. Of |v|, weighed.
+    """
+    rng = np.random.default_rng(78)
+    n = 16
+    keys, values = line(rng, n, 2, dim, rng.integers(0, 9, n) * 8.0)  # 0..64 over 16
+    q = np.zeros((1 if kind == "decode" else 12, 2, dim))
+    q[:, :, 0] = 0.5 * dim ** 0.5 if dim == 64 else 4.0
+    got, want, mass = [], [], []
+    for seed in range(40):
+        values = oracle.round_e4m3(np.clip(rng.standard_normal((n, 2, dim)) * 90, -448, 448))
+        s = Sequence(kind, "f32", 2, 2, dim, keys, values, np.full(1, -4), np.full(1, -6), q, new=12)
+        got.append((s.run(*s.new_token(rng)) if kind == "decode" else s.run()).double().cpu().numpy())
+        k, v = (s.cache.values(0, plane, s.at) for plane in (0, 1))
+        end = np.arange(n - s.new, n)
+        w, _ = expect(s.q.double().cpu().numpy(), k, v, end, s.scale, **numerics(kind, "f32", dim, n))
+        m, _ = expect(s.q.double().cpu().numpy(), k, np.abs(v), end, s.scale, **numerics(kind, "f32", dim, n))
+        want.append(w), mass.append(m)
+    off = np.abs(np.array(got) - want) / np.array(mass)
+    assert off.max() <= (0.7 * 2.0 ** -24 + 4 * 2.0 ** -23 * 0.7 + 2.0 ** -23 + 2.0 ** -23 + 6 * TINY) * 2
+    # A rounding is some 0.4 * 2^-24 in the mean square. Those of single keys average out; three do not: the sum's, the
+    # division's and the result's.
+    assert np.sqrt((off ** 2).mean()) <= 0.75 * 2.0 ** -24
