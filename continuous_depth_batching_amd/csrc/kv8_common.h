@@ -243,8 +243,9 @@ template <typename T> constexpr int kValueRaise = sizeof(T) == 4 ? 7 : 0;
 // The unit that values are widened in and products with them counted in: 2^(ref - 127). fp16 holds the values of a
 // tile exactly if its scale is at most the unit and no more than 2^kExact below it, so the unit moves where a tile's
 // is not, and the accumulators, fp32, move with it: up with a larger scale, and down for a smaller one, but never
-// more than 2^60 below the largest scale met, so that 2^30 products of 2^31 at most stay within fp32. Values that
-// are 2^(60 + kExact) and more below the largest met lose bits, and vanish 2^9 below that.
+// more than 2^60 below the largest scale met, so that 2^30 products of 2^31 at most stay within fp32. Values of
+// tiles 2^(60 + kExact) and more below the largest scale met lose bits, the last of them 2^94 below it (fp32 models:
+// 2^101).
 template <typename T> struct ValueUnit {
   static constexpr int kExact = sizeof(T) == 4 ? 11 : 15, kDeep = 60;
   int ref = 1, met = 1;

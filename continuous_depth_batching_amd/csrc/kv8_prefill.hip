@@ -133,8 +133,8 @@ CDB_DEVICE uint32_t nan_bytes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x010101
 // fp32 models raise by a product, which is exact: in the exponent it would cost one near 0 some of its bits.
 constexpr float kSlack = 6.f, kRaise = 9.f;
 
-// Waves a SIMD: three where the registers allow it without spills (5000 tokens of 55 heads x 96, 360 us against 380);
-// for bf16 heads of 128 they would spill 27, and take 904 and 125 us for 900 and 113.
+// Waves a SIMD: three where the registers allow it (bf16 heads of 96 spill 2; 5000 tokens of 55 such heads took 360 us
+// against 380); bf16 heads of 128 would spill 27, and take 904 and 125 us for 900 and 113.
 template <typename T, int D> constexpr int kPrefillWaves = D == 64 || (sizeof(T) == 2 && D == 96) ? 3 : 2;
 
 template <typename T, int D>
