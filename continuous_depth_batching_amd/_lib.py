@@ -28,6 +28,7 @@ CDB_DECODE_SCRATCH_BYTES = 16 << 20  # include/cdb_amd.h
 CDB_DECODE_STAGE_PLAN = 1
 CDB_DECODE_STAGE_ATTEND = 2
 CDB_LAYOUT_MAX_SEQS = 4000
+CDB_SAMPLE_MAX_VOCAB = 1 << 20
 CDB_LAYOUT_TOKENS_FULL, CDB_LAYOUT_TILES_FULL, CDB_LAYOUT_NO_BLOCKS, CDB_LAYOUT_BAD_REQUEST = 1, 2, 4, 8
 
 _P = c_void_p
@@ -217,6 +218,15 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _P, _P, c_int32, _P, _P, c_int32, c_int32,  # past, lens, num_seqs, table, table_row, table rows, width
             _P, c_int32, c_int32, _P, _P, _P, c_int32,  # free, num_free, block_size, cu_q, positions, rows, capacity
             _P, _P, c_int32, _P, _P,  # tile_seq, tile_q0, tile_capacity, counts, stream
+        ],
+    ),
+    "cdb_sample_workspace_bytes": (c_int64, [c_int32, c_int32]),
+    "cdb_sample": (
+        c_int32,
+        [
+            _P, c_int64, _P, _P, _P, _P, _P,  # logits, row_stride, uniform, temperature, top_k, top_p, min_p
+            _P, _P, _P, c_int64,  # tokens, logprobs, workspace, workspace_bytes
+            c_int32, c_int32, c_int32, _P,  # rows, vocab, dtype, stream
         ],
     ),
 }

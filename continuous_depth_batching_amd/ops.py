@@ -795,6 +795,82 @@ def _(logits):
     return logits.new_empty(logits.shape[:-1], dtype=torch.int64)
 
 
+def sample_workspace_bytes(rows: int, vocab: int) -> int:
+    n = int(_lib.lib().cdb_sample_workspace_bytes(rows, vocab))
+    if n < 0:
+        raise ValueError(f"no sampling of {rows} rows of {vocab} logits (up to {_lib.CDB_SAMPLE_MAX_VOCAB})")
+    return n
+
+
+def sample_raw(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None,
+               top_k: torch.Tensor | None, top_p: torch.Tensor | None, min_p: torch.Tensor | None,
+               tokens: torch.Tensor, logprobs: torch.Tensor, workspace: torch.Tensor) -> None:
+    """Launch ``cdb_sample``: one token a row of logits [rows, vocab], drawn with ``uniform`` float64 [rows] in [0, 1).
+
+    ``temperature``, ``top_p`` and ``min_p`` float32 and ``top_k`` int32 have an entry a row, or are None (1 and no
+    filter); a temperature not above 0 is greedy. Kept are the ``top_k`` largest, of those the shortest beginning
+    (largest first, lower index first among equals) that holds ``top_p`` of their weight, and of those the ones that
+    weigh at least ``min_p`` times the largest. ``tokens`` int64 gets the token, -1 where every logit is -inf or NaN,
+    and ``logprobs`` float32 the logarithm of its share of the kept weight. Rows may lie apart. ``workspace``: any
+    dense tensor of ``sample_workspace_bytes`` bytes; calls that may overlap need one each."""
+
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    if vocab == 0 or (vocab > 1 and logits.stride(1) != 1) or (rows > 1 and logits.stride(0) < vocab):
+        raise ValueError("logits must have unit stride along a vocabulary of at least one token and rows apart")
+    for name, t, dtype in (("uniform", uniform, torch.float64), ("temperature", temperature, torch.float32),
+                           ("top_k", top_k, torch.int32), ("top_p", top_p, torch.float32),
+                           ("min_p", min_p, torch.float32), ("tokens", tokens, torch.int64),
+                           ("logprobs", logprobs, torch.float32)):
+        if t is None:
+            continue
+        if t.dtype is not dtype:
+            raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+        if t.shape != (rows,) or not t.is_contiguous():
+            raise ValueError(f"{name} must be contiguous with an entry per row")
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    kv8._require_here(logits, uniform, temperature, top_k, top_p, min_p, tokens, logprobs, workspace)
+    code = _lib.lib().cdb_sample(logits.data_ptr(), logits.stride(0), uniform.data_ptr(), _ptr(temperature),
+                                 _ptr(top_k), _ptr(top_p), _ptr(min_p), tokens.data_ptr(), logprobs.data_ptr(),
+                                 workspace.data_ptr(), workspace.nbytes, rows, vocab, dtype_code(logits.dtype),
+                                 _stream())
+    if code:
+        _lib.check(code, "cdb_sample")
+
+
+@torch.library.custom_op("cdb::sample", mutates_args=(), device_types="cuda")
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.Tensor | None, top_k: torch.Tensor | None,
+           top_p: torch.Tensor | None, min_p: torch.Tensor | None) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens int64 [rows] drawn from logits [rows, vocab], and their log-probabilities; see ``sample_raw``."""
+
+    if logits.dim() != 2:
+        raise ValueError("logits must be [rows, vocab]")
+    rows, vocab = logits.shape
+    tokens = torch.empty(rows, dtype=torch.int64, device=logits.device)
+    logprobs = torch.empty(rows, dtype=torch.float32, device=logits.device)
+    workspace = torch.empty(sample_workspace_bytes(rows, vocab), dtype=torch.uint8, device=logits.device)
+    sample_raw(logits, uniform, temperature, top_k, top_p, min_p, tokens, logprobs, workspace)
+    return tokens, logprobs
+
+
+@sample.register_fake
+def _(logits, uniform, temperature, top_k, top_p, min_p):
+    rows = logits.shape[0]
+    return logits.new_empty(rows, dtype=torch.int64), logits.new_empty(rows, dtype=torch.float32)
+
+
+def lm_head_sample(x: torch.Tensor, weight: torch.Tensor, packed: torch.Tensor | None, uniform: torch.Tensor,
+                   temperature: torch.Tensor | None = None, top_k: torch.Tensor | None = None,
+                   top_p: torch.Tensor | None = None, min_p: torch.Tensor | None = None
+                   ) -> tuple[torch.Tensor, torch.Tensor]:
+    """Tokens of a coda batch drawn from the logits x @ weight.T, and their log-probabilities: ``lm_head_argmax``
+    for sampled requests; arguments as ``sample_raw``."""
+
+    return torch.ops.cdb.sample(linear_auto(x, weight, packed, False), uniform, temperature, top_k, top_p, min_p)
+
+
 @dataclass
 class GateState:
     """Device-resident exit-policy state, one entry per hidden-bank slot."""

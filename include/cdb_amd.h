@@ -487,6 +487,34 @@ int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs,
                      int32_t token_capacity, int32_t* tile_seq, int32_t* tile_q0, int32_t tile_capacity,
                      int32_t* counts, hipStream_t stream);
 
+/* ---------------------------------------------------------------------------
+ * Drawing tokens
+ * ------------------------------------------------------------------------ */
+
+enum { CDB_SAMPLE_MAX_VOCAB = 1 << 20 };
+
+/* Workspace bytes of cdb_sample (-1 for invalid arguments). */
+int64_t cdb_sample_workspace_bytes(int32_t rows, int32_t vocab);
+
+/* One token a row of logits [rows, vocab] (rows row_stride elements apart), drawn with the given numbers uniform
+ * [rows] in [0, 1): beside cdb_argmax, which takes the largest. Token i weighs exp((x_i - max x) / temperature);
+ * tokens are ordered by logit, the larger first and the lower index among equals.
+ *   top_k: the first k of the order are kept (0 and less, or vocab and more: all);
+ *   top_p: of those, the shortest beginning that holds top_p of what they weigh together, one token at least
+ *   (1 and more: all);
+ *   min_p: of those, the ones that weigh at least min_p times the largest (0 and less: all; 1 and more: its equals).
+ * Drawn is the first kept token, by index, at which the running weight of the kept ones passes uniform times their
+ * total; numbers outside [0, 1) count as the nearest inside. temperature, top_k, top_p and min_p have an entry a row,
+ * or are null: 1 and no filter. A temperature not above 0 takes the first token of the order (the index cdb_argmax
+ * gives, where no logit is NaN). Logits of -infinity and NaN are never drawn; where one is +infinity only such are.
+ * tokens [rows]; logprobs [rows]: the logarithm of the drawn token's share of the kept weight. A row without a token
+ * to draw gets -1 and -infinity. Weights are counted in units of 2^-46 of the largest (vocabularies above 65536: of
+ * 2^-(62 - ceil(log2 vocab))) and summed exactly, so a row's token depends on nothing but the row. */
+int cdb_sample(const void* logits, int64_t row_stride, const double* uniform, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs,
+               void* workspace, int64_t workspace_bytes, int32_t rows, int32_t vocab, int32_t dtype,
+               hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1,0 +1,204 @@
+"""Sampled tokens (cdb_sample through torch.ops.cdb.sample and ops.sample_raw) against the float64 definition.
+
+Tokens have to be equal: the kernel's weights are exact to 2^-44 of themselves and 2^-47 of the largest, so it could
+differ only where the given number, or p, falls within about V * 2^-47 of a border between two tokens. The numbers are
+drawn from a fixed seed and fall on no such border, or exactly on one that both sides compute exactly. A log-probability
+is the fp32 rounding of a value off by 2^-40 at most: 2^-24 relative, and 2^-38 near 0."""
+
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from continuous_depth_batching_amd import ops
+from oracle import sampling
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def run(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    rows = logits.shape[0]
+
+    def dev(v, dtype):
+        if v is None:
+            return None
+        return torch.as_tensor(np.broadcast_to(np.asarray(v), (rows,)).copy()).to(dtype).to(DEV)
+
+    tok, lp = torch.ops.cdb.sample(logits.to(DEV), dev(u, torch.float64), dev(temperature, torch.float32),
+                                   dev(top_k, torch.int32), dev(top_p, torch.float32), dev(min_p, torch.float32))
+    return tok.cpu(), lp.cpu()
+
+
+def check(logits, u, temperature=None, top_k=None, top_p=None, min_p=None):
+    got, lp = run(logits, u, temperature, top_k, top_p, min_p)
+    x = logits.double().cpu().numpy()
+    rows = x.shape[0]
+
+    def at(v, r, default, f32):
+        if v is None:
+            return default
+        y = np.broadcast_to(np.asarray(v), (rows,))[r]
+        return float(np.float32(y)) if f32 else y
+
+    for r in range(rows):
+        token, logprob = sampling.draw(x[r], float(at(u, r, 0.0, False)), at(temperature, r, 1.0, True),
+                                       int(at(top_k, r, 0, False)), at(top_p, r, 1.0, True), at(min_p, r, 0.0, True))
+        assert int(got[r]) == token, (r, int(got[r]), token)
+        if math.isinf(logprob):
+            assert float(lp[r]) == logprob
+        else:
+            assert abs(float(lp[r]) - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -38, (r, float(lp[r]), logprob)
+
+
+def logits_of(rows, vocab, dtype, seed, spread=2.5):
+    gen = torch.Generator().manual_seed(seed)
+    x = torch.randn(rows, vocab, generator=gen) * spread
+    x[:, ::max(1, vocab // 9)] += 2 * spread
+    return x.to(dtype)
+
+
+FILTERS = {
+    "none": {},
+    "temperature": dict(temperature=[0.3, 0.7, 1.0, 2.0, 40.0]),
+    "top_k": dict(top_k=[1, 2, 7, 100, 5000]),
+    "top_p": dict(top_p=[0.05, 0.5, 0.9, 0.99, 0.9999]),
+    "min_p": dict(min_p=[0.01, 0.1, 0.5, 0.999, 1.0]),
+    "all": dict(temperature=[0.6, 0.8, 1.0, 1.3, 0.0], top_k=[5, 50, 0, 1000, 3], top_p=[0.9, 0.5, 0.95, 0.8, 0.3],
+                min_p=[0.0, 0.02, 0.1, 0.05, 0.5]),
+}
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [1, 2, 7, 63, 1025, 8191, 50001])
+@pytest.mark.parametrize("name", sorted(FILTERS))
+def test_matches_definition(name, vocab, dtype):
+    u = np.random.default_rng(vocab).random(5)
+    check(logits_of(5, vocab, dtype, seed=vocab), u, **FILTERS[name])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_equal_logits_go_by_index(dtype):
+    # Every logit the same, more of them than a list holds: borders are whole numbers, computed exactly by both.
+    vocab = 40000
+    x = torch.zeros(4, vocab, dtype=dtype)
+    check(x, [0.0, 0.5, 0.25, 0.999], top_k=[3, 30000, 0, 0], top_p=[1.0, 1.0, 0.5, 0.125])
+    check(x[:1], [0.9999999], top_k=[1])
+    got, _ = run(x, [0.5, 0.5, 0.5, 0.5], temperature=[0.0] * 4)
+    assert got.tolist() == [0, 0, 0, 0]
+
+
+def test_zeros_of_both_signs_are_equal():
+    x = torch.tensor([[-0.0, 0.0, -0.0, 0.0, -1.0]], dtype=torch.float32)
+    for u in (0.0, 0.3, 0.6, 0.99):
+        check(x, [u], top_k=[2])
+    check(x, [0.9], temperature=[0.0])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("name", sorted(FILTERS))
+def test_masked_infinite_and_nan_logits(name, dtype):
+    x = logits_of(5, 4099, dtype, seed=5)
+    x[0, 1:] = -math.inf                      # one token left
+    x[1] = -math.inf                          # nothing left
+    x[2, 100:] = float("nan")                 # NaN is never drawn
+    x[3, [7, 400, 4000]] = math.inf           # only these
+    x[4, :] = torch.finfo(dtype).min          # the lowest value is a value
+    x[4, 17] = -math.inf
+    u = [0.7, 0.5, 0.3, 0.8, 0.9]
+    check(x, u, **FILTERS[name])
+    nan = torch.full((1, 33), float("nan"), dtype=dtype)
+    got, lp = run(nan, [0.5])
+    assert got.tolist() == [-1] and lp.tolist() == [-math.inf]
+
+
+def test_extreme_temperatures_and_parameters():
+    x = logits_of(6, 3001, torch.float32, seed=9)
+    inf, nan = math.inf, float("nan")
+    check(x, [0.2, 0.4, 0.6, 0.8, 0.1, 0.9], temperature=[1e-30, 1e30, 1e-3, 1e-38, 300.0, 1.0],
+          top_k=[-3, 0, 3000, 3001, 2 ** 31 - 1, 4])
+    got, _ = run(x, [0.5] * 6, temperature=[-1.0, nan, 0.0, inf, 1.0, 1.0], top_p=[1, 1, 1, 1, -1.0, 0.0],
+                 min_p=[0, 0, 0, 0, -1.0, 7.0])
+    best = x.argmax(dim=1)
+    for r in (0, 1, 2, 4, 5):
+        assert int(got[r]) == int(best[r])
+    assert int(got[3]) == 1500  # an endless temperature makes all 3001 tokens equal
+    big = torch.tensor([[3e38, -3e38, 2.9e38, 0.0]])
+    check(big, [0.5], temperature=[1e38])
+    check(big, [0.99], temperature=[1e38], top_p=[0.95])
+
+
+def test_numbers_outside_the_unit_interval_are_the_nearest_inside():
+    x = logits_of(4, 999, torch.float32, seed=2, spread=0.5)
+    got, _ = run(x, [-3.0, float("nan"), 1.0, 8.0])
+    assert got[:2].tolist() == [0, 0] and got[2:].tolist() == [998, 998]
+
+
+def test_frequencies_follow_the_weights():
+    # 200000 evenly spread numbers: each token's count is its share to within one number.
+    x = torch.tensor([[0.3, -math.inf, 1.7, -0.5, 1.7, 0.0]])
+    n = 200000
+    u = (np.arange(n) + 0.5) / n
+    got, _ = run(x.expand(n, 6).contiguous(), u)
+    counts = torch.bincount(got, minlength=6).double()
+    assert (counts - torch.softmax(x[0].double(), 0) * n).abs().max() <= 1
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("offset", [0, 1, 3, 7])
+def test_strided_and_unaligned_rows(dtype, offset):
+    base = logits_of(3, 2100, dtype, seed=offset).to(DEV)
+    view = base[:, offset:offset + 2050 - offset]
+    u = np.random.default_rng(offset).random(3)
+    check(view, u, top_k=[40, 0, 900], top_p=[0.9, 0.9, 1.0])
+
+
+def test_rows_do_not_depend_on_the_batch_and_captured_calls_repeat():
+    x = logits_of(40, 20000, torch.bfloat16, seed=4).to(DEV)
+    u = torch.rand(40, dtype=torch.float64, generator=torch.Generator().manual_seed(1)).to(DEV)
+    t = torch.full((40,), 0.8, device=DEV)
+    p = torch.full((40,), 0.9, device=DEV)
+    tok = torch.empty(40, dtype=torch.int64, device=DEV)
+    lp = torch.empty(40, device=DEV)
+    ws = torch.empty(ops.sample_workspace_bytes(40, 20000), dtype=torch.uint8, device=DEV)
+    ops.sample_raw(x, u, t, None, p, None, tok, lp, ws)
+    eager, eager_lp = tok.clone(), lp.clone()
+    for r in (0, 17, 39):
+        one, one_lp = torch.ops.cdb.sample(x[r:r + 1], u[r:r + 1], t[:1], None, p[:1], None)
+        assert int(one) == int(eager[r]) and float(one_lp) == float(eager_lp[r])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        ops.sample_raw(x, u, t, None, p, None, tok, lp, ws)
+    for _ in range(3):
+        tok.fill_(-7)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(tok, eager) and torch.equal(lp, eager_lp)
+    u.copy_(u.flip(0))
+    graph.replay()
+    again, _ = torch.ops.cdb.sample(x, u, t, None, p, None)
+    assert torch.equal(tok, again)
+
+
+def test_lm_head_sample_draws_from_its_logits():
+    gen = torch.Generator().manual_seed(3)
+    w = (torch.randn(4096, 256, generator=gen) * 0.2).bfloat16().to(DEV)
+    x = torch.randn(6, 256, generator=gen).bfloat16().to(DEV)
+    u = torch.rand(6, dtype=torch.float64, generator=gen).to(DEV)
+    packed = ops.maybe_pack_linear_weight(w)
+    tok, lp = ops.lm_head_sample(x, w, packed, u, top_p=torch.full((6,), 0.8, device=DEV))
+    logits = torch.ops.cdb.linear(x, w, packed, False)
+    for r in range(6):
+        token, logprob = sampling.draw(logits[r].double().cpu().numpy(), float(u[r]), top_p=float(np.float32(0.8)))
+        assert int(tok[r]) == token and abs(float(lp[r]) - logprob) <= 2.0 ** -24 * abs(logprob) + 2.0 ** -38
+    cold, _ = ops.lm_head_sample(x, w, packed, u, temperature=torch.zeros(6, device=DEV))
+    assert torch.equal(cold, ops.lm_head_argmax(x, w, packed))
+
+
+def test_no_rows():
+    tok, lp = torch.ops.cdb.sample(torch.empty(0, 9, device=DEV), torch.empty(0, dtype=torch.float64, device=DEV),
+                                   None, None, None, None)
+    assert tok.shape == (0,) and lp.shape == (0,)
