@@ -45,6 +45,7 @@ FILE_FLAGS = {
     "prefill_attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kv8_prefill.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "kv8_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "prefix_decode.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 

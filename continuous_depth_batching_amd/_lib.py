@@ -28,6 +28,7 @@ CDB_DECODE_SCRATCH_BYTES = 16 << 20  # include/cdb_amd.h
 CDB_DECODE_STAGE_PLAN = 1
 CDB_DECODE_STAGE_ATTEND = 2
 CDB_LAYOUT_MAX_SEQS = 4000
+CDB_PREFIX_QUERIES, CDB_PREFIX_MAX_PARTS = 16, 64
 CDB_SAMPLE_MAX_VOCAB = 1 << 20
 CDB_LAYOUT_TOKENS_FULL, CDB_LAYOUT_TILES_FULL, CDB_LAYOUT_NO_BLOCKS, CDB_LAYOUT_BAD_REQUEST = 1, 2, 4, 8
 
@@ -218,6 +219,20 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _P, _P, c_int32, _P, _P, c_int32, c_int32,  # past, lens, num_seqs, table, table_row, table rows, width
             _P, c_int32, c_int32, _P, _P, _P, c_int32,  # free, num_free, block_size, cu_q, positions, rows, capacity
             _P, _P, c_int32, _P, _P,  # tile_seq, tile_q0, tile_capacity, counts, stream
+        ],
+    ),
+    "cdb_prefix_decode_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
+    "cdb_prefix_decode_attention": (
+        c_int32,
+        [
+            _P, _P, _P, _P, _P,  # q, k_new, v_new, k_pool, v_pool
+            c_int64, c_int32, c_int64, _P, c_int32,  # layer_stride, layers, pool_blocks, cache_layer, cache_layer0
+            _P, _P, c_int32, c_int32, _P,  # block_table, table_row, table_rows, table_width, seqlens
+            _P, _P, c_int32, c_int32, _P, _P,  # rope_cos, rope_sin, rope_style, max_positions, q_bias, k_bias
+            _P, c_int32, _P, c_int32, _P, c_int32, _P,  # listed, n, groups, n, items, n, row_info
+            _P, _P, c_int64,  # out, workspace, workspace_bytes
+            c_int32, c_int32, c_int32, c_int32, c_int32,  # rows, H, Hkv, D, block_size
+            c_float, c_int64, c_int64, c_int32, _P,  # scale, q_stride, kv_stride, dtype, stream
         ],
     ),
     "cdb_sample_workspace_bytes": (c_int64, [c_int32, c_int32]),

@@ -258,6 +258,202 @@ def _(q, k_new, v_new, kv_pool, cache_layer, cache_layer0, block_table, table_ro
     return torch.empty_like(q)
 
 
+# ---------------------------------------------------------------------------
+# Decode attention of rows that share prefixes.
+# ---------------------------------------------------------------------------
+
+PREFIX_QUERIES = _lib.CDB_PREFIX_QUERIES
+
+
+@dataclass(frozen=True)
+class PrefixDecodePlan:
+    """Work list of ``prefix_decode_attention_raw`` (include/cdb_amd.h, cdb_prefix_decode_attention), as numpy arrays or,
+    after ``to``, int32 tensors: it names rows and prefixes, not positions, so it serves every layer and every step in
+    which the rows, their order and their prefixes stay.
+
+    listed    [n] rows with a prefix, group by group
+    groups    [groups, 4]: (first place in listed, rows, tokens of the prefix, first item)
+    items     [m, 4]: (group, first query, first token, end token)
+    row_info  [rows, 4]: (first query in the group, tokens of the prefix, the group's first item, parts)
+    """
+
+    listed: "np.ndarray | torch.Tensor"
+    groups: "np.ndarray | torch.Tensor"
+    items: "np.ndarray | torch.Tensor"
+    row_info: "np.ndarray | torch.Tensor"
+
+    @property
+    def num_rows(self) -> int:
+        return self.row_info.shape[0]
+
+    @property
+    def num_items(self) -> int:
+        return self.items.shape[0]
+
+    def to(self, device: torch.device | str) -> "PrefixDecodePlan":
+        """The plan on a device, by one copy."""
+
+        import numpy as np
+
+        arrays = [np.asarray(a, dtype=np.int32) for a in (self.listed, self.groups, self.items, self.row_info)]
+        flat = torch.from_numpy(np.concatenate([a.ravel() for a in arrays])).to(device)
+        parts = flat.split([a.size for a in arrays])
+        return PrefixDecodePlan(*(x.view(a.shape) for x, a in zip(parts, arrays)))
+
+
+def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np.ndarray", *, num_heads: int,
+                       num_kv_heads: int, num_cus: int = 256) -> PrefixDecodePlan:
+    """The work list of a decode batch: row b belongs to group ``group[b]`` (negative: to none) and begins with that
+    group's ``lengths[group[b]]`` tokens. Rows of one group sit at the same cache layer: rows at two loop depths of a
+    layout with a slot a step are two groups.
+
+    Prefixes are cut into parts of about equal length, enough of them to give every CU two workgroups while a part
+    keeps 128 tokens, and at most 64. A row's rounding depends on its prefix's parts."""
+
+    import numpy as np
+
+    group = np.asarray(group, dtype=np.int64).reshape(-1)
+    lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
+    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
+        raise ValueError(f"{num_heads} query heads cannot share {num_kv_heads} KV heads evenly")
+    if group.size and int(group.max()) >= lengths.size:
+        raise ValueError(f"row in group {int(group.max())} of {lengths.size}")
+    if lengths.size and (int(lengths.min()) < 0 or int(lengths.max()) > 1 << 30):
+        raise ValueError("prefixes have from 0 to 2 ** 30 tokens")
+    share = num_heads // num_kv_heads
+    order = np.argsort(group, kind="stable")
+    order = order[group[order] >= 0]
+    order = order[lengths[group[order]] > 0]  # a prefix of no tokens is none
+    info = np.zeros((group.size, 4), dtype=np.int64)
+    names, first, counts = np.unique(group[order], return_index=True, return_counts=True)
+    tokens = lengths[names]
+    runs = (counts * share + PREFIX_QUERIES - 1) // PREFIX_QUERIES
+    each = max(128, -(-int((runs * tokens).sum()) * num_kv_heads // (2 * int(num_cus))))
+    parts = np.minimum(-(-tokens // each), _lib.CDB_PREFIX_MAX_PARTS)
+    items, groups = [], []
+    for n, (at, count, length, run, part) in enumerate(zip(first.tolist(), counts.tolist(), tokens.tolist(),
+                                                           runs.tolist(), parts.tolist())):
+        item0 = len(items)
+        groups.append((at, count, length, item0))
+        step = -(-length // part)
+        step = -(-step // 32) * 32
+        part = -(-length // step)
+        ends = [min(length, (k + 1) * step) for k in range(part)]
+        items.extend((n, q * PREFIX_QUERIES, k * step, ends[k]) for q in range(run) for k in range(part))
+        rows = order[at:at + count]
+        info[rows, 0] = np.arange(count) * share
+        info[rows, 1], info[rows, 2], info[rows, 3] = length, item0, part
+    def array(a, shape):
+        return np.asarray(a, dtype=np.int32).reshape(shape)
+    return PrefixDecodePlan(listed=array(order, -1), groups=array(groups, (-1, 4)), items=array(items, (-1, 4)),
+                            row_info=array(info, (-1, 4)))
+
+
+def prefix_decode_workspace_bytes(plan: PrefixDecodePlan, num_heads: int, num_kv_heads: int, head_dim: int,
+                                  max_own: int) -> int:
+    """Workspace of launches of this plan whose rows hold up to ``max_own`` tokens behind their prefix, the new one
+    among them. Rows with more are served too; the number of their chunks, and with it their rounding, then depends
+    on how many rows share the workspace."""
+
+    n = int(_lib.lib().cdb_prefix_decode_workspace_bytes(plan.num_rows, plan.num_items, num_heads, num_kv_heads,
+                                                         head_dim, max_own))
+    if n < 0:
+        raise ValueError("invalid arguments for the workspace size")
+    return n
+
+
+def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, view: KVPoolView,
+                                cache_layer: torch.Tensor | None, cache_layer0: int, block_table: torch.Tensor,
+                                table_row: torch.Tensor | None, seqlens: torch.Tensor,
+                                rope_cos: torch.Tensor | None, rope_sin: torch.Tensor | None, rope_style: int,
+                                q_bias: torch.Tensor | None, k_bias: torch.Tensor | None, plan: PrefixDecodePlan,
+                                out: torch.Tensor, workspace: torch.Tensor, scale: float) -> torch.Tensor:
+    """Launch ``cdb_prefix_decode_attention`` (no allocation): ``paged_decode_attention_raw`` for rows of which some
+    begin with the same tokens, named by ``plan`` (``prefix_decode_plan``, on the device). Append each row's new token
+    at position ``seqlens[b]`` and attend over positions 0..seqlens[b] (negative: a padding row, zero output); a group's
+    common tokens are read once, through its first row's table row. ``workspace`` is any dense tensor of
+    ``prefix_decode_workspace_bytes`` bytes. Calls that may overlap need a workspace each."""
+
+    pool, block = view.pool, view.block_size
+    if pool.dim() != 5 or pool.shape[1] != 2 or not pool.is_contiguous():
+        raise ValueError("the pool must be a contiguous [layers, 2, rows, Hkv, D] tensor")
+    layers, _, pool_rows, heads_kv, dim = pool.shape
+    if block < 16 or block & (block - 1) or pool_rows % block:
+        raise ValueError(f"block_size must be a power of two of at least 16 that divides the pool's rows, got {block}")
+    shape, dt = q.shape, q.dtype
+    if len(shape) != 3 or shape[2] != dim:
+        raise ValueError(f"q must be [rows, H, {dim}]")
+    num_rows, num_heads = shape[0], shape[1]
+    if k_new.shape != (num_rows, heads_kv, dim) or v_new.shape != k_new.shape:
+        raise ValueError(f"k_new and v_new must be [{num_rows}, {heads_kv}, {dim}]")
+    if k_new.dtype is not dt or v_new.dtype is not dt or pool.dtype is not dt:
+        raise TypeError("q, k_new, v_new and the pool must share a dtype")
+    if num_heads == 0 or num_heads % heads_kv:
+        raise ValueError(f"{num_heads} query heads cannot share {heads_kv} KV heads evenly")
+    if out.shape != shape or out.dtype is not dt or not out.is_contiguous():
+        raise ValueError("out must be contiguous and match q")
+    table_rows, width = kv8._check_table(block_table)
+    kv8._check_ints("seqlens", seqlens, num_rows)
+    if table_row is not None:
+        kv8._check_ints("table_row", table_row, num_rows)
+    elif table_rows < num_rows:
+        raise ValueError("block_table needs a row per batch row when table_row is not given")
+    if cache_layer is not None:
+        kv8._check_ints("cache_layer", cache_layer, num_rows)
+    max_positions = kv8._check_rope(rope_style, rope_cos, rope_sin, dim)
+    kv8._check_bias("q_bias", q_bias, num_heads, dim, dt)
+    kv8._check_bias("k_bias", k_bias, heads_kv, dim, dt)
+    listed, groups, items, info = plan.listed, plan.groups, plan.items, plan.row_info
+    if not isinstance(info, torch.Tensor):
+        raise TypeError("the plan must be on the device: plan.to(device)")
+    num_listed, num_groups, num_items = listed.shape[0], groups.shape[0], items.shape[0]
+    for name, t, n in (("plan.listed", listed, num_listed), ("plan.groups", groups, 4 * num_groups),
+                       ("plan.items", items, 4 * num_items), ("plan.row_info", info, 4 * num_rows)):
+        kv8._check_ints(name, t, n)
+    if not workspace.is_contiguous():
+        raise ValueError("workspace must be contiguous")
+    q_stride = kv8._row_stride("q", q, num_rows, num_heads, dim)
+    kv_stride = kv8._row_stride("k_new", k_new, num_rows, heads_kv, dim)
+    if kv8._row_stride("v_new", v_new, num_rows, heads_kv, dim) != kv_stride:
+        raise ValueError("k_new and v_new must share a row stride")
+    kv8._require_here(q, k_new, v_new, pool, cache_layer, block_table, table_row, seqlens, rope_cos, rope_sin, q_bias,
+                      k_bias, listed, groups, items, info, out, workspace)
+    code = _lib.lib().cdb_prefix_decode_attention(
+        q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), view.k_ptr, view.v_ptr, view.layer_stride, layers,
+        pool_rows // block, _ptr(cache_layer), cache_layer0, block_table.data_ptr(), _ptr(table_row), table_rows, width,
+        seqlens.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
+        listed.data_ptr(), num_listed, groups.data_ptr(), num_groups, items.data_ptr(), num_items, info.data_ptr(),
+        out.data_ptr(), workspace.data_ptr(), workspace.nbytes, num_rows, num_heads, heads_kv, dim, block, scale,
+        q_stride, kv_stride, dtype_code(dt), _stream())
+    if code:
+        _lib.check(code, "cdb_prefix_decode_attention")
+    return out
+
+
+@torch.library.custom_op("cdb::prefix_decode_attention", mutates_args=("kv_pool", "workspace"), device_types="cuda")
+def prefix_decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, kv_pool: torch.Tensor,
+                            cache_layer: torch.Tensor | None, cache_layer0: int, block_table: torch.Tensor,
+                            table_row: torch.Tensor | None, seqlens: torch.Tensor, rope_cos: torch.Tensor | None,
+                            rope_sin: torch.Tensor | None, rope_style: int, q_bias: torch.Tensor | None,
+                            k_bias: torch.Tensor | None, listed: torch.Tensor, groups: torch.Tensor,
+                            items: torch.Tensor, row_info: torch.Tensor, workspace: torch.Tensor, block_size: int,
+                            scale: float) -> torch.Tensor:
+    """Paged decode attention of rows that share prefixes, with fused RoPE + KV append over ``kv_pool``
+    [num_cache_layers, 2, pool_blocks * block_size, Hkv, D]; the plan's four tensors as in ``PrefixDecodePlan``. See
+    ``prefix_decode_attention_raw``."""
+
+    out = q.new_empty(q.shape)
+    return prefix_decode_attention_raw(q, k_new, v_new, KVPoolView(kv_pool, block_size), cache_layer, cache_layer0,
+                                       block_table, table_row, seqlens, rope_cos, rope_sin, rope_style, q_bias, k_bias,
+                                       PrefixDecodePlan(listed, groups, items, row_info), out, workspace, scale)
+
+
+@prefix_decode_attention.register_fake
+def _(q, k_new, v_new, kv_pool, cache_layer, cache_layer0, block_table, table_row, seqlens, rope_cos, rope_sin,
+      rope_style, q_bias, k_bias, listed, groups, items, row_info, workspace, block_size, scale):
+    return q.new_empty(q.shape)
+
+
 def softmax_scale(head_dim: int) -> float:
     return 1.0 / math.sqrt(head_dim)
 

@@ -488,6 +488,50 @@ int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs,
                      int32_t* counts, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------
+ * Rows that share prefixes
+ * ------------------------------------------------------------------------ */
+
+enum {
+  CDB_PREFIX_QUERIES = 16,   /* queries (row, head) of an item */
+  CDB_PREFIX_MAX_PARTS = 64  /* parts that a prefix is cut into */
+};
+
+/* Workspace bytes of cdb_prefix_decode_attention for num_rows rows, num_items items and rows of up to max_own tokens of
+ * their own (-1 for invalid arguments). Rows with more are served too, in fewer and longer chunks, whose number depends
+ * on how many rows share the workspace. */
+int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, int32_t num_heads, int32_t num_kv_heads,
+                                          int32_t head_dim, int32_t max_own);
+
+/* cdb_paged_decode_attention for rows that begin with the same tokens, which are read once for all of them: rotate the
+ * row's new query and key, append key and value at position seqlens[b] of the row's cache layer, attend over positions
+ * 0..seqlens[b]. Arguments as there, but for the plan; block_size is a power of two of at least 16, and the block table
+ * has table_rows rows. Rotations are fp32 and rounded once, to the cache's type (that call rounds bf16 after each step).
+ *
+ * Group n's rows are listed[groups[4n]] and the groups[4n + 1] - 1 behind it; they hold the same first groups[4n + 2]
+ * tokens, at the same slots of the same cache layer or as copies. These are read through the table row and cache layer
+ * of the group's first row; the others only from there on. Queries of a group are counted row by row, the group's
+ * num_heads / num_kv_heads heads of a KV head each; items [num_items][4] = (group, first query, a multiple of
+ * CDB_PREFIX_QUERIES; first token; end token): the parts of a group's tokens for one run of queries follow each other,
+ * and the runs of a group too. (-1, ..) is no item. row_info [num_rows][4] = (row's first query in its group, tokens of
+ * its prefix, its group's first item, parts), zeros for a row without a group. A row is listed at most once.
+ *
+ * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
+ * or the angles' range or inside its prefix, its cache layer or table row out of range, or its layer not its group's;
+ * NaN too where a block outside the pool is met, for all rows of the group if it is in the prefix. Calls that may
+ * overlap need a workspace each. */
+int cdb_prefix_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_pool, void* v_pool,
+                                int64_t layer_stride, int32_t num_cache_layers, int64_t pool_blocks,
+                                const int32_t* cache_layer, int32_t cache_layer0, const int32_t* block_table,
+                                const int32_t* table_row, int32_t table_rows, int32_t table_width,
+                                const int32_t* seqlens, const float* rope_cos, const float* rope_sin,
+                                int32_t rope_style, int32_t max_positions, const void* q_bias, const void* k_bias,
+                                const int32_t* listed, int32_t num_listed, const int32_t* groups, int32_t num_groups,
+                                const int32_t* items, int32_t num_items, const int32_t* row_info, void* out,
+                                void* workspace, int64_t workspace_bytes, int32_t num_rows, int32_t num_heads,
+                                int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
+                                int64_t q_stride, int64_t kv_stride, int32_t dtype, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------
  * Drawing tokens
  * ------------------------------------------------------------------------ */
 
