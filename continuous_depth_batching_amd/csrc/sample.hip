@@ -7,13 +7,19 @@
 //   T not above 0: the first token of the order.
 //
 // Where u and p cut is decided by sums over as many as V tokens, whose shares may be far below what fp32 sums
-// keep, so weights are fp64 exponentials (2^-44 relative) rounded to fixed point, 2^-46 of the largest weight, and
+// keep, so weights are fp64 exponentials (2^-38 relative) rounded to fixed point, 2^-46 of the largest weight, and
 // every sum is an integer: exact, and so the same in any order of the additions, atomic ones among them.
 //
-// One workgroup of 16 waves takes a row; a wave owns a run of consecutive tokens, 16 bytes a lane at a time.
-// The place where top-k or top-p cuts is found by histograms in LDS: of the distance to the maximum first, then,
-// while more tokens than a list holds share the bin, of (logit, index) as one number over the bin's range; the
-// tokens of the last bin are sorted.
+// One workgroup of 16 waves takes a row; a wave owns a run of consecutive tokens, 8 of them a lane at a time.
+//   A first pass leaves the largest logit of each of 2048 parts of the row.
+//   top-k: the k-th largest of these is a bound that k tokens at least reach, and mostly not many more. min-p gives its
+//   bound at once. A second pass collects the tokens above the bound, and the rest is done on that list, in LDS.
+//   top-p: the second pass adds up what lies at each distance from the maximum (a histogram in LDS), which says where
+//   the share ends; the tokens above are collected if they are few.
+//   Where many tokens are kept, those of the bin in which the filter ends are collected to find the place where it
+//   does, and a last pass weighs the kept tokens in index order.
+// On lists, histograms over ranges of (logit, index) as one number narrow a range down to 128 tokens, which are
+// ordered by counting.
 
 #include "cdb_common.h"
 #include "../../include/cdb_amd.h"
@@ -22,9 +28,12 @@ namespace cdb {
 
 constexpr int kSampleThreads = 1024;
 constexpr int kSampleWaves = kSampleThreads / kWave;
-constexpr int kBins = 1024;  // one a thread
-constexpr int kList = 2048;  // tokens of the bin that is sorted, two a thread
-static_assert(kBins == kSampleThreads && kList == 2 * kSampleThreads, "one bin and two places a thread");
+constexpr int kBins = 1024;      // one a thread
+constexpr int kList = 2048;      // tokens of a list, two a thread
+constexpr int kShort = 128;      // ordered by counting, 8 threads a token
+constexpr int kPartRank = 1200;  // a part's maximum of this rank is reached by some 1800 tokens where they lie as they fall
+constexpr int kRun = 8;          // tokens a lane takes at a time
+static_assert(kBins == kSampleThreads && kList == 2 * kSampleThreads && kShort * 8 == kSampleThreads, "shares of a thread");
 
 struct SampleParams {
   const void* logits;
@@ -37,22 +46,21 @@ struct SampleParams {
   int32_t vocab, unit_log2;  // weights are counted in units of 2^-unit_log2
 };
 
-// 2^y for y <= 0 in fp64: 2^f for |f| <= 1/2 by a polynomial through its values at the zeros of a Chebyshev
-// polynomial (off by 3.7e-14 of the value at most), exact at 0.
-CDB_DEVICE double power_of_two(double y, int raise) {
-  const double n = __builtin_rint(y), f = y - n;
-  double p = 0x1.b63880a30e9ffp-24;
-  p = __builtin_fma(p, f, 0x1.63d136366db24p-20);
-  p = __builtin_fma(p, f, 0x1.ffcb9515a8016p-17);
-  p = __builtin_fma(p, f, 0x1.4308ac85aa947p-13);
-  p = __builtin_fma(p, f, 0x1.5d87fe86fe88ep-10);
-  p = __builtin_fma(p, f, 0x1.3b2ab7181b755p-7);
-  p = __builtin_fma(p, f, 0x1.c6b08d7047e52p-5);
-  p = __builtin_fma(p, f, 0x1.ebfbdff823cedp-3);
-  p = __builtin_fma(p, f, 0x1.62e42fefa39efp-1);
+// 2^(y + raise) in fp64, for y from about -1000 to 0 and a whole `raise`: 2^f for |f| <= 1/2 by a polynomial through its
+// values at 0 and the zeros of a Chebyshev polynomial (off by 2.1e-12 of the value at most), exact at f = 0.
+CDB_DEVICE double power_of_two(double y, double magic) {
+  // magic = 1.5 * 2^52 + raise: the sum's last bits are y rounded to a whole number, and raise.
+  const double t = y + magic, f = y - (t - magic);
+  double p = 0x1.63b2d7971923fp-20;
+  p = __builtin_fma(p, f, 0x1.00c0e4e15189cp-16);
+  p = __builtin_fma(p, f, 0x1.4308c7183d6a2p-13);
+  p = __builtin_fma(p, f, 0x1.5d877598350dep-10);
+  p = __builtin_fma(p, f, 0x1.3b2ab70ad2565p-7);
+  p = __builtin_fma(p, f, 0x1.c6b08da70cce3p-5);
+  p = __builtin_fma(p, f, 0x1.ebfbdff82a734p-3);
+  p = __builtin_fma(p, f, 0x1.62e42fef9cc69p-1);
   p = __builtin_fma(p, f, 1.0);
-  // Far exponents give 0 whatever they are; kept within what an int holds.
-  return __builtin_ldexp(p, (int)fmax(n, -4096.0) + raise);
+  return __builtin_ldexp(p, (int)(uint32_t)__builtin_bit_cast(uint64_t, t));
 }
 
 // Logits as numbers in their order, with the index below: larger logits first, the lower index among equals.
@@ -65,34 +73,78 @@ CDB_DEVICE uint32_t logit_key(float x) {
 CDB_DEVICE float logit_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key & 0x7fffffffu : ~key); }
 CDB_DEVICE uint64_t place_of(float x, int i) { return ((uint64_t)logit_key(x) << 32) | (uint32_t)~i; }
 
-CDB_DEVICE uint64_t shfl_u64(uint64_t v, int lane) {
-  const uint32_t lo = __builtin_amdgcn_ds_bpermute(lane << 2, (int)(uint32_t)v);
-  const uint32_t hi = __builtin_amdgcn_ds_bpermute(lane << 2, (int)(uint32_t)(v >> 32));
+// A word and its neighbour by DPP, 0 where there is none or the row is masked.
+template <int kCtrl, int kRows = 0xf> CDB_DEVICE uint64_t dpp_u64(uint64_t v) {
+  const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)v, kCtrl, kRows, 0xf, true);
+  const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(v >> 32), kCtrl, kRows, 0xf, true);
   return ((uint64_t)hi << 32) | lo;
-}
-CDB_DEVICE uint64_t wave_total(uint64_t v) {
-#pragma unroll
-  for (int m = 32; m >= 1; m >>= 1) v += shfl_u64(v, __lane_id() ^ m);
-  return v;
 }
 // Sum over this lane and those before it.
 CDB_DEVICE uint64_t wave_running(uint64_t v) {
-  const int lane = __lane_id();
-#pragma unroll
-  for (int m = 1; m < 64; m <<= 1) {
-    const uint64_t o = shfl_u64(v, max(lane - m, 0));
-    v += lane >= m ? o : 0;
-  }
+  v += dpp_u64<0x111>(v);  // row_shr 1, 2, 4, 8
+  v += dpp_u64<0x112>(v);
+  v += dpp_u64<0x114>(v);
+  v += dpp_u64<0x118>(v);
+  v += dpp_u64<0x142, 0xa>(v);  // lane 15 of each row to the next row, lane 31 to the upper half
+  v += dpp_u64<0x143, 0xc>(v);
   return v;
+}
+CDB_DEVICE uint32_t wave_running32(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xf, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xa, 0xf, true);
+  v += __builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xc, 0xf, true);
+  return v;
+}
+CDB_DEVICE uint64_t read_lane(uint64_t v, int lane) {
+  const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = __builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), lane);
+  return ((uint64_t)hi << 32) | lo;
+}
+CDB_DEVICE uint64_t wave_total(uint64_t v) { return read_lane(wave_running(v), 63); }
+CDB_DEVICE uint64_t wave_most(uint64_t v) {
+  v = max(v, dpp_u64<0x111>(v));
+  v = max(v, dpp_u64<0x112>(v));
+  v = max(v, dpp_u64<0x114>(v));
+  v = max(v, dpp_u64<0x118>(v));
+  v = max(v, dpp_u64<0x142, 0xa>(v));
+  v = max(v, dpp_u64<0x143, 0xc>(v));
+  return read_lane(v, 63);
+}
+// Sum over 8 consecutive lanes.
+CDB_DEVICE uint64_t eight_total(uint64_t v) {
+  v += dpp_u64<0xb1>(v);   // quad_perm 1 0 3 2
+  v += dpp_u64<0x4e>(v);   // quad_perm 2 3 0 1
+  v += dpp_u64<0x141>(v);  // half mirror
+  return v;
+}
+CDB_DEVICE void add_to(uint64_t* p, uint64_t v) {
+  atomicAdd(reinterpret_cast<unsigned long long*>(p), (unsigned long long)v);
+}
+CDB_DEVICE void raise_to(uint64_t* p, uint64_t v) {
+  atomicMax(reinterpret_cast<unsigned long long*>(p), (unsigned long long)v);
+}
+CDB_DEVICE void lower_to(uint64_t* p, uint64_t v) {
+  atomicMin(reinterpret_cast<unsigned long long*>(p), (unsigned long long)v);
+}
+// The range of the workgroup's places, of which a lane knows the least and the most, to words that hold ~0 and 0.
+CDB_DEVICE void widen(uint64_t* lo, uint64_t* hi, uint64_t least, uint64_t most) {
+  const uint64_t a = ~wave_most(~least), b = wave_most(most);
+  if (__lane_id() == 0) {
+    lower_to(lo, a);
+    raise_to(hi, b);
+  }
 }
 
 struct SampleShared {
   uint64_t mass[kBins];
   uint64_t list[kList];
-  uint32_t count[kBins];
+  uint64_t few[kShort], few_mass[kShort];
   uint64_t wave64[kSampleWaves], lo, hi, before;
   float wave32[kSampleWaves];
-  int32_t bin, found;
+  int32_t bin, found, found_few;
 };
 
 // Sum over this thread and those before it; `total` is the sum over all. Meets the workgroup twice.
@@ -113,23 +165,23 @@ CDB_DEVICE uint64_t block_running(uint64_t v, SampleShared& s, uint64_t& total) 
   return before + run;
 }
 
-// A row's logits as a lane meets them: vectors of 16 bytes, aligned, of which the first and the last may stick out
-// of the row. Wave w owns vectors [64 w turns, 64 (w + 1) turns), lane by lane.
+// A row's logits as a lane meets them: runs of 8 tokens, at addresses aligned for 16-byte loads, of which the first
+// and the last may stick out of the row. Wave w owns runs [64 w turns, 64 (w + 1) turns), lane by lane.
 template <typename T> struct SampleRow {
-  static constexpr int E = 16 / (int)sizeof(T);
-  const T* base;  // of vector 0, aligned
-  int skip;       // elements of vector 0 before the row
+  typedef Vec<T, kRun> Run;
+  const T* base;  // of run 0, aligned
+  int skip;       // elements of run 0 before the row
   int vocab, turns, first;
 
-  CDB_DEVICE Vec<T, E> fetch(int v) const {
-    Vec<T, E> x;
-    const int i0 = v * E - skip;
-    if (i0 >= 0 && i0 <= vocab - E) {
-      x.load(base + (int64_t)v * E);
+  CDB_DEVICE Run fetch(int n) const {
+    Run x;
+    const int i0 = n * kRun - skip;
+    if (i0 >= 0 && i0 <= vocab - kRun) {
+      x.load(base + (int64_t)n * kRun);
     } else {
 #pragma unroll
-      for (int e = 0; e < E; ++e)
-        x.set(e, i0 + e >= 0 && i0 + e < vocab ? Elem<T>::load(base + (int64_t)v * E + e) : -INFINITY);
+      for (int e = 0; e < kRun; ++e)
+        x.set(e, i0 + e >= 0 && i0 + e < vocab ? Elem<T>::load(base + (int64_t)n * kRun + e) : -INFINITY);
     }
     return x;
   }
@@ -137,37 +189,71 @@ template <typename T> struct SampleRow {
     skip = (int)(((uintptr_t)row & 15) / sizeof(T));
     base = row - skip;
     vocab = n;
-    const int vectors = (skip + n + E - 1) / E;
-    turns = (vectors + kSampleThreads - 1) / kSampleThreads;
+    const int runs = (skip + n + kRun - 1) / kRun;
+    turns = (runs + kSampleThreads - 1) / kSampleThreads;
     first = (threadIdx.x >> 6) * turns * kWave + (threadIdx.x & 63);
   }
-  CDB_DEVICE int index(int j) const { return (first + j * kWave) * E - skip; }
-  // f(vector, index of its first element) for the lane's vectors, in order.
-  template <typename F> CDB_DEVICE void each_vector(F f) const {
-    for (int j = 0; j < turns; ++j) f(fetch(first + j * kWave), index(j));
-  }
-  template <typename F> CDB_DEVICE void each(F f) const {
-    each_vector([&](const Vec<T, E>& x, int i) __attribute__((always_inline)) {
+  // f(turn, run, index of its first token) for the lane's runs, in order; U of them, or the next one, load together.
+  template <int U, typename F> CDB_DEVICE void each(F f) const {
+    if constexpr (U == 1) {
+      Run x = fetch(first);
+      for (int j = 0; j < turns; ++j) {
+        const Run next = fetch(first + min(j + 1, turns - 1) * kWave);
+        f(j, x, (first + j * kWave) * kRun - skip);
+        x = next;
+      }
+    } else {
+      for (int j0 = 0; j0 < turns; j0 += U) {
+        Run x[U];
 #pragma unroll
-      for (int e = 0; e < E; ++e) f(x.get(e), i + e);
-    });
+        for (int u = 0; u < U; ++u) x[u] = fetch(first + min(j0 + u, turns - 1) * kWave);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          if (j0 + u < turns) f(j0 + u, x[u], (first + (j0 + u) * kWave) * kRun - skip);
+      }
+    }
   }
 };
+// The largest of a run, NaN passed over.
+template <typename Run> CDB_DEVICE float largest(const Run& x) {
+  float m = x.get(0);
+#pragma unroll
+  for (int e = 1; e < kRun; ++e) m = fmaxf(m, x.get(e));
+  return m;
+}
 
-// What a logit weighs.
-struct Weigher {
-  double top, rate;  // log2(e) / T
-  float top_f, bins_per;  // bins of the first histogram per unit of logit
-  int unit_log2;
-  bool endless;  // the maximum is infinite: nothing else weighs anything
+// What a logit weighs. kPlain: the maximum is finite and, over the temperature, below 2^20, so one product and sum
+// gives the exponent (all exponents are off by the same 2^-33 at most, which divides out); otherwise the difference
+// is taken first, and where the maximum is infinite nothing else weighs anything.
+template <bool kPlain> struct Weigher {
+  double top, rate, offset, magic;  // rate: log2(e) / T
+  float top_f, bins_per;            // bins of the first histogram per unit of logit
 
+  // In units. -infinity and NaN give less than half a unit.
   CDB_DEVICE double of(float x) const {
-    if (endless) return x == top_f ? __builtin_ldexp(1.0, unit_log2) : 0.0;
-    return power_of_two(((double)x - top) * rate, unit_log2);
+    double y;
+    if constexpr (kPlain) {
+      y = __builtin_fma((double)x, rate, offset);
+    } else {
+      y = x == top_f ? 0.0 : ((double)x - top) * rate;
+    }
+    return power_of_two(fmax(y, -1000.0), magic);
   }
-  CDB_DEVICE static uint64_t units(double w) {
-    // Rounded to a whole number below 2^52 by the sum's own rounding.
-    return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xfffffffffffffull;
+  // A weight rounded to a whole number of units, by the rounding of a sum with 2^52.
+  CDB_DEVICE static uint64_t units(double w) { return __builtin_bit_cast(uint64_t, w + 0x1p52) & 0xfffffffffffffull; }
+  CDB_DEVICE uint64_t units_of(float x) const { return units(of(x)); }
+  // What a run's tokens weigh together, those that `keep` holds for: the sum with 2^52 stays on each until the end.
+  template <typename Run, typename F> CDB_DEVICE uint64_t units_of_run(const Run& x, F keep) const {
+    uint64_t sum = 0;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) {
+      const double v = of(x.get(e));
+      sum += __builtin_bit_cast(uint64_t, (keep(e, v) ? v : 0.0) + 0x1p52);
+    }
+    return sum - kRun * 0x4330000000000000ull;
+  }
+  template <typename Run> CDB_DEVICE uint64_t units_of_run(const Run& x) const {
+    return units_of_run(x, [](int, double) { return true; });
   }
   // Falls, or stays, as the logit rises.
   CDB_DEVICE int bin(float x) const {
@@ -176,123 +262,462 @@ struct Weigher {
   }
 };
 
-// Tokens sorted by place, the first of the order first. n <= kList; the rest of `list` up to a power of two is
-// filled with 0, which sorts last.
-CDB_DEVICE void sort_places(uint64_t* list, int n) {
-  int size = 2;
-  while (size < n) size <<= 1;
-  for (int i = n + threadIdx.x; i < size; i += kSampleThreads) list[i] = 0;
+// The tokens that a cut leaves: all that can be drawn, or those up to a place of the order.
+struct Limit {
+  float last;
+  int index;
+  bool every;
+  CDB_DEVICE static Limit none() { return {0.f, 0, true}; }
+  CDB_DEVICE static Limit at(uint64_t place) { return {logit_of((uint32_t)(place >> 32)), (int)~(uint32_t)place, false}; }
+  CDB_DEVICE bool keeps(float x, int i) const {
+    return (every & (x > -INFINITY)) | (!every & ((x > last) | ((x == last) & (i <= index))));
+  }
+};
+
+// Puts the tokens of a run for which keep(logit, index) holds on the list; beyond its end they are only counted. For
+// whole waves.
+template <typename Run, typename F>
+CDB_DEVICE void append(SampleShared& s, const Run& x, int i, F keep) {
+  uint32_t mask = 0;
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) mask |= keep(x.get(e), i + e) ? 1u << e : 0u;
+  if (!__any(mask != 0)) return;
+  const uint32_t upto = wave_running32(__popc(mask));
+  const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
+  int at = 0;
+  if (__lane_id() == 63) at = atomicAdd(&s.found, (int)all);
+  at = __builtin_amdgcn_readlane(at, 63) + (int)upto - __popc(mask);
+  if (mask == 0) return;
+#pragma unroll
+  for (int e = 0; e < kRun; ++e)
+    if (mask & (1u << e)) {
+      if (at < kList) s.list[at] = place_of(x.get(e), i + e);
+      ++at;
+    }
+}
+
+// Of a histogram in `mass`, ordered as the tokens are: the last bin that counts before which, `before` included, less
+// than the goal lies, or -1. `before` becomes what lies before that bin.
+CDB_DEVICE int last_bin(SampleShared& s, uint64_t upto, uint64_t& before, double goal) {
+  const int t = threadIdx.x;
+  const uint64_t mine = s.mass[t], here = before + upto - mine;
+  const bool starts = mine != 0 && (double)here < goal;
+  // Bins that start are the first ones that count, so a wave's last lane that does is its last.
+  const uint64_t lanes = __ballot(starts);
+  if (t == 0) s.bin = -1;
   __syncthreads();
-  for (int k = 2; k <= size; k <<= 1) {
-    for (int j = k >> 1; j > 0; j >>= 1) {
-      for (int t = threadIdx.x; t < size / 2; t += kSampleThreads) {
-        const int a = 2 * t - (t & (j - 1)), b = a + j;
-        const uint64_t x = list[a], y = list[b];
-        const bool rises = (a & k) != 0;
-        if ((x < y) != rises) {
-          list[a] = y;
-          list[b] = x;
+  if (lanes != 0 && (t & 63) == 63 - __clzll(lanes)) atomicMax(&s.bin, t);
+  __syncthreads();
+  const int b = s.bin;
+  if (t == max(b, 0)) s.before = here;
+  __syncthreads();
+  before = s.before;
+  return b;
+}
+
+// The place of the last kept token of the list's n whose place is `limit` at least. Kept are those before which, with
+// the `before` that is not on the list, less than the goal lies: kMass, of what they weigh; otherwise a number of
+// tokens. share: the goal is that share of what they weigh. The first is always kept.
+template <bool kMass, typename W>
+CDB_DEVICE uint64_t pick(SampleShared& s, const W& w, int n, uint64_t limit, uint64_t before, double goal, bool share) {
+  const int t = threadIdx.x, lane = t & 63;
+  uint64_t place[2], q[2], lo = ~0ull, hi = 0;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    place[e] = t + e * kSampleThreads < n ? s.list[t + e * kSampleThreads] : 0;
+    if (place[e] < limit) place[e] = 0;
+    q[e] = place[e] == 0 ? 0 : kMass ? w.units_of(logit_of((uint32_t)(place[e] >> 32))) : 1;
+    if (place[e] != 0) {
+      lo = min(lo, place[e]);
+      hi = max(hi, place[e]);
+    }
+  }
+  if (t == 0) {
+    s.lo = ~0ull;
+    s.hi = 0;
+  }
+  __syncthreads();
+  widen(&s.lo, &s.hi, lo, hi);
+  __syncthreads();
+  lo = s.lo;
+  hi = s.hi;
+  for (;;) {
+    const int shift = max(0, 64 - __clzll(hi - lo) - 10);
+    s.mass[t] = 0;
+    if (t == 0) s.found_few = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (place[e] >= lo && place[e] <= hi) add_to(&s.mass[(int)((hi - place[e]) >> shift)], q[e]);
+    __syncthreads();
+    uint64_t total;
+    const uint64_t upto = block_running(s.mass[t], s, total);
+    if (share) {
+      goal *= (double)total;
+      share = false;
+    }
+    goal = fmax(goal, 0x1p-60);
+    const int b = max(last_bin(s, upto, before, goal), 0);
+    hi -= (uint64_t)b << shift;
+    lo = max(lo, hi - (((uint64_t)1 << shift) - 1));
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (place[e] >= lo && place[e] <= hi) {
+        const int at = atomicAdd(&s.found_few, 1);
+        if (at < kShort) {
+          s.few[at] = place[e];
+          s.few_mass[at] = q[e];
         }
       }
+    __syncthreads();
+    const int m = s.found_few;
+    if (m <= kShort) {
+      const int i = t >> 3;
+      const uint64_t mine = i < m ? s.few[i] : 0;
+      uint64_t larger = 0;
+      for (int j = t & 7; j < m; j += 8) larger += s.few[j] > mine ? s.few_mass[j] : 0;
+      larger = eight_total(larger);
+      if (t == 0) s.lo = hi;  // the bin holds a token: the first of its range is kept if no other is
       __syncthreads();
+      if ((lane & 7) == 0 && i < m && (double)(before + larger) < goal) lower_to(&s.lo, mine);
+      __syncthreads();
+      const uint64_t last = s.lo;
+      __syncthreads();
+      return last;
     }
+    __syncthreads();  // all have read how many there were
   }
 }
 
-// The place of the last kept token among those at `limit` and before it in the order. Kept are those before which
-// less than the goal lies: kMass, a share of what they weigh together; otherwise a number of tokens. The first is
-// always kept.
-template <bool kMass, typename Row>
-CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const Weigher& w, uint64_t limit, double goal) {
+// The place of the last kept token of the row, as `pick`, among those that `limit` leaves. `bin`: of those up to the
+// first histogram's `bin`, if it was made already (0 or more), before which `before` lies.
+template <bool kMass, typename Row, typename W>
+CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const W& w, const Limit& limit, double goal, int bin,
+                        uint64_t before) {
+  typedef typename Row::Run Run;
   const int t = threadIdx.x;
-  uint64_t lo = limit, hi = ~0ull, before = 0;
-  bool linear = true;
-  for (;;) {
-    // How much lies in each bin.
-    const int shift = linear ? 0 : max(0, 64 - __clzll(hi - lo) - 10);
-    auto bin_of = [&](float x, uint64_t place) __attribute__((always_inline)) -> int {
-      return linear ? w.bin(x) : (int)((hi - place) >> shift);
-    };
+  uint64_t lo = 0, hi = ~0ull, total;
+  if (bin < 0) {
     s.mass[t] = 0;
-    s.count[t] = 0;
     __syncthreads();
-    row.each([&](float x, int i) __attribute__((always_inline)) {
-      if (!(x > -INFINITY)) return;
-      const uint64_t place = place_of(x, i);
-      if (place < lo || place > hi) return;
-      const int b = bin_of(x, place);
-      atomicAdd(&s.count[b], 1u);
-      if constexpr (kMass)
-        atomicAdd(reinterpret_cast<unsigned long long*>(&s.mass[b]), (unsigned long long)Weigher::units(w.of(x)));
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        const float y = x.get(e);
+        const uint64_t q = kMass ? w.units_of(y) : 1;
+        if (limit.keeps(y, i + e)) add_to(&s.mass[w.bin(y)], q);
+      }
     });
     __syncthreads();
-    const uint64_t mine = kMass ? s.mass[t] : s.count[t];
-    uint64_t total;
-    const uint64_t upto = block_running(mine, s, total);
-    if (linear) {
-      if (kMass) goal *= (double)total;
-      goal = fmax(goal, 0x1p-60);
-    }
-    // The last bin with tokens before which less than the goal lies.
-    const bool starts = s.count[t] != 0 && (double)(before + upto - mine) < goal;
-    if (t == 0) s.bin = -1;
-    __syncthreads();
-    if (starts) atomicMax(&s.bin, t);
-    __syncthreads();
-    const int b = s.bin;
-    if (t == b) s.before = before + upto - mine;
+    const uint64_t upto = block_running(s.mass[t], s, total);
+    if (kMass) goal *= (double)total;
+    goal = fmax(goal, 0x1p-60);
+    bin = max(last_bin(s, upto, before, goal), 0);
+  }
+  // The tokens of the bin; while they are too many, of a part of the range that they take.
+  int shift = -1;  // of the histogram over [lo, hi], or the first one's
+  for (;;) {
+    auto inside = [&](float x, int i) __attribute__((always_inline)) -> bool {
+      if (shift < 0) return limit.keeps(x, i) & (w.bin(x) == bin);
+      const uint64_t place = place_of(x, i);
+      return limit.keeps(x, i) & (place >= lo) & (place <= hi);
+    };
     if (t == 0) {
       s.found = 0;
       s.lo = ~0ull;
       s.hi = 0;
     }
     __syncthreads();
-    const int n = (int)min(s.count[b], 0x7fffffffu);
-    before = s.before;
-    auto inside = [&](float x, uint64_t place) __attribute__((always_inline)) -> bool {
-      return place >= lo && place <= hi && bin_of(x, place) == b;
-    };
-    if (n <= kList) {
-      row.each([&](float x, int i) __attribute__((always_inline)) {
-        if (!(x > -INFINITY)) return;
-        const uint64_t place = place_of(x, i);
-        if (inside(x, place)) s.list[atomicAdd(&s.found, 1)] = place;
-      });
-      __syncthreads();
-      sort_places(s.list, n);
-      uint64_t q[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint64_t place = 2 * t + e < n ? s.list[2 * t + e] : 0;
-        q[e] = place == 0 ? 0 : kMass ? Weigher::units(w.of(logit_of((uint32_t)(place >> 32)))) : 1;
-      }
-      const uint64_t sum = block_running(q[0] + q[1], s, total) - q[0] - q[1];
-      if (t == 0) s.bin = 0;
-      __syncthreads();
-      if (2 * t < n && (double)(before + sum) < goal) atomicMax(&s.bin, 2 * t);
-      if (2 * t + 1 < n && (double)(before + sum + q[0]) < goal) atomicMax(&s.bin, 2 * t + 1);
-      __syncthreads();
-      const uint64_t last = s.list[s.bin];
-      __syncthreads();
-      return last;
-    }
-    // Too many: the range that they take.
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { append(s, x, i, inside); });
+    __syncthreads();
+    if (s.found <= kList) return pick<kMass>(s, w, s.found, 0, before, goal, false);
     uint64_t least = ~0ull, most = 0;
-    row.each([&](float x, int i) __attribute__((always_inline)) {
-      if (!(x > -INFINITY)) return;
-      const uint64_t place = place_of(x, i);
-      if (inside(x, place)) {
-        least = min(least, place);
-        most = max(most, place);
-      }
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (inside(x.get(e), i + e)) {
+          const uint64_t place = place_of(x.get(e), i + e);
+          least = min(least, place);
+          most = max(most, place);
+        }
     });
-    atomicMin(reinterpret_cast<unsigned long long*>(&s.lo), (unsigned long long)least);
-    atomicMax(reinterpret_cast<unsigned long long*>(&s.hi), (unsigned long long)most);
+    widen(&s.lo, &s.hi, least, most);
     __syncthreads();
     lo = s.lo;
     hi = s.hi;
-    linear = false;
+    shift = max(0, 64 - __clzll(hi - lo) - 10);
+    s.mass[t] = 0;
     __syncthreads();
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (inside(x.get(e), i + e))
+          add_to(&s.mass[(int)((hi - place_of(x.get(e), i + e)) >> shift)], kMass ? w.units_of(x.get(e)) : 1);
+    });
+    __syncthreads();
+    const uint64_t upto = block_running(s.mass[t], s, total);
+    hi -= (uint64_t)max(last_bin(s, upto, before, goal), 0) << shift;
+    lo = max(lo, hi - (((uint64_t)1 << shift) - 1));
+  }
+}
+
+// What the filters of a row ask for.
+struct Filters {
+  int k;         // 0: all
+  double p;      // 1: all
+  double u;      // the given number
+  double size, least;  // share of the largest that a kept token weighs at least, and in units
+  bool by_count, by_share, by_size;
+};
+
+template <typename W>
+CDB_DEVICE void give(const SampleParams& P, int64_t r, const W& w, uint64_t place, uint64_t total) {
+  const float x = logit_of((uint32_t)(place >> 32));
+  const double share = x == w.top_f ? 0.0 : ((double)x - w.top) * (w.rate * 0.6931471805599453);
+  P.tokens[r] = (int)~(uint32_t)place;
+  P.logprobs[r] = (float)(share - log(__builtin_ldexp((double)total, -P.unit_log2)));
+}
+
+// The running weight that must be passed, of kept tokens that weigh `total` units; the largest token has a weight, so
+// one passes it.
+CDB_DEVICE uint64_t goal_of(double u, uint64_t total) {
+  return u > 0.0 ? min((uint64_t)(fmin(u, 1.0) * (double)total), total - 1) : 0;
+}
+
+// Draws from the list of the row's first n tokens, n <= kShort, in any order, of which top-k leaves k at most; goal:
+// the weight that top-p asks for, if it is known (0 or more).
+template <typename W>
+CDB_DEVICE void draw_short(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f, int n,
+                           double goal) {
+  // 8 threads a token, which each compare it with every eighth.
+  const int t = threadIdx.x, i = t >> 3, part = t & 7;
+  const uint64_t place = i < n ? s.list[i] : 0;
+  const double weight = place == 0 ? 0.0 : w.of(logit_of((uint32_t)(place >> 32)));
+  const uint64_t mine = W::units(weight);
+  if (part == 0) s.few_mass[i] = mine;
+  if (t == 0) s.before = 0;
+  __syncthreads();
+  uint64_t before = 0, count = 0, total = 0;
+  for (int j = part; j < n; j += 8) {
+    const bool larger = s.list[j] > place;
+    before += larger ? s.few_mass[j] : 0;
+    count += larger;
+  }
+  before = eight_total(before);
+  count = eight_total(count);
+  bool kept = place != 0 && (!f.by_count || count < (uint64_t)f.k);
+  if (f.by_share) {
+    if (goal < 0.0) {
+      // The last that top-k leaves has the others before it.
+      if (part == 0 && place != 0 && (count + 1 == (uint64_t)f.k || (count + 1 == (uint64_t)n && n < f.k)))
+        s.before = before + mine;
+      __syncthreads();
+      goal = f.p * (double)s.before;
+    }
+    kept = kept && (count == 0 || (double)before < goal);
+  }
+  kept = kept && weight >= f.least;
+  __syncthreads();
+  if (part == 0) s.few_mass[i] = kept ? mine : 0;
+  __syncthreads();
+  before = 0;
+  for (int j = part; j < n; j += 8) {
+    const uint64_t q = s.few_mass[j];
+    before += (uint32_t)s.list[j] > (uint32_t)place ? q : 0;  // a lower index
+    total += q;
+  }
+  before = eight_total(before);
+  total = eight_total(total);
+  const uint64_t at = goal_of(f.u, total);
+  if (part == 0 && kept && at >= before && at < before + mine) give(P, r, w, place, total);
+}
+
+// The same for n <= kList.
+template <typename W>
+CDB_DEVICE void draw_list(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f, int n,
+                          double goal) {
+  const int t = threadIdx.x;
+  uint64_t limit = 1;
+  if (f.by_count) limit = pick<false>(s, w, n, limit, 0, (double)f.k, false);
+  if (f.by_share) limit = pick<true>(s, w, n, limit, 0, goal < 0.0 ? f.p : goal, goal < 0.0);
+  uint64_t place[2], q[2];
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    place[e] = t + e * kSampleThreads < n ? s.list[t + e * kSampleThreads] : 0;
+    const double weight = w.of(logit_of((uint32_t)(place[e] >> 32)));
+    q[e] = place[e] >= limit && weight >= f.least ? W::units(weight) : 0;
+  }
+  // By index: the bin of up to 1024 neighbours, then the token.
+  const int shift = max(0, 32 - __clz(P.vocab - 1) - 10);
+  uint64_t total, goal_at = 0, sum = 0;
+  int base = 0;
+  for (int step = 0; step < 2; ++step) {
+    s.mass[t] = 0;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int i = (int)~(uint32_t)place[e] - base, at = step == 0 ? i >> shift : i;
+      if (q[e] != 0 && at >= 0 && at < (step == 0 ? kBins : 1 << shift)) add_to(&s.mass[at], q[e]);
+    }
+    __syncthreads();
+    const uint64_t mine = s.mass[t], upto = block_running(mine, s, total);
+    if (step == 0) {
+      sum = total;
+      goal_at = goal_of(f.u, total);
+    }
+    if (goal_at >= upto - mine && goal_at < upto) {
+      s.bin = t;
+      s.before = upto - mine;
+    }
+    __syncthreads();
+    if (step == 0) {
+      base = s.bin << shift;
+      goal_at -= s.before;
+    }
+  }
+  const int token = base + s.bin;
+#pragma unroll
+  for (int e = 0; e < 2; ++e)
+    if (q[e] != 0 && (int)~(uint32_t)place[e] == token) give(P, r, w, place[e], sum);
+}
+
+// Collects the tokens up to bin b of the first histogram; how many they are.
+template <typename T, typename W>
+CDB_DEVICE int collect(const SampleRow<T>& row, SampleShared& s, const W& w, int b) {
+  const float edge = b >= kBins - 1 ? NAN : (float)(b + 1);  // the last bin has no end
+  if (threadIdx.x == 0) s.found = 0;
+  __syncthreads();
+  auto inside = [&](float x, int) __attribute__((always_inline)) -> bool {
+    const float d = x == w.top_f ? 0.f : w.top_f - x;
+    return (x > -INFINITY) & !(d * w.bins_per >= edge);
+  };
+  row.template each<4>([&](int, const typename SampleRow<T>::Run& x, int i) __attribute__((always_inline)) {
+    if (__any(inside(largest(x), 0))) append(s, x, i, inside);
+  });
+  __syncthreads();
+  return s.found;
+}
+
+// Draws by collecting the tokens that may be kept in a list. False, for all threads, where they may be too many; `bin`,
+// `before` and `goal` then tell what is known of where top-p ends.
+template <typename T, typename W>
+CDB_DEVICE bool draw_few(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s, const W& w,
+                         const Filters& f, const float* part_top, int& bin, uint64_t& before, double& goal) {
+  if (f.by_count && f.k > kPartRank) return false;
+  const int t = threadIdx.x;
+  uint64_t total;
+  int b = kBins - 1;
+  if (f.by_count) {
+    s.mass[t] = 0;
+    if (t == 0) s.bin = kBins - 1;
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < 2; ++e)
+      if (part_top[e] > -INFINITY) add_to(&s.mass[w.bin(part_top[e])], 1);
+    __syncthreads();
+    const uint64_t mine = s.mass[t], upto = block_running(mine, s, total);
+    if (upto >= (uint64_t)f.k && upto - mine < (uint64_t)f.k) s.bin = t;
+    __syncthreads();
+    b = s.bin;
+  } else if (f.by_share) {
+    s.mass[t] = 0;
+    if (t == 0) s.found = 0;
+    __syncthreads();
+    row.template each<1>([&](int, const typename SampleRow<T>::Run& x, int) __attribute__((always_inline)) {
+      uint64_t q[kRun];
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) q[e] = w.units_of(x.get(e));
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (q[e] != 0) add_to(&s.mass[w.bin(x.get(e))], q[e]);
+    });
+    __syncthreads();
+    const uint64_t upto = block_running(s.mass[t], s, total);
+    goal = fmax(f.p * (double)total, 0x1p-60);
+    b = bin = max(last_bin(s, upto, before, goal), 0);
+    // The parts whose largest logit lies up to there tell about how many tokens do.
+    const int parts = __popcll(__ballot(part_top[0] > -INFINITY && w.bin(part_top[0]) <= b)) +
+                      __popcll(__ballot(part_top[1] > -INFINITY && w.bin(part_top[1]) <= b));
+    if ((t & 63) == 0) atomicAdd(&s.found, parts);
+    __syncthreads();
+    const bool many = s.found > kPartRank;
+    __syncthreads();
+    if (many) return false;
+  }
+  if (f.by_size && !f.by_share) {
+    const double far = -log2(f.size) * (kBins / 46.0) + 1.0;
+    b = min(b, (int)fmin(far, (double)(kBins - 1)));
+  }
+  const int n = collect(row, s, w, b);
+  if (n > kList) return false;
+  if (n <= kShort) draw_short(P, r, s, w, f, n, goal);
+  else draw_list(P, r, s, w, f, n, goal);
+  return true;
+}
+
+// Draws by weighing every kept token in index order.
+template <typename T, typename W>
+CDB_DEVICE void draw_many(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s, const W& w,
+                          const Filters& f, int bin, uint64_t before, double goal) {
+  typedef typename SampleRow<T>::Run Run;
+  const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
+  Limit limit = Limit::none();
+  if (f.by_count) limit = Limit::at(cut<false>(row, s, w, limit, (double)f.k, -1, 0));
+  if (f.by_share) limit = Limit::at(cut<true>(row, s, w, limit, bin < 0 ? f.p : goal, bin, bin < 0 ? 0 : before));
+  auto of_run = [&](const Run& x, int i) __attribute__((always_inline)) -> uint64_t {
+    if (limit.every && !f.by_size) return w.units_of_run(x);
+    if (!__any(limit.every || largest(x) >= limit.last)) return 0;
+    return w.units_of_run(x, [&](int e, double v) __attribute__((always_inline)) -> bool {
+      return limit.keeps(x.get(e), i + e) & (v >= f.least);
+    });
+  };
+  // Where the running weight passes the goal: the wave, the turn of that wave (a wave of this workgroup each), the
+  // lane, the token.
+  uint64_t sum = 0, total = 0;
+  row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { sum += of_run(x, i); });
+  sum = wave_total(sum);
+  __syncthreads();
+  if (lane == 0) s.wave64[wave] = sum;
+  __syncthreads();
+#pragma unroll
+  for (int v = 0; v < kSampleWaves; ++v) total += s.wave64[v];
+  const uint64_t at_goal = goal_of(f.u, total);
+  int owner = 0;
+  before = 0;
+#pragma unroll
+  for (int v = 0; v < kSampleWaves - 1; ++v) {
+    const uint64_t upto = before + s.wave64[v];
+    if (v == owner && upto <= at_goal) {
+      before = upto;
+      owner = v + 1;
+    }
+  }
+  const int each = (row.turns + kSampleWaves - 1) / kSampleWaves;  // turns of the owner that a wave takes
+  const int from = wave * each, to = min(row.turns, from + each);
+  const int base = owner * row.turns * kWave + lane;
+  uint64_t all = 0;
+  for (int j = from; j < to; ++j)
+    all += wave_total(of_run(row.fetch(base + j * kWave), (base + j * kWave) * kRun - row.skip));
+  __syncthreads();
+  if (lane == 0) s.wave64[wave] = all;
+  __syncthreads();
+  for (int v = 0; v < wave; ++v) before += s.wave64[v];
+  if (at_goal < before || at_goal >= before + all) return;
+  for (int j = from; j < to; ++j) {
+    const int i = (base + j * kWave) * kRun - row.skip;
+    const Run x = row.fetch(base + j * kWave);
+    const uint64_t mine = of_run(x, i), upto = before + wave_running(mine);
+    uint64_t at = upto - mine;
+    if (at_goal >= at && at_goal < upto) {
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        const double v = w.of(x.get(e));
+        const uint64_t q = limit.keeps(x.get(e), i + e) && v >= f.least ? W::units(v) : 0;
+        if (at_goal >= at && at_goal < at + q) give(P, r, w, place_of(x.get(e), i + e), total);
+        at += q;
+      }
+    }
+    before = read_lane(upto, 63);
   }
 }
 
@@ -304,11 +729,23 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams P) 
   SampleRow<T> row;
   row.open(static_cast<const T*>(P.logits) + r * P.row_stride, P.vocab);
 
-  float top = -INFINITY;
-  row.each([&](float x, int) __attribute__((always_inline)) { top = fmaxf(top, x); });  // passes over NaN
-  top = wave_max(top);
+  // Loaded with the row's first tokens: a load of its own would cost each its time.
+  const float temperature = P.temperature == nullptr ? 1.f : P.temperature[r];
+  const int k = P.top_k == nullptr ? 0 : P.top_k[r];
+  const float p = P.top_p == nullptr ? 1.f : P.top_p[r], m = P.min_p == nullptr || !(P.min_p[r] > 0.f) ? 0.f : fminf(P.min_p[r], 1.f);
+  Filters f;
+  f.u = P.uniform[r];
+
+  float part_top[2] = {-INFINITY, -INFINITY};  // of the thread's even and odd turns
+  row.template each<8>([&](int j, const typename SampleRow<T>::Run& x, int) __attribute__((always_inline)) {
+    const float m = largest(x);
+    if (j & 1) part_top[1] = fmaxf(part_top[1], m);
+    else part_top[0] = fmaxf(part_top[0], m);
+  });
+  const float mine = fmaxf(part_top[0], part_top[1]);
+  float top = wave_max(mine);
   if (lane == 0) s.wave32[wave] = top;
-  if (t == 0) s.bin = 0x7fffffff;
+  if (t == 0) s.bin = 0x7fffffff;  // the lowest index, of a greedy row
   __syncthreads();
 #pragma unroll
   for (int w = 0; w < kSampleWaves; ++w) top = fmaxf(top, s.wave32[w]);
@@ -319,11 +756,15 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams P) 
     }
     return;
   }
-  const float temperature = P.temperature == nullptr ? 1.f : P.temperature[r];
   if (!(temperature > 0.f)) {
-    int best = 0x7fffffff;
-    row.each([&](float x, int i) __attribute__((always_inline)) { if (x == top) best = min(best, i); });
-    if (best != 0x7fffffff) atomicMin(&s.bin, best);
+    if (mine == top) {
+      int best = 0x7fffffff;
+      row.template each<4>([&](int, const typename SampleRow<T>::Run& x, int i) __attribute__((always_inline)) {
+#pragma unroll
+        for (int e = 0; e < kRun; ++e) best = x.get(e) == top ? min(best, i + e) : best;
+      });
+      atomicMin(&s.bin, best);
+    }
     __syncthreads();
     if (t == 0) {
       P.tokens[r] = s.bin;
@@ -331,70 +772,35 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams P) 
     }
     return;
   }
-  Weigher w;
-  w.top = top;
-  w.top_f = top;
-  w.rate = 1.4426950408889634 / (double)temperature;
-  w.bins_per = (float)fmin(w.rate * (kBins / 46.0), 1e30);
-  w.unit_log2 = P.unit_log2;
-  w.endless = top == INFINITY;
-
-  // The place of the last token that top-k and top-p keep.
-  uint64_t limit = 1;
-  const int k = P.top_k == nullptr ? 0 : P.top_k[r];
-  if (k > 0 && k < P.vocab) limit = cut<false>(row, s, w, limit, (double)k);
-  const float p = P.top_p == nullptr ? 1.f : P.top_p[r];
-  if (p < 1.f) limit = cut<true>(row, s, w, limit, (double)p);
-  const float last = logit_of((uint32_t)(limit >> 32));
-  const bool all = limit == 1;
-  const int last_index = (int)~(uint32_t)limit;
-  const float m = P.min_p == nullptr ? 0.f : fminf(P.min_p[r], 1.f);
-  const double least = m > 0.f ? __builtin_ldexp((double)m, P.unit_log2) : 0.0;
-  auto weight = [&](float x, int i) __attribute__((always_inline)) -> uint64_t {
-    const bool kept = all ? x > -INFINITY : x > last || (x == last && i <= last_index);
-    if (!kept) return 0;
-    const double v = w.of(x);
-    return v >= least ? Weigher::units(v) : 0;
+  f.k = k;
+  f.p = p;
+  f.size = m;
+  f.by_count = k > 0 && k < P.vocab;
+  f.by_share = p < 1.f;
+  f.by_size = m > 0.f;
+  auto set_up = [&](auto& w) __attribute__((always_inline)) {
+    w.top = top;
+    w.top_f = top;
+    w.rate = 1.4426950408889634 / (double)temperature;
+    w.offset = -w.top * w.rate;
+    w.magic = 0x1.8p52 + (double)P.unit_log2;
+    w.bins_per = (float)fmin(w.rate * (kBins / 46.0), 1e30);
+    f.least = f.by_size ? f.size * w.of(top) : 0.0;
   };
-
-  uint64_t sum = 0, total;
-  row.each([&](float x, int i) __attribute__((always_inline)) { sum += weight(x, i); });
-  sum = wave_total(sum);
-  __syncthreads();
-  if (lane == 0) s.wave64[wave] = sum;
-  __syncthreads();
-  uint64_t before = 0;
-  total = 0;
-#pragma unroll
-  for (int v = 0; v < kSampleWaves; ++v) {
-    const uint64_t x = s.wave64[v];
-    before += v < wave ? x : 0;
-    total += x;
+  if (fabs((double)top * (1.4426950408889634 / (double)temperature)) < 0x1p20) {
+    Weigher<true> w;
+    set_up(w);
+    int bin = -1;
+    uint64_t before = 0;
+    double goal = -1.0;
+    if ((f.by_count || f.by_share || f.by_size) && draw_few(P, r, row, s, w, f, part_top, bin, before, goal)) return;
+    __syncthreads();
+    draw_many(P, r, row, s, w, f, bin, before, goal);
+  } else {
+    Weigher<false> w;
+    set_up(w);
+    draw_many(P, r, row, s, w, f, -1, 0, -1.0);
   }
-  // The running weight that must be passed; the largest token has a weight, so one does pass.
-  const double u = P.uniform[r];
-  const uint64_t goal = u > 0.0 ? min((uint64_t)(fmin(u, 1.0) * (double)total), total - 1) : 0;
-  if (goal < before || goal >= before + sum) return;
-  row.each_vector([&](const Vec<T, SampleRow<T>::E>& x, int i) __attribute__((always_inline)) {
-    uint64_t mine = 0;
-#pragma unroll
-    for (int e = 0; e < SampleRow<T>::E; ++e) mine += weight(x.get(e), i + e);
-    const uint64_t run = wave_running(mine);
-    uint64_t at = before + run - mine;
-    if (goal >= at && goal < at + mine) {
-      for (int e = 0; e < SampleRow<T>::E; ++e) {
-        const float y = x.get(e);
-        const uint64_t q = weight(y, i + e);
-        if (goal >= at && goal < at + q) {
-          const double share = w.endless ? 0.0 : ((double)y - w.top) * (w.rate * 0.6931471805599453);
-          P.tokens[r] = i + e;
-          P.logprobs[r] = (float)(share - log(__builtin_ldexp((double)total, -P.unit_log2)));
-        }
-        at += q;
-      }
-    }
-    before += shfl_u64(run, 63);
-  });
 }
 
 template <typename T> static int sample_type(const SampleParams& P, int rows, hipStream_t stream) {
