@@ -23,11 +23,15 @@
 
 namespace cdb {
 
-constexpr int kWaves = 4;
+constexpr int kWaves = 8;        // of a prefix's workgroup
+constexpr int kRowWaves = 2;     // of a row's
 constexpr int kChunk = 1024;     // own tokens of a workgroup
 constexpr int kMaxChunks = 64;   // of a row; longer contexts take longer chunks
 constexpr int kMaxParts = CDB_PREFIX_MAX_PARTS;  // of a prefix
 constexpr int kColumns = 16;     // queries of a product
+constexpr int kQueries = CDB_PREFIX_QUERIES;  // of an item, 32 a wave
+constexpr int kItem = CDB_PREFIX_ITEM;        // words of an item
+static_assert(kQueries % 32 == 0 && kQueries <= 32 * kWaves, "queries of an item's waves");
 static_assert(kMaxParts <= 64, "a lane weighs a part");
 
 struct PrefixParams {
@@ -38,10 +42,10 @@ struct PrefixParams {
   int32_t cache_layer0, num_layers, table_rows, table_width, max_positions, bs_log2;
   const float *cos, *sin;
   const void *q_bias, *k_bias;
-  const int32_t *listed, *groups, *items, *row_info;
-  int32_t num_listed, num_groups, num_items;
+  const int32_t *listed, *items, *row_info;
+  int32_t num_listed, num_items;
   void* out;
-  float* shared;   // [items][KV heads][kColumns][D + 2]: O, the maximum and the sum of a prefix's part
+  float* shared;   // [items][KV heads][kQueries][D + 2]: O, the maximum and the sum of a prefix's part
   float* partials; // [rows][heads][max_chunks][D + 2]: the same of a chunk of own tokens
   uint64_t* tags;  // [rows][KV heads][slices][max_chunks]: equal to `tag` where this call's partials are whole
   uint64_t tag;
@@ -78,7 +82,8 @@ template <int D> struct StepRegs<bf16_t, D> {
 
   CDB_DEVICE void load_key(int a, const char* tile, uint32_t token, int g) {
 #pragma unroll
-    for (int j = 0; j < kRuns; ++j) k[a][j] = *reinterpret_cast<const u32x4_t*>(tile + (token + (32 * j + 8 * g) * 2u));
+    for (int j = 0; j < kRuns; ++j)
+      k[a][j] = *reinterpret_cast<const u32x4_t*>(tile + (token + (32 * j + 8 * g) * 2u));
   }
   CDB_DEVICE void load_value(int i, const char* tile, uint32_t token, int r) {
     const char* p = tile + (token + (uint32_t)r * (D / 8));
@@ -94,43 +99,58 @@ template <int D> struct StepRegs<bf16_t, D> {
       for (int w = 0; w < kWords; ++w) v[i][w] = x.w[w];
     }
   }
-  // Elements d and d + 1 (d even) of column c, scaled already, to LDS.
-  static CDB_DEVICE void store_query(uint32_t* to, int c, int d, float x0, float x1) {
-    to += ((d >> 5) * 64 + ((d & 31) >> 3) * 16 + c) * 4 + ((d & 7) >> 1);
-    const uint32_t y = pack_bf16x2(x0, x1);
-    to[0] = y;
-    to[kRuns * 64 * 4] = pack_bf16x2(x0 - __uint_as_float(y << 16), x1 - __uint_as_float(y & 0xffff0000u));
-  }
-  CDB_DEVICE void scores(const uint32_t* query, int lane, f32x4_t* s) const {
+  // Elements d..d + 7 of column c, scaled already, to LDS.
+  static CDB_DEVICE void store_query(uint32_t* to, int c, int d, const float* x) {
+    to += ((d >> 5) * 64 + ((d & 31) >> 3) * 16 + c) * 4;
+    u32x4_t hi, lo;
 #pragma unroll
-    for (int a = 0; a < kTiles; ++a) s[a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < 4; ++i) {
+      hi[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
+      lo[i] = pack_bf16x2(x[2 * i] - __uint_as_float(hi[i] << 16), x[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
+    }
+    *reinterpret_cast<u32x4_t*>(to) = hi;
+    *reinterpret_cast<u32x4_t*>(to + kRuns * 64 * 4) = lo;
+  }
+  template <int NC> CDB_DEVICE void scores(const uint32_t* query, const int* slot, f32x4_t (*s)[kTiles]) const {
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a) s[n][a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int p = 1; p >= 0; --p)
 #pragma unroll
-      for (int j = 0; j < kRuns; ++j) {
-        const bf16x8_t q = *reinterpret_cast<const bf16x8_t*>(query + ((p * kRuns + j) * 64 + lane) * 4);
+      for (int j = 0; j < kRuns; ++j)
 #pragma unroll
-        for (int a = 0; a < kTiles; ++a)
-          s[a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[a][j]), q, s[a], 0, 0, 0);
-      }
+        for (int n = 0; n < NC; ++n) {
+          const bf16x8_t q = *reinterpret_cast<const bf16x8_t*>(query + slot[n] * 4 + (p * kRuns + j) * 64 * 4);
+#pragma unroll
+          for (int a = 0; a < kTiles; ++a)
+            s[n][a] =
+                __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[a][j]), q, s[n][a], 0, 0, 0);
+        }
   }
-  CDB_DEVICE void accumulate(const f32x4_t* p, f32x4_t* acc) const {
-    union { uint32_t w[4]; bf16x8_t v; } hi, lo;
+  template <int NC> CDB_DEVICE void accumulate(const f32x4_t (*p)[kTiles], f32x4_t (*acc)[D / 16]) const {
+    union { uint32_t w[4]; bf16x8_t v; } hi[NC], lo[NC];
 #pragma unroll
-    for (int i = 0; i < 8; i += 2) {
-      const float x = p[i >> 2][i & 3], y = p[i >> 2][(i & 3) + 1];
-      hi.w[i >> 1] = pack_bf16x2(x, y);
-      lo.w[i >> 1] = pack_bf16x2(x - __uint_as_float(hi.w[i >> 1] << 16),
-                                 y - __uint_as_float(hi.w[i >> 1] & 0xffff0000u));
-    }
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int i = 0; i < 8; i += 2) {
+        const float x = p[n][i >> 2][i & 3], y = p[n][i >> 2][(i & 3) + 1];
+        const uint32_t w = pack_bf16x2(x, y);
+        hi[n].w[i >> 1] = w;
+        lo[n].w[i >> 1] = pack_bf16x2(x - __uint_as_float(w << 16), y - __uint_as_float(w & 0xffff0000u));
+      }
 #pragma unroll
     for (int m = 0; m < D / 16; ++m) {
       union { uint32_t w[4]; bf16x8_t v; } x;
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         x.w[i] = __builtin_amdgcn_perm(v[2 * i + 1][m >> 1], v[2 * i][m >> 1], m & 1 ? 0x07060302u : 0x05040100u);
-      acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, lo.v, acc[m], 0, 0, 0);
-      acc[m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, hi.v, acc[m], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, lo[n].v, acc[n][m], 0, 0, 0);
+        acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, hi[n].v, acc[n][m], 0, 0, 0);
+      }
     }
   }
 };
@@ -151,173 +171,255 @@ template <int D> struct StepRegs<float, D> {
 #pragma unroll
     for (int w = 0; w < kWords; ++w) v[i][w] = x.get(w);
   }
-  static CDB_DEVICE void store_query(uint32_t* to, int c, int d, float x0, float x1) {
-    to += ((d >> 4) * 64 + ((d & 15) >> 2) * 16 + c) * 4 + (d & 3);
-    to[0] = __float_as_uint(x0);
-    to[1] = __float_as_uint(x1);
+  static CDB_DEVICE void store_query(uint32_t* to, int c, int d, const float* x) {
+    to += ((d >> 4) * 64 + ((d & 15) >> 2) * 16 + c) * 4;
+    *reinterpret_cast<f32x4_t*>(to) = (f32x4_t){x[0], x[1], x[2], x[3]};
+    *reinterpret_cast<f32x4_t*>(to + 16 * 4) = (f32x4_t){x[4], x[5], x[6], x[7]};
   }
-  CDB_DEVICE void scores(const uint32_t* query, int lane, f32x4_t* s) const {
-    s[0] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+  template <int NC> CDB_DEVICE void scores(const uint32_t* query, const int* slot, f32x4_t (*s)[kTiles]) const {
 #pragma unroll
-    for (int j = 0; j < kRuns; ++j) {
-      const f32x4_t q = *reinterpret_cast<const f32x4_t*>(query + (j * 64 + lane) * 4);
+    for (int n = 0; n < NC; ++n) s[n][0] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s[0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][j][i], q[i], s[0], 0, 0, 0);
-    }
+    for (int j = 0; j < kRuns; ++j)
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const f32x4_t q = *reinterpret_cast<const f32x4_t*>(query + slot[n] * 4 + j * 64 * 4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s[n][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][j][i], q[i], s[n][0], 0, 0, 0);
+      }
   }
-  CDB_DEVICE void accumulate(const f32x4_t* p, f32x4_t* acc) const {
+  template <int NC> CDB_DEVICE void accumulate(const f32x4_t (*p)[kTiles], f32x4_t (*acc)[D / 16]) const {
 #pragma unroll
     for (int m = 0; m < D / 16; ++m)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) acc[m] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][m], p[0][i], acc[m], 0, 0, 0);
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int n = 0; n < NC; ++n)
+          acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][m], p[n][0][i], acc[n][m], 0, 0, 0);
   }
 };
 
-// A wave's running maximum and sum (of query r, over the lane's own tokens) and O^T: rows are elements, row x of
-// product m element x * D / 16 + m.
-template <typename T, int D> struct Walk {
+// A wave's running maxima and sums for NC times 16 queries (of query r, over the lane's own tokens) and O^T: rows are
+// elements, row x of product m element x * D / 16 + m.
+template <typename T, int D, int NC> struct Walk {
   static constexpr int kTiles = StepRegs<T, D>::kTiles;
-  float top, sum;
+  float top[NC], sum[NC];
   bool missing;
-  f32x4_t acc[D / 16];
+  f32x4_t acc[NC][D / 16];
+  int lane;
 
-  CDB_DEVICE void start() {
-    top = -INFINITY;
-    sum = 0.f;
+  CDB_DEVICE void start(int l) {
+    lane = l;
     missing = false;
 #pragma unroll
-    for (int m = 0; m < D / 16; ++m) acc[m] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    for (int n = 0; n < NC; ++n) {
+      top[n] = -INFINITY;
+      sum[n] = 0.f;
+#pragma unroll
+      for (int m = 0; m < D / 16; ++m) acc[n][m] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
+    }
   }
   // Scores, in units of log2, to weights. Tokens outside [lo, hi) of a tile have none.
-  CDB_DEVICE void weigh(f32x4_t* s, const int* lo, const int* hi, int g) {
-    float most = top;
+  CDB_DEVICE void weigh(f32x4_t (*s)[kTiles], const int* lo, const int* hi, int g) {
+    bool edge = false;
+#pragma unroll
+    for (int a = 0; a < kTiles; ++a) edge = edge || lo[a] > 0 || hi[a] < 16;
+    if (edge) {
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool in = 4 * g + i >= lo[a] && 4 * g + i < hi[a];
+#pragma unroll
+          for (int n = 0; n < NC; ++n) s[n][a][i] = in ? s[n][a][i] : -INFINITY;
+        }
+    }
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float most = top[n];
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) most = fmaxf(most, s[n][a][i]);
+      if (__any(most > top[n])) {
+        most = column_max(most);
+        const float keep = top[n] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top[n] - most);  // the first finds zeros
+        sum[n] *= keep;
+#pragma unroll
+        for (int m = 0; m < D / 16; ++m) acc[n][m] *= keep;
+        top[n] = most;
+      }
+      const float from = top[n] == -INFINITY ? 0.f : top[n];
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s[n][a][i] = __builtin_amdgcn_exp2f(s[n][a][i] - from);
+          sum[n] += s[n][a][i];
+        }
+    }
+  }
+  // Tokens [lo, hi), step `first` of every `stride`: `open` puts the first step on its way, `tokens` walks.
+  StepRegs<T, D> x;
+  int64_t where;  // lane j: byte offset of tile window + j
+  int lo, hi, first, stride, count, window;
+
+  CDB_DEVICE int64_t offset(int j) const {
+    const uint32_t a = __builtin_amdgcn_readlane((int)(uint32_t)where, j);
+    const uint32_t b = __builtin_amdgcn_readlane((int)(uint32_t)(where >> 32), j);
+    return (int64_t)(((uint64_t)b << 32) | a);
+  }
+  // Of a tile that sticks out of the range the nearest token inside stands for those outside; the last step's second
+  // tile may be missing: the first stands in for it.
+  CDB_DEVICE int bounds(int step, int a, int& b0, int& b1) const {
+    const int j = min(kTiles * step + a, count - 1), t = ((lo >> 4) + window + j) * 16;
+    b0 = max(lo - t, 0);
+    b1 = min(hi - t, 16);
+    return j;
+  }
+  CDB_DEVICE void load_keys(const Tokens& at, int step, int r, int g) {
 #pragma unroll
     for (int a = 0; a < kTiles; ++a) {
-      if (lo[a] > 0 || hi[a] < 16) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) s[a][i] = 4 * g + i >= lo[a] && 4 * g + i < hi[a] ? s[a][i] : -INFINITY;
-      }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) most = fmaxf(most, s[a][i]);
+      int b0, b1;
+      const int64_t tile = offset(bounds(step, a, b0, b1));
+      x.load_key(a, at.k + tile, (uint32_t)min(max(r, b0), b1 - 1) * (uint32_t)at.row_bytes, g);
     }
-    most = column_max(most);
-    if (__any(most > top)) {
-      const float keep = top == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(top - most);  // the first finds zeros
-      sum *= keep;
-#pragma unroll
-      for (int m = 0; m < D / 16; ++m) acc[m] *= keep;
-      top = most;
-    }
-    const float from = top == -INFINITY ? 0.f : top;
-#pragma unroll
-    for (int a = 0; a < kTiles; ++a)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[a][i] = __builtin_amdgcn_exp2f(s[a][i] - from);
-        sum += s[a][i];
-      }
   }
-  // Tokens [lo, hi), step `first` of every `stride`.
-  CDB_DEVICE void tokens(const Tokens& at, const uint32_t* query, int lo, int hi, int first, int stride) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    if (lo >= hi) return;
-    const int t0 = lo >> 4, tiles = ((hi + 15) >> 4) - t0;
-    const uint32_t row_bytes = (uint32_t)at.row_bytes;
-    for (int window = 0; window < tiles; window += 64) {
-      const int count = min(64, tiles - window);
-      int64_t where = 0;
-      bool lost = false;
-      if (lane < count) where = at.at((t0 + window + lane) * 16, lost);
-      missing = missing || __ballot(lost) != 0;
-      auto offset = [&](int j) __attribute__((always_inline)) -> int64_t {
-        const uint32_t a = __builtin_amdgcn_readlane((int)(uint32_t)where, j);
-        const uint32_t b = __builtin_amdgcn_readlane((int)(uint32_t)(where >> 32), j);
-        return (int64_t)(((uint64_t)b << 32) | a);
-      };
-      StepRegs<T, D> x;
-      int from[kTiles], to[kTiles];
-      // Of a tile that sticks out of the range the nearest token inside stands for those outside; the last step's
-      // second tile may be missing: the first stands in for it.
-      auto bounds = [&](int step, int a, int& b0, int& b1) __attribute__((always_inline)) -> int {
-        const int j = min(kTiles * step + a, count - 1), t = (t0 + window + j) * 16;
-        b0 = max(lo - t, 0);
-        b1 = min(hi - t, 16);
-        return j;
-      };
-      auto load_keys = [&](int step) __attribute__((always_inline)) {
+  CDB_DEVICE void load_values(const Tokens& at, int step, int r, int g) {
 #pragma unroll
-        for (int a = 0; a < kTiles; ++a) {
-          int b0, b1;
-          const int64_t tile = offset(bounds(step, a, b0, b1));
-          x.load_key(a, at.k + tile, (uint32_t)min(max(r, b0), b1 - 1) * row_bytes, g);
-        }
-      };
-      auto load_values = [&](int step) __attribute__((always_inline)) {
+    for (int a = 0; a < kTiles; ++a) {
+      int b0, b1;
+      const int64_t tile = offset(bounds(step, a, b0, b1));
 #pragma unroll
-        for (int a = 0; a < kTiles; ++a) {
-          int b0, b1;
-          const int64_t tile = offset(bounds(step, a, b0, b1));
+      for (int i = 0; i < 4; ++i)
+        x.load_value(4 * a + i, at.v + tile, (uint32_t)min(max(4 * g + i, b0), b1 - 1) * (uint32_t)at.row_bytes, r);
+    }
+  }
+  CDB_DEVICE void look_up(const Tokens& at, int w) {
+    const int r = lane & 15, g = lane >> 4;
+    window = w;
+    count = min(64, ((hi + 15) >> 4) - (lo >> 4) - w);
+    where = 0;
+    bool lost = false;
+    if (lane < count) where = at.at(((lo >> 4) + w + lane) * 16, lost);
+    missing = missing || __ballot(lost) != 0;
+    if (kTiles * first < count) {
+      load_keys(at, first, r, g);
+      __builtin_amdgcn_sched_barrier(0);  // keys before values, as in the steps: the waits count on it
+      load_values(at, first, r, g);
+    }
+  }
+  CDB_DEVICE void open(const Tokens& at, int from, int to, int which, int of) {
+    lo = from;
+    hi = to;
+    first = which;
+    stride = of;
+    count = 0;
+    if (lo < hi) look_up(at, 0);
+  }
+  // The lane's place in the query operands: columns without a query read the last one's.
+  CDB_DEVICE void slots(int cols, int* slot) const {
 #pragma unroll
-          for (int i = 0; i < 4; ++i)
-            x.load_value(4 * a + i, at.v + tile, (uint32_t)min(max(4 * g + i, b0), b1 - 1) * row_bytes, r);
-        }
-      };
+    for (int n = 0; n < NC; ++n) {
+      const int c = min(16 * n + (lane & 15), cols - 1);
+      slot[n] = (c >> 4) * (StepRegs<T, D>::kQueryWords / 4) + (lane & 48) + (c & 15);
+    }
+  }
+  CDB_DEVICE void tokens(const Tokens& at, const uint32_t* query, int cols) {
+    int slot[NC];
+    slots(cols, slot);
+    const int r = lane & 15, g = lane >> 4;
+    const int tiles = lo < hi ? ((hi + 15) >> 4) - (lo >> 4) : 0;
+    for (int w = 0; w < tiles; w += 64) {
+      if (w != 0) look_up(at, w);
       const int steps = (count + kTiles - 1) / kTiles;
-      if (first < steps) {
-        load_keys(first);
-        __builtin_amdgcn_sched_barrier(0);  // keys before values, as in the steps: the waits count on it
-        load_values(first);
-      }
       for (int step = first; step < steps; step += stride) {
         // The loads ahead repeat the step at the end: a branch around them would make the wait for this step's
         // values one for the next keys too.
         const int ahead = step + stride < steps ? step + stride : step;
-        f32x4_t s[kTiles];
-        x.scores(query, lane, s);
-        load_keys(ahead);
+        f32x4_t s[NC][kTiles];
+        x.template scores<NC>(query, slot, s);
+        load_keys(at, ahead, r, g);
+        int from[kTiles], to[kTiles];
 #pragma unroll
         for (int a = 0; a < kTiles; ++a) {
           bounds(step, a, from[a], to[a]);
           if (kTiles * step + a >= count) to[a] = 0;
         }
         weigh(s, from, to, g);
-        x.accumulate(s, acc);
+        x.template accumulate<NC>(s, acc);
         __builtin_amdgcn_sched_barrier(0);
-        load_values(ahead);
+        load_values(at, ahead, r, g);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   }
-  // O, the maximum and the sum of each column to LDS: [column][D + 4].
-  CDB_DEVICE void leave(float* to, int cols) {
-    const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-    float total = column_sum(sum);
-    if (missing) total = NAN;
-    if (r >= cols) return;
-    float* mine = to + r * (D + 4);
+  // O, the maximum and the sum of each column: [column][stride].
+  CDB_DEVICE void leave(float* to, int cols, int stride) {
+    const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-    for (int i = 0; i < 4; ++i)
+    for (int n = 0; n < NC; ++n) {
+      float total = column_sum(sum[n]);
+      if (missing) total = NAN;
+      if (16 * n + r >= cols) continue;
+      float* mine = to + (16 * n + r) * stride;
 #pragma unroll
-      for (int m = 0; m < D / 16; m += 2)
-        *reinterpret_cast<f32x2_t*>(mine + (4 * g + i) * (D / 16) + m) = (f32x2_t){acc[m][i], acc[m + 1][i]};
-    if (g == 0) {
-      mine[D] = total == 0.f ? -INFINITY : top;  // no token yet, or none above -infinity
-      mine[D + 1] = total;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < D / 16; m += 2)
+          *reinterpret_cast<f32x2_t*>(mine + (4 * g + i) * (D / 16) + m) = (f32x2_t){acc[n][m][i], acc[n][m + 1][i]};
+      if (g == 0) {
+        mine[D] = total == 0.f ? -INFINITY : top[n];  // no token yet, or none above -infinity
+        mine[D + 1] = total;
+      }
+    }
+  }
+  // Takes in what another wave has left for the same columns.
+  CDB_DEVICE void join(const float* from, int cols, int stride) {
+    const int r = lane & 15, g = lane >> 4;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float* other = from + min(16 * n + r, cols - 1) * stride;
+      const float most = fmaxf(top[n], other[D]), base = most == -INFINITY ? 0.f : most;
+      const float f0 = __builtin_amdgcn_exp2f(top[n] - base), f1 = __builtin_amdgcn_exp2f(other[D] - base);
+      sum[n] = fmaf(sum[n], f0, g == 0 ? f1 * other[D + 1] : 0.f);  // a column's sum is that of its four lanes
+      top[n] = most;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int m = 0; m < D / 16; m += 2) {
+          const f32x2_t y = *reinterpret_cast<const f32x2_t*>(other + (4 * g + i) * (D / 16) + m);
+          acc[n][m][i] = fmaf(acc[n][m][i], f0, f1 * y[0]);
+          acc[n][m + 1][i] = fmaf(acc[n][m + 1][i], f0, f1 * y[1]);
+        }
     }
   }
 };
 
-// Query head `head` of row b, rotated and scaled, as column c of the query operand: a wave's work.
+// 16 elements of a column of the query operands: of query head `head` of row b at position p, rotated and scaled; NaN,
+// or zeros, where there is no such query.
 template <typename T, int D, int STYLE>
-CDB_DEVICE void turn_query(const PrefixParams& P, uint32_t* query, int c, int b, int head, int p) {
-  const int lane = threadIdx.x & 63, d = min(2 * lane, D - 2);
-  const int64_t angle = STYLE == 0 ? 0 : (int64_t)p * (D / 2);
-  const T* bias = static_cast<const T*>(P.q_bias);
-  float x[2];
-  load_rotated<T, D, STYLE, 2>(static_cast<const T*>(P.q) + b * P.q_stride + (int64_t)head * D,
-                               bias == nullptr ? nullptr : bias + (int64_t)head * D, P.cos + angle, P.sin + angle, d,
-                               P.vec, x);
-  if (2 * lane < D) StepRegs<T, D>::store_query(query, c, d, mul_rn(x[0], P.scale_log2), mul_rn(x[1], P.scale_log2));
+CDB_DEVICE void turn_query(const PrefixParams& P, uint32_t* query, int c, int piece, int b, int head, int p, float none) {
+  const int d = STYLE == 1 ? 8 * piece : 16 * piece;
+  float x[8], y[8];
+  if (p >= 0) {
+    const int64_t angle = STYLE == 0 ? 0 : (int64_t)p * (D / 2);
+    const T* bias = static_cast<const T*>(P.q_bias);
+    load_rotated_pair<T, D, STYLE, 8>(static_cast<const T*>(P.q) + b * P.q_stride + (int64_t)head * D,
+                                      bias == nullptr ? nullptr : bias + (int64_t)head * D, P.cos + angle,
+                                      P.sin + angle, d, P.vec, x, y);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      x[i] = mul_rn(x[i], P.scale_log2);
+      y[i] = mul_rn(y[i], P.scale_log2);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = y[i] = none;
+  }
+  query += (c >> 4) * StepRegs<T, D>::kQueryWords;
+  StepRegs<T, D>::store_query(query, c & 15, d, x);
+  StepRegs<T, D>::store_query(query, c & 15, STYLE == 1 ? d + D / 2 : d + 8, y);
 }
 
 // What a row's launch arguments come to: whether it is padding, or has none of its own that can be served.
@@ -347,21 +449,24 @@ template <typename T, int D> CDB_DEVICE Tokens tokens_of(const PrefixParams& P, 
   return x;
 }
 
+// Words of LDS: the queries, and in their place later what half of the waves leave to the other half.
+template <typename T, int D> struct AttendLds {
+  static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kQueries / 16), kJoin = kWaves / 2 * 32 * (D + 4);
+  static constexpr int kWords = kQ > kJoin ? kQ : kJoin;
+};
+
 template <typename T, int D, int STYLE>
-__global__ void __launch_bounds__(64 * kWaves) prefix_attend_kernel(PrefixParams P) {
-  __shared__ __align__(16) uint32_t query[StepRegs<T, D>::kQueryWords];
-  __shared__ __align__(16) float join[kWaves * kColumns * (D + 4)];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+__global__ void __launch_bounds__(64 * kWaves, 2) prefix_attend_kernel(PrefixParams P) {
+  __shared__ __align__(16) uint32_t lds[AttendLds<T, D>::kWords];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int item = blockIdx.x / P.num_kv_heads, kvh = blockIdx.x - item * P.num_kv_heads;
-  const int n = P.items[4 * item], q0 = P.items[4 * item + 1];
-  if (n < 0 || n >= P.num_groups) return;  // no item
-  const int first = P.groups[4 * n], count = P.groups[4 * n + 1], length = P.groups[4 * n + 2];
-  if (count <= 0 || count > P.num_listed || first < 0 || first > P.num_listed - count) return;
+  const int4 head = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[0];
+  const int4 tail = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[1];
+  const int first = head.x, count = head.y, leader = head.z, length = head.w, q0 = tail.x, lo = tail.y, hi = tail.z;
+  if (count <= 0 || count > P.num_listed || first < 0 || first > P.num_listed - count) return;  // no item
   const int64_t queries = (int64_t)count * P.group;
   if (q0 < 0 || q0 >= queries) return;
-  const int cols = (int)min((int64_t)kColumns, queries - q0);
-  int lo = P.items[4 * item + 2], hi = P.items[4 * item + 3];
-  const int leader = P.listed[first];
+  const int cols = (int)min((int64_t)kQueries, queries - q0);
   int layer = -1, trow = -1;
   if (leader >= 0 && leader < P.num_rows) {
     layer = P.cache_layer0 + (P.cache_layer == nullptr ? 0 : P.cache_layer[leader]);
@@ -369,49 +474,41 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_attend_kernel(PrefixParams
   }
   const bool bad = layer < 0 || layer >= P.num_layers || trow < 0 || trow >= P.table_rows || lo < 0 || hi > length ||
                    (int64_t)length > ((int64_t)P.table_width << P.bs_log2);
-  for (int c = wave; c < kColumns; c += kWaves) {
-    const int at = q0 + min(c, cols - 1);
-    const int b = P.listed[first + at / P.group];
-    const int p = b >= 0 && b < P.num_rows ? P.seqlens[b] : -1;
-    if (p >= 0 && (STYLE == 0 || p < P.max_positions))
-      turn_query<T, D, STYLE>(P, query, c, b, kvh * P.group + at % P.group, p);
-    else if (2 * (threadIdx.x & 63) < D)  // a padding row, or one that gets NaN
-      StepRegs<T, D>::store_query(query, c, 2 * (threadIdx.x & 63), 0.f, 0.f);
-  }
-  __syncthreads();
-  Walk<T, D> walk;
-  walk.start();
+  // 32 queries a wave; where that leaves waves over, several take the same queries and every so-manieth step.
+  const int runs = cols <= 32 ? 1 : cols <= 64 ? 2 : 4, run = wave & (runs - 1), part = wave / runs, parts = kWaves / runs;
+  const int mine = min(32, cols - 32 * run);  // may be none
+  const Tokens at_prefix = tokens_of<T, D>(P, bad ? 0 : layer, bad ? 0 : trow, kvh);
+  Walk<T, D, 2> walk;
+  walk.start(lane);
   if (bad) walk.missing = true;
-  else walk.tokens(tokens_of<T, D>(P, layer, trow, kvh), query, lo, hi, wave, kWaves);
-  walk.leave(join + wave * cols * (D + 4), cols);
-  __syncthreads();
-  float* to = P.shared + ((int64_t)item * P.num_kv_heads + kvh) * kColumns * (D + 2);
-  for (int i = threadIdx.x; i < cols * D; i += 64 * kWaves) {
-    const int c = i / D, d = i - c * D;
-    float m[kWaves], most = -INFINITY, o = 0.f, l = 0.f;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      m[w] = join[(w * cols + c) * (D + 4) + D];
-      most = fmaxf(most, m[w]);
-    }
-    const float from = most == -INFINITY ? 0.f : most;
-#pragma unroll
-    for (int w = 0; w < kWaves; ++w) {
-      const float* x = join + (w * cols + c) * (D + 4);
-      const float f = __builtin_amdgcn_exp2f(m[w] - from);
-      o = fmaf(f, x[d], o);
-      l = fmaf(f, x[D + 1], l);
-    }
-    to[c * (D + 2) + d] = o;
-    if (d == 0) {
-      to[c * (D + 2) + D] = most;
-      to[c * (D + 2) + D + 1] = l;
-    }
+  walk.open(at_prefix, bad || mine <= 0 ? 0 : lo, bad || mine <= 0 ? 0 : hi, part, parts);
+  constexpr int kPieces = D / 16;
+#pragma unroll 2
+  for (int i = threadIdx.x; i < cols * kPieces; i += 64 * kWaves) {
+    const int c = i / kPieces, at = q0 + c;
+    const int b = P.listed[first + at / P.group];
+    int p = b >= 0 && b < P.num_rows ? P.seqlens[b] : -1;
+    // A padding row, or one that gets NaN: for not being at its group's cache layer, from here.
+    const bool stranger = p >= 0 && P.cache_layer != nullptr && P.cache_layer0 + P.cache_layer[b] != layer;
+    if (stranger || (STYLE != 0 && p >= P.max_positions)) p = -1;
+    turn_query<T, D, STYLE>(P, lds, c, i - c * kPieces, b, kvh * P.group + at % P.group, p, stranger ? NAN : 0.f);
   }
+  __syncthreads();
+  if (mine > 0) walk.tokens(at_prefix, lds + 2 * run * StepRegs<T, D>::kQueryWords, mine);
+  float* to = P.shared + ((int64_t)item * P.num_kv_heads + kvh) * kQueries * (D + 2);
+  // Waves with the same queries are joined in halves.
+  float* join = reinterpret_cast<float*>(lds) + run * 32 * (D + 4);
+  for (int half = parts >> 1; half > 0; half >>= 1) {
+    __syncthreads();
+    if (mine > 0 && part >= half && part < 2 * half) walk.leave(join + (part - half) * runs * 32 * (D + 4), mine, D + 4);
+    __syncthreads();
+    if (mine > 0 && part < half) walk.join(join + part * runs * 32 * (D + 4), mine, D + 4);
+  }
+  if (mine > 0 && part == 0) walk.leave(to + 32 * run * (D + 2), mine, D + 2);
 }
 
 template <typename T, int D, int STYLE>
-__global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams P) {
+__global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(PrefixParams P) {
   __shared__ __align__(16) uint32_t query[StepRegs<T, D>::kQueryWords];
   __shared__ __align__(16) T fresh[2][D];
   __shared__ float weights[kColumns][kMaxChunks + kMaxParts];
@@ -428,20 +525,13 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
   const int n0 = P.row_info[4 * b], item0 = P.row_info[4 * b + 2], parts = P.row_info[4 * b + 3];
   if (parts == 0) {
     row.bad = row.bad || row.own != 0;
-  } else if (!row.bad) {
-    const int64_t last = item0 + (((int64_t)n0 + P.group - 1) / kColumns + 1) * parts;  // behind the row's last item
-    if (parts < 0 || parts > kMaxParts || n0 < 0 || item0 < 0 || last > P.num_items) {
-      row.bad = true;
-    } else {
-      const int n = P.items[4 * item0], first = n >= 0 && n < P.num_groups ? P.groups[4 * n] : -1;
-      const int leader = first >= 0 && first < P.num_listed ? P.listed[first] : -1;
-      row.bad = leader < 0 || leader >= P.num_rows ||
-                (P.cache_layer != nullptr && P.cache_layer[leader] != P.cache_layer[b]);
-    }
+  } else {
+    const int64_t last = item0 + (((int64_t)n0 + P.group - 1) / kQueries + 1) * parts;  // behind the row's last item
+    row.bad = row.bad || parts < 0 || parts > kMaxParts || n0 < 0 || item0 < 0 || last > P.num_items;
   }
   if (p < 0 || row.bad) {
     if (chunk == 0)
-      for (int i = threadIdx.x; i < P.group * D; i += 64 * kWaves) Elem<T>::store(out + i, p < 0 ? 0.f : NAN);
+      for (int i = threadIdx.x; i < P.group * D; i += 64 * kRowWaves) Elem<T>::store(out + i, p < 0 ? 0.f : NAN);
     return;
   }
   // A row with more chunks than the workspace has partials for takes longer ones.
@@ -457,12 +547,18 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
 
   for (int slice = 0; slice < P.group; slice += kColumns) {
     const int cols = min(kColumns, P.group - slice);
-    for (int c = wave; c < kColumns; c += kWaves)
-      turn_query<T, D, STYLE>(P, query, c, b, kvh * P.group + slice + min(c, cols - 1), p);
-    Walk<T, D> walk;
-    walk.start();
-    if (ends && wave == kWaves - 1) {
-      const int lane = threadIdx.x & 63, d = min(2 * lane, D - 2);
+    // Opaque, so that nothing derived from the lane is kept over the loop (it takes one turn but for groups of more
+    // than 16, and the registers are needed inside).
+    int tid = threadIdx.x;
+    __asm__ volatile("" : "+v"(tid));
+    const int lane = tid & 63;
+    Walk<T, D, 1> walk;
+    walk.start(lane);
+    walk.open(at, lo, hi, wave, kRowWaves);  // on its way before the queries are turned
+    for (int i = tid; i < cols * (D / 16); i += 64 * kRowWaves)
+      turn_query<T, D, STYLE>(P, query, i / (D / 16), i % (D / 16), b, kvh * P.group + slice + i / (D / 16), p, 0.f);
+    if (ends && wave == kRowWaves - 1) {
+      const int d = min(2 * lane, D - 2);
       const int64_t angle = STYLE == 0 ? 0 : (int64_t)p * (D / 2), from = b * P.kv_stride + (int64_t)kvh * D;
       const T* bias = static_cast<const T*>(P.k_bias);
       float x[2], y[2];
@@ -471,7 +567,7 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
                                    P.cos + angle, P.sin + angle, d, P.vec, x);
       bool lost = false;
       const int64_t tile = at.at(p & ~15, lost) + (int64_t)(p & 15) * at.row_bytes;
-      walk.missing = lost;
+      walk.missing = walk.missing || lost;
       Vec<T, 2> k, v;
       k.set_pair(0, x[0], x[1]);
       v.set_pair(0, y[0], y[1]);
@@ -485,44 +581,44 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
       }
     }
     __syncthreads();
-    if (ends && wave == kWaves - 1) {
+    walk.tokens(at, query, cols);
+    if (ends && wave == kRowWaves - 1) {
       // The new token as the first of a tile.
-      const int lane = threadIdx.x & 63, r = lane & 15, g = lane >> 4;
-      StepRegs<T, D> x;
+      const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-      for (int a = 0; a < StepRegs<T, D>::kTiles; ++a) x.load_key(a, reinterpret_cast<const char*>(fresh[0]), 0, g);
+      for (int a = 0; a < StepRegs<T, D>::kTiles; ++a) walk.x.load_key(a, reinterpret_cast<const char*>(fresh[0]), 0, g);
 #pragma unroll
       for (int i = 0; i < 4 * StepRegs<T, D>::kTiles; ++i)
-        x.load_value(i, reinterpret_cast<const char*>(fresh[1]), 0, r);
-      f32x4_t s[StepRegs<T, D>::kTiles];
-      x.scores(query, lane, s);
+        walk.x.load_value(i, reinterpret_cast<const char*>(fresh[1]), 0, r);
+      f32x4_t s[1][StepRegs<T, D>::kTiles];
+      int slot[1];
+      walk.slots(cols, slot);
+      walk.x.template scores<1>(query, slot, s);
       const int from[2] = {0, 0}, to[2] = {1, 0};
       walk.weigh(s, from, to, g);
-      x.accumulate(s, walk.acc);
+      walk.x.template accumulate<1>(s, walk.acc);
     }
-    walk.tokens(at, query, lo, hi, wave, kWaves);
-    walk.leave(join + wave * cols * kPlace, cols);
+    walk.leave(join + wave * cols * kPlace, cols, kPlace);
     __syncthreads();
 
-    const int tid = threadIdx.x, lane = tid & 63;
-    const int64_t shared_stride = (int64_t)P.num_kv_heads * kColumns * (D + 2);
+    const int64_t shared_stride = (int64_t)P.num_kv_heads * kQueries * (D + 2);
     auto shared_of = [&](int c) __attribute__((always_inline)) -> const float* {
       const int n = n0 + slice + c;
-      return P.shared + (((int64_t)item0 + n / kColumns * parts) * P.num_kv_heads + kvh) * kColumns * (D + 2) +
-             n % kColumns * (D + 2);
+      return P.shared + (((int64_t)item0 + n / kQueries * parts) * P.num_kv_heads + kvh) * kQueries * (D + 2) +
+             n % kQueries * (D + 2);
     };
     if (chunks > 1) {
-      for (int i = tid; i < cols * D; i += 64 * kWaves) {
+      for (int i = tid; i < cols * D; i += 64 * kRowWaves) {
         const int c = i / D, d = i - c * D;
-        float m[kWaves], most = -INFINITY, o = 0.f, l = 0.f;
+        float m[kRowWaves], most = -INFINITY, o = 0.f, l = 0.f;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < kRowWaves; ++w) {
           m[w] = join[(w * cols + c) * kPlace + D];
           most = fmaxf(most, m[w]);
         }
         const float from = most == -INFINITY ? 0.f : most;
 #pragma unroll
-        for (int w = 0; w < kWaves; ++w) {
+        for (int w = 0; w < kRowWaves; ++w) {
           const float* x = join + (w * cols + c) * kPlace;
           const float f = __builtin_amdgcn_exp2f(m[w] - from);
           o = fmaf(f, x[d], o);
@@ -558,9 +654,9 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
       }
     }
     // Weights of the waves, or of the chunks, and of the prefix's parts, a wave a column.
-    const int mine = chunks > 1 ? chunks : kWaves;
+    const int mine = chunks > 1 ? chunks : kRowWaves;
     const float* rows = P.partials + ((int64_t)b * P.num_heads + kvh * P.group + slice) * P.max_chunks * (D + 2);
-    for (int c = wave; c < cols; c += kWaves) {
+    for (int c = wave; c < cols; c += kRowWaves) {
       float m0 = -INFINITY, l0 = 0.f, m1 = -INFINITY, l1 = 0.f;
       if (lane < mine) {
         if (chunks > 1) {
@@ -584,14 +680,23 @@ __global__ void __launch_bounds__(64 * kWaves) prefix_decode_kernel(PrefixParams
       if (lane < parts) weights[c][kMaxChunks + lane] = f1 / total;
     }
     __syncthreads();
-    for (int i = tid; i < cols * (D / 2); i += 64 * kWaves) {
+    for (int i = tid; i < cols * (D / 2); i += 64 * kRowWaves) {
       const int c = i / (D / 2), d = 2 * (i - c * (D / 2));
       float o0 = 0.f, o1 = 0.f;
       const float* x = shared_of(c) + d;
-      for (int n = 0; n < parts; ++n) {
-        const f32x2_t y = *reinterpret_cast<const f32x2_t*>(x + n * shared_stride);
-        o0 = fmaf(weights[c][kMaxChunks + n], y[0], o0);
-        o1 = fmaf(weights[c][kMaxChunks + n], y[1], o1);
+      for (int n = 0; n < parts; n += 8) {
+        f32x2_t y[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          y[j] = *reinterpret_cast<const f32x2_t*>(x + (int64_t)min(n + j, parts - 1) * shared_stride);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+          const float f = n + j < parts ? weights[c][kMaxChunks + min(n + j, kMaxParts - 1)] : 0.f;
+          if (n + j < parts) {
+            o0 = fmaf(f, y[j][0], o0);
+            o1 = fmaf(f, y[j][1], o1);
+          }
+        }
       }
       for (int n = 0; n < mine; ++n) {
         float y0, y1;
@@ -628,8 +733,8 @@ template <typename T, int D, int STYLE> static int prefix_style(const PrefixPara
   }
   const int64_t most = ((int64_t)P.table_width << P.bs_log2) / kChunk + 1;
   const dim3 grid((unsigned)(P.num_rows * P.num_kv_heads), (unsigned)min((int64_t)P.max_chunks, most));
-  const size_t lds = sizeof(float) * kWaves * min(P.group, kColumns) * (D + 4);
-  prefix_decode_kernel<T, D, STYLE><<<grid, wg, lds, stream>>>(P);
+  const size_t lds = sizeof(float) * kRowWaves * min(P.group, kColumns) * (D + 4);
+  prefix_decode_kernel<T, D, STYLE><<<grid, dim3(64 * kRowWaves), lds, stream>>>(P);
   return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;
 }
 template <typename T, int D> static int prefix_dim(const PrefixParams& P, int style, hipStream_t stream) {
@@ -652,7 +757,7 @@ static int64_t chunk_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head
 }
 // Bytes of the partials of prefixes, a multiple of 16.
 static int64_t shared_bytes(int64_t num_items, int32_t num_kv_heads, int32_t head_dim) {
-  return num_items * num_kv_heads * kColumns * (head_dim + 2) * 4;
+  return num_items * num_kv_heads * kQueries * (head_dim + 2) * 4;
 }
 
 // A tag that no other call of this process has, and that memory does not hold by chance.
@@ -681,8 +786,8 @@ extern "C" int cdb_prefix_decode_attention(
     int32_t num_cache_layers, int64_t pool_blocks, const int32_t* cache_layer, int32_t cache_layer0,
     const int32_t* block_table, const int32_t* table_row, int32_t table_rows, int32_t table_width,
     const int32_t* seqlens, const float* rope_cos, const float* rope_sin, int32_t rope_style, int32_t max_positions,
-    const void* q_bias, const void* k_bias, const int32_t* listed, int32_t num_listed, const int32_t* groups,
-    int32_t num_groups, const int32_t* items, int32_t num_items, const int32_t* row_info, void* out, void* workspace,
+    const void* q_bias, const void* k_bias, const int32_t* listed, int32_t num_listed, const int32_t* items,
+    int32_t num_items, const int32_t* row_info, void* out, void* workspace,
     int64_t workspace_bytes, int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
     int32_t block_size, float scale, int64_t q_stride, int64_t kv_stride, int32_t dtype, hipStream_t stream) {
   using namespace cdb;
@@ -691,7 +796,7 @@ extern "C" int cdb_prefix_decode_attention(
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   if (num_rows < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows <= 0 ||
       table_width <= 0 || num_cache_layers <= 0 || pool_blocks <= 0 || pool_blocks > 0x7fffffffll || num_listed < 0 ||
-      num_groups < 0 || num_items < 0)
+      num_items < 0)
     return CDB_ERR_SHAPE;
   if (block_size < 16 || (block_size & (block_size - 1)) != 0) return CDB_ERR_SHAPE;
   if (num_rows == 0) return CDB_OK;
@@ -699,7 +804,7 @@ extern "C" int cdb_prefix_decode_attention(
       block_table == nullptr || seqlens == nullptr || row_info == nullptr || out == nullptr || workspace == nullptr)
     return CDB_ERR_NULL;
   if (rope_style != 0 && (rope_cos == nullptr || rope_sin == nullptr)) return CDB_ERR_NULL;
-  if (num_items != 0 && (listed == nullptr || groups == nullptr || items == nullptr)) return CDB_ERR_NULL;
+  if (num_items != 0 && (listed == nullptr || items == nullptr)) return CDB_ERR_NULL;
   if (rope_style != 0 && max_positions <= 0) return CDB_ERR_SHAPE;
   const int size = dtype == CDB_DTYPE_F32 ? 4 : 2;
   const int64_t row = (int64_t)num_kv_heads * head_dim;
@@ -713,7 +818,7 @@ extern "C" int cdb_prefix_decode_attention(
   if (kv_stride == 0) kv_stride = row;
   if (q_stride < (int64_t)num_heads * head_dim || kv_stride < row) return CDB_ERR_SHAPE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(k_pool) % 16 != 0 ||
-      reinterpret_cast<uintptr_t>(v_pool) % 16 != 0 || layer_stride * size % 16 != 0)
+      reinterpret_cast<uintptr_t>(v_pool) % 16 != 0 || reinterpret_cast<uintptr_t>(items) % 16 != 0 || layer_stride * size % 16 != 0)
     return CDB_ERR_SHAPE;
   const int64_t left = workspace_bytes - shared_bytes(num_items, num_kv_heads, head_dim);
   const int64_t chunks = left < 0 ? 0 : min(left / (num_rows * chunk_bytes(num_heads, num_kv_heads, head_dim)),
@@ -728,8 +833,8 @@ extern "C" int cdb_prefix_decode_attention(
   P.max_positions = rope_style != 0 ? max_positions : 0;
   P.bs_log2 = __builtin_ctz(block_size);
   P.q_bias = q_bias; P.k_bias = k_bias;
-  P.listed = listed; P.groups = groups; P.items = items; P.row_info = row_info;
-  P.num_listed = num_listed; P.num_groups = num_groups; P.num_items = num_items;
+  P.listed = listed; P.items = items; P.row_info = row_info;
+  P.num_listed = num_listed; P.num_items = num_items;
   P.out = out; P.shared = static_cast<float*>(workspace);
   P.partials = P.shared + shared_bytes(num_items, num_kv_heads, head_dim) / 4;
   P.max_chunks = (int32_t)chunks;

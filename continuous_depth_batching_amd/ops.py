@@ -272,13 +272,11 @@ class PrefixDecodePlan:
     which the rows, their order and their prefixes stay.
 
     listed    [n] rows with a prefix, group by group
-    groups    [groups, 4]: (first place in listed, rows, tokens of the prefix, first item)
-    items     [m, 4]: (group, first query, first token, end token)
+    items     [m, 8]: (the group's first place in listed, rows, first row and tokens, first query, first and end token, 0)
     row_info  [rows, 4]: (first query in the group, tokens of the prefix, the group's first item, parts)
     """
 
     listed: "np.ndarray | torch.Tensor"
-    groups: "np.ndarray | torch.Tensor"
     items: "np.ndarray | torch.Tensor"
     row_info: "np.ndarray | torch.Tensor"
 
@@ -295,10 +293,10 @@ class PrefixDecodePlan:
 
         import numpy as np
 
-        arrays = [np.asarray(a, dtype=np.int32) for a in (self.listed, self.groups, self.items, self.row_info)]
+        arrays = [np.asarray(a, dtype=np.int32) for a in (self.items, self.row_info, self.listed)]  # items aligned
         flat = torch.from_numpy(np.concatenate([a.ravel() for a in arrays])).to(device)
-        parts = flat.split([a.size for a in arrays])
-        return PrefixDecodePlan(*(x.view(a.shape) for x, a in zip(parts, arrays)))
+        items, info, listed = (x.view(a.shape) for x, a in zip(flat.split([a.size for a in arrays]), arrays))
+        return PrefixDecodePlan(listed=listed, items=items, row_info=info)
 
 
 def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np.ndarray", *, num_heads: int,
@@ -307,8 +305,9 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
     group's ``lengths[group[b]]`` tokens. Rows of one group sit at the same cache layer: rows at two loop depths of a
     layout with a slot a step are two groups.
 
-    Prefixes are cut into parts of about equal length, enough of them to give every CU two workgroups while a part
-    keeps 128 tokens, and at most 64. A row's rounding depends on its prefix's parts."""
+    Prefixes are cut into parts of about equal length, enough of them to give every CU a workgroup while a part keeps
+    128 tokens, and at most 64 (a part costs each of its queries a partial result, written and read again). A row's
+    rounding depends on its prefix's parts."""
 
     import numpy as np
 
@@ -328,25 +327,21 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
     names, first, counts = np.unique(group[order], return_index=True, return_counts=True)
     tokens = lengths[names]
     runs = (counts * share + PREFIX_QUERIES - 1) // PREFIX_QUERIES
-    each = max(128, -(-int((runs * tokens).sum()) * num_kv_heads // (2 * int(num_cus))))
-    parts = np.minimum(-(-tokens // each), _lib.CDB_PREFIX_MAX_PARTS)
-    items, groups = [], []
-    for n, (at, count, length, run, part) in enumerate(zip(first.tolist(), counts.tolist(), tokens.tolist(),
-                                                           runs.tolist(), parts.tolist())):
-        item0 = len(items)
-        groups.append((at, count, length, item0))
+    each = max(128, -(-int((runs * tokens).sum()) * num_kv_heads // int(num_cus)))
+    parts = np.minimum(np.maximum(tokens // each, 1), _lib.CDB_PREFIX_MAX_PARTS)
+    items = []
+    for at, count, length, run, part in zip(first.tolist(), counts.tolist(), tokens.tolist(), runs.tolist(),
+                                            parts.tolist()):
+        item0, rows = len(items), order[at:at + count]
         step = -(-length // part)
         step = -(-step // 32) * 32
         part = -(-length // step)
-        ends = [min(length, (k + 1) * step) for k in range(part)]
-        items.extend((n, q * PREFIX_QUERIES, k * step, ends[k]) for q in range(run) for k in range(part))
-        rows = order[at:at + count]
+        items.extend((at, count, int(rows[0]), length, q * PREFIX_QUERIES, k * step, min(length, (k + 1) * step), 0)
+                     for q in range(run) for k in range(part))
         info[rows, 0] = np.arange(count) * share
         info[rows, 1], info[rows, 2], info[rows, 3] = length, item0, part
-    def array(a, shape):
-        return np.asarray(a, dtype=np.int32).reshape(shape)
-    return PrefixDecodePlan(listed=array(order, -1), groups=array(groups, (-1, 4)), items=array(items, (-1, 4)),
-                            row_info=array(info, (-1, 4)))
+    return PrefixDecodePlan(listed=order.astype(np.int32), row_info=info.astype(np.int32),
+                            items=np.asarray(items, dtype=np.int32).reshape(-1, _lib.CDB_PREFIX_ITEM))
 
 
 def prefix_decode_workspace_bytes(plan: PrefixDecodePlan, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -403,12 +398,12 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     max_positions = kv8._check_rope(rope_style, rope_cos, rope_sin, dim)
     kv8._check_bias("q_bias", q_bias, num_heads, dim, dt)
     kv8._check_bias("k_bias", k_bias, heads_kv, dim, dt)
-    listed, groups, items, info = plan.listed, plan.groups, plan.items, plan.row_info
+    listed, items, info = plan.listed, plan.items, plan.row_info
     if not isinstance(info, torch.Tensor):
         raise TypeError("the plan must be on the device: plan.to(device)")
-    num_listed, num_groups, num_items = listed.shape[0], groups.shape[0], items.shape[0]
-    for name, t, n in (("plan.listed", listed, num_listed), ("plan.groups", groups, 4 * num_groups),
-                       ("plan.items", items, 4 * num_items), ("plan.row_info", info, 4 * num_rows)):
+    num_listed, num_items = listed.shape[0], items.shape[0]
+    for name, t, n in (("plan.listed", listed, num_listed), ("plan.items", items, _lib.CDB_PREFIX_ITEM * num_items),
+                       ("plan.row_info", info, 4 * num_rows)):
         kv8._check_ints(name, t, n)
     if not workspace.is_contiguous():
         raise ValueError("workspace must be contiguous")
@@ -417,12 +412,12 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     if kv8._row_stride("v_new", v_new, num_rows, heads_kv, dim) != kv_stride:
         raise ValueError("k_new and v_new must share a row stride")
     kv8._require_here(q, k_new, v_new, pool, cache_layer, block_table, table_row, seqlens, rope_cos, rope_sin, q_bias,
-                      k_bias, listed, groups, items, info, out, workspace)
+                      k_bias, listed, items, info, out, workspace)
     code = _lib.lib().cdb_prefix_decode_attention(
         q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), view.k_ptr, view.v_ptr, view.layer_stride, layers,
         pool_rows // block, _ptr(cache_layer), cache_layer0, block_table.data_ptr(), _ptr(table_row), table_rows, width,
         seqlens.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
-        listed.data_ptr(), num_listed, groups.data_ptr(), num_groups, items.data_ptr(), num_items, info.data_ptr(),
+        listed.data_ptr(), num_listed, items.data_ptr(), num_items, info.data_ptr(),
         out.data_ptr(), workspace.data_ptr(), workspace.nbytes, num_rows, num_heads, heads_kv, dim, block, scale,
         q_stride, kv_stride, dtype_code(dt), _stream())
     if code:
@@ -435,22 +430,22 @@ def prefix_decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.T
                             cache_layer: torch.Tensor | None, cache_layer0: int, block_table: torch.Tensor,
                             table_row: torch.Tensor | None, seqlens: torch.Tensor, rope_cos: torch.Tensor | None,
                             rope_sin: torch.Tensor | None, rope_style: int, q_bias: torch.Tensor | None,
-                            k_bias: torch.Tensor | None, listed: torch.Tensor, groups: torch.Tensor,
+                            k_bias: torch.Tensor | None, listed: torch.Tensor,
                             items: torch.Tensor, row_info: torch.Tensor, workspace: torch.Tensor, block_size: int,
                             scale: float) -> torch.Tensor:
     """Paged decode attention of rows that share prefixes, with fused RoPE + KV append over ``kv_pool``
-    [num_cache_layers, 2, pool_blocks * block_size, Hkv, D]; the plan's four tensors as in ``PrefixDecodePlan``. See
+    [num_cache_layers, 2, pool_blocks * block_size, Hkv, D]; the plan's three tensors as in ``PrefixDecodePlan``. See
     ``prefix_decode_attention_raw``."""
 
     out = q.new_empty(q.shape)
     return prefix_decode_attention_raw(q, k_new, v_new, KVPoolView(kv_pool, block_size), cache_layer, cache_layer0,
                                        block_table, table_row, seqlens, rope_cos, rope_sin, rope_style, q_bias, k_bias,
-                                       PrefixDecodePlan(listed, groups, items, row_info), out, workspace, scale)
+                                       PrefixDecodePlan(listed, items, row_info), out, workspace, scale)
 
 
 @prefix_decode_attention.register_fake
 def _(q, k_new, v_new, kv_pool, cache_layer, cache_layer0, block_table, table_row, seqlens, rope_cos, rope_sin,
-      rope_style, q_bias, k_bias, listed, groups, items, row_info, workspace, block_size, scale):
+      rope_style, q_bias, k_bias, listed, items, row_info, workspace, block_size, scale):
     return q.new_empty(q.shape)
 
 

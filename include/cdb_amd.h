@@ -492,7 +492,8 @@ int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs,
  * ------------------------------------------------------------------------ */
 
 enum {
-  CDB_PREFIX_QUERIES = 16,   /* queries (row, head) of an item */
+  CDB_PREFIX_QUERIES = 128,  /* queries (row, head) of an item */
+  CDB_PREFIX_ITEM = 8,       /* words of an item */
   CDB_PREFIX_MAX_PARTS = 64  /* parts that a prefix is cut into */
 };
 
@@ -507,26 +508,27 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
  * 0..seqlens[b]. Arguments as there, but for the plan; block_size is a power of two of at least 16, and the block table
  * has table_rows rows. Rotations are fp32 and rounded once, to the cache's type (that call rounds bf16 after each step).
  *
- * Group n's rows are listed[groups[4n]] and the groups[4n + 1] - 1 behind it; they hold the same first groups[4n + 2]
- * tokens, at the same slots of the same cache layer or as copies. These are read through the table row and cache layer
- * of the group's first row; the others only from there on. Queries of a group are counted row by row, the group's
- * num_heads / num_kv_heads heads of a KV head each; items [num_items][4] = (group, first query, a multiple of
- * CDB_PREFIX_QUERIES; first token; end token): the parts of a group's tokens for one run of queries follow each other,
- * and the runs of a group too. (-1, ..) is no item. row_info [num_rows][4] = (row's first query in its group, tokens of
- * its prefix, its group's first item, parts), zeros for a row without a group. A row is listed at most once.
+ * The rows of a group follow each other in listed; they hold the same first tokens, at the same slots of the same cache
+ * layer or as copies, which are read through the table row and cache layer of the group's first row; the others are
+ * read only from there on. Queries of a group are counted row by row, the group's num_heads / num_kv_heads heads of a
+ * KV head each. items [num_items][CDB_PREFIX_ITEM] (16-byte aligned) = (the group's first place in listed, its rows, its
+ * first row, tokens of its prefix, first query, a multiple of CDB_PREFIX_QUERIES, first token, end token, 0): the parts
+ * of a group's tokens for one run of queries follow each other, and the runs of a group too; 0 rows is no item. row_info
+ * [num_rows][4] = (row's first query in its group, tokens of its prefix, its group's first item, parts), zeros for a
+ * row without a group. A row is listed at most once.
  *
  * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
- * or the angles' range or inside its prefix, its cache layer or table row out of range, or its layer not its group's;
- * NaN too where a block outside the pool is met, for all rows of the group if it is in the prefix. Calls that may
- * overlap need a workspace each. */
+ * or the angles' range or inside its prefix, or its cache layer or table row out of range; NaN where its cache layer is
+ * not its group's first row's, and where a block outside the pool is met, for all rows of the group if it is in the
+ * prefix. Calls that may overlap need a workspace each. */
 int cdb_prefix_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_pool, void* v_pool,
                                 int64_t layer_stride, int32_t num_cache_layers, int64_t pool_blocks,
                                 const int32_t* cache_layer, int32_t cache_layer0, const int32_t* block_table,
                                 const int32_t* table_row, int32_t table_rows, int32_t table_width,
                                 const int32_t* seqlens, const float* rope_cos, const float* rope_sin,
                                 int32_t rope_style, int32_t max_positions, const void* q_bias, const void* k_bias,
-                                const int32_t* listed, int32_t num_listed, const int32_t* groups, int32_t num_groups,
-                                const int32_t* items, int32_t num_items, const int32_t* row_info, void* out,
+                                const int32_t* listed, int32_t num_listed, const int32_t* items, int32_t num_items,
+                                const int32_t* row_info, void* out,
                                 void* workspace, int64_t workspace_bytes, int32_t num_rows, int32_t num_heads,
                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
                                 int64_t q_stride, int64_t kv_stride, int32_t dtype, hipStream_t stream);

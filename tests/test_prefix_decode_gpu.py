@@ -147,10 +147,9 @@ def test_blocks_outside_the_pool_give_nan():
 
 def test_malformed_plans_stay_in_bounds():
     s = ph.make([0, 0, 1], [200, 90], [4, 5, 6], dead=0.0)
-    names = ("listed", "groups", "items", "row_info")
-    for name in names:
+    for name in ("listed", "items", "row_info"):
         for value in (-1, 1 << 20, -(1 << 31), (1 << 31) - 1):
-            for column in range(1 if name == "listed" else 4):
+            for column in range({"listed": 1, "items": 8, "row_info": 4}[name]):
                 t = getattr(s.plan, name).clone()
                 if name == "listed":
                     t[:] = value
@@ -163,7 +162,7 @@ def test_malformed_plans_stay_in_bounds():
 def test_padded_items_are_none():
     s = ph.make([0, 0, 1], [200, 90], [4, 5, 6], dead=0.0)
     want = ph.call(s).clone()
-    items = torch.cat([s.plan.items, torch.full((5, 4), -1, dtype=torch.int32, device="cuda")])
+    items = torch.cat([s.plan.items, torch.full((5, 8), -1, dtype=torch.int32, device="cuda")])
     plan = replace(s.plan, items=items)
     ws = torch.empty(ops.prefix_decode_workspace_bytes(plan, 8, 4, 64, 10), dtype=torch.uint8, device="cuda")
     assert torch.equal(ph.call(s, plan=plan, workspace=ws), want)
@@ -237,7 +236,7 @@ def test_the_registered_operator():
     want, pool = ph.call(s).clone(), s.pool.clone()
     got = torch.ops.cdb.prefix_decode_attention(
         s.q, s.k, s.v, pool, s.layer, s.layer0, s.table, None, s.seq, s.cos, s.sin, s.rope, s.q_bias, s.k_bias,
-        s.plan.listed, s.plan.groups, s.plan.items, s.plan.row_info, s.workspace, s.block, s.scale)
+        s.plan.listed, s.plan.items, s.plan.row_info, s.workspace, s.block, s.scale)
     assert torch.equal(got, want) and torch.equal(pool, s.pool)
 
 

@@ -23,16 +23,16 @@ def cover(plan, group, lengths, heads, kv):
             assert not plan.row_info[b].any()
             continue
         assert length == lengths[n] and 1 <= parts <= _lib.CDB_PREFIX_MAX_PARTS
-        name = plan.items[item0, 0]
-        first, count, tokens, at = plan.groups[name]
-        assert tokens == length and at == item0
+        first, count, leader, tokens = plan.items[item0, :4]
+        assert tokens == length and leader == plan.listed[first] and not plan.items[:, 7].any()
         assert b in plan.listed[first:first + count] and plan.listed[first + q0 // share] == b and q0 % share == 0
         for q in range(q0, q0 + share):
             run = item0 + q // ops.PREFIX_QUERIES * parts
             of = plan.items[run:run + parts]
-            assert (of[:, 0] == name).all() and (of[:, 1] == q // ops.PREFIX_QUERIES * ops.PREFIX_QUERIES).all()
-            assert of[0, 2] == 0 and of[-1, 3] == length and (of[1:, 2] == of[:-1, 3]).all()
-            assert (of[:, 2] < of[:, 3]).all()
+            assert (of[:, :4] == plan.items[item0, :4]).all()
+            assert (of[:, 4] == q // ops.PREFIX_QUERIES * ops.PREFIX_QUERIES).all()
+            assert of[0, 5] == 0 and of[-1, 6] == length and (of[1:, 5] == of[:-1, 6]).all()
+            assert (of[:, 5] < of[:, 6]).all()
 
 
 @pytest.mark.parametrize("heads,kv", [(1, 1), (16, 16), (32, 8), (28, 4), (7, 1), (64, 1)])
@@ -53,7 +53,7 @@ def test_plans_of_nothing():
     plan = ops.prefix_decode_plan([-1, -1], [], num_heads=4, num_kv_heads=4)
     assert plan.num_rows == 2 and plan.num_items == 0 and not plan.row_info.any()
     device = plan.to("cpu")
-    assert device.row_info.shape == (2, 4) and device.items.shape == (0, 4) and device.row_info.dtype is torch.int32
+    assert device.row_info.shape == (2, 4) and device.items.shape == (0, 8) and device.row_info.dtype is torch.int32
 
 
 @pytest.mark.parametrize("group,lengths,heads,kv", [([0, 2], [5, 5], 4, 4), ([0], [-1], 4, 4), ([0], [1 << 31], 4, 4),
@@ -68,7 +68,7 @@ def code(**over):
     a = dict(q=fake, k_new=fake, v_new=fake, k_pool=fake, v_pool=fake, layer_stride=64 * 16 * 256, layers=2,
              pool_blocks=64, cache_layer=None, cache_layer0=0, block_table=fake, table_row=None, table_rows=4,
              table_width=8, seqlens=fake, cos=fake, sin=fake, style=1, max_positions=100, q_bias=None, k_bias=None,
-             listed=fake, num_listed=4, groups=fake, num_groups=1, items=fake, num_items=1, row_info=fake, out=fake,
+             listed=fake, num_listed=4, items=fake, num_items=1, row_info=fake, out=fake,
              workspace=fake, nbytes=1 << 24, rows=4, heads=4, kv=4, dim=64, block=16, scale=0.1, q_stride=0,
              kv_stride=0, dtype=_lib.CDB_DTYPE_BF16, stream=None)
     a.update(over)
@@ -86,7 +86,7 @@ odd = ctypes.c_void_p(0x1004)
     (dict(table_rows=3), _lib.CDB_ERR_SHAPE), (dict(table_width=1 << 27), _lib.CDB_ERR_SHAPE),
     (dict(layers=0), _lib.CDB_ERR_SHAPE), (dict(pool_blocks=0), _lib.CDB_ERR_SHAPE),
     (dict(pool_blocks=1 << 31), _lib.CDB_ERR_SHAPE), (dict(num_listed=-1), _lib.CDB_ERR_SHAPE),
-    (dict(num_groups=-1), _lib.CDB_ERR_SHAPE), (dict(num_items=-1), _lib.CDB_ERR_SHAPE),
+    (dict(num_items=-1), _lib.CDB_ERR_SHAPE), (dict(items=odd), _lib.CDB_ERR_SHAPE),
     (dict(block=8), _lib.CDB_ERR_SHAPE), (dict(block=48), _lib.CDB_ERR_SHAPE),
     (dict(layer_stride=64 * 16 * 256 - 8), _lib.CDB_ERR_SHAPE), (dict(scale=0.0), _lib.CDB_ERR_SHAPE),
     (dict(scale=float("inf")), _lib.CDB_ERR_SHAPE), (dict(scale=float("nan")), _lib.CDB_ERR_SHAPE),
@@ -96,7 +96,7 @@ odd = ctypes.c_void_p(0x1004)
     (dict(kv=1 << 22, heads=1 << 22, layers=1), _lib.CDB_ERR_SHAPE),
     (dict(q=None), _lib.CDB_ERR_NULL), (dict(k_pool=None), _lib.CDB_ERR_NULL), (dict(out=None), _lib.CDB_ERR_NULL),
     (dict(row_info=None), _lib.CDB_ERR_NULL), (dict(listed=None), _lib.CDB_ERR_NULL),
-    (dict(groups=None), _lib.CDB_ERR_NULL), (dict(items=None), _lib.CDB_ERR_NULL),
+    (dict(items=None), _lib.CDB_ERR_NULL),
     (dict(cos=None), _lib.CDB_ERR_NULL), (dict(workspace=None), _lib.CDB_ERR_NULL),
     (dict(nbytes=100), _lib.CDB_ERR_CAPACITY), (dict(nbytes=-1), _lib.CDB_ERR_CAPACITY),
     (dict(rows=0), _lib.CDB_OK),
@@ -134,7 +134,7 @@ def scene():
     (lambda s: setattr(s, "plan", s.host_plan), TypeError),
     (lambda s: setattr(s, "plan", replace(s.plan, items=s.plan.items.long())), TypeError),
     (lambda s: setattr(s, "plan", replace(s.plan, row_info=s.plan.row_info[:2])), ValueError),
-    (lambda s: setattr(s, "plan", replace(s.plan, groups=s.plan.groups[:, :3])), ValueError),
+    (lambda s: setattr(s, "plan", replace(s.plan, items=s.plan.items[:, :3])), ValueError),
     (lambda s: setattr(s, "workspace", s.workspace[::2]), ValueError),
     (lambda s: None, RuntimeError),  # tensors of the CPU
 ])
@@ -157,5 +157,5 @@ def test_operator_is_registered():
         q, k = torch.empty(3, 8, 64, device="cuda"), torch.empty(3, 4, 64, device="cuda")
         out = torch.ops.cdb.prefix_decode_attention(q, k, k, torch.empty(1, 2, 64, 4, 64, device="cuda"), None, 0,
                                                     ints(3, 4), None, ints(3), None, None, 0, None, None, ints(3),
-                                                    ints(1, 4), ints(1, 4), ints(3, 4), ints(9), 16, 0.125)
+                                                    ints(1, 8), ints(3, 4), ints(9), 16, 0.125)
         assert out.shape == q.shape
