@@ -28,7 +28,7 @@ CDB_DECODE_SCRATCH_BYTES = 16 << 20  # include/cdb_amd.h
 CDB_DECODE_STAGE_PLAN = 1
 CDB_DECODE_STAGE_ATTEND = 2
 CDB_LAYOUT_MAX_SEQS = 4000
-CDB_PREFIX_QUERIES, CDB_PREFIX_ITEM, CDB_PREFIX_MAX_PARTS = 128, 8, 64
+CDB_PREFIX_QUERIES, CDB_PREFIX_FEW, CDB_PREFIX_ITEM, CDB_PREFIX_MAX_PARTS = 128, 16, 8, 64
 CDB_SAMPLE_MAX_VOCAB = 1 << 20
 CDB_LAYOUT_TOKENS_FULL, CDB_LAYOUT_TILES_FULL, CDB_LAYOUT_NO_BLOCKS, CDB_LAYOUT_BAD_REQUEST = 1, 2, 4, 8
 
@@ -229,7 +229,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             c_int64, c_int32, c_int64, _P, c_int32,  # layer_stride, layers, pool_blocks, cache_layer, cache_layer0
             _P, _P, c_int32, c_int32, _P,  # block_table, table_row, table_rows, table_width, seqlens
             _P, _P, c_int32, c_int32, _P, _P,  # rope_cos, rope_sin, rope_style, max_positions, q_bias, k_bias
-            _P, c_int32, _P, c_int32, _P,  # listed, n, items, n, row_info
+            _P, c_int32, _P, c_int32, c_int32, _P,  # listed, n, items, n, few, row_info
             _P, _P, c_int64,  # out, workspace, workspace_bytes
             c_int32, c_int32, c_int32, c_int32, c_int32,  # rows, H, Hkv, D, block_size
             c_float, c_int64, c_int64, c_int32, _P,  # scale, q_stride, kv_stride, dtype, stream

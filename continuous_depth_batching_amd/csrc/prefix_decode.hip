@@ -23,15 +23,17 @@
 
 namespace cdb {
 
-constexpr int kWaves = 8;        // of a prefix's workgroup
 constexpr int kRowWaves = 2;     // of a row's
 constexpr int kChunk = 1024;     // own tokens of a workgroup
 constexpr int kMaxChunks = 64;   // of a row; longer contexts take longer chunks
 constexpr int kMaxParts = CDB_PREFIX_MAX_PARTS;  // of a prefix
 constexpr int kColumns = 16;     // queries of a product
-constexpr int kQueries = CDB_PREFIX_QUERIES;  // of an item, 32 a wave
+constexpr int kQueries = CDB_PREFIX_QUERIES;  // of an item
 constexpr int kItem = CDB_PREFIX_ITEM;        // words of an item
-static_assert(kQueries % 32 == 0 && kQueries <= 32 * kWaves, "queries of an item's waves");
+static_assert(CDB_PREFIX_FEW == kColumns && kQueries == 128, "queries of an item's waves");
+// A prefix's workgroup: four waves of the same 16 queries, each with every fourth step; or four of 32 queries each on
+// two parts of the tokens.
+template <bool kFew> constexpr int kWaves = kFew ? 4 : 8;
 static_assert(kMaxParts <= 64, "a lane weighs a part");
 
 struct PrefixParams {
@@ -43,7 +45,7 @@ struct PrefixParams {
   const float *cos, *sin;
   const void *q_bias, *k_bias;
   const int32_t *listed, *items, *row_info;
-  int32_t num_listed, num_items;
+  int32_t num_listed, num_items, num_few;
   void* out;
   float* shared;   // [items][KV heads][kQueries][D + 2]: O, the maximum and the sum of a prefix's part
   float* partials; // [rows][heads][max_chunks][D + 2]: the same of a chunk of own tokens
@@ -108,26 +110,27 @@ template <int D> struct StepRegs<bf16_t, D> {
       hi[i] = pack_bf16x2(x[2 * i], x[2 * i + 1]);
       lo[i] = pack_bf16x2(x[2 * i] - __uint_as_float(hi[i] << 16), x[2 * i + 1] - __uint_as_float(hi[i] & 0xffff0000u));
     }
-    *reinterpret_cast<u32x4_t*>(to) = hi;
-    *reinterpret_cast<u32x4_t*>(to + kRuns * 64 * 4) = lo;
+    *reinterpret_cast<u32x4_t*>(to) = lo;
+    *reinterpret_cast<u32x4_t*>(to + kRuns * 64 * 4) = hi;
   }
-  template <int NC> CDB_DEVICE void scores(const uint32_t* query, const int* slot, f32x4_t (*s)[kTiles]) const {
+  typedef bf16x8_t Operand;
+  static constexpr int kOperands = 2 * kRuns;  // of a query: the second parts, then the first ones
+  // query(n, i): operand i of column tile n.
+  template <int NC, typename F> CDB_DEVICE void scores(F query, f32x4_t (*s)[kTiles]) const {
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int a = 0; a < kTiles; ++a) s[n][a] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int p = 1; p >= 0; --p)
+    for (int i = 0; i < kOperands; ++i)
 #pragma unroll
-      for (int j = 0; j < kRuns; ++j)
+      for (int n = 0; n < NC; ++n) {
+        const Operand q = query(n, i);
 #pragma unroll
-        for (int n = 0; n < NC; ++n) {
-          const bf16x8_t q = *reinterpret_cast<const bf16x8_t*>(query + slot[n] * 4 + (p * kRuns + j) * 64 * 4);
-#pragma unroll
-          for (int a = 0; a < kTiles; ++a)
-            s[n][a] =
-                __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[a][j]), q, s[n][a], 0, 0, 0);
-        }
+        for (int a = 0; a < kTiles; ++a)
+          s[n][a] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[a][i % kRuns]), q, s[n][a],
+                                                            0, 0, 0);
+      }
   }
   template <int NC> CDB_DEVICE void accumulate(const f32x4_t (*p)[kTiles], f32x4_t (*acc)[D / 16]) const {
     union { uint32_t w[4]; bf16x8_t v; } hi[NC], lo[NC];
@@ -149,6 +152,9 @@ template <int D> struct StepRegs<bf16_t, D> {
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, lo[n].v, acc[n][m], 0, 0, 0);
+      }
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
         acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(x.v, hi[n].v, acc[n][m], 0, 0, 0);
       }
     }
@@ -176,14 +182,16 @@ template <int D> struct StepRegs<float, D> {
     *reinterpret_cast<f32x4_t*>(to) = (f32x4_t){x[0], x[1], x[2], x[3]};
     *reinterpret_cast<f32x4_t*>(to + 16 * 4) = (f32x4_t){x[4], x[5], x[6], x[7]};
   }
-  template <int NC> CDB_DEVICE void scores(const uint32_t* query, const int* slot, f32x4_t (*s)[kTiles]) const {
+  typedef f32x4_t Operand;
+  static constexpr int kOperands = kRuns;
+  template <int NC, typename F> CDB_DEVICE void scores(F query, f32x4_t (*s)[kTiles]) const {
 #pragma unroll
     for (int n = 0; n < NC; ++n) s[n][0] = (f32x4_t){0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int j = 0; j < kRuns; ++j)
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        const f32x4_t q = *reinterpret_cast<const f32x4_t*>(query + slot[n] * 4 + j * 64 * 4);
+        const Operand q = query(n, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) s[n][0] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[0][j][i], q[i], s[n][0], 0, 0, 0);
       }
@@ -196,6 +204,42 @@ template <int D> struct StepRegs<float, D> {
 #pragma unroll
         for (int n = 0; n < NC; ++n)
           acc[n][m] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[i][m], p[n][0][i], acc[n][m], 0, 0, 0);
+  }
+};
+
+// The staged walk: a workgroup's waves that take the same tokens share them in LDS. Two parts of the tokens are walked
+// side by side, by four waves each; a part's step lies as [keys, values][token][D], rows 16 bytes apart, which spreads
+// the operands' reads over all banks. While a step is multiplied the next one's loads are on the way.
+template <typename T, int D> struct Stage {
+  static constexpr int kTiles = StepRegs<T, D>::kTiles, kStep = 16 * kTiles;
+  static constexpr int kPieces = D * (int)sizeof(T) / 16, kUnits = (kPieces + 15) / 16;  // 16 bytes of a row; a thread's
+  static constexpr int kRow = D * (int)sizeof(T) + 16, kPlane = kStep * kRow, kPart = 2 * kPlane, kBytes = 2 * kPart;
+  u32x4_t w[2][kTiles][kUnits];
+
+  // `i` of the part's 256 threads: piece i % 16 (and every 16th from there) of row i / 16 of each tile.
+  CDB_DEVICE void load(const Tokens& at, const int64_t* tile, const int* b0, const int* b1, int i) {
+#pragma unroll
+    for (int a = 0; a < kTiles; ++a) {
+      const uint32_t row = (uint32_t)min(max(i >> 4, b0[a]), b1[a] - 1) * (uint32_t)at.row_bytes;
+#pragma unroll
+      for (int u = 0; u < kUnits; ++u) {
+        const uint32_t piece = min((i & 15) + 16 * u, kPieces - 1) * 16;
+        w[0][a][u] = *reinterpret_cast<const u32x4_t*>(at.k + tile[a] + (row + piece));
+        w[1][a][u] = *reinterpret_cast<const u32x4_t*>(at.v + tile[a] + (row + piece));
+      }
+    }
+  }
+  CDB_DEVICE void store(char* part, int i) const {
+#pragma unroll
+    for (int p = 0; p < 2; ++p)
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+        for (int u = 0; u < kUnits; ++u) {
+          const int piece = (i & 15) + 16 * u;
+          if (kPieces % 16 == 0 || piece < kPieces)
+            *reinterpret_cast<u32x4_t*>(part + p * kPlane + (16 * a + (i >> 4)) * kRow + piece * 16) = w[p][a][u];
+        }
   }
 };
 
@@ -325,6 +369,10 @@ template <typename T, int D, int NC> struct Walk {
       slot[n] = (c >> 4) * (StepRegs<T, D>::kQueryWords / 4) + (lane & 48) + (c & 15);
     }
   }
+  // Operand i of column tile n as it lies in LDS.
+  CDB_DEVICE static typename StepRegs<T, D>::Operand operand(const uint32_t* query, const int* slot, int n, int i) {
+    return *reinterpret_cast<const typename StepRegs<T, D>::Operand*>(query + slot[n] * 4 + i * 64 * 4);
+  }
   CDB_DEVICE void tokens(const Tokens& at, const uint32_t* query, int cols) {
     int slot[NC];
     slots(cols, slot);
@@ -338,7 +386,7 @@ template <typename T, int D, int NC> struct Walk {
         // values one for the next keys too.
         const int ahead = step + stride < steps ? step + stride : step;
         f32x4_t s[NC][kTiles];
-        x.template scores<NC>(query, slot, s);
+        x.template scores<NC>([&](int n, int i) __attribute__((always_inline)) { return operand(query, slot, n, i); }, s);
         load_keys(at, ahead, r, g);
         int from[kTiles], to[kTiles];
 #pragma unroll
@@ -352,6 +400,81 @@ template <typename T, int D, int NC> struct Walk {
         load_values(at, ahead, r, g);
         __builtin_amdgcn_sched_barrier(0);
       }
+    }
+  }
+  // The staged walk over [lo, hi) for all of a workgroup's threads; `lds` holds the queries, which every wave takes from
+  // there first. A wave without queries only loads.
+  CDB_DEVICE void shared_tokens(const Tokens& at, uint32_t* lds, int run, int part, int cols, int from, int to) {
+    typedef Stage<T, D> S;
+    typedef typename StepRegs<T, D>::Operand Operand;
+    constexpr int kOps = StepRegs<T, D>::kOperands;
+    const int r = lane & 15, g = lane >> 4, i = threadIdx.x & 255;
+    lo = from;
+    hi = to;
+    const int tiles = ((hi + 15) >> 4) - (lo >> 4), steps = (tiles + kTiles - 1) / kTiles, turns = (steps + 1) / 2;
+    window = -64;
+    // Two turns' loads are on the way while one is multiplied. The loads at the end repeat the last step: a branch
+    // around them would make the waits for the turn before ones for them too.
+    S stage[2];
+    auto load = [&](S& to_stage, int turn) __attribute__((always_inline)) {
+      const int step = min(2 * turn + part, steps - 1), first_tile = kTiles * step;
+      if (first_tile >= window + 64) {
+        window = first_tile & ~63;
+        count = min(64, tiles - window);
+        bool lost = false;
+        where = 0;
+        if (lane < count) where = at.at(((lo >> 4) + window + lane) * 16, lost);
+        missing = missing || __ballot(lost) != 0;
+      }
+      int64_t tile[kTiles];
+      int b0[kTiles], b1[kTiles];
+#pragma unroll
+      for (int a = 0; a < kTiles; ++a) tile[a] = offset(bounds(step - window / kTiles, a, b0[a], b1[a]));
+      to_stage.load(at, tile, b0, b1, i);
+    };
+    load(stage[0], 0);
+    load(stage[1], 1);
+    Operand q[NC][kOps];
+    int slot[NC];
+    slots(max(cols, 1), slot);
+#pragma unroll
+    for (int n = 0; n < NC; ++n)
+#pragma unroll
+      for (int o = 0; o < kOps; ++o) q[n][o] = operand(lds + NC * run * StepRegs<T, D>::kQueryWords, slot, n, o);
+    __syncthreads();  // the tokens take the queries' place
+    char* ring = reinterpret_cast<char*>(lds) + part * S::kPart;
+    stage[0].store(ring, i);
+    lds_barrier();
+    auto turn_of = [&](int turn, S& free_stage, const S& next_stage, const char* now, char* next)
+                       __attribute__((always_inline)) {
+      const int step = 2 * turn + part;
+      load(free_stage, turn + 2);
+      if (cols > 0 && step < steps) {
+#pragma unroll
+        for (int a = 0; a < kTiles; ++a) x.load_key(a, now + a * 16 * S::kRow, r * S::kRow, g);
+        f32x4_t s[NC][kTiles];
+        x.template scores<NC>([&](int n, int o) __attribute__((always_inline)) { return q[n][o]; }, s);
+#pragma unroll
+        for (int a = 0; a < kTiles; ++a)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            x.load_value(4 * a + e, now + S::kPlane + a * 16 * S::kRow, (4 * g + e) * S::kRow, r);
+        int first_in[kTiles], end_in[kTiles];
+#pragma unroll
+        for (int a = 0; a < kTiles; ++a) {
+          const int t = ((lo >> 4) + kTiles * step + a) * 16;
+          first_in[a] = max(lo - t, 0);
+          end_in[a] = min(hi - t, 16);
+        }
+        weigh(s, first_in, end_in, g);
+        x.template accumulate<NC>(s, acc);
+      }
+      next_stage.store(next, i);
+      lds_barrier();
+    };
+    for (int turn = 0; turn < turns; turn += 2) {
+      turn_of(turn, stage[0], stage[1], ring, ring + S::kBytes);
+      if (turn + 1 < turns) turn_of(turn + 1, stage[1], stage[0], ring + S::kBytes, ring);
     }
   }
   // O, the maximum and the sum of each column: [column][stride].
@@ -449,24 +572,27 @@ template <typename T, int D> CDB_DEVICE Tokens tokens_of(const PrefixParams& P, 
   return x;
 }
 
-// Words of LDS: the queries, and in their place later what half of the waves leave to the other half.
-template <typename T, int D> struct AttendLds {
-  static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kQueries / 16), kJoin = kWaves / 2 * 32 * (D + 4);
-  static constexpr int kWords = kQ > kJoin ? kQ : kJoin;
+// Words of LDS: the queries, and in their place later the staged tokens, and what half of the waves leave to the others.
+template <typename T, int D, bool kFew> struct AttendLds {
+  static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kFew ? 1 : kQueries / 16);
+  static constexpr int kJoin = kWaves<kFew> / 2 * (kFew ? 16 : 32) * (D + 4), kStages = kFew ? 0 : Stage<T, D>::kBytes / 2;
+  static constexpr int kMost = kQ > kJoin ? kQ : kJoin, kWords = kMost > kStages ? kMost : kStages;
 };
 
-template <typename T, int D, int STYLE>
-__global__ void __launch_bounds__(64 * kWaves, 2) prefix_attend_kernel(PrefixParams P) {
-  __shared__ __align__(16) uint32_t lds[AttendLds<T, D>::kWords];
+template <typename T, int D, int STYLE, bool kFew>
+__global__ void __launch_bounds__(64 * kWaves<kFew>, (kFew ? 3 : 2)) prefix_attend_kernel(PrefixParams P) {
+  constexpr int kThreads = 64 * kWaves<kFew>, NC = kFew ? 1 : 2;
+  __shared__ __align__(16) uint32_t lds[AttendLds<T, D, kFew>::kWords];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int item = blockIdx.x / P.num_kv_heads, kvh = blockIdx.x - item * P.num_kv_heads;
+  const int at_item = blockIdx.x / P.num_kv_heads, kvh = blockIdx.x - at_item * P.num_kv_heads;
+  const int item = at_item + (kFew ? 0 : P.num_few);
   const int4 head = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[0];
   const int4 tail = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[1];
   const int first = head.x, count = head.y, leader = head.z, length = head.w, q0 = tail.x, lo = tail.y, hi = tail.z;
   if (count <= 0 || count > P.num_listed || first < 0 || first > P.num_listed - count) return;  // no item
   const int64_t queries = (int64_t)count * P.group;
   if (q0 < 0 || q0 >= queries) return;
-  const int cols = (int)min((int64_t)kQueries, queries - q0);
+  const int cols = (int)min((int64_t)(kFew ? kColumns : kQueries), queries - q0);
   int layer = -1, trow = -1;
   if (leader >= 0 && leader < P.num_rows) {
     layer = P.cache_layer0 + (P.cache_layer == nullptr ? 0 : P.cache_layer[leader]);
@@ -474,17 +600,16 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attend_kernel(PrefixPar
   }
   const bool bad = layer < 0 || layer >= P.num_layers || trow < 0 || trow >= P.table_rows || lo < 0 || hi > length ||
                    (int64_t)length > ((int64_t)P.table_width << P.bs_log2);
-  // 32 queries a wave; where that leaves waves over, several take the same queries and every so-manieth step.
-  const int runs = cols <= 32 ? 1 : cols <= 64 ? 2 : 4, run = wave & (runs - 1), part = wave / runs, parts = kWaves / runs;
-  const int mine = min(32, cols - 32 * run);  // may be none
+  const int runs = kFew ? 1 : 4, run = wave & (runs - 1), part = wave / runs, parts = kWaves<kFew> / runs;
+  const int mine = min(16 * NC, cols - 16 * NC * run);  // may be none
   const Tokens at_prefix = tokens_of<T, D>(P, bad ? 0 : layer, bad ? 0 : trow, kvh);
-  Walk<T, D, 2> walk;
+  Walk<T, D, NC> walk;
   walk.start(lane);
   if (bad) walk.missing = true;
-  walk.open(at_prefix, bad || mine <= 0 ? 0 : lo, bad || mine <= 0 ? 0 : hi, part, parts);
+  if constexpr (kFew) walk.open(at_prefix, bad ? 0 : lo, bad ? 0 : hi, part, parts);
   constexpr int kPieces = D / 16;
 #pragma unroll 2
-  for (int i = threadIdx.x; i < cols * kPieces; i += 64 * kWaves) {
+  for (int i = threadIdx.x; i < cols * kPieces; i += kThreads) {
     const int c = i / kPieces, at = q0 + c;
     const int b = P.listed[first + at / P.group];
     int p = b >= 0 && b < P.num_rows ? P.seqlens[b] : -1;
@@ -494,17 +619,22 @@ __global__ void __launch_bounds__(64 * kWaves, 2) prefix_attend_kernel(PrefixPar
     turn_query<T, D, STYLE>(P, lds, c, i - c * kPieces, b, kvh * P.group + at % P.group, p, stranger ? NAN : 0.f);
   }
   __syncthreads();
-  if (mine > 0) walk.tokens(at_prefix, lds + 2 * run * StepRegs<T, D>::kQueryWords, mine);
+  if constexpr (kFew) {
+    walk.tokens(at_prefix, lds, mine);
+  } else if (!bad && lo < hi) {
+    walk.shared_tokens(at_prefix, lds, run, part, mine, lo, hi);
+  }
   float* to = P.shared + ((int64_t)item * P.num_kv_heads + kvh) * kQueries * (D + 2);
   // Waves with the same queries are joined in halves.
-  float* join = reinterpret_cast<float*>(lds) + run * 32 * (D + 4);
+  float* join = reinterpret_cast<float*>(lds) + run * 16 * NC * (D + 4);
+  constexpr int kSlot = 16 * NC * (D + 4);
   for (int half = parts >> 1; half > 0; half >>= 1) {
     __syncthreads();
-    if (mine > 0 && part >= half && part < 2 * half) walk.leave(join + (part - half) * runs * 32 * (D + 4), mine, D + 4);
+    if (mine > 0 && part >= half && part < 2 * half) walk.leave(join + (part - half) * runs * kSlot, mine, D + 4);
     __syncthreads();
-    if (mine > 0 && part < half) walk.join(join + part * runs * 32 * (D + 4), mine, D + 4);
+    if (mine > 0 && part < half) walk.join(join + part * runs * kSlot, mine, D + 4);
   }
-  if (mine > 0 && part == 0) walk.leave(to + 32 * run * (D + 2), mine, D + 2);
+  if (mine > 0 && part == 0) walk.leave(to + 16 * NC * run * (D + 2), mine, D + 2);
 }
 
 template <typename T, int D, int STYLE>
@@ -522,12 +652,14 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
   const int p = row.p;
   T* out = static_cast<T*>(P.out) + ((int64_t)b * P.num_heads + (int64_t)kvh * P.group) * D;
   // The row's queries within its group, and the prefix's parts.
-  const int n0 = P.row_info[4 * b], item0 = P.row_info[4 * b + 2], parts = P.row_info[4 * b + 3];
+  const int n0 = P.row_info[4 * b], item0 = P.row_info[4 * b + 2], given = P.row_info[4 * b + 3];
+  row.bad = row.bad || given < -kMaxParts || given > kMaxParts;
+  const int parts = row.bad ? 0 : given < 0 ? -given : given, each = given < 0 ? kColumns : kQueries;  // queries of an item
   if (parts == 0) {
     row.bad = row.bad || row.own != 0;
   } else {
-    const int64_t last = item0 + (((int64_t)n0 + P.group - 1) / kQueries + 1) * parts;  // behind the row's last item
-    row.bad = row.bad || parts < 0 || parts > kMaxParts || n0 < 0 || item0 < 0 || last > P.num_items;
+    const int64_t last = item0 + (((int64_t)n0 + P.group - 1) / each + 1) * parts;  // behind the row's last item
+    row.bad = row.bad || n0 < 0 || item0 < 0 || last > P.num_items;
   }
   if (p < 0 || row.bad) {
     if (chunk == 0)
@@ -593,7 +725,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
       f32x4_t s[1][StepRegs<T, D>::kTiles];
       int slot[1];
       walk.slots(cols, slot);
-      walk.x.template scores<1>(query, slot, s);
+      walk.x.template scores<1>(
+          [&](int n, int i) __attribute__((always_inline)) { return walk.operand(query, slot, n, i); }, s);
       const int from[2] = {0, 0}, to[2] = {1, 0};
       walk.weigh(s, from, to, g);
       walk.x.template accumulate<1>(s, walk.acc);
@@ -604,8 +737,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
     const int64_t shared_stride = (int64_t)P.num_kv_heads * kQueries * (D + 2);
     auto shared_of = [&](int c) __attribute__((always_inline)) -> const float* {
       const int n = n0 + slice + c;
-      return P.shared + (((int64_t)item0 + n / kQueries * parts) * P.num_kv_heads + kvh) * kQueries * (D + 2) +
-             n % kQueries * (D + 2);
+      return P.shared + (((int64_t)item0 + n / each * parts) * P.num_kv_heads + kvh) * kQueries * (D + 2) +
+             n % each * (D + 2);
     };
     if (chunks > 1) {
       for (int i = tid; i < cols * D; i += 64 * kRowWaves) {
@@ -726,9 +859,14 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
 }
 
 template <typename T, int D, int STYLE> static int prefix_style(const PrefixParams& P, hipStream_t stream) {
-  const dim3 wg(64 * kWaves);
-  if (P.num_items > 0) {
-    prefix_attend_kernel<T, D, STYLE><<<dim3((unsigned)(P.num_items * P.num_kv_heads)), wg, 0, stream>>>(P);
+  if (P.num_few > 0) {
+    prefix_attend_kernel<T, D, STYLE, true>
+        <<<dim3((unsigned)(P.num_few * P.num_kv_heads)), dim3(64 * kWaves<true>), 0, stream>>>(P);
+    if (hipGetLastError() != hipSuccess) return CDB_ERR_HIP;
+  }
+  if (P.num_items > P.num_few) {
+    prefix_attend_kernel<T, D, STYLE, false>
+        <<<dim3((unsigned)((P.num_items - P.num_few) * P.num_kv_heads)), dim3(64 * kWaves<false>), 0, stream>>>(P);
     if (hipGetLastError() != hipSuccess) return CDB_ERR_HIP;
   }
   const int64_t most = ((int64_t)P.table_width << P.bs_log2) / kChunk + 1;
@@ -787,7 +925,7 @@ extern "C" int cdb_prefix_decode_attention(
     const int32_t* block_table, const int32_t* table_row, int32_t table_rows, int32_t table_width,
     const int32_t* seqlens, const float* rope_cos, const float* rope_sin, int32_t rope_style, int32_t max_positions,
     const void* q_bias, const void* k_bias, const int32_t* listed, int32_t num_listed, const int32_t* items,
-    int32_t num_items, const int32_t* row_info, void* out, void* workspace,
+    int32_t num_items, int32_t num_few, const int32_t* row_info, void* out, void* workspace,
     int64_t workspace_bytes, int32_t num_rows, int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
     int32_t block_size, float scale, int64_t q_stride, int64_t kv_stride, int32_t dtype, hipStream_t stream) {
   using namespace cdb;
@@ -796,7 +934,7 @@ extern "C" int cdb_prefix_decode_attention(
   if (head_dim != 64 && head_dim != 96 && head_dim != 128) return CDB_ERR_UNSUPPORTED;
   if (num_rows < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 || table_rows <= 0 ||
       table_width <= 0 || num_cache_layers <= 0 || pool_blocks <= 0 || pool_blocks > 0x7fffffffll || num_listed < 0 ||
-      num_items < 0)
+      num_items < 0 || num_few < 0 || num_few > num_items)
     return CDB_ERR_SHAPE;
   if (block_size < 16 || (block_size & (block_size - 1)) != 0) return CDB_ERR_SHAPE;
   if (num_rows == 0) return CDB_OK;
@@ -834,7 +972,7 @@ extern "C" int cdb_prefix_decode_attention(
   P.bs_log2 = __builtin_ctz(block_size);
   P.q_bias = q_bias; P.k_bias = k_bias;
   P.listed = listed; P.items = items; P.row_info = row_info;
-  P.num_listed = num_listed; P.num_items = num_items;
+  P.num_listed = num_listed; P.num_items = num_items; P.num_few = num_few;
   P.out = out; P.shared = static_cast<float*>(workspace);
   P.partials = P.shared + shared_bytes(num_items, num_kv_heads, head_dim) / 4;
   P.max_chunks = (int32_t)chunks;

@@ -113,6 +113,14 @@ CDB_DEVICE uint64_t wave_most(uint64_t v) {
   v = max(v, dpp_u64<0x143, 0xc>(v));
   return read_lane(v, 63);
 }
+// The largest of the wave's values.
+CDB_DEVICE float wave_largest(float v) {
+  v = row16_max(v);
+  const float a = fmaxf(v, __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 16)));
+  const float b = fmaxf(__uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 32)),
+                        __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), 48)));
+  return __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(fmaxf(a, b))));
+}
 // Sum over 8 consecutive lanes.
 CDB_DEVICE uint64_t eight_total(uint64_t v) {
   v += dpp_u64<0xb1>(v);   // quad_perm 1 0 3 2
@@ -171,28 +179,42 @@ template <typename T> struct SampleRow {
   typedef Vec<T, kRun> Run;
   const T* base;  // of run 0, aligned
   int skip;       // elements of run 0 before the row
-  int vocab, turns, first;
+  int vocab, turns, first, first_whole, last_whole;  // runs that lie in the row
 
+  // The runs n[0..U): loaded together, those that stick out of the row (or lie behind it) mended afterwards, so that no
+  // load waits for another.
+  template <int U> CDB_DEVICE void fetch(const int* n, Run* x) const {
+    int c[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      c[u] = last_whole < first_whole ? -1 : min(max(n[u], first_whole), last_whole);
+      if (last_whole >= first_whole) x[u].load(base + (int64_t)c[u] * kRun);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      if (n[u] != c[u]) {
+        const int i0 = n[u] * kRun - skip;
+#pragma unroll
+        for (int e = 0; e < kRun; ++e)
+          x[u].set(e, i0 + e >= 0 && i0 + e < vocab ? Elem<T>::load(base + (int64_t)n[u] * kRun + e) : -INFINITY);
+      }
+  }
   CDB_DEVICE Run fetch(int n) const {
     Run x;
-    const int i0 = n * kRun - skip;
-    if (i0 >= 0 && i0 <= vocab - kRun) {
-      x.load(base + (int64_t)n * kRun);
-    } else {
-#pragma unroll
-      for (int e = 0; e < kRun; ++e)
-        x.set(e, i0 + e >= 0 && i0 + e < vocab ? Elem<T>::load(base + (int64_t)n * kRun + e) : -INFINITY);
-    }
+    fetch<1>(&n, &x);
     return x;
   }
   CDB_DEVICE void open(const T* row, int n) {
     skip = (int)(((uintptr_t)row & 15) / sizeof(T));
     base = row - skip;
     vocab = n;
+    first_whole = skip == 0 ? 0 : 1;
+    last_whole = (skip + n) / kRun - 1;
     const int runs = (skip + n + kRun - 1) / kRun;
     turns = (runs + kSampleThreads - 1) / kSampleThreads;
     first = (threadIdx.x >> 6) * turns * kWave + (threadIdx.x & 63);
   }
+  CDB_DEVICE int wave_of(int i) const { return (skip + i) / kRun / (turns * kWave); }
   // f(turn, run, index of its first token) for the lane's runs, in order; U of them, or the next one, load together.
   template <int U, typename F> CDB_DEVICE void each(F f) const {
     if constexpr (U == 1) {
@@ -205,8 +227,10 @@ template <typename T> struct SampleRow {
     } else {
       for (int j0 = 0; j0 < turns; j0 += U) {
         Run x[U];
+        int n[U];
 #pragma unroll
-        for (int u = 0; u < U; ++u) x[u] = fetch(first + min(j0 + u, turns - 1) * kWave);
+        for (int u = 0; u < U; ++u) n[u] = first + min(j0 + u, turns - 1) * kWave;
+        fetch<U>(n, x);
 #pragma unroll
         for (int u = 0; u < U; ++u)
           if (j0 + u < turns) f(j0 + u, x[u], (first + (j0 + u) * kWave) * kRun - skip);
@@ -274,13 +298,8 @@ struct Limit {
   }
 };
 
-// Puts the tokens of a run for which keep(logit, index) holds on the list; beyond its end they are only counted. For
-// whole waves.
-template <typename Run, typename F>
-CDB_DEVICE void append(SampleShared& s, const Run& x, int i, F keep) {
-  uint32_t mask = 0;
-#pragma unroll
-  for (int e = 0; e < kRun; ++e) mask |= keep(x.get(e), i + e) ? 1u << e : 0u;
+// Puts the tokens of a run whose bits are set on the list; beyond its end they are only counted. For whole waves.
+template <typename Run> CDB_DEVICE void append(SampleShared& s, const Run& x, int i, uint32_t mask) {
   if (!__any(mask != 0)) return;
   const uint32_t upto = wave_running32(__popc(mask));
   const uint32_t all = __builtin_amdgcn_readlane(upto, 63);
@@ -294,6 +313,14 @@ CDB_DEVICE void append(SampleShared& s, const Run& x, int i, F keep) {
       if (at < kList) s.list[at] = place_of(x.get(e), i + e);
       ++at;
     }
+}
+
+// The bits of a run's tokens for which keep(logit, index) holds.
+template <typename Run, typename F> CDB_DEVICE uint32_t bits_of(const Run& x, int i, F keep) {
+  uint32_t mask = 0;
+#pragma unroll
+  for (int e = 0; e < kRun; ++e) mask |= keep(x.get(e), i + e) ? 1u << e : 0u;
+  return mask;
 }
 
 // Of a histogram in `mass`, ordered as the tokens are: the last bin that counts before which, `before` included, less
@@ -389,6 +416,22 @@ CDB_DEVICE uint64_t pick(SampleShared& s, const W& w, int n, uint64_t limit, uin
   }
 }
 
+// What the tokens that `limit` leaves weigh (or how many they are), by their distance from the maximum, to `mass`.
+template <bool kMass, typename Row, typename W>
+CDB_DEVICE void histogram(const Row& row, SampleShared& s, const W& w, const Limit& limit) {
+  s.mass[threadIdx.x] = 0;
+  __syncthreads();
+  row.template each<1>([&](int, const typename Row::Run& x, int i) __attribute__((always_inline)) {
+    uint64_t q[kRun];
+#pragma unroll
+    for (int e = 0; e < kRun; ++e) q[e] = kMass ? w.units_of(x.get(e)) : 1;
+#pragma unroll
+    for (int e = 0; e < kRun; ++e)
+      if ((q[e] != 0) & limit.keeps(x.get(e), i + e)) add_to(&s.mass[w.bin(x.get(e))], q[e]);
+  });
+  __syncthreads();
+}
+
 // The place of the last kept token of the row, as `pick`, among those that `limit` leaves. `bin`: of those up to the
 // first histogram's `bin`, if it was made already (0 or more), before which `before` lies.
 template <bool kMass, typename Row, typename W>
@@ -398,17 +441,7 @@ CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const W& w, const Limit
   const int t = threadIdx.x;
   uint64_t lo = 0, hi = ~0ull, total;
   if (bin < 0) {
-    s.mass[t] = 0;
-    __syncthreads();
-    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
-#pragma unroll
-      for (int e = 0; e < kRun; ++e) {
-        const float y = x.get(e);
-        const uint64_t q = kMass ? w.units_of(y) : 1;
-        if (limit.keeps(y, i + e)) add_to(&s.mass[w.bin(y)], q);
-      }
-    });
-    __syncthreads();
+    histogram<kMass>(row, s, w, limit);
     const uint64_t upto = block_running(s.mass[t], s, total);
     if (kMass) goal *= (double)total;
     goal = fmax(goal, 0x1p-60);
@@ -428,7 +461,7 @@ CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const W& w, const Limit
       s.hi = 0;
     }
     __syncthreads();
-    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { append(s, x, i, inside); });
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { append(s, x, i, bits_of(x, i, inside)); });
     __syncthreads();
     if (s.found <= kList) return pick<kMass>(s, w, s.found, 0, before, goal, false);
     uint64_t least = ~0ull, most = 0;
@@ -592,7 +625,7 @@ CDB_DEVICE int collect(const SampleRow<T>& row, SampleShared& s, const W& w, int
     return (x > -INFINITY) & !(d * w.bins_per >= edge);
   };
   row.template each<4>([&](int, const typename SampleRow<T>::Run& x, int i) __attribute__((always_inline)) {
-    if (__any(inside(largest(x), 0))) append(s, x, i, inside);
+    if (__any(inside(largest(x), 0))) append(s, x, i, bits_of(x, i, inside));
   });
   __syncthreads();
   return s.found;
@@ -620,18 +653,8 @@ CDB_DEVICE bool draw_few(const SampleParams& P, int64_t r, const SampleRow<T>& r
     __syncthreads();
     b = s.bin;
   } else if (f.by_share) {
-    s.mass[t] = 0;
     if (t == 0) s.found = 0;
-    __syncthreads();
-    row.template each<1>([&](int, const typename SampleRow<T>::Run& x, int) __attribute__((always_inline)) {
-      uint64_t q[kRun];
-#pragma unroll
-      for (int e = 0; e < kRun; ++e) q[e] = w.units_of(x.get(e));
-#pragma unroll
-      for (int e = 0; e < kRun; ++e)
-        if (q[e] != 0) add_to(&s.mass[w.bin(x.get(e))], q[e]);
-    });
-    __syncthreads();
+    histogram<true>(row, s, w, Limit::none());
     const uint64_t upto = block_running(s.mass[t], s, total);
     goal = fmax(f.p * (double)total, 0x1p-60);
     b = bin = max(last_bin(s, upto, before, goal), 0);
@@ -663,22 +686,72 @@ CDB_DEVICE void draw_many(const SampleParams& P, int64_t r, const SampleRow<T>& 
   const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
   Limit limit = Limit::none();
   if (f.by_count) limit = Limit::at(cut<false>(row, s, w, limit, (double)f.k, -1, 0));
-  if (f.by_share) limit = Limit::at(cut<true>(row, s, w, limit, bin < 0 ? f.p : goal, bin, bin < 0 ? 0 : before));
+  uint64_t sum = 0, total = 0;
+  bool weighed = false;
+  if (f.by_share) {
+    if (bin < 0) {
+      histogram<true>(row, s, w, limit);
+      const uint64_t upto = block_running(s.mass[t], s, total);
+      goal = fmax(f.p * (double)total, 0x1p-60);
+      before = 0;
+      bin = max(last_bin(s, upto, before, goal), 0);
+    }
+    // The tokens before the bin in which the share ends are kept and weighed, those of the bin collected.
+    if (t == 0) s.found = 0;
+    __syncthreads();
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+      if (!__any(w.bin(largest(x)) <= bin)) return;
+      uint32_t above = 0, here = 0;
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) {
+        const float y = x.get(e);
+        const int b = limit.keeps(y, i + e) ? w.bin(y) : kBins;
+        above |= b < bin ? 1u << e : 0u;
+        here |= b == bin ? 1u << e : 0u;
+      }
+      sum += w.units_of_run(x, [&](int e, double v) __attribute__((always_inline)) -> bool {
+        return (above >> e & 1) & (v >= f.least);
+      });
+      append(s, x, i, here);
+    });
+    __syncthreads();
+    const int n = s.found;
+    weighed = n <= kList;
+    __syncthreads();  // all have read it
+    if (weighed) {
+      const uint64_t last = pick<true>(s, w, n, 0, before, goal, false);
+      limit = Limit::at(last);
+      sum = wave_total(sum);
+      if (lane == 0) s.wave64[wave] = sum;
+      __syncthreads();
+      for (int j = t; j < n; j += kSampleThreads) {
+        const uint64_t place = s.list[j];
+        const double v = w.of(logit_of((uint32_t)(place >> 32)));
+        if (place >= last && v >= f.least) add_to(&s.wave64[row.wave_of((int)~(uint32_t)place)], W::units(v));
+      }
+    } else {
+      limit = Limit::at(cut<true>(row, s, w, limit, goal, bin, before));
+    }
+  }
   auto of_run = [&](const Run& x, int i) __attribute__((always_inline)) -> uint64_t {
     if (limit.every && !f.by_size) return w.units_of_run(x);
-    if (!__any(limit.every || largest(x) >= limit.last)) return 0;
     return w.units_of_run(x, [&](int e, double v) __attribute__((always_inline)) -> bool {
       return limit.keeps(x.get(e), i + e) & (v >= f.least);
     });
   };
+  if (!weighed) {
+    sum = 0;
+    row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+      if (__any(limit.every || largest(x) >= limit.last)) sum += of_run(x, i);
+    });
+    sum = wave_total(sum);
+    __syncthreads();
+    if (lane == 0) s.wave64[wave] = sum;
+  }
+  __syncthreads();
   // Where the running weight passes the goal: the wave, the turn of that wave (a wave of this workgroup each), the
   // lane, the token.
-  uint64_t sum = 0, total = 0;
-  row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { sum += of_run(x, i); });
-  sum = wave_total(sum);
-  __syncthreads();
-  if (lane == 0) s.wave64[wave] = sum;
-  __syncthreads();
+  total = 0;
 #pragma unroll
   for (int v = 0; v < kSampleWaves; ++v) total += s.wave64[v];
   const uint64_t at_goal = goal_of(f.u, total);
@@ -743,7 +816,7 @@ __global__ void __launch_bounds__(kSampleThreads) sample_kernel(SampleParams P) 
     else part_top[0] = fmaxf(part_top[0], m);
   });
   const float mine = fmaxf(part_top[0], part_top[1]);
-  float top = wave_max(mine);
+  float top = wave_largest(mine);
   if (lane == 0) s.wave32[wave] = top;
   if (t == 0) s.bin = 0x7fffffff;  // the lowest index, of a greedy row
   __syncthreads();

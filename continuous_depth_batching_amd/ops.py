@@ -262,7 +262,7 @@ def _(q, k_new, v_new, kv_pool, cache_layer, cache_layer0, block_table, table_ro
 # Decode attention of rows that share prefixes.
 # ---------------------------------------------------------------------------
 
-PREFIX_QUERIES = _lib.CDB_PREFIX_QUERIES
+PREFIX_QUERIES, PREFIX_FEW = _lib.CDB_PREFIX_QUERIES, _lib.CDB_PREFIX_FEW
 
 
 @dataclass(frozen=True)
@@ -273,12 +273,15 @@ class PrefixDecodePlan:
 
     listed    [n] rows with a prefix, group by group
     items     [m, 8]: (the group's first place in listed, rows, first row and tokens, first query, first and end token, 0)
-    row_info  [rows, 4]: (first query in the group, tokens of the prefix, the group's first item, parts)
+    row_info  [rows, 4]: (first query in the group, tokens of the prefix, the group's first item, parts, negative where
+              the items are of the few)
+    few       the items of groups with few queries, which come first
     """
 
     listed: "np.ndarray | torch.Tensor"
     items: "np.ndarray | torch.Tensor"
     row_info: "np.ndarray | torch.Tensor"
+    few: int
 
     @property
     def num_rows(self) -> int:
@@ -296,7 +299,7 @@ class PrefixDecodePlan:
         arrays = [np.asarray(a, dtype=np.int32) for a in (self.items, self.row_info, self.listed)]  # items aligned
         flat = torch.from_numpy(np.concatenate([a.ravel() for a in arrays])).to(device)
         items, info, listed = (x.view(a.shape) for x, a in zip(flat.split([a.size for a in arrays]), arrays))
-        return PrefixDecodePlan(listed=listed, items=items, row_info=info)
+        return PrefixDecodePlan(listed=listed, items=items, row_info=info, few=self.few)
 
 
 def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np.ndarray", *, num_heads: int,
@@ -305,9 +308,10 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
     group's ``lengths[group[b]]`` tokens. Rows of one group sit at the same cache layer: rows at two loop depths of a
     layout with a slot a step are two groups.
 
-    Prefixes are cut into parts of about equal length, enough of them to give every CU a workgroup while a part keeps
-    128 tokens, and at most 64 (a part costs each of its queries a partial result, written and read again). A row's
-    rounding depends on its prefix's parts."""
+    Prefixes are cut into parts of about equal length, at least 128 tokens and at most 64 parts: as many as give every
+    CU a workgroup, as a part costs each of its queries a partial result, written and read again; three times as many
+    where a group has 32 queries at most, whose workgroups run three to a CU. A row's rounding depends on its prefix's
+    parts."""
 
     import numpy as np
 
@@ -326,22 +330,28 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
     info = np.zeros((group.size, 4), dtype=np.int64)
     names, first, counts = np.unique(group[order], return_index=True, return_counts=True)
     tokens = lengths[names]
-    runs = (counts * share + PREFIX_QUERIES - 1) // PREFIX_QUERIES
-    each = max(128, -(-int((runs * tokens).sum()) * num_kv_heads // int(num_cus)))
-    parts = np.minimum(np.maximum(tokens // each, 1), _lib.CDB_PREFIX_MAX_PARTS)
+    few = counts * share <= 2 * PREFIX_FEW
+    sizes = np.where(few, PREFIX_FEW, PREFIX_QUERIES)
+    runs = (counts * share + sizes - 1) // sizes
     items = []
-    for at, count, length, run, part in zip(first.tolist(), counts.tolist(), tokens.tolist(), runs.tolist(),
-                                            parts.tolist()):
-        item0, rows = len(items), order[at:at + count]
-        step = -(-length // part)
-        step = -(-step // 32) * 32
-        part = -(-length // step)
-        items.extend((at, count, int(rows[0]), length, q * PREFIX_QUERIES, k * step, min(length, (k + 1) * step), 0)
-                     for q in range(run) for k in range(part))
-        info[rows, 0] = np.arange(count) * share
-        info[rows, 1], info[rows, 2], info[rows, 3] = length, item0, part
+    num_few = 0
+    for kind, wanted in ((True, 3 * int(num_cus)), (False, int(num_cus))):
+        of = np.flatnonzero(few == kind)
+        each = max(128, -(-int((runs[of] * tokens[of]).sum()) * num_kv_heads // wanted))
+        for n in of.tolist():
+            item0, at, count, length = len(items), int(first[n]), int(counts[n]), int(tokens[n])
+            part = min(max(length // each, 1), _lib.CDB_PREFIX_MAX_PARTS)
+            step = -(-length // part)
+            step = -(-step // 32) * 32
+            part = -(-length // step)
+            rows = order[at:at + count]
+            items.extend((at, count, int(rows[0]), length, q * int(sizes[n]), k * step, min(length, (k + 1) * step), 0)
+                         for q in range(int(runs[n])) for k in range(part))
+            info[rows, 0] = np.arange(count) * share
+            info[rows, 1], info[rows, 2], info[rows, 3] = length, item0, -part if kind else part
+        num_few = len(items) if kind else num_few
     return PrefixDecodePlan(listed=order.astype(np.int32), row_info=info.astype(np.int32),
-                            items=np.asarray(items, dtype=np.int32).reshape(-1, _lib.CDB_PREFIX_ITEM))
+                            items=np.asarray(items, dtype=np.int32).reshape(-1, _lib.CDB_PREFIX_ITEM), few=num_few)
 
 
 def prefix_decode_workspace_bytes(plan: PrefixDecodePlan, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -402,6 +412,8 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     if not isinstance(info, torch.Tensor):
         raise TypeError("the plan must be on the device: plan.to(device)")
     num_listed, num_items = listed.shape[0], items.shape[0]
+    if not 0 <= plan.few <= num_items:
+        raise ValueError(f"{plan.few} of the plan's {num_items} items cannot be the few")
     for name, t, n in (("plan.listed", listed, num_listed), ("plan.items", items, _lib.CDB_PREFIX_ITEM * num_items),
                        ("plan.row_info", info, 4 * num_rows)):
         kv8._check_ints(name, t, n)
@@ -417,7 +429,7 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
         q.data_ptr(), k_new.data_ptr(), v_new.data_ptr(), view.k_ptr, view.v_ptr, view.layer_stride, layers,
         pool_rows // block, _ptr(cache_layer), cache_layer0, block_table.data_ptr(), _ptr(table_row), table_rows, width,
         seqlens.data_ptr(), _ptr(rope_cos), _ptr(rope_sin), rope_style, max_positions, _ptr(q_bias), _ptr(k_bias),
-        listed.data_ptr(), num_listed, items.data_ptr(), num_items, info.data_ptr(),
+        listed.data_ptr(), num_listed, items.data_ptr(), num_items, plan.few, info.data_ptr(),
         out.data_ptr(), workspace.data_ptr(), workspace.nbytes, num_rows, num_heads, heads_kv, dim, block, scale,
         q_stride, kv_stride, dtype_code(dt), _stream())
     if code:
@@ -430,22 +442,22 @@ def prefix_decode_attention(q: torch.Tensor, k_new: torch.Tensor, v_new: torch.T
                             cache_layer: torch.Tensor | None, cache_layer0: int, block_table: torch.Tensor,
                             table_row: torch.Tensor | None, seqlens: torch.Tensor, rope_cos: torch.Tensor | None,
                             rope_sin: torch.Tensor | None, rope_style: int, q_bias: torch.Tensor | None,
-                            k_bias: torch.Tensor | None, listed: torch.Tensor,
-                            items: torch.Tensor, row_info: torch.Tensor, workspace: torch.Tensor, block_size: int,
+                            k_bias: torch.Tensor | None, listed: torch.Tensor, items: torch.Tensor,
+                            row_info: torch.Tensor, few: int, workspace: torch.Tensor, block_size: int,
                             scale: float) -> torch.Tensor:
     """Paged decode attention of rows that share prefixes, with fused RoPE + KV append over ``kv_pool``
-    [num_cache_layers, 2, pool_blocks * block_size, Hkv, D]; the plan's three tensors as in ``PrefixDecodePlan``. See
+    [num_cache_layers, 2, pool_blocks * block_size, Hkv, D]; the plan's parts as in ``PrefixDecodePlan``. See
     ``prefix_decode_attention_raw``."""
 
     out = q.new_empty(q.shape)
     return prefix_decode_attention_raw(q, k_new, v_new, KVPoolView(kv_pool, block_size), cache_layer, cache_layer0,
                                        block_table, table_row, seqlens, rope_cos, rope_sin, rope_style, q_bias, k_bias,
-                                       PrefixDecodePlan(listed, items, row_info), out, workspace, scale)
+                                       PrefixDecodePlan(listed, items, row_info, few), out, workspace, scale)
 
 
 @prefix_decode_attention.register_fake
 def _(q, k_new, v_new, kv_pool, cache_layer, cache_layer0, block_table, table_row, seqlens, rope_cos, rope_sin,
-      rope_style, q_bias, k_bias, listed, items, row_info, workspace, block_size, scale):
+      rope_style, q_bias, k_bias, listed, items, row_info, few, workspace, block_size, scale):
     return q.new_empty(q.shape)
 
 

@@ -493,6 +493,7 @@ int cdb_batch_layout(const int32_t* past, const int32_t* lens, int32_t num_seqs,
 
 enum {
   CDB_PREFIX_QUERIES = 128,  /* queries (row, head) of an item */
+  CDB_PREFIX_FEW = 16,       /* of the first num_few items: those of groups with few queries */
   CDB_PREFIX_ITEM = 8,       /* words of an item */
   CDB_PREFIX_MAX_PARTS = 64  /* parts that a prefix is cut into */
 };
@@ -512,10 +513,11 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
  * layer or as copies, which are read through the table row and cache layer of the group's first row; the others are
  * read only from there on. Queries of a group are counted row by row, the group's num_heads / num_kv_heads heads of a
  * KV head each. items [num_items][CDB_PREFIX_ITEM] (16-byte aligned) = (the group's first place in listed, its rows, its
- * first row, tokens of its prefix, first query, a multiple of CDB_PREFIX_QUERIES, first token, end token, 0): the parts
- * of a group's tokens for one run of queries follow each other, and the runs of a group too; 0 rows is no item. row_info
- * [num_rows][4] = (row's first query in its group, tokens of its prefix, its group's first item, parts), zeros for a
- * row without a group. A row is listed at most once.
+ * first row, tokens of its prefix, first query, a multiple of the item's queries, first token, end token, 0): the parts
+ * of a group's tokens for one run of queries follow each other, and the runs of a group too; 0 rows is no item. The
+ * first num_few items have CDB_PREFIX_FEW queries each, the others CDB_PREFIX_QUERIES. row_info [num_rows][4] = (row's
+ * first query in its group, tokens of its prefix, its group's first item, parts, negative where the items are of the
+ * first num_few), zeros for a row without a group. A row is listed at most once.
  *
  * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
  * or the angles' range or inside its prefix, or its cache layer or table row out of range; NaN where its cache layer is
@@ -528,7 +530,7 @@ int cdb_prefix_decode_attention(const void* q, const void* k_new, const void* v_
                                 const int32_t* seqlens, const float* rope_cos, const float* rope_sin,
                                 int32_t rope_style, int32_t max_positions, const void* q_bias, const void* k_bias,
                                 const int32_t* listed, int32_t num_listed, const int32_t* items, int32_t num_items,
-                                const int32_t* row_info, void* out,
+                                int32_t num_few, const int32_t* row_info, void* out,
                                 void* workspace, int64_t workspace_bytes, int32_t num_rows, int32_t num_heads,
                                 int32_t num_kv_heads, int32_t head_dim, int32_t block_size, float scale,
                                 int64_t q_stride, int64_t kv_stride, int32_t dtype, hipStream_t stream);

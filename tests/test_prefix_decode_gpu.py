@@ -236,7 +236,7 @@ def test_the_registered_operator():
     want, pool = ph.call(s).clone(), s.pool.clone()
     got = torch.ops.cdb.prefix_decode_attention(
         s.q, s.k, s.v, pool, s.layer, s.layer0, s.table, None, s.seq, s.cos, s.sin, s.rope, s.q_bias, s.k_bias,
-        s.plan.listed, s.plan.items, s.plan.row_info, s.workspace, s.block, s.scale)
+        s.plan.listed, s.plan.items, s.plan.row_info, s.plan.few, s.workspace, s.block, s.scale)
     assert torch.equal(got, want) and torch.equal(pool, s.pool)
 
 

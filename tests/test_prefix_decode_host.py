@@ -22,15 +22,18 @@ def cover(plan, group, lengths, heads, kv):
         if n < 0 or lengths[n] == 0:
             assert not plan.row_info[b].any()
             continue
+        size = ops.PREFIX_FEW if parts < 0 else ops.PREFIX_QUERIES
+        assert (item0 < plan.few) == (parts < 0)
+        parts = abs(parts)
         assert length == lengths[n] and 1 <= parts <= _lib.CDB_PREFIX_MAX_PARTS
         first, count, leader, tokens = plan.items[item0, :4]
         assert tokens == length and leader == plan.listed[first] and not plan.items[:, 7].any()
         assert b in plan.listed[first:first + count] and plan.listed[first + q0 // share] == b and q0 % share == 0
         for q in range(q0, q0 + share):
-            run = item0 + q // ops.PREFIX_QUERIES * parts
+            run = item0 + q // size * parts
             of = plan.items[run:run + parts]
             assert (of[:, :4] == plan.items[item0, :4]).all()
-            assert (of[:, 4] == q // ops.PREFIX_QUERIES * ops.PREFIX_QUERIES).all()
+            assert (of[:, 4] == q // size * size).all()
             assert of[0, 5] == 0 and of[-1, 6] == length and (of[1:, 5] == of[:-1, 6]).all()
             assert (of[:, 5] < of[:, 6]).all()
 
@@ -68,7 +71,7 @@ def code(**over):
     a = dict(q=fake, k_new=fake, v_new=fake, k_pool=fake, v_pool=fake, layer_stride=64 * 16 * 256, layers=2,
              pool_blocks=64, cache_layer=None, cache_layer0=0, block_table=fake, table_row=None, table_rows=4,
              table_width=8, seqlens=fake, cos=fake, sin=fake, style=1, max_positions=100, q_bias=None, k_bias=None,
-             listed=fake, num_listed=4, items=fake, num_items=1, row_info=fake, out=fake,
+             listed=fake, num_listed=4, items=fake, num_items=1, num_few=1, row_info=fake, out=fake,
              workspace=fake, nbytes=1 << 24, rows=4, heads=4, kv=4, dim=64, block=16, scale=0.1, q_stride=0,
              kv_stride=0, dtype=_lib.CDB_DTYPE_BF16, stream=None)
     a.update(over)
@@ -86,7 +89,7 @@ odd = ctypes.c_void_p(0x1004)
     (dict(table_rows=3), _lib.CDB_ERR_SHAPE), (dict(table_width=1 << 27), _lib.CDB_ERR_SHAPE),
     (dict(layers=0), _lib.CDB_ERR_SHAPE), (dict(pool_blocks=0), _lib.CDB_ERR_SHAPE),
     (dict(pool_blocks=1 << 31), _lib.CDB_ERR_SHAPE), (dict(num_listed=-1), _lib.CDB_ERR_SHAPE),
-    (dict(num_items=-1), _lib.CDB_ERR_SHAPE), (dict(items=odd), _lib.CDB_ERR_SHAPE),
+    (dict(num_items=-1), _lib.CDB_ERR_SHAPE), (dict(num_few=2), _lib.CDB_ERR_SHAPE), (dict(num_few=-1), _lib.CDB_ERR_SHAPE), (dict(items=odd), _lib.CDB_ERR_SHAPE),
     (dict(block=8), _lib.CDB_ERR_SHAPE), (dict(block=48), _lib.CDB_ERR_SHAPE),
     (dict(layer_stride=64 * 16 * 256 - 8), _lib.CDB_ERR_SHAPE), (dict(scale=0.0), _lib.CDB_ERR_SHAPE),
     (dict(scale=float("inf")), _lib.CDB_ERR_SHAPE), (dict(scale=float("nan")), _lib.CDB_ERR_SHAPE),
@@ -132,6 +135,7 @@ def scene():
     (lambda s: setattr(s, "cos", s.cos[:, :3]), ValueError),
     (lambda s: setattr(s, "q_bias", torch.zeros(8, 64)), ValueError),
     (lambda s: setattr(s, "plan", s.host_plan), TypeError),
+    (lambda s: setattr(s, "plan", replace(s.plan, few=99)), ValueError),
     (lambda s: setattr(s, "plan", replace(s.plan, items=s.plan.items.long())), TypeError),
     (lambda s: setattr(s, "plan", replace(s.plan, row_info=s.plan.row_info[:2])), ValueError),
     (lambda s: setattr(s, "plan", replace(s.plan, items=s.plan.items[:, :3])), ValueError),
@@ -157,5 +161,5 @@ def test_operator_is_registered():
         q, k = torch.empty(3, 8, 64, device="cuda"), torch.empty(3, 4, 64, device="cuda")
         out = torch.ops.cdb.prefix_decode_attention(q, k, k, torch.empty(1, 2, 64, 4, 64, device="cuda"), None, 0,
                                                     ints(3, 4), None, ints(3), None, None, 0, None, None, ints(3),
-                                                    ints(1, 8), ints(3, 4), ints(9), 16, 0.125)
+                                                    ints(1, 8), ints(3, 4), 1, ints(9), 16, 0.125)
         assert out.shape == q.shape
