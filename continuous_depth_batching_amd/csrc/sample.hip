@@ -10,16 +10,22 @@
 // keep, so weights are fp64 exponentials (2^-38 relative) rounded to fixed point, 2^-46 of the largest weight, and
 // every sum is an integer: exact, and so the same in any order of the additions, atomic ones among them.
 //
-// One workgroup of 16 waves takes a row; a wave owns a run of consecutive tokens, 8 of them a lane at a time.
+// One workgroup takes a row; a wave owns a run of consecutive tokens, 8 of them a lane at a time.
 //   A first pass leaves the largest logit of each of 2048 parts of the row.
 //   top-k: the k-th largest of these is a bound that k tokens at least reach, and mostly not many more. min-p gives its
 //   bound at once. A second pass collects the tokens above the bound, and the rest is done on that list, in LDS.
 //   top-p: the second pass adds up what lies at each distance from the maximum (a histogram in LDS), which says where
 //   the share ends; the tokens above are collected if they are few.
-//   Where many tokens are kept, those of the bin in which the filter ends are collected to find the place where it
-//   does, and a last pass weighs the kept tokens in index order.
+//   Where many tokens are kept, the pass after that weighs the tokens above the bin in which the filter ends and
+//   collects those of the bin, whose place is then found on the list. Without a filter one pass weighs all tokens.
 // On lists, histograms over ranges of (logit, index) as one number narrow a range down to 128 tokens, which are
 // ordered by counting.
+//
+// Bounds: a row lies with one CU, which reads it at 25 GB/s a row where 256 run (the first pass over 256 rows of 131072
+// fp32 logits takes 21 us, 6.4 TB/s, a later one 19 and more from the last cache), and weighs 5.5 tokens a nanosecond,
+// 19 fp64 instructions each. So one row of 49152 bf16 logits with all filters takes 13 us, of which the passes are 3
+// and the rest is launch, loads and meetings that wait for each other; 256 rows with mixed ones 48, 256 of 131072 fp32
+// logits 118: the row that keeps 99 % at T = 1.5 bounds them with the first pass 22, histogram 36, weights 37, place 8.
 
 #include <cfloat>
 
@@ -41,8 +47,8 @@ struct SampleParams {
   int32_t vocab, unit_log2;  // weights are counted in units of 2^-unit_log2
 };
 
-// 2^(y + raise) in fp64, for y from about -1000 to 0 and a whole `raise`: 2^f for |f| <= 1/2 by a polynomial through its
-// values at 0 and the zeros of a Chebyshev polynomial (off by 2.1e-12 of the value at most), exact at f = 0.
+// 2^(y + raise) in fp64, for y from about -1000 to 0 and a whole `raise`: 2^f for |f| <= 1/2 by a polynomial through
+// its values at 0 and the zeros of a Chebyshev polynomial (off by 2.1e-12 of the value at most), exact at f = 0.
 CDB_DEVICE double power_of_two(double y, double magic) {
   // magic = 1.5 * 2^52 + raise: the sum's last bits are y rounded to a whole number, and raise.
   const double t = y + magic, f = y - (t - magic);
@@ -137,11 +143,12 @@ CDB_DEVICE void widen(uint64_t* lo, uint64_t* hi, uint64_t least, uint64_t most)
 // The work of a workgroup of kSampleThreads threads on its row.
 template <int kSampleThreads> struct Sampler {
   static constexpr int kSampleWaves = kSampleThreads / kWave;
-  static constexpr int kBins = 1024, kBinsEach = kBins / kSampleThreads;      // a thread's lie side by side
-  static constexpr int kList = 2048, kListEach = kList / kSampleThreads;      // tokens of a list
-  static constexpr int kParts = 2048, kPartsEach = kParts / kSampleThreads;   // of a row: a thread's runs, dealt out in turn
-  static constexpr int kPartRank = 1200;  // a part's maximum of this rank is reached by some 1800 tokens where they lie as they fall
-  static constexpr int kShort = 128, kSharers = kSampleThreads / kShort;      // tokens ordered by counting, threads a token
+  static constexpr int kBins = 1024, kBinsEach = kBins / kSampleThreads;     // a thread's lie side by side
+  static constexpr int kList = 2048, kListEach = kList / kSampleThreads;     // tokens of a list
+  static constexpr int kParts = 2048, kPartsEach = kParts / kSampleThreads;  // of a row: a thread's runs in turn
+  // A part's maximum of this rank is reached by some 1800 tokens, where they lie as they fall.
+  static constexpr int kPartRank = 1200;
+  static constexpr int kShort = 128, kSharers = kSampleThreads / kShort;  // tokens ordered by counting, threads a token
   static_assert(kBinsEach >= 1 && kPartsEach <= 8 && kSharers >= 1 && kSharers <= 8, "shares of a thread");
 
   // Sum over the kSharers lanes of a token.
@@ -156,7 +163,7 @@ template <int kSampleThreads> struct Sampler {
     uint64_t list[kList];
     uint64_t few[kShort], few_mass[kShort];
     uint64_t wave64[kSampleWaves], lo, hi, before;
-    float wave32[kSampleWaves], edge[2];
+    float wave32[kSampleWaves], low32[kSampleWaves], edge[2];
     int32_t bin, found, found_few;
   };
 
@@ -186,8 +193,8 @@ template <int kSampleThreads> struct Sampler {
     int skip;       // elements of run 0 before the row
     int vocab, turns, first, first_whole, last_whole;  // runs that lie in the row
 
-    // The runs n[0..U): loaded together, those that stick out of the row (or lie behind it) mended afterwards, so that no
-    // load waits for another.
+    // The runs n[0..U): loaded together, those that stick out of the row (or lie behind it) mended afterwards, so that
+    // no load waits for another.
     template <int U> CDB_DEVICE void fetch(const int* n, Run* x) const {
       int c[U];
 #pragma unroll
@@ -294,13 +301,14 @@ template <int kSampleThreads> struct Sampler {
       const float d = !kPlain && x == top_f ? 0.f : top_f - x;
       return (int)fminf(d * bins_per, (float)(kBins - 1));
     }
-    // The logits of bin b, from `lo` to `hi`, for the workgroup, which meets once: the first wave narrows the range of all
-    // logits up to the maximum, half of it for each end, 32 places at a time.
+    // The logits of bin b, from `lo` to `hi`, for the workgroup, which meets once: the first wave narrows the range of
+    // all logits up to the maximum, half of it for each end, 32 places at a time.
     CDB_DEVICE void edges(SampleShared& s, int b, float& lo, float& hi) const {
       if (threadIdx.x < kWave) {
         const int lane = threadIdx.x;
         const bool upper = lane >= 32;
-        uint32_t out = logit_key(-FLT_MAX) - 1, in = logit_key(top_f);  // bins of `in` are b - upper at most, of `out` not
+        // The bin of `in` is b - upper at most, that of `out` is not.
+        uint32_t out = logit_key(-FLT_MAX) - 1, in = logit_key(top_f);
         while (__any(in - out > 1)) {
           const uint32_t mid = out + (uint32_t)(((uint64_t)(in - out) * ((lane & 31) + 1)) / 33);
           const uint64_t all = __ballot(mid != out && bin(logit_of(mid)) <= b - upper);
@@ -325,7 +333,9 @@ template <int kSampleThreads> struct Sampler {
     int index;
     bool every;
     CDB_DEVICE static Limit none() { return {0.f, 0, true}; }
-    CDB_DEVICE static Limit at(uint64_t place) { return {logit_of((uint32_t)(place >> 32)), (int)~(uint32_t)place, false}; }
+    CDB_DEVICE static Limit at(uint64_t place) {
+      return {logit_of((uint32_t)(place >> 32)), (int)~(uint32_t)place, false};
+    }
     CDB_DEVICE bool keeps(float x, int i) const {
       return (every & (x > -INFINITY)) | (!every & ((x > last) | ((x == last) & (i <= index))));
     }
@@ -364,8 +374,9 @@ template <int kSampleThreads> struct Sampler {
     if (threadIdx.x == 0) s.bin = -1;
     __syncthreads();
   }
-  // Of a whole histogram in `mass`, ordered as the tokens are: the last bin that counts before which, `before` included,
-  // less than the goal lies. share: the goal is that share of the histogram. `before` becomes what lies before that bin.
+  // Of a whole histogram in `mass`, ordered as the tokens are: the last bin that counts before which, `before`
+  // included, less than the goal lies. share: the goal is that share of the histogram. `before` becomes what lies
+  // before that bin.
   static CDB_DEVICE int last_bin(SampleShared& s, uint64_t& before, double& goal, bool share, uint64_t& total) {
     const int t = threadIdx.x;
     uint64_t q[kBinsEach], sum = 0;
@@ -402,7 +413,8 @@ template <int kSampleThreads> struct Sampler {
   // the `before` that is not on the list, less than the goal lies: kMass, of what they weigh; otherwise a number of
   // tokens. share: the goal is that share of what they weigh. The first is always kept.
   template <bool kMass, typename W>
-  static CDB_DEVICE uint64_t pick(SampleShared& s, const W& w, int n, uint64_t limit, uint64_t before, double goal, bool share) {
+  static CDB_DEVICE uint64_t pick(SampleShared& s, const W& w, int n, uint64_t limit, uint64_t before, double goal,
+                                  bool share) {
     const int t = threadIdx.x;
     uint64_t place[kListEach], q[kListEach], lo = ~0ull, hi = 0, total;
 #pragma unroll
@@ -487,8 +499,8 @@ template <int kSampleThreads> struct Sampler {
   // The place of the last kept token of the row, as `pick`, among those that `limit` leaves. `bin`: of those up to the
   // first histogram's `bin`, if it was made already (0 or more), before which `before` lies.
   template <bool kMass, typename Row, typename W>
-  static CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const W& w, const Limit& limit, double goal, int bin,
-                          uint64_t before) {
+  static CDB_DEVICE uint64_t cut(const Row& row, SampleShared& s, const W& w, const Limit& limit, double goal,
+                                 int bin, uint64_t before) {
     typedef typename Row::Run Run;
     const int t = threadIdx.x;
     uint64_t lo = 0, hi = ~0ull, total;
@@ -510,7 +522,9 @@ template <int kSampleThreads> struct Sampler {
         s.hi = 0;
       }
       __syncthreads();
-      row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) { append(s, x, i, bits_of(x, i, inside)); });
+      row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+        append(s, x, i, bits_of(x, i, inside));
+      });
       __syncthreads();
       if (s.found <= kList) return pick<kMass>(s, w, s.found, 0, before, goal, false);
       uint64_t least = ~0ull, most = 0;
@@ -566,8 +580,8 @@ template <int kSampleThreads> struct Sampler {
   // Draws from the list of the row's first n tokens, n <= kShort, in any order, of which top-k leaves k at most; goal:
   // the weight that top-p asks for, if it is known (0 or more).
   template <typename W>
-  static CDB_DEVICE void draw_short(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f, int n,
-                             double goal) {
+  static CDB_DEVICE void draw_short(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f,
+                                    int n, double goal) {
     // kSharers threads a token, which each compare it with their share of the others.
     const int t = threadIdx.x, i = t / kSharers, part = t % kSharers;
     const uint64_t place = i < n ? s.list[i] : 0;
@@ -613,8 +627,8 @@ template <int kSampleThreads> struct Sampler {
 
   // The same for n <= kList.
   template <typename W>
-  static CDB_DEVICE void draw_list(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f, int n,
-                            double goal) {
+  static CDB_DEVICE void draw_list(const SampleParams& P, int64_t r, SampleShared& s, const W& w, const Filters& f,
+                                   int n, double goal) {
     const int t = threadIdx.x;
     uint64_t limit = 1;
     if (f.by_count) limit = pick<false>(s, w, n, limit, 0, (double)f.k, false);
@@ -666,12 +680,14 @@ template <int kSampleThreads> struct Sampler {
       if (q[e] != 0 && (int)~(uint32_t)place[e] == base) give(P, r, w, place[e], sum);
   }
 
-  // Collects the tokens up to bin b of the first histogram; how many they are.
-  template <typename T, typename W>
-  static CDB_DEVICE int collect(const SampleRow<T>& row, SampleShared& s, const W& w, int b) {
+  // A logit that all of the first b + 1 bins, of which `per` lie in a unit of logit, reach. (top - x) * per below b + 1
+  // is off by 2^-22 of itself at most, and rounding the difference here keeps the order of the logits.
+  static CDB_DEVICE float reached(float top, float per, int b) { return top - (float)(b + 1) / per * 1.000001f; }
+  // Collects the tokens that reach `bound`; how many they are.
+  template <typename T> static CDB_DEVICE int collect(const SampleRow<T>& row, SampleShared& s, float bound) {
     if (threadIdx.x == 0) s.found = 0;
     __syncthreads();
-    auto inside = [&](float x, int) __attribute__((always_inline)) -> bool { return (x > -INFINITY) & (w.bin(x) <= b); };
+    auto inside = [&](float x, int) __attribute__((always_inline)) -> bool { return x >= bound; };
     row.template each<sizeof(T) == 2 ? 8 : 4>(
         [&](int, const typename SampleRow<T>::Run& x, int i) __attribute__((always_inline)) {
           if (__any(inside(largest(x), 0))) append(s, x, i, bits_of(x, i, inside));
@@ -680,24 +696,30 @@ template <int kSampleThreads> struct Sampler {
     return s.found;
   }
 
-  // Draws by collecting the tokens that may be kept in a list. False, for all threads, where they may be too many; `bin`,
-  // `before` and `goal` then tell what is known of where top-p ends.
+  // Draws by collecting the tokens that may be kept in a list. False, for all threads, where they may be too many;
+  // `bin`, `before` and `goal` then tell what is known of where top-p ends.
   template <typename T, typename W>
-  static CDB_DEVICE bool draw_few(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s, const W& w,
-                           const Filters& f, const float* part_top, int& bin, uint64_t& before, double& goal) {
+  static CDB_DEVICE bool draw_few(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s,
+                                  const W& w, const Filters& f, const float* part_top, float least, int& bin,
+                                  uint64_t& before, double& goal) {
     if (f.by_count && f.k > kPartRank) return false;
     const int t = threadIdx.x;
     uint64_t total;
     int b = kBins - 1;
+    float bound = -FLT_MAX;
     if (f.by_count) {
+      // By the bins of the weights the k-th token may lie in the last one with most of the row, too many for a list:
+      // 256 mixed rows of 131072, among them k = 1000 at T = 0.3, took 280 us. With bins from the largest of the parts'
+      // maxima to the least they take 118.
+      const float width = (float)(kBins - 1) / (w.top_f - least), per = width <= FLT_MAX ? width : 0.f;
       clear_bins(s);
 #pragma unroll
       for (int e = 0; e < kPartsEach; ++e)
-        if (part_top[e] > -INFINITY) add_to(&s.mass[w.bin(part_top[e])], 1);
+        if (part_top[e] > -INFINITY) add_to(&s.mass[(int)fminf((w.top_f - part_top[e]) * per, (float)(kBins - 1))], 1);
       uint64_t parts_before = 0;
       double rank = (double)f.k;
       const int last = last_bin(s, parts_before, rank, false, total);
-      if (total >= (uint64_t)f.k) b = last;
+      if (total >= (uint64_t)f.k) bound = fmaxf(least, reached(w.top_f, per, last));
     } else if (f.by_share) {
       if (t == 0) s.found = 0;
       histogram<true>(row, s, w, Limit::none());
@@ -706,7 +728,8 @@ template <int kSampleThreads> struct Sampler {
       // The parts whose largest logit lies up to there tell about how many tokens do.
       int parts = 0;
 #pragma unroll
-      for (int e = 0; e < kPartsEach; ++e) parts += __popcll(__ballot(part_top[e] > -INFINITY && w.bin(part_top[e]) <= b));
+      for (int e = 0; e < kPartsEach; ++e)
+        parts += __popcll(__ballot(part_top[e] > -INFINITY && w.bin(part_top[e]) <= b));
       if ((t & 63) == 0) atomicAdd(&s.found, parts);
       __syncthreads();
       const bool many = s.found > kPartRank;
@@ -717,7 +740,8 @@ template <int kSampleThreads> struct Sampler {
       const double far = -log2(f.size) * (kBins / 46.0) + 1.0;
       b = min(b, (int)fmin(far, (double)(kBins - 1)));
     }
-    const int n = collect(row, s, w, b);
+    if (b < kBins - 1) bound = fmaxf(bound, reached(w.top_f, w.bins_per, b));
+    const int n = collect(row, s, bound);
     if (n > kList) return false;
     if (n <= kShort) draw_short(P, r, s, w, f, n, goal);
     else draw_list(P, r, s, w, f, n, goal);
@@ -726,8 +750,8 @@ template <int kSampleThreads> struct Sampler {
 
   // Draws by weighing every kept token in index order.
   template <typename T, typename W>
-  static CDB_DEVICE void draw_many(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s, const W& w,
-                            const Filters& f, int bin, uint64_t before, double goal) {
+  static CDB_DEVICE void draw_many(const SampleParams& P, int64_t r, const SampleRow<T>& row, SampleShared& s,
+                                   const W& w, const Filters& f, int bin, uint64_t before, double goal) {
     typedef typename SampleRow<T>::Run Run;
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     Limit limit = Limit::none();
@@ -859,11 +883,12 @@ template <int kSampleThreads> struct Sampler {
     // Loaded with the row's first tokens: a load of its own would cost each its time.
     const float temperature = P.temperature == nullptr ? 1.f : P.temperature[r];
     const int k = P.top_k == nullptr ? 0 : P.top_k[r];
-    const float p = P.top_p == nullptr ? 1.f : P.top_p[r], m = P.min_p == nullptr || !(P.min_p[r] > 0.f) ? 0.f : fminf(P.min_p[r], 1.f);
+    const float p = P.top_p == nullptr ? 1.f : P.top_p[r];
+    const float m = P.min_p == nullptr || !(P.min_p[r] > 0.f) ? 0.f : fminf(P.min_p[r], 1.f);
     Filters f;
     f.u = P.uniform[r];
 
-    float part_top[kPartsEach], mine = -INFINITY;
+    float part_top[kPartsEach], mine = -INFINITY, least = INFINITY;  // of the parts' largest: the largest, the least
 #pragma unroll
     for (int e = 0; e < kPartsEach; ++e) part_top[e] = -INFINITY;
     for (int j0 = 0; j0 < row.turns; j0 += 8) {
@@ -877,13 +902,23 @@ template <int kSampleThreads> struct Sampler {
         if (j0 + u < row.turns) part_top[u % kPartsEach] = fmaxf(part_top[u % kPartsEach], largest(x[u]));
     }
 #pragma unroll
-    for (int e = 0; e < kPartsEach; ++e) mine = fmaxf(mine, part_top[e]);
+    for (int e = 0; e < kPartsEach; ++e) {
+      mine = fmaxf(mine, part_top[e]);
+      least = fminf(least, part_top[e] > -INFINITY ? part_top[e] : INFINITY);
+    }
     float top = wave_largest(mine);
-    if (lane == 0) s.wave32[wave] = top;
+    least = -wave_largest(-least);
+    if (lane == 0) {
+      s.wave32[wave] = top;
+      s.low32[wave] = least;
+    }
     if (t == 0) s.bin = 0x7fffffff;  // the lowest index, of a greedy row
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < kSampleWaves; ++w) top = fmaxf(top, s.wave32[w]);
+    for (int w = 0; w < kSampleWaves; ++w) {
+      top = fmaxf(top, s.wave32[w]);
+      least = fminf(least, s.low32[w]);
+    }
     if (top == -INFINITY) {
       if (t == 0) {
         P.tokens[r] = -1;
@@ -928,7 +963,8 @@ template <int kSampleThreads> struct Sampler {
       int bin = -1;
       uint64_t before = 0;
       double goal = -1.0;
-      if ((f.by_count || f.by_share || f.by_size) && draw_few(P, r, row, s, w, f, part_top, bin, before, goal)) return;
+      if ((f.by_count || f.by_share || f.by_size) && draw_few(P, r, row, s, w, f, part_top, least, bin, before, goal))
+        return;
       __syncthreads();
       draw_many(P, r, row, s, w, f, bin, before, goal);
     } else {
@@ -946,8 +982,8 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleParams P) {
 }
 
 template <typename T> static int sample_type(const SampleParams& P, int rows, hipStream_t stream) {
-  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster: 256 rows of 49152 take 47 us
-  // with 1024 threads and 52 with 512, one row 12.2 and 13; 356 rows of 1438 take 30 and 14.5, 95 of 368 19 and 15.
+  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster: 256 rows of 49152 take 48 us
+  // with 1024 threads and 52 with 512; 356 rows of 1438 take 30 and 14.5, 298 of 82 27 and 16, 95 of 368 19 and 15.
   if (rows > 256 || P.vocab <= 8192) sample_kernel<T, 512><<<dim3((unsigned)rows), dim3(512), 0, stream>>>(P);
   else sample_kernel<T, 1024><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(P);
   return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;

@@ -137,6 +137,53 @@ def test_numbers_outside_the_unit_interval_are_the_nearest_inside():
     assert got[:2].tolist() == [0, 0] and got[2:].tolist() == [998, 998]
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+@pytest.mark.parametrize("vocab", [8192, 8193, 70001])
+def test_many_tokens_kept_by_several_filters(vocab, dtype):
+    # More than a list holds by top-k, by top-p and by min-p, and together; low temperatures at which most tokens weigh
+    # less than a unit, where the k-th of them is far behind the last that weighs anything.
+    x = logits_of(10, vocab, dtype, seed=vocab)
+    check(x, np.random.default_rng(vocab + 1).random(10),
+          temperature=[0.3, 0.05, 0.3, 3.0, 3.0, 3.0, 9.0, 9.0, 1.0, 0.01],
+          top_k=[1000, 1200, 1201, 5000, 5000, 0, 0, 7000, 2500, 900],
+          top_p=[1.0, 0.9999, 0.9, 0.97, 1.0, 0.97, 1.0, 0.999, 0.9999999, 0.5],
+          min_p=[0.0, 0.0, 1e-9, 0.0, 1e-3, 1e-3, 1e-2, 1e-4, 0.0, 0.0])
+
+
+def test_more_rows_than_compute_units_of_a_long_vocabulary():
+    rows, vocab = 260, 9001
+    x = logits_of(rows, vocab, torch.float32, seed=21)
+    kinds = [dict(top_k=0, top_p=1.0, min_p=0.0), dict(top_k=40, top_p=0.9, min_p=0.0),
+             dict(top_k=0, top_p=0.95, min_p=0.0), dict(top_k=3000, top_p=0.99, min_p=0.0),
+             dict(top_k=0, top_p=1.0, min_p=0.01)]
+    check(x, np.random.default_rng(22).random(rows), temperature=[(0.0, 0.5, 1.0, 2.5)[r % 4] for r in range(rows)],
+          **{n: [kinds[r % 5][n] for r in range(rows)] for n in ("top_k", "top_p", "min_p")})
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_logits_crowded_around_the_border(dtype):
+    # Almost all logits have two values next to each other, so a bin holds more than a list and is narrowed by index.
+    vocab = 20011
+    x = torch.full((6, vocab), 1.0, dtype=dtype)
+    x[:, ::3] = 1.0078125
+    x[:, 5] = 9.0
+    x[4:, 6] = -30.0
+    check(x, [0.1, 0.5, 0.77, 0.93, 0.31, 0.9], top_k=[0, 6000, 6671, 9000, 0, 1100],
+          top_p=[0.7, 1.0, 0.9, 0.5, 0.9, 0.99], min_p=[0.0, 0.0, 0.0, 0.0, 1e-4, 0.0])
+
+
+def test_far_apart_logits_and_high_temperatures():
+    # Differences beyond the type's range, and none at all among the largest of the parts.
+    x = torch.zeros(4, 4000)
+    x[0, ::2], x[0, 1::2] = 3e38, -3e38
+    x[1, 7], x[1, 9] = 3.4e38, -3.4e38
+    x[2, 1::8] = 5.0
+    x[3] = torch.linspace(-3e38, 3e38, 4000)
+    check(x, [0.3, 0.6, 0.9, 0.999], temperature=[1e38, 3e38, 1.0, 2e38], top_k=[1100, 30, 400, 1000])
+    check(x, [0.3, 0.6, 0.9, 0.999], temperature=[1e38, 3e38, 1.0, 2e38], top_p=[0.9, 0.5, 0.99, 0.3])
+    check(x, [0.3, 0.6, 0.9, 0.999], temperature=[1e38, 3e38, 1.0, 2e38], min_p=[0.01, 0.5, 0.1, 0.05])
+
+
 def test_frequencies_follow_the_weights():
     # 200000 evenly spread numbers: each token's count is its share to within one number.
     x = torch.tensor([[0.3, -math.inf, 1.7, -0.5, 1.7, 0.0]])
