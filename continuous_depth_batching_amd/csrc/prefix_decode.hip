@@ -1,19 +1,27 @@
 // Decode attention of rows that share prefixes, over the paged cache in the model's type.
 //
 // Row b attends over positions 0..p_b of its cache layer. Rows of a group begin with the same tokens; these are read
-// once for all of them, each row's own tokens by the row:
-//   prefix_attend_kernel  a workgroup takes 16 queries (row, head) of a group and one KV head and a part of the
-//                         prefix's tokens, and leaves the unnormalised sum, the maximum and the sum of weights;
-//   prefix_decode_kernel  a workgroup takes one row and KV head and 1024 of the row's own tokens, rotates and appends
-//                         the new one, and joins what it has with the prefix's parts (a row with several chunks: the
-//                         workgroup that ends last does).
+// once for all of them, each row's own tokens by the row, and what the two leave is joined: with m, l and O a part's
+// largest score, sum of weights and weighted sum of values, M = max m, out = sum 2^(m - M) O / sum 2^(m - M) l.
+//   prefix_attend_kernel  a workgroup takes 16 or 128 queries (row, head) of a group, one KV head and a part of the
+//                         prefix's tokens, and leaves m, l and O of each query;
+//   prefix_decode_kernel  a workgroup of two waves takes one row and KV head and 1024 of the row's own tokens, rotates
+//                         and appends the new one, and joins what it has with the prefix's parts (a row with several
+//                         chunks: the workgroup that ends last does).
 // Both walk tokens 32 (fp32: 16) at a time, a wave each, with a running maximum and sum:
 //   S^T = K Q^T, bf16: v_mfma_f32_16x16x32_bf16 on keys as they lie in memory, with the rotated query, already scaled,
 //   as two bf16 parts (2^-17 of an element together);
 //   O^T = V^T P^T with P as two bf16 parts; values are turned to the operand's order by one byte permutation for two
-//   of them.
+//   of them. One part of Q and P each would halve the products and lose what the one-row kernel keeps, which holds both
+//   in fp32.
 // fp32 takes v_mfma_f32_16x16x4_f32, which rounds nothing but the sums. Both products are 16 queries wide; columns
 // without a query repeat the last one. A lane's scores are those of the tokens whose values it holds, so P never moves.
+//
+// Bounds, bf16, heads of 128: own tokens, by the bytes: 256 rows x 16 KV heads of 32 to 512 own tokens take 95 us,
+// 3.8 TB/s, of the 127 us with 2 x 2048 shared ones, whose part is bound by the products' chain (30 us). 32000 tokens
+// shared by 64 rows of 32 heads on 8 KV heads: 85 us, in which a SIMD has matrix work for 27 and vector work (weights
+// and their parts) for 25, at two waves that wait for the same steps; the rows' own tokens take 20 more.
+
 #include <atomic>
 #include <chrono>
 
@@ -31,8 +39,11 @@ constexpr int kColumns = 16;     // queries of a product
 constexpr int kQueries = CDB_PREFIX_QUERIES;  // of an item
 constexpr int kItem = CDB_PREFIX_ITEM;        // words of an item
 static_assert(CDB_PREFIX_FEW == kColumns && kQueries == 128, "queries of an item's waves");
-// A prefix's workgroup: four waves of the same 16 queries, each with every fourth step; or four of 32 queries each on
-// two parts of the tokens.
+// A prefix's workgroup: four waves of the same 16 queries, each with every fourth step, loaded by itself; or four of 32
+// queries each on two parts of the tokens, which share a step's loads in LDS. The plan takes the first kind for groups
+// of up to 32 queries: 8 groups of 8 (32, 33, 64) queries on 2048 tokens, 16 KV heads, take 41 (64, 76, 121) us with
+// their own tokens on the first kind and 49 (73, 74, 105) on the second; one group on 16000 tokens 41 (54, 70, 80) and
+// 46 (50, 52, 56).
 template <bool kFew> constexpr int kWaves = kFew ? 4 : 8;
 static_assert(kMaxParts <= 64, "a lane weighs a part");
 
@@ -209,10 +220,13 @@ template <int D> struct StepRegs<float, D> {
 
 // The staged walk: a workgroup's waves that take the same tokens share them in LDS. Two parts of the tokens are walked
 // side by side, by four waves each; a part's step lies as [keys, values][token][D], rows 16 bytes apart, which spreads
-// the operands' reads over all banks. While a step is multiplied the next one's loads are on the way.
+// the operands' reads over all banks. While a step is multiplied the next one's loads are on the way. Computing the
+// next step's scores while this one is weighed, with a third step in LDS, takes 252 registers and turns the 105 us of
+// the 32000 tokens above into 113.
 template <typename T, int D> struct Stage {
   static constexpr int kTiles = StepRegs<T, D>::kTiles, kStep = 16 * kTiles;
-  static constexpr int kPieces = D * (int)sizeof(T) / 16, kUnits = (kPieces + 15) / 16;  // 16 bytes of a row; a thread's
+  static constexpr int kPieces = D * (int)sizeof(T) / 16;  // of 16 bytes, of a row
+  static constexpr int kUnits = (kPieces + 15) / 16;       // of a thread
   static constexpr int kRow = D * (int)sizeof(T) + 16, kPlane = kStep * kRow, kPart = 2 * kPlane, kBytes = 2 * kPart;
   u32x4_t w[2][kTiles][kUnits];
 
@@ -386,7 +400,8 @@ template <typename T, int D, int NC> struct Walk {
         // values one for the next keys too.
         const int ahead = step + stride < steps ? step + stride : step;
         f32x4_t s[NC][kTiles];
-        x.template scores<NC>([&](int n, int i) __attribute__((always_inline)) { return operand(query, slot, n, i); }, s);
+        x.template scores<NC>(
+            [&](int n, int i) __attribute__((always_inline)) { return operand(query, slot, n, i); }, s);
         load_keys(at, ahead, r, g);
         int from[kTiles], to[kTiles];
 #pragma unroll
@@ -402,8 +417,8 @@ template <typename T, int D, int NC> struct Walk {
       }
     }
   }
-  // The staged walk over [lo, hi) for all of a workgroup's threads; `lds` holds the queries, which every wave takes from
-  // there first. A wave without queries only loads.
+  // The staged walk over [lo, hi) for all of a workgroup's threads; `lds` holds the queries, which every wave takes
+  // from there first. A wave without queries only loads.
   CDB_DEVICE void shared_tokens(const Tokens& at, uint32_t* lds, int run, int part, int cols, int from, int to) {
     typedef Stage<T, D> S;
     typedef typename StepRegs<T, D>::Operand Operand;
@@ -522,7 +537,8 @@ template <typename T, int D, int NC> struct Walk {
 // 16 elements of a column of the query operands: of query head `head` of row b at position p, rotated and scaled; NaN,
 // or zeros, where there is no such query.
 template <typename T, int D, int STYLE>
-CDB_DEVICE void turn_query(const PrefixParams& P, uint32_t* query, int c, int piece, int b, int head, int p, float none) {
+CDB_DEVICE void turn_query(const PrefixParams& P, uint32_t* query, int c, int piece, int b, int head, int p,
+                           float none) {
   const int d = STYLE == 1 ? 8 * piece : 16 * piece;
   float x[8], y[8];
   if (p >= 0) {
@@ -572,10 +588,11 @@ template <typename T, int D> CDB_DEVICE Tokens tokens_of(const PrefixParams& P, 
   return x;
 }
 
-// Words of LDS: the queries, and in their place later the staged tokens, and what half of the waves leave to the others.
+// Words of LDS: the queries, and in their place later the staged tokens, and what half of the waves leave to the other.
 template <typename T, int D, bool kFew> struct AttendLds {
   static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kFew ? 1 : kQueries / 16);
-  static constexpr int kJoin = kWaves<kFew> / 2 * (kFew ? 16 : 32) * (D + 4), kStages = kFew ? 0 : Stage<T, D>::kBytes / 2;
+  static constexpr int kJoin = kWaves<kFew> / 2 * (kFew ? 16 : 32) * (D + 4);
+  static constexpr int kStages = kFew ? 0 : Stage<T, D>::kBytes / 2;
   static constexpr int kMost = kQ > kJoin ? kQ : kJoin, kWords = kMost > kStages ? kMost : kStages;
 };
 
@@ -654,7 +671,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
   // The row's queries within its group, and the prefix's parts.
   const int n0 = P.row_info[4 * b], item0 = P.row_info[4 * b + 2], given = P.row_info[4 * b + 3];
   row.bad = row.bad || given < -kMaxParts || given > kMaxParts;
-  const int parts = row.bad ? 0 : given < 0 ? -given : given, each = given < 0 ? kColumns : kQueries;  // queries of an item
+  const int parts = row.bad ? 0 : given < 0 ? -given : given;
+  const int each = given < 0 ? kColumns : kQueries;  // queries of an item
   if (parts == 0) {
     row.bad = row.bad || row.own != 0;
   } else {
@@ -718,7 +736,8 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
       // The new token as the first of a tile.
       const int r = lane & 15, g = lane >> 4;
 #pragma unroll
-      for (int a = 0; a < StepRegs<T, D>::kTiles; ++a) walk.x.load_key(a, reinterpret_cast<const char*>(fresh[0]), 0, g);
+      for (int a = 0; a < StepRegs<T, D>::kTiles; ++a)
+        walk.x.load_key(a, reinterpret_cast<const char*>(fresh[0]), 0, g);
 #pragma unroll
       for (int i = 0; i < 4 * StepRegs<T, D>::kTiles; ++i)
         walk.x.load_value(i, reinterpret_cast<const char*>(fresh[1]), 0, r);
@@ -956,7 +975,8 @@ extern "C" int cdb_prefix_decode_attention(
   if (kv_stride == 0) kv_stride = row;
   if (q_stride < (int64_t)num_heads * head_dim || kv_stride < row) return CDB_ERR_SHAPE;
   if (reinterpret_cast<uintptr_t>(workspace) % 16 != 0 || reinterpret_cast<uintptr_t>(k_pool) % 16 != 0 ||
-      reinterpret_cast<uintptr_t>(v_pool) % 16 != 0 || reinterpret_cast<uintptr_t>(items) % 16 != 0 || layer_stride * size % 16 != 0)
+      reinterpret_cast<uintptr_t>(v_pool) % 16 != 0 || reinterpret_cast<uintptr_t>(items) % 16 != 0 ||
+      layer_stride * size % 16 != 0)
     return CDB_ERR_SHAPE;
   const int64_t left = workspace_bytes - shared_bytes(num_items, num_kv_heads, head_dim);
   const int64_t chunks = left < 0 ? 0 : min(left / (num_rows * chunk_bytes(num_heads, num_kv_heads, head_dim)),
