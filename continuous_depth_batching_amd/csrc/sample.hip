@@ -16,16 +16,17 @@
 //   bound at once. A second pass collects the tokens above the bound, and the rest is done on that list, in LDS.
 //   top-p: the second pass adds up what lies at each distance from the maximum (a histogram in LDS), which says where
 //   the share ends; the tokens above are collected if they are few.
-//   Where many tokens are kept, the pass after that weighs the tokens above the bin in which the filter ends and
-//   collects those of the bin, whose place is then found on the list. Without a filter one pass weighs all tokens.
+//   Where many tokens are kept, the pass after that collects those of the bin in which the filter ends, whose place is
+//   then found on the list, and weighs the tokens above the bin, if it is not known what each wave's weigh: workgroups
+//   of 16 waves have a histogram for each. Without a filter one pass weighs all tokens.
 // On lists, histograms over ranges of (logit, index) as one number narrow a range down to 128 tokens, which are
 // ordered by counting.
 //
 // Bounds: a row lies with one CU, which reads it at 25 GB/s a row where 256 run (the first pass over 256 rows of 131072
-// fp32 logits takes 21 us, 6.4 TB/s, a later one 19 and more from the last cache), and weighs 5.5 tokens a nanosecond,
-// 19 fp64 instructions each. So one row of 49152 bf16 logits with all filters takes 13 us, of which the passes are 3
-// and the rest is launch, loads and meetings that wait for each other; 256 rows with mixed ones 48, 256 of 131072 fp32
-// logits 118: the row that keeps 99 % at T = 1.5 bounds them with the first pass 22, histogram 36, weights 37, place 8.
+// fp32 logits takes 21 us, 6.4 TB/s, a later one 19 from the last cache), and weighs 5.5 tokens a nanosecond, some 25
+// instructions of 4 cycles each. So one row of 49152 bf16 logits with all filters takes 14 us, of which the passes are
+// 3 and the rest is launch, loads and meetings that wait for each other; 256 rows with mixed ones 41, 256 of 131072
+// fp32 logits 88: what bounds them is a row that keeps 99 % at T = 1.5, or top-k and top-p together.
 
 #include <cfloat>
 
@@ -149,6 +150,10 @@ template <int kSampleThreads> struct Sampler {
   // A part's maximum of this rank is reached by some 1800 tokens, where they lie as they fall.
   static constexpr int kPartRank = 1200;
   static constexpr int kShort = 128, kSharers = kSampleThreads / kShort;  // tokens ordered by counting, threads a token
+  // Whether each wave has a histogram of its own, which saves weighing the kept tokens again: one workgroup to a CU has
+  // the LDS for that. 64 rows of 65536 flat fp32 logits with top-p take 41 us so and 50 without, 256 rows of 131072
+  // mixed ones 88 and 118.
+  static constexpr bool kApart = kSampleThreads == 1024;
   static_assert(kBinsEach >= 1 && kPartsEach <= 8 && kSharers >= 1 && kSharers <= 8, "shares of a thread");
 
   // Sum over the kSharers lanes of a token.
@@ -159,7 +164,7 @@ template <int kSampleThreads> struct Sampler {
     return v;
   }
   struct SampleShared {
-    uint64_t mass[kBins];
+    uint64_t mass[kBins], apart[kApart ? kSampleWaves : 1][kApart ? kBins : 1];
     uint64_t list[kList];
     uint64_t few[kShort], few_mass[kShort];
     uint64_t wave64[kSampleWaves], lo, hi, before;
@@ -496,6 +501,32 @@ template <int kSampleThreads> struct Sampler {
     });
   }
 
+  // The same of all tokens' weights, with what each wave's tokens weigh to `apart`.
+  template <typename Row, typename W>
+  static CDB_DEVICE void histogram_apart(const Row& row, SampleShared& s, const W& w) {
+    const int t = threadIdx.x;
+    uint64_t* mine = s.apart[t >> 6];
+#pragma unroll
+    for (int e = 0; e < kBins; e += kWave) mine[e + (t & 63)] = 0;
+    row.template each<1>([&](int, const typename Row::Run& x, int) __attribute__((always_inline)) {
+      uint64_t q[kRun];
+#pragma unroll
+      for (int e = 0; e < kRun; ++e) q[e] = w.units_of(x.get(e));
+#pragma unroll
+      for (int e = 0; e < kRun; ++e)
+        if (q[e] != 0) add_to(&mine[w.bin(x.get(e))], q[e]);
+    });
+    __syncthreads();
+#pragma unroll
+    for (int e = 0; e < kBinsEach; ++e) {
+      uint64_t sum = 0;
+#pragma unroll
+      for (int v = 0; v < kSampleWaves; ++v) sum += s.apart[v][t * kBinsEach + e];
+      s.mass[t * kBinsEach + e] = sum;
+    }
+    if (t == 0) s.bin = -1;
+  }
+
   // The place of the last kept token of the row, as `pick`, among those that `limit` leaves. `bin`: of those up to the
   // first histogram's `bin`, if it was made already (0 or more), before which `before` lies.
   template <bool kMass, typename Row, typename W>
@@ -707,6 +738,9 @@ template <int kSampleThreads> struct Sampler {
     uint64_t total;
     int b = kBins - 1;
     float bound = -FLT_MAX;
+    // (Of top-k's tokens all are needed to tell what top-p's share of them is.)
+    if (f.by_size && !(f.by_count && f.by_share))
+      b = (int)fmin(-log2(f.size) * (kBins / 46.0) + 1.0, (double)(kBins - 1));
     if (f.by_count) {
       // By the bins of the weights the k-th token may lie in the last one with most of the row, too many for a list:
       // 256 mixed rows of 131072, among them k = 1000 at T = 0.3, took 280 us. With bins from the largest of the parts'
@@ -722,9 +756,11 @@ template <int kSampleThreads> struct Sampler {
       if (total >= (uint64_t)f.k) bound = fmaxf(least, reached(w.top_f, per, last));
     } else if (f.by_share) {
       if (t == 0) s.found = 0;
-      histogram<true>(row, s, w, Limit::none());
+      if constexpr (kApart) histogram_apart(row, s, w);
+      else histogram<true>(row, s, w, Limit::none());
       goal = f.p;
-      b = bin = last_bin(s, before, goal, true, total);
+      bin = last_bin(s, before, goal, true, total);
+      b = min(b, bin);
       // The parts whose largest logit lies up to there tell about how many tokens do.
       int parts = 0;
 #pragma unroll
@@ -735,10 +771,6 @@ template <int kSampleThreads> struct Sampler {
       const bool many = s.found > kPartRank;
       __syncthreads();
       if (many) return false;
-    }
-    if (f.by_size && !f.by_share) {
-      const double far = -log2(f.size) * (kBins / 46.0) + 1.0;
-      b = min(b, (int)fmin(far, (double)(kBins - 1)));
     }
     if (b < kBins - 1) bound = fmaxf(bound, reached(w.top_f, w.bins_per, b));
     const int n = collect(row, s, bound);
@@ -758,6 +790,7 @@ template <int kSampleThreads> struct Sampler {
     if (f.by_count) limit = Limit::at(cut<false>(row, s, w, limit, (double)f.k, -1, 0));
     uint64_t sum = 0, total = 0;
     bool weighed = false;
+    const bool apart = kApart && bin >= 0;
     if (f.by_share) {
       if (bin < 0) {
         histogram<true>(row, s, w, limit);
@@ -769,30 +802,41 @@ template <int kSampleThreads> struct Sampler {
       if (t == 0) s.found = 0;
       float lo, hi;
       w.edges(s, bin, lo, hi);
-      row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
-        const float m = largest(x);
-        if (!__any(m >= lo)) return;
-        Logits above;  // -infinity weighs nothing
-        uint32_t here = 0;
+      if (apart && limit.every && !f.by_size) {
+        // What the wave's tokens before the bin weigh is known.
+        for (int e = lane; e < bin; e += kWave) sum += s.apart[kApart ? wave : 0][kApart ? e : 0];
+        row.template each<sizeof(T) == 2 ? 8 : 4>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+          if (!__any(largest(x) >= lo)) return;
+          append(s, x, i, bits_of(x, i, [&](float y, int) __attribute__((always_inline)) -> bool {
+            return (y >= lo) & (y <= hi);
+          }));
+        });
+      } else {
+        row.template each<1>([&](int, const Run& x, int i) __attribute__((always_inline)) {
+          const float m = largest(x);
+          if (!__any(m >= lo)) return;
+          Logits above;  // -infinity weighs nothing
+          uint32_t here = 0;
 #pragma unroll
-        for (int e = 0; e < kRun; ++e) {
-          const float y = x.get(e);
-          above.v[e] = y > hi ? y : -INFINITY;
-          here |= (y >= lo) & (y <= hi) ? 1u << e : 0u;
-        }
-        if (limit.every && !f.by_size) {
-          sum += w.units_of_run(above);
-        } else {
-          uint32_t kept = 0;
+          for (int e = 0; e < kRun; ++e) {
+            const float y = x.get(e);
+            above.v[e] = y > hi ? y : -INFINITY;
+            here |= (y >= lo) & (y <= hi) ? 1u << e : 0u;
+          }
+          if (limit.every && !f.by_size) {
+            sum += w.units_of_run(above);
+          } else {
+            uint32_t kept = 0;
 #pragma unroll
-          for (int e = 0; e < kRun; ++e) kept |= limit.keeps(x.get(e), i + e) ? 1u << e : 0u;
-          here &= kept;
-          sum += w.units_of_run(above, [&](int e, double v) __attribute__((always_inline)) -> bool {
-            return (kept >> e & 1) & (v >= f.least);
-          });
-        }
-        append(s, x, i, here);
-      });
+            for (int e = 0; e < kRun; ++e) kept |= limit.keeps(x.get(e), i + e) ? 1u << e : 0u;
+            here &= kept;
+            sum += w.units_of_run(above, [&](int e, double v) __attribute__((always_inline)) -> bool {
+              return (kept >> e & 1) & (v >= f.least);
+            });
+          }
+          append(s, x, i, here);
+        });
+      }
       __syncthreads();
       const int n = s.found;
       weighed = n <= kList;

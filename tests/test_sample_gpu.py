@@ -150,6 +150,22 @@ def test_many_tokens_kept_by_several_filters(vocab, dtype):
           min_p=[0.0, 0.0, 1e-9, 0.0, 1e-3, 1e-3, 1e-2, 1e-4, 0.0, 0.0])
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_top_p_and_min_p_end_near_each_other(dtype):
+    # Many tokens kept; the largest weights lie close together, so min-p ends before, in and behind the bins in which
+    # top-p does.
+    vocab, shares = 20011, [0.2, 0.5, 0.8, 0.95, 0.999]
+    for temperature in (3.0, 8.0, 40.0):
+        x = logits_of(1, vocab, dtype, seed=31, spread=2.0).expand(40, vocab).contiguous()
+        top = (x[0].double() / temperature).sort(descending=True).values
+        w = (top - top[0]).exp()
+        ends = [float(w[int((w.cumsum(0) < p * w.sum()).sum())]) for p in shares]  # what top-p's last token weighs
+        top_p = [p for p in shares for _ in range(8)]
+        min_p = [e * f for e in ends for f in (0.2, 0.9, 0.97, 0.999, 1.0, 1.001, 1.03, 1.1)]
+        check(x, np.random.default_rng(int(temperature)).random(40), temperature=[temperature] * 40, top_p=top_p,
+              min_p=[min(1.0, m) for m in min_p])
+
+
 def test_more_rows_than_compute_units_of_a_long_vocabulary():
     rows, vocab = 260, 9001
     x = logits_of(rows, vocab, torch.float32, seed=21)
