@@ -319,6 +319,8 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
     lengths = np.asarray(lengths, dtype=np.int64).reshape(-1)
     if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads:
         raise ValueError(f"{num_heads} query heads cannot share {num_kv_heads} KV heads evenly")
+    if num_cus <= 0:
+        raise ValueError(f"no plan for {num_cus} CUs")
     if group.size and int(group.max()) >= lengths.size:
         raise ValueError(f"row in group {int(group.max())} of {lengths.size}")
     if lengths.size and (int(lengths.min()) < 0 or int(lengths.max()) > 1 << 30):

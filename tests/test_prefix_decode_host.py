@@ -66,6 +66,11 @@ def test_plans_that_make_no_sense(group, lengths, heads, kv):
         ops.prefix_decode_plan(group, lengths, num_heads=heads, num_kv_heads=kv)
 
 
+def test_plans_for_no_compute_units():
+    with pytest.raises(ValueError):
+        ops.prefix_decode_plan([0, 0], [100], num_heads=4, num_kv_heads=4, num_cus=0)
+
+
 def code(**over):
     fake = ctypes.c_void_p(0x1000)  # refused on the host: no kernel sees it
     a = dict(q=fake, k_new=fake, v_new=fake, k_pool=fake, v_pool=fake, layer_stride=64 * 16 * 256, layers=2,

@@ -1,9 +1,10 @@
 """Sampled tokens (cdb_sample through torch.ops.cdb.sample and ops.sample_raw) against the float64 definition.
 
-Tokens have to be equal: the kernel's weights are exact to 2^-44 of themselves and 2^-47 of the largest, so it could
-differ only where the given number, or p, falls within about V * 2^-47 of a border between two tokens. The numbers are
-drawn from a fixed seed and fall on no such border, or exactly on one that both sides compute exactly. A log-probability
-is the fp32 rounding of a value off by 2^-40 at most: 2^-24 relative, and 2^-38 near 0."""
+Tokens have to be equal: the kernel's weights are off by 2^-38 of themselves and, by rounding to whole units, by 2^-47 of
+the largest (2^-46 above 65536 tokens), so it could differ only where the given number, or p, falls within about 2^-38 of a
+border between two tokens. The numbers are drawn from a fixed seed and fall on no such border, or exactly on one that both
+sides compute exactly. A log-probability is the fp32 rounding, 2^-24 relative, of a value that is off by what the kept
+weight is: 2^-38."""
 
 from __future__ import annotations
 
