@@ -170,6 +170,7 @@ template <int kSampleThreads> struct Sampler {
     uint64_t wave64[kSampleWaves], lo, hi, before;
     float wave32[kSampleWaves], low32[kSampleWaves], edge[2];
     int32_t bin, found, found_few;
+    __align__(16) uint32_t ends[2 * kRun];  // the runs that stick out of the row, as the row's type
   };
 
   // Sum over this thread and those before it; `total` is the sum over all. Meets the workgroup twice.
@@ -196,7 +197,8 @@ template <int kSampleThreads> struct Sampler {
     typedef Vec<T, kRun> Run;
     const T* base;  // of run 0, aligned
     int skip;       // elements of run 0 before the row
-    int vocab, turns, first, first_whole, last_whole;  // runs that lie in the row
+    const T* ends;  // run 0 and the last one, if they stick out, -infinity outside
+    int vocab, turns, first, first_whole, last_whole, last;  // runs that lie in the row; the last one that touches it
 
     // The runs n[0..U): loaded together, those that stick out of the row (or lie behind it) mended afterwards, so that
     // no load waits for another.
@@ -210,10 +212,12 @@ template <int kSampleThreads> struct Sampler {
 #pragma unroll
       for (int u = 0; u < U; ++u)
         if (n[u] != c[u]) {
-          const int i0 = n[u] * kRun - skip;
+          if (n[u] <= last) {
+            x[u].load(ends + (n[u] == 0 ? 0 : kRun));
+          } else {
 #pragma unroll
-          for (int e = 0; e < kRun; ++e)
-            x[u].set(e, i0 + e >= 0 && i0 + e < vocab ? Elem<T>::load(base + (int64_t)n[u] * kRun + e) : -INFINITY);
+            for (int e = 0; e < kRun; ++e) x[u].set(e, -INFINITY);
+          }
         }
     }
     CDB_DEVICE Run fetch(int n) const {
@@ -221,13 +225,21 @@ template <int kSampleThreads> struct Sampler {
       fetch<1>(&n, &x);
       return x;
     }
-    CDB_DEVICE void open(const T* row, int n) {
+    CDB_DEVICE void open(SampleShared& s, const T* row, int n) {
       skip = (int)(((uintptr_t)row & 15) / sizeof(T));
       base = row - skip;
       vocab = n;
       first_whole = skip == 0 ? 0 : 1;
       last_whole = (skip + n) / kRun - 1;
-      const int runs = (skip + n + kRun - 1) / kRun;
+      const int runs = (skip + n + kRun - 1) / kRun, t = threadIdx.x;
+      last = runs - 1;
+      T* to = reinterpret_cast<T*>(s.ends);
+      ends = to;
+      if (skip != 0 || (skip + n) % kRun != 0) {
+        const int i = (t < kRun ? 0 : last * kRun) + t % kRun - skip;
+        if (t < 2 * kRun) Elem<T>::store(to + t, i >= 0 && i < n ? Elem<T>::load(row + i) : -INFINITY);
+        __syncthreads();
+      }
       turns = (runs + kSampleThreads - 1) / kSampleThreads;
       first = (threadIdx.x >> 6) * turns * kWave + (threadIdx.x & 63);
     }
@@ -922,7 +934,7 @@ template <int kSampleThreads> struct Sampler {
     const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const int64_t r = blockIdx.x;
     SampleRow<T> row;
-    row.open(static_cast<const T*>(P.logits) + r * P.row_stride, P.vocab);
+    row.open(s, static_cast<const T*>(P.logits) + r * P.row_stride, P.vocab);
 
     // Loaded with the row's first tokens: a load of its own would cost each its time.
     const float temperature = P.temperature == nullptr ? 1.f : P.temperature[r];
