@@ -1,7 +1,7 @@
 """Sampled tokens (cdb_sample through torch.ops.cdb.sample and ops.sample_raw) against the float64 definition.
 
 Tokens have to be equal: the kernel's weights are off by 2^-38 of themselves and, by rounding to whole units, by 2^-47 of
-the largest (2^-46 above 65536 tokens), so it could differ only where the given number, or p, falls within about 2^-38 of a
+the largest (2^-43 at 2^20 tokens), so it could differ only where the given number, or p, falls within about 2^-38 of a
 border between two tokens. The numbers are drawn from a fixed seed and fall on no such border, or exactly on one that both
 sides compute exactly. A log-probability is the fp32 rounding, 2^-24 relative, of a value that is off by what the kept
 weight is: 2^-38."""
@@ -165,6 +165,33 @@ def test_top_p_and_min_p_end_near_each_other(dtype):
         min_p = [e * f for e in ends for f in (0.2, 0.9, 0.97, 0.999, 1.0, 1.001, 1.03, 1.1)]
         check(x, np.random.default_rng(int(temperature)).random(40), temperature=[temperature] * 40, top_p=top_p,
               min_p=[min(1.0, m) for m in min_p])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32], ids=["bf16", "f32"])
+def test_largest_vocabulary(dtype):
+    vocab = 1 << 20
+    x = logits_of(6, vocab, dtype, seed=41, spread=1.0)
+    check(x, [0.999999, 0.2, 0.5, 0.8, 0.4, 0.7], temperature=[1.0, 1.0, 2.0, 1.0, 0.7, 0.0],
+          top_k=[0, 50, 0, 40000, 1100, 0], top_p=[1.0, 0.9, 0.97, 1.0, 0.9, 1.0],
+          min_p=[0.0, 0.0, 0.0, 0.0, 0.0, 0.0])
+
+
+def test_calls_on_two_streams_at_once():
+    sets = [logits_of(40, 5003 + 31000 * i, torch.bfloat16, seed=50 + i).to(DEV) for i in range(2)]
+    u = torch.rand(40, dtype=torch.float64, generator=torch.Generator().manual_seed(3)).to(DEV)
+    p = torch.full((40,), 0.95, device=DEV)
+    want = [torch.ops.cdb.sample(x, u, None, None, p, None) for x in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(8):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(torch.ops.cdb.sample(sets[i], u, None, None, p, None))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for tok, lp in got[i]:
+            assert torch.equal(tok, want[i][0]) and torch.equal(lp, want[i][1])
 
 
 def test_more_rows_than_compute_units_of_a_long_vocabulary():
