@@ -522,7 +522,8 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
  * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
  * or the angles' range or inside its prefix, or its cache layer or table row out of range; NaN where its cache layer is
  * not its group's first row's, and where a block outside the pool is met, for all rows of the group if it is in the
- * prefix. Calls that may overlap need a workspace each. */
+ * prefix. A value that is infinite makes its element infinite in every row that sees the token (NaN where the token's
+ * weight vanishes in fp32), a key whose score is -infinity has no weight. Calls that may overlap need a workspace each. */
 int cdb_prefix_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_pool, void* v_pool,
                                 int64_t layer_stride, int32_t num_cache_layers, int64_t pool_blocks,
                                 const int32_t* cache_layer, int32_t cache_layer0, const int32_t* block_table,
