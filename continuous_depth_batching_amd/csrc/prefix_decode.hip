@@ -624,12 +624,22 @@ __global__ void __launch_bounds__(64 * kWaves<kFew>, (kFew ? 3 : 2)) prefix_atte
   const int item = at_item + (kFew ? 0 : P.num_few);
   const int4 head = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[0];
   const int4 tail = reinterpret_cast<const int4*>(P.items + (int64_t)kItem * item)[1];
-  const int first = head.x, count = head.y, leader = head.z, length = head.w, q0 = tail.x, lo = tail.y, hi = tail.z;
+  const int first = head.x, count = head.y, length = head.w, q0 = tail.x, lo = tail.y, hi = tail.z;
   if (count <= 0 || count > P.num_listed || first < 0 || first > P.num_listed - count) return;  // no item
   const int64_t queries = (int64_t)count * P.group;
   if (q0 < 0 || q0 >= queries) return;
   const int cols = (int)min((int64_t)(kFew ? kColumns : kQueries), queries - q0);
-  int layer = -1, trow = -1;
+  // The row through which the tokens are read: the group's first, or the first behind it that is no padding.
+  int leader = head.z, layer = -1, trow = -1;
+  if (leader >= 0 && leader < P.num_rows && P.seqlens[leader] < 0) {
+    leader = -1;
+    for (int i = 0; i < count && leader < 0; i += kWave) {
+      const int b = i + lane < count ? P.listed[first + i + lane] : -1;
+      const uint64_t live = __ballot(b >= 0 && b < P.num_rows && P.seqlens[b] >= 0);
+      if (live != 0) leader = __builtin_amdgcn_readlane(b, __ffsll((unsigned long long)live) - 1);
+    }
+    if (leader < 0) return;  // no row that asks for the tokens
+  }
   if (leader >= 0 && leader < P.num_rows) {
     layer = P.cache_layer0 + (P.cache_layer == nullptr ? 0 : P.cache_layer[leader]);
     trow = P.table_row == nullptr ? leader : P.table_row[leader];

@@ -510,20 +510,21 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
  * has table_rows rows. Rotations are fp32 and rounded once, to the cache's type (that call rounds bf16 after each step).
  *
  * The rows of a group follow each other in listed; they hold the same first tokens, at the same slots of the same cache
- * layer or as copies, which are read through the table row and cache layer of the group's first row; the others are
- * read only from there on. Queries of a group are counted row by row, the group's num_heads / num_kv_heads heads of a
- * KV head each. items [num_items][CDB_PREFIX_ITEM] (16-byte aligned) = (the group's first place in listed, its rows, its
- * first row, tokens of its prefix, first query, a multiple of the item's queries, first token, end token, 0): the parts
- * of a group's tokens for one run of queries follow each other, and the runs of a group too; 0 rows is no item. The
- * first num_few items have CDB_PREFIX_FEW queries each, the others CDB_PREFIX_QUERIES. row_info [num_rows][4] = (row's
- * first query in its group, tokens of its prefix, its group's first item, parts, negative where the items are of the
- * first num_few), zeros for a row without a group. A row is listed at most once.
+ * layer or as copies, which are read through the table row and cache layer of the group's first row that is no padding;
+ * the others are read only from there on. Queries of a group are counted row by row, the group's num_heads /
+ * num_kv_heads heads of a KV head each. items [num_items][CDB_PREFIX_ITEM] (16-byte aligned) = (the group's first place
+ * in listed, its rows, its first row, tokens of its prefix, first query, a multiple of the item's queries, first token,
+ * end token, 0): the parts of a group's tokens for one run of queries follow each other, and the runs of a group too; 0
+ * rows is no item. The first num_few items have CDB_PREFIX_FEW queries each, the others CDB_PREFIX_QUERIES. row_info
+ * [num_rows][4] = (row's first query in its group, tokens of its prefix, its group's first item, parts, negative where
+ * the items are of the first num_few), zeros for a row without a group. A row is listed at most once.
  *
  * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
  * or the angles' range or inside its prefix, or its cache layer or table row out of range; NaN where its cache layer is
- * not its group's first row's, and where a block outside the pool is met, for all rows of the group if it is in the
- * prefix. A value that is infinite makes its element infinite in every row that sees the token (NaN where the token's
- * weight vanishes in fp32), a key whose score is -infinity has no weight. Calls that may overlap need a workspace each. */
+ * not that of the row through which its group's tokens are read, and where a block outside the pool is met, for all rows
+ * of the group if it is in the prefix. A value that is infinite makes its element infinite in every row that sees the
+ * token (NaN where the token's weight vanishes in fp32), a key whose score is -infinity has no weight. Calls that may
+ * overlap need a workspace each. */
 int cdb_prefix_decode_attention(const void* q, const void* k_new, const void* v_new, void* k_pool, void* v_pool,
                                 int64_t layer_stride, int32_t num_cache_layers, int64_t pool_blocks,
                                 const int32_t* cache_layer, int32_t cache_layer0, const int32_t* block_table,
