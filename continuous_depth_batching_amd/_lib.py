@@ -221,6 +221,7 @@ SIGNATURES: dict[str, tuple[object, list[object]]] = {
             _P, _P, c_int32, _P, _P,  # tile_seq, tile_q0, tile_capacity, counts, stream
         ],
     ),
+    "cdb_prefix_decode_plan_workspace_bytes": (c_int64, [c_int32] * 7),
     "cdb_prefix_decode_workspace_bytes": (c_int64, [c_int32, c_int32, c_int32, c_int32, c_int32, c_int32]),
     "cdb_prefix_decode_attention": (
         c_int32,

@@ -58,7 +58,7 @@ struct PrefixParams {
   const int32_t *listed, *items, *row_info;
   int32_t num_listed, num_items, num_few;
   void* out;
-  float* shared;   // [items][KV heads][kQueries][D + 2]: O, the maximum and the sum of a prefix's part
+  float* shared;   // [items][KV heads][queries of the item's kind][D + 2]: O, the maximum and the sum of a prefix's part
   float* partials; // [rows][heads][max_chunks][D + 2]: the same of a chunk of own tokens
   uint64_t* tags;  // [rows][KV heads][slices][max_chunks]: equal to `tag` where this call's partials are whole
   uint64_t tag;
@@ -67,6 +67,12 @@ struct PrefixParams {
   int64_t q_stride, kv_stride;
   bool vec;
 };
+
+// Queries that an item has room for, and where the first of them lies: queries of all items before it.
+template <bool kFew> constexpr int kRoom = kFew ? kColumns : kQueries;
+CDB_DEVICE int64_t room_of(const PrefixParams& P, int64_t item, bool few) {
+  return few ? item * kColumns : item * kQueries - (int64_t)P.num_few * (kQueries - kColumns);
+}
 
 // Where one KV head's tokens of a table row lie, 16 at a time.
 struct Tokens {
@@ -609,7 +615,7 @@ template <typename T, int D> CDB_DEVICE Tokens tokens_of(const PrefixParams& P, 
 
 // Words of LDS: the queries, and in their place later the staged tokens, and what half of the waves leave to the other.
 template <typename T, int D, bool kFew> struct AttendLds {
-  static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kFew ? 1 : kQueries / 16);
+  static constexpr int kQ = StepRegs<T, D>::kQueryWords * (kRoom<kFew> / 16);
   static constexpr int kJoin = kWaves<kFew> / 2 * (kFew ? 16 : 32) * (D + 4);
   static constexpr int kStages = kFew ? 0 : Stage<T, D>::kBytes / 2;
   static constexpr int kMost = kQ > kJoin ? kQ : kJoin, kWords = kMost > kStages ? kMost : kStages;
@@ -628,7 +634,7 @@ __global__ void __launch_bounds__(64 * kWaves<kFew>, (kFew ? 3 : 2)) prefix_atte
   if (count <= 0 || count > P.num_listed || first < 0 || first > P.num_listed - count) return;  // no item
   const int64_t queries = (int64_t)count * P.group;
   if (q0 < 0 || q0 >= queries) return;
-  const int cols = (int)min((int64_t)(kFew ? kColumns : kQueries), queries - q0);
+  const int cols = (int)min((int64_t)kRoom<kFew>, queries - q0);
   // The row through which the tokens are read: the group's first, or the first behind it that is no padding.
   int leader = head.z, layer = -1, trow = -1;
   if (leader >= 0 && leader < P.num_rows && P.seqlens[leader] < 0) {
@@ -670,7 +676,7 @@ __global__ void __launch_bounds__(64 * kWaves<kFew>, (kFew ? 3 : 2)) prefix_atte
   } else if (!bad && lo < hi) {
     walk.shared_tokens(at_prefix, lds, run, part, mine, lo, hi);
   }
-  float* to = P.shared + ((int64_t)item * P.num_kv_heads + kvh) * kQueries * (D + 2);
+  float* to = P.shared + (room_of(P, item, kFew) * P.num_kv_heads + kvh * kRoom<kFew>) * (D + 2);
   // Waves with the same queries are joined in halves.
   float* join = reinterpret_cast<float*>(lds) + run * 16 * NC * (D + 4);
   constexpr int kSlot = 16 * NC * (D + 4);
@@ -701,12 +707,13 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
   const int n0 = P.row_info[4 * b], item0 = P.row_info[4 * b + 2], given = P.row_info[4 * b + 3];
   row.bad = row.bad || given < -kMaxParts || given > kMaxParts;
   const int parts = row.bad ? 0 : given < 0 ? -given : given;
-  const int each = given < 0 ? kColumns : kQueries;  // queries of an item
+  const bool few = given < 0;
+  const int each_log2 = few ? 4 : 7, each = 1 << each_log2;  // queries of an item
   if (parts == 0) {
     row.bad = row.bad || row.own != 0;
   } else {
-    const int64_t last = item0 + (((int64_t)n0 + P.group - 1) / each + 1) * parts;  // behind the row's last item
-    row.bad = row.bad || n0 < 0 || item0 < 0 || last > P.num_items;
+    const int64_t last = item0 + ((((int64_t)n0 + P.group - 1) >> each_log2) + 1) * parts;  // behind the row's last item
+    row.bad = row.bad || n0 < 0 || item0 < (few ? 0 : P.num_few) || last > (few ? P.num_few : P.num_items);
   }
   if (p < 0 || row.bad) {
     if (chunk == 0)
@@ -784,11 +791,11 @@ __global__ void __launch_bounds__(64 * kRowWaves, 3) prefix_decode_kernel(Prefix
     walk.leave(join + wave * cols * kPlace, cols, kPlace);
     __syncthreads();
 
-    const int64_t shared_stride = (int64_t)P.num_kv_heads * kQueries * (D + 2);
+    const int64_t shared_stride = (int64_t)P.num_kv_heads * each * (D + 2);
+    const float* shared0 = P.shared + (room_of(P, item0, few) * P.num_kv_heads + kvh * each) * (D + 2);
     auto shared_of = [&](int c) __attribute__((always_inline)) -> const float* {
       const int n = n0 + slice + c;
-      return P.shared + (((int64_t)item0 + n / each * parts) * P.num_kv_heads + kvh) * kQueries * (D + 2) +
-             n % each * (D + 2);
+      return shared0 + (n >> each_log2) * parts * shared_stride + (n & (each - 1)) * (D + 2);
     };
     if (chunks > 1) {
       for (int i = tid; i < cols * D; i += 64 * kRowWaves) {
@@ -944,8 +951,8 @@ static int64_t chunk_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head
   return (int64_t)num_heads * (head_dim + 2) * 4 + num_kv_heads * slices * 8;
 }
 // Bytes of the partials of prefixes, a multiple of 16.
-static int64_t shared_bytes(int64_t num_items, int32_t num_kv_heads, int32_t head_dim) {
-  return num_items * num_kv_heads * kQueries * (head_dim + 2) * 4;
+static int64_t shared_bytes(int64_t num_few, int64_t num_items, int32_t num_kv_heads, int32_t head_dim) {
+  return (num_few * kColumns + (num_items - num_few) * kQueries) * num_kv_heads * (head_dim + 2) * 4;
 }
 
 // A tag that no other call of this process has, and that memory does not hold by chance.
@@ -959,14 +966,20 @@ static uint64_t next_tag() {
 
 }  // namespace cdb
 
-extern "C" int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, int32_t num_heads,
-                                                     int32_t num_kv_heads, int32_t head_dim, int32_t max_own) {
-  if (num_rows < 0 || num_items < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
+extern "C" int64_t cdb_prefix_decode_plan_workspace_bytes(int32_t num_rows, int32_t num_few, int32_t num_items,
+                                                          int32_t num_heads, int32_t num_kv_heads, int32_t head_dim,
+                                                          int32_t max_own) {
+  if (num_rows < 0 || num_few < 0 || num_items < num_few || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads != 0 ||
       head_dim <= 0 || max_own <= 0)
     return -1;
   const int64_t chunks = min(((int64_t)max_own + cdb::kChunk - 1) / cdb::kChunk, (int64_t)cdb::kMaxChunks);
-  return cdb::shared_bytes(num_items, num_kv_heads, head_dim) +
+  return cdb::shared_bytes(num_few, num_items, num_kv_heads, head_dim) +
          max((int64_t)num_rows, (int64_t)1) * chunks * cdb::chunk_bytes(num_heads, num_kv_heads, head_dim);
+}
+
+extern "C" int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, int32_t num_heads,
+                                                     int32_t num_kv_heads, int32_t head_dim, int32_t max_own) {
+  return cdb_prefix_decode_plan_workspace_bytes(num_rows, 0, num_items, num_heads, num_kv_heads, head_dim, max_own);
 }
 
 extern "C" int cdb_prefix_decode_attention(
@@ -1009,7 +1022,7 @@ extern "C" int cdb_prefix_decode_attention(
       reinterpret_cast<uintptr_t>(v_pool) % 16 != 0 || reinterpret_cast<uintptr_t>(items) % 16 != 0 ||
       layer_stride * size % 16 != 0)
     return CDB_ERR_SHAPE;
-  const int64_t left = workspace_bytes - shared_bytes(num_items, num_kv_heads, head_dim);
+  const int64_t left = workspace_bytes - shared_bytes(num_few, num_items, num_kv_heads, head_dim);
   const int64_t chunks = left < 0 ? 0 : min(left / (num_rows * chunk_bytes(num_heads, num_kv_heads, head_dim)),
                                             (int64_t)kMaxChunks);
   if (chunks < 1) return CDB_ERR_CAPACITY;
@@ -1025,7 +1038,7 @@ extern "C" int cdb_prefix_decode_attention(
   P.listed = listed; P.items = items; P.row_info = row_info;
   P.num_listed = num_listed; P.num_items = num_items; P.num_few = num_few;
   P.out = out; P.shared = static_cast<float*>(workspace);
-  P.partials = P.shared + shared_bytes(num_items, num_kv_heads, head_dim) / 4;
+  P.partials = P.shared + shared_bytes(num_few, num_items, num_kv_heads, head_dim) / 4;
   P.max_chunks = (int32_t)chunks;
   P.slices = (num_heads / num_kv_heads + kColumns - 1) / kColumns;
   P.tags = reinterpret_cast<uint64_t*>(P.partials + (int64_t)num_rows * num_heads * chunks * (head_dim + 2));

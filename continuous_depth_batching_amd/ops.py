@@ -362,8 +362,8 @@ def prefix_decode_workspace_bytes(plan: PrefixDecodePlan, num_heads: int, num_kv
     among them. Rows with more are served too; the number of their chunks, and with it their rounding, then depends
     on how many rows share the workspace."""
 
-    n = int(_lib.lib().cdb_prefix_decode_workspace_bytes(plan.num_rows, plan.num_items, num_heads, num_kv_heads,
-                                                         head_dim, max_own))
+    n = int(_lib.lib().cdb_prefix_decode_plan_workspace_bytes(plan.num_rows, plan.few, plan.num_items, num_heads,
+                                                              num_kv_heads, head_dim, max_own))
     if n < 0:
         raise ValueError("invalid arguments for the workspace size")
     return n

@@ -498,9 +498,14 @@ enum {
   CDB_PREFIX_MAX_PARTS = 64  /* parts that a prefix is cut into */
 };
 
-/* Workspace bytes of cdb_prefix_decode_attention for num_rows rows, num_items items and rows of up to max_own tokens of
- * their own (-1 for invalid arguments). Rows with more are served too, in fewer and longer chunks, whose number depends
- * on how many rows share the workspace. */
+/* Workspace bytes of cdb_prefix_decode_attention for num_rows rows, num_items items, the first num_few of them of few
+ * queries, and rows of up to max_own tokens of their own (-1 for invalid arguments). Rows with more are served too, in
+ * fewer and longer chunks, whose number depends on how many rows share the workspace. */
+int64_t cdb_prefix_decode_plan_workspace_bytes(int32_t num_rows, int32_t num_few, int32_t num_items, int32_t num_heads,
+                                               int32_t num_kv_heads, int32_t head_dim, int32_t max_own);
+
+/* The same where num_few is not known: enough for any. An item of few queries needs CDB_PREFIX_FEW /
+ * CDB_PREFIX_QUERIES of what this counts for it. */
 int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, int32_t num_heads, int32_t num_kv_heads,
                                           int32_t head_dim, int32_t max_own);
 
