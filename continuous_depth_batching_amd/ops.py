@@ -310,8 +310,12 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
 
     Prefixes are cut into parts of about equal length, at least 128 tokens and at most 64 parts: as many as give every
     CU a workgroup, as a part costs each of its queries a partial result, written and read again; three times as many
-    where a group has 32 queries at most, whose workgroups run three to a CU. A row's rounding depends on its prefix's
-    parts."""
+    where a group has 32 queries at most, whose workgroups run three to a CU.
+
+    So the parts follow from all groups of the batch, and the kind of workgroup from the size of the row's own group. A
+    row's rounding depends on both, and on nothing else of the batch: where a neighbour that joins or leaves changes
+    neither, the row keeps its bits; where it does, the result may differ in its last ones, unlike
+    ``paged_decode_attention``'s, whose rows do not depend on each other."""
 
     import numpy as np
 

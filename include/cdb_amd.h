@@ -524,6 +524,10 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
  * [num_rows][4] = (row's first query in its group, tokens of its prefix, its group's first item, parts, negative where
  * the items are of the first num_few), zeros for a row without a group. A row is listed at most once.
  *
+ * A row's result depends, in its last bits, on the parts that the plan cuts its prefix into and on which of the two kinds
+ * its items are, but not on what else is in the plan or the batch, while the workspace has a chunk for each 1024 of its
+ * own tokens.
+ *
  * A row of negative position is padding: zeros. NaN for a row, and no append, where its position is out of the table's
  * or the angles' range or inside its prefix, or its cache layer or table row out of range; NaN where its cache layer is
  * not that of the row through which its group's tokens are read, and where a block outside the pool is met, for all rows
