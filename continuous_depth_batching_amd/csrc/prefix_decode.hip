@@ -12,8 +12,9 @@
 //   S^T = K Q^T, bf16: v_mfma_f32_16x16x32_bf16 on keys as they lie in memory, with the rotated query, already scaled,
 //   as two bf16 parts (2^-16 of an element together);
 //   O^T = V^T P^T with P as two bf16 parts; values are turned to the operand's order by one byte permutation for two
-//   of them. One part of Q and P each would halve the products and lose what the one-row kernel keeps, which holds both
-//   in fp32.
+//   of them. One part of Q and P each would halve the products and leave 2^-9 of an element, which is what the kernel
+//   for rows without prefixes has (paged_decode_attention.hip: queries rounded to bf16 when rotated, weights for their
+//   product). Here the result is the formula's on the cached numbers to one rounding, the output's, in any cut.
 // fp32 takes v_mfma_f32_16x16x4_f32, which rounds nothing but the sums. Both products are 16 queries wide; columns
 // without a query repeat the last one. A lane's scores are those of the tokens whose values it holds, so P never moves.
 //

@@ -512,7 +512,8 @@ int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, i
 /* cdb_paged_decode_attention for rows that begin with the same tokens, which are read once for all of them: rotate the
  * row's new query and key, append key and value at position seqlens[b] of the row's cache layer, attend over positions
  * 0..seqlens[b]. Arguments as there, but for the plan; block_size is a power of two of at least 16, and the block table
- * has table_rows rows. Rotations are fp32 and rounded once, to the cache's type (that call rounds bf16 after each step).
+ * has table_rows rows. Rotations are fp32: the key is rounded once, to the cache's type, and the query is not (that call
+ * rounds both, in bf16 after each step, and so appends other bits in bf16).
  *
  * The rows of a group follow each other in listed; they hold the same first tokens, at the same slots of the same cache
  * layer or as copies, which are read through the table row and cache layer of the group's first row that is no padding;
