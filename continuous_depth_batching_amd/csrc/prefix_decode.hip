@@ -1,7 +1,8 @@
 // Decode attention of rows that share prefixes, over the paged cache in the model's type.
 //
 // Row b attends over positions 0..p_b of its cache layer. Rows of a group begin with the same tokens; these are read
-// once for all of them, each row's own tokens by the row, and what the two leave is joined: with m, l and O a part's
+// once for 16 or 128 of the group's queries of a KV head, each row's own tokens by the row, and what the two leave is
+// joined: with m, l and O a part's
 // largest score, sum of weights and weighted sum of values, M = max m, out = sum 2^(m - M) O / sum 2^(m - M) l.
 //   prefix_attend_kernel  a workgroup takes 16 or 128 queries (row, head) of a group, one KV head and a part of the
 //                         prefix's tokens, and leaves m, l and O of each query;

@@ -382,7 +382,8 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     """Launch ``cdb_prefix_decode_attention`` (no allocation): ``paged_decode_attention_raw`` for rows of which some
     begin with the same tokens, named by ``plan`` (``prefix_decode_plan``, on the device). Append each row's new token
     at position ``seqlens[b]`` and attend over positions 0..seqlens[b] (negative: a padding row, zero output); a group's
-    common tokens are read once, through the table row of its first row that is no padding. ``workspace`` is any dense tensor of
+    common tokens are read through the table row of its first row that is no padding, once for each 128 of its queries
+    of a KV head (16 in a group of up to 32). ``workspace`` is any dense tensor of
     ``prefix_decode_workspace_bytes`` bytes. Calls that may overlap need a workspace each."""
 
     pool, block = view.pool, view.block_size

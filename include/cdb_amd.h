@@ -509,7 +509,8 @@ int64_t cdb_prefix_decode_plan_workspace_bytes(int32_t num_rows, int32_t num_few
 int64_t cdb_prefix_decode_workspace_bytes(int32_t num_rows, int32_t num_items, int32_t num_heads, int32_t num_kv_heads,
                                           int32_t head_dim, int32_t max_own);
 
-/* cdb_paged_decode_attention for rows that begin with the same tokens, which are read once for all of them: rotate the
+/* cdb_paged_decode_attention for rows that begin with the same tokens, which are read once for each CDB_PREFIX_FEW or
+ * CDB_PREFIX_QUERIES queries of a KV head that share them (128 rows of as many heads as KV heads: once): rotate the
  * row's new query and key, append key and value at position seqlens[b] of the row's cache layer, attend over positions
  * 0..seqlens[b]. Arguments as there, but for the plan; block_size is a power of two of at least 16, and the block table
  * has table_rows rows. Rotations are fp32: the key is rounded once, to the cache's type, and the query is not (that call
