@@ -26,7 +26,10 @@
 // fp32 logits takes 21 us, 6.4 TB/s, a later one 19 from the last cache), and weighs 5.5 tokens a nanosecond, some 25
 // instructions of 4 cycles each. So one row of 49152 bf16 logits with all filters takes 13 us, of which the passes are
 // 3 and the rest is launch, loads, meetings and instruction fetches that wait for each other; 256 rows with mixed ones
-// 38, 256 of 131072 fp32 logits 89: what bounds them is a row that keeps 99 % at T = 1.5, or top-k and top-p together.
+// 38, 256 of 131072 fp32 logits 88: what bounds them is a row that keeps 99 % at T = 1.5, or top-k and top-p together.
+// A kernel is 160 to 170 KB of instructions, as all of this stands in it for finite and for other maxima, and holds 128
+// registers a lane at four waves a SIMD: 512 threads spill 20 (20 bytes a lane of scratch), 1024 spill 58 in bf16 and 75
+// in fp32 (80 bytes).
 
 #include <cfloat>
 
@@ -151,8 +154,8 @@ template <int kSampleThreads> struct Sampler {
   static constexpr int kPartRank = 1200;
   static constexpr int kShort = 128, kSharers = kSampleThreads / kShort;  // tokens ordered by counting, threads a token
   // Whether each wave has a histogram of its own, which saves weighing the kept tokens again: one workgroup to a CU has
-  // the LDS for that. 64 rows of 65536 flat fp32 logits with top-p take 41 us so and 50 without, 256 rows of 131072
-  // mixed ones 88 and 118.
+  // the LDS for that. 64 rows of 65536 flat fp32 logits with top-p take 40 us so and 48 without, 256 rows of 131072
+  // mixed ones 87 and 103.
   static constexpr bool kApart = kSampleThreads == 1024;
   static_assert(kBinsEach >= 1 && kPartsEach <= 8 && kSharers >= 1 && kSharers <= 8, "shares of a thread");
 
@@ -755,8 +758,8 @@ template <int kSampleThreads> struct Sampler {
       b = (int)fmin(-log2(f.size) * (kBins / 46.0) + 1.0, (double)(kBins - 1));
     if (f.by_count) {
       // By the bins of the weights the k-th token may lie in the last one with most of the row, too many for a list:
-      // 256 mixed rows of 131072, among them k = 1000 at T = 0.3, took 280 us. With bins from the largest of the parts'
-      // maxima to the least they take 118.
+      // 256 mixed rows of 131072, among them k = 1000 at T = 0.3, take 275 us. With bins from the largest of the parts'
+      // maxima to the least they take 87.
       const float width = (float)(kBins - 1) / (w.top_f - least), per = width <= FLT_MAX ? width : 0.f;
       clear_bins(s);
 #pragma unroll
@@ -983,7 +986,7 @@ template <int kSampleThreads> struct Sampler {
       return;
     }
     // Out of the way, as are the other rare branches here: what follows has to be fetched, and at a few instructions a
-    // wave that takes longer than running it (one row 13.8 us without, 12.9 with; 33 rows of 32771 15.6 and 14.1).
+    // wave that takes longer than running it (one row 14.3 us without, 13.4 with; 33 rows of 32771 15.9 and 14.5).
     if (__builtin_expect(!(temperature > 0.f), 0)) {
       if (mine == top) {
         int best = 0x7fffffff;
@@ -1040,8 +1043,11 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleParams P) {
 }
 
 template <typename T> static int sample_type(const SampleParams& P, int rows, hipStream_t stream) {
-  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster: 256 rows of 49152 take 48 us
-  // with 1024 threads and 52 with 512; 356 rows of 1438 take 30 and 14.5, 298 of 82 27 and 16, 95 of 368 19 and 15.
+  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster and has a histogram a wave: 256
+  // rows of 49152 take 38 us with 1024 threads and 46 with 512, one 13.4 and 13.8, 64 flat ones of 65536 40 and 54; 356
+  // rows of 1438 34 and 24, 298 of 82 26 and 15, 95 of 368 22 and 18, 64 of 8000 46 and 43. Of more rows than CUs two run
+  // at a time: 512 rows of 49152 take 65 and 60, but 300 of them 40 and 47, 257 fp32 rows of 131072 89 and 117: just
+  // above 256 rows the rule is the slower choice.
   if (rows > 256 || P.vocab <= 8192) sample_kernel<T, 512><<<dim3((unsigned)rows), dim3(512), 0, stream>>>(P);
   else sample_kernel<T, 1024><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(P);
   return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;
