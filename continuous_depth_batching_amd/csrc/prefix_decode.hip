@@ -19,10 +19,12 @@
 // fp32 takes v_mfma_f32_16x16x4_f32, which rounds nothing but the sums. Both products are 16 queries wide; columns
 // without a query repeat the last one. A lane's scores are those of the tokens whose values it holds, so P never moves.
 //
-// Bounds, bf16, heads of 128: own tokens, by the bytes: 256 rows x 16 KV heads of 32 to 512 own tokens take 95 us,
-// 3.8 TB/s, of the 127 us with 2 x 2048 shared ones, whose part is bound by the products' chain (30 us). 32000 tokens
-// shared by 64 rows of 32 heads on 8 KV heads: 85 us, in which a SIMD has matrix work for 27 and vector work (weights
-// and their parts) for 25, at two waves that wait for the same steps; the rows' own tokens take 20 more.
+// Bounds, bf16, heads of 128: own tokens, by the bytes: 256 rows x 16 KV heads of 32 to 512 own tokens take 93 us,
+// 3.9 TB/s, of the 125 us with 2 x 2048 shared ones, whose part is bound by the products' chain (30 us). 32000 tokens
+// shared by 64 rows of 32 heads on 8 KV heads: 84 us, in which a SIMD has matrix work for 27 and vector work (weights
+// and their parts) for as much, at two waves that wait for the same steps; the rows' own tokens take 20 more. In fp32,
+// 64 rows of 16 heads after 2048 tokens take 31, 47 and 49 us with heads of 64, 96 and 128 (floors 7, 10 and 14); heads
+// of 96 keep 144 bytes a lane in scratch there, though nothing spills.
 
 #include <atomic>
 #include <chrono>
@@ -43,9 +45,10 @@ constexpr int kItem = CDB_PREFIX_ITEM;        // words of an item
 static_assert(CDB_PREFIX_FEW == kColumns && kQueries == 128, "queries of an item's waves");
 // A prefix's workgroup: four waves of the same 16 queries, each with every fourth step, loaded by itself; or four of 32
 // queries each on two parts of the tokens, which share a step's loads in LDS. The plan takes the first kind for groups
-// of up to 32 queries: 8 groups of 8 (32, 33, 64) queries on 2048 tokens, 16 KV heads, take 41 (64, 76, 121) us with
-// their own tokens on the first kind and 49 (73, 74, 105) on the second; one group on 16000 tokens 41 (54, 70, 80) and
-// 46 (50, 52, 56).
+// of up to 32 queries: 8 groups of 8 (32, 33, 64) queries on 2048 tokens, 16 KV heads, take 41 (64, 74, 121) us with
+// their own tokens on the first kind and 50 (74, 76, 106) on the second; one group of 16 (24, 33) on 16000 tokens 43
+// (54, 72) and 50 (52, 54); 2 of 8 (24, 64) on 8000, 32 heads on 8, 40 (39, 46) and 38 (40, 43). So the rule, which
+// sees neither the tokens nor the KV heads, loses up to 7% for few queries on long prefixes of few KV heads.
 template <bool kFew> constexpr int kWaves = kFew ? 4 : 8;
 static_assert(kMaxParts <= 64, "a lane weighs a part");
 

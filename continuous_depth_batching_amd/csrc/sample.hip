@@ -1043,11 +1043,11 @@ __global__ void __launch_bounds__(kThreads, 4) sample_kernel(SampleParams P) {
 }
 
 template <typename T> static int sample_type(const SampleParams& P, int rows, hipStream_t stream) {
-  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster and has a histogram a wave: 256
-  // rows of 49152 take 38 us with 1024 threads and 46 with 512, one 13.4 and 13.8, 64 flat ones of 65536 40 and 54; 356
-  // rows of 1438 34 and 24, 298 of 82 26 and 15, 95 of 368 22 and 18, 64 of 8000 46 and 43. Of more rows than CUs two run
-  // at a time: 512 rows of 49152 take 65 and 60, but 300 of them 40 and 47, 257 fp32 rows of 131072 89 and 117: just
-  // above 256 rows the rule is the slower choice.
+  // A CU holds two workgroups of 512, or one of 1024, which passes over a long row faster and has a histogram a wave:
+  // 256 rows of 49152 take 38 us with 1024 threads and 46 with 512, one 13.4 and 13.8, 64 flat ones of 65536 40 and 54;
+  // 356 rows of 1438 34 and 24, 298 of 82 26 and 15, 95 of 368 22 and 18, 64 of 8000 46 and 43. Of more rows than CUs
+  // two run at a time: 512 rows of 49152 take 65 and 60, but 300 of them 40 and 47, 257 fp32 rows of 131072 89 and 117:
+  // just above 256 rows the rule is the slower choice.
   if (rows > 256 || P.vocab <= 8192) sample_kernel<T, 512><<<dim3((unsigned)rows), dim3(512), 0, stream>>>(P);
   else sample_kernel<T, 1024><<<dim3((unsigned)rows), dim3(1024), 0, stream>>>(P);
   return hipGetLastError() == hipSuccess ? CDB_OK : CDB_ERR_HIP;

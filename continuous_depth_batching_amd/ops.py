@@ -306,7 +306,8 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
                        num_kv_heads: int, num_cus: int = 256) -> PrefixDecodePlan:
     """The work list of a decode batch: row b belongs to group ``group[b]`` (negative: to none) and begins with that
     group's ``lengths[group[b]]`` tokens. Rows of one group sit at the same cache layer: rows at two loop depths of a
-    layout with a slot a step are two groups.
+    layout with a slot a step are two groups. Made on the host (25-100 us, and 25 for ``to``), and again when a row
+    joins or changes its group; rows that end may stay as padding.
 
     Prefixes are cut into parts of about equal length, at least 128 tokens and at most 64 parts: as many as give every
     CU a workgroup, as a part costs each of its queries a partial result, written and read again; three times as many
