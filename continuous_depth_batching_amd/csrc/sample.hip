@@ -28,8 +28,8 @@
 // 3 and the rest is launch, loads, meetings and instruction fetches that wait for each other; 256 rows with mixed ones
 // 38, 256 of 131072 fp32 logits 88: what bounds them is a row that keeps 99 % at T = 1.5, or top-k and top-p together.
 // A kernel is 160 to 170 KB of instructions, as all of this stands in it for finite and for other maxima, and holds 128
-// registers a lane at four waves a SIMD: 512 threads spill 20 (20 bytes a lane of scratch), 1024 spill 58 in bf16 and 75
-// in fp32 (80 bytes).
+// registers a lane at four waves a SIMD: 512 threads spill 22 in bf16 and 20 in fp32 (28 and 20 bytes a lane of
+// scratch), 1024 spill 64 and 73 (84 bytes).
 
 #include <cfloat>
 
@@ -609,12 +609,13 @@ template <int kSampleThreads> struct Sampler {
     bool by_count, by_share, by_size;
   };
 
+  // The share is that of the weight as it was summed, in which what all exponents are off by divides out (kPlain), and
+  // one token alone has all of it: its weight may be a rounding above the total.
   template <typename W>
   static CDB_DEVICE void give(const SampleParams& P, int64_t r, const W& w, uint64_t place, uint64_t total) {
-    const float x = logit_of((uint32_t)(place >> 32));
-    const double share = x == w.top_f ? 0.0 : ((double)x - w.top) * (w.rate * 0.6931471805599453);
+    const double weight = w.of(logit_of((uint32_t)(place >> 32)));
     P.tokens[r] = (int)~(uint32_t)place;
-    P.logprobs[r] = (float)(share - log(__builtin_ldexp((double)total, -P.unit_log2)));
+    P.logprobs[r] = W::units(weight) == total ? 0.f : (float)fmin(log(weight / (double)total), 0.0);
   }
 
   // The running weight that must be passed, of kept tokens that weigh `total` units; the largest token has a weight, so
