@@ -1023,7 +1023,7 @@ def sample_raw(logits: torch.Tensor, uniform: torch.Tensor, temperature: torch.T
     (largest first, lower index first among equals) that holds ``top_p`` of their weight, and of those the ones that
     weigh at least ``min_p`` times the largest. ``tokens`` int64 gets the token, -1 where every logit is -inf or NaN,
     and ``logprobs`` float32 the logarithm of its share of the kept weight. Rows may lie apart. ``workspace``: any
-    dense tensor of ``sample_workspace_bytes`` bytes; calls that may overlap need one each."""
+    dense tensor of ``sample_workspace_bytes`` bytes, which is none at present."""
 
     if logits.dim() != 2:
         raise ValueError("logits must be [rows, vocab]")

@@ -569,8 +569,10 @@ int64_t cdb_sample_workspace_bytes(int32_t rows, int32_t vocab);
  * or are null: 1 and no filter. A temperature not above 0 takes the first token of the order (the index cdb_argmax
  * gives, where no logit is NaN). Logits of -infinity and NaN are never drawn; where one is +infinity only such are.
  * tokens [rows]; logprobs [rows]: the logarithm of the drawn token's share of the kept weight, 0 for a token that is
- * kept alone and never above. A row without a token to draw gets -1 and -infinity. Weights are counted in units of 2^-46 of the largest (vocabularies above 65536: of
- * 2^-(62 - ceil(log2 vocab))) and summed exactly, so a row's token depends on nothing but the row. */
+ * kept alone and never above. A row without a token to draw gets -1 and -infinity. Weights are counted in units of 2^-46
+ * of the largest (vocabularies above 65536: of 2^-(62 - ceil(log2 vocab))) and summed exactly, so a row's token depends
+ * on nothing but the row; what weighs less than half a unit is never drawn. workspace holds nothing at present, as its
+ * size says, and may be null. */
 int cdb_sample(const void* logits, int64_t row_stride, const double* uniform, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* min_p, int64_t* tokens, float* logprobs,
                void* workspace, int64_t workspace_bytes, int32_t rows, int32_t vocab, int32_t dtype,
