@@ -19,10 +19,9 @@
 // codes; 118 with chunks of 512 tokens, 128 with a merge launch of its own); 21 rows of 4k..32k tokens, 32 heads
 // on 8 x 128, 113 us (5.2 TB/s); one row of 900 tokens 9.6-10.5 us, a chain of latencies: position, block ids,
 // tiles and query, 7 pairs a wave, the join. The same loads without arithmetic take 85 and 104 us.
-#include <atomic>
-#include <chrono>
 #include <type_traits>
 
+#include "call_tag.h"
 #include "cdb_amd.h"
 #include "kv8_common.h"
 #include "kv8_host.h"
@@ -728,15 +727,6 @@ namespace cdb {
 static int64_t chunk_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head_dim) {
   const int64_t slices = ((int64_t)num_heads / num_kv_heads + 15) / 16;
   return (int64_t)num_heads * (head_dim + 2) * 4 + num_kv_heads * slices * 8;
-}
-
-// A tag that no other call of this process has, and that memory does not hold by chance.
-static uint64_t next_tag() {
-  static std::atomic<uint64_t> calls{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() << 20};
-  uint64_t z = calls.fetch_add(1, std::memory_order_relaxed) * 0x9e3779b97f4a7c15ull;
-  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
-  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
-  return (z ^ (z >> 31)) | 1;
 }
 
 }  // namespace cdb

@@ -26,9 +26,7 @@
 // 64 rows of 16 heads after 2048 tokens take 31, 47 and 49 us with heads of 64, 96 and 128 (floors 7, 10 and 14); heads
 // of 96 keep 144 bytes a lane in scratch there, though nothing spills.
 
-#include <atomic>
-#include <chrono>
-
+#include "call_tag.h"
 #include "cdb_amd.h"
 #include "kv8_common.h"
 #include "kv8_host.h"
@@ -958,15 +956,6 @@ static int64_t chunk_bytes(int32_t num_heads, int32_t num_kv_heads, int32_t head
 // Bytes of the partials of prefixes, a multiple of 16.
 static int64_t shared_bytes(int64_t num_few, int64_t num_items, int32_t num_kv_heads, int32_t head_dim) {
   return (num_few * kColumns + (num_items - num_few) * kQueries) * num_kv_heads * (head_dim + 2) * 4;
-}
-
-// A tag that no other call of this process has, and that memory does not hold by chance.
-static uint64_t next_tag() {
-  static std::atomic<uint64_t> calls{(uint64_t)std::chrono::steady_clock::now().time_since_epoch().count() << 20};
-  uint64_t z = calls.fetch_add(1, std::memory_order_relaxed) * 0x9e3779b97f4a7c15ull;
-  z = (z ^ (z >> 30)) * 0xbf58476d1ce4e5b9ull;
-  z = (z ^ (z >> 27)) * 0x94d049bb133111ebull;
-  return (z ^ (z >> 31)) | 1;
 }
 
 }  // namespace cdb
