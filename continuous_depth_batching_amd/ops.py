@@ -276,12 +276,14 @@ class PrefixDecodePlan:
     row_info  [rows, 4]: (first query in the group, tokens of the prefix, the group's first item, parts, negative where
               the items are of the few)
     few       the items of groups with few queries, which come first
+    share     query heads a KV head, by which queries are counted; 0 where it is not known
     """
 
     listed: "np.ndarray | torch.Tensor"
     items: "np.ndarray | torch.Tensor"
     row_info: "np.ndarray | torch.Tensor"
     few: int
+    share: int = 0
 
     @property
     def num_rows(self) -> int:
@@ -299,7 +301,7 @@ class PrefixDecodePlan:
         arrays = [np.asarray(a, dtype=np.int32) for a in (self.items, self.row_info, self.listed)]  # items aligned
         flat = torch.from_numpy(np.concatenate([a.ravel() for a in arrays])).to(device)
         items, info, listed = (x.view(a.shape) for x, a in zip(flat.split([a.size for a in arrays]), arrays))
-        return PrefixDecodePlan(listed=listed, items=items, row_info=info, few=self.few)
+        return PrefixDecodePlan(listed=listed, items=items, row_info=info, few=self.few, share=self.share)
 
 
 def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np.ndarray", *, num_heads: int,
@@ -358,7 +360,8 @@ def prefix_decode_plan(group: "list[int] | np.ndarray", lengths: "list[int] | np
             info[rows, 1], info[rows, 2], info[rows, 3] = length, item0, -part if kind else part
         num_few = len(items) if kind else num_few
     return PrefixDecodePlan(listed=order.astype(np.int32), row_info=info.astype(np.int32),
-                            items=np.asarray(items, dtype=np.int32).reshape(-1, _lib.CDB_PREFIX_ITEM), few=num_few)
+                            items=np.asarray(items, dtype=np.int32).reshape(-1, _lib.CDB_PREFIX_ITEM), few=num_few,
+                            share=share)
 
 
 def prefix_decode_workspace_bytes(plan: PrefixDecodePlan, num_heads: int, num_kv_heads: int, head_dim: int,
@@ -419,6 +422,8 @@ def prefix_decode_attention_raw(q: torch.Tensor, k_new: torch.Tensor, v_new: tor
     listed, items, info = plan.listed, plan.items, plan.row_info
     if not isinstance(info, torch.Tensor):
         raise TypeError("the plan must be on the device: plan.to(device)")
+    if plan.share not in (0, num_heads // heads_kv):
+        raise ValueError(f"the plan is for {plan.share} query heads a KV head, not for {num_heads // heads_kv}")
     num_listed, num_items = listed.shape[0], items.shape[0]
     if not 0 <= plan.few <= num_items:
         raise ValueError(f"{plan.few} of the plan's {num_items} items cannot be the few")
