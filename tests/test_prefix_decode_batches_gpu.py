@@ -55,3 +55,28 @@ def test_a_row_cut_alike_has_the_same_bits_in_any_batch(heads, kv, dtype):
         same = [i for i, b in enumerate(rows) if shape_of(part.host_plan, i) == shape_of(whole, b)]
         assert size < 70 or len(same) >= size // 2  # smaller ones leave few queries of the large group
         assert torch.equal(got[same], want[[rows[i] for i in same]])
+
+
+def test_calls_on_two_streams_at_once():
+    scenes = [ph.make([0] * 9 + [1] * 40 + [-1], [900, 333], [1 + 31 * b % 97 for b in range(49)] + [2900], heads=4, kv=4,
+                      dim=128, seed=i, dead=0.0) for i in range(2)]
+    want = [ph.call(s).clone() for s in scenes]
+    streams = [torch.cuda.Stream() for _ in scenes]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(6):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got[i].append(ph.call(scenes[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(out, want[i]) for out in got[i])
+
+
+def test_no_rows():
+    s = ph.make([0, -1], [40], [3, 4])
+    plan = ops.prefix_decode_plan([], [40], num_heads=8, num_kv_heads=4).to("cuda")
+    s.q, s.k, s.v, s.seq, s.layer = (t[:0] for t in (s.q, s.k, s.v, s.seq, s.layer))
+    before = s.pool.clone()
+    assert ph.call(s, plan=plan).shape == (0, 8, 64)
+    assert torch.equal(s.pool.isnan(), before.isnan())

@@ -24,7 +24,7 @@ def batch(rows, vocab, dtype, seed):
     x[::7, ::2] = -math.inf
     x[3] = 1.0
     x[4] = -math.inf
-    x[5, 100] = math.inf
+    x[5, 100 % vocab] = math.inf
 
     def pick(values, dtype):
         return torch.from_numpy(rng.choice(np.asarray(values), size=rows)).to(dtype).to(DEV)
@@ -54,3 +54,12 @@ def test_a_row_is_drawn_alike_in_any_batch(vocab, dtype):
         head = {k: None if v is None else v[:256] for k, v in only.items()}
         few, few_logprobs = torch.ops.cdb.sample(*head.values())
         assert torch.equal(few, tokens[:256]) and torch.equal(few_logprobs, logprobs[:256]), names
+
+
+def test_many_rows():
+    b = batch(70001, 40, torch.float32, 5)
+    tokens, logprobs = torch.ops.cdb.sample(*b.values())
+    at = torch.arange(69900, 70001, device=DEV)
+    few, few_logprobs = torch.ops.cdb.sample(*(v[at] for v in b.values()))
+    assert torch.equal(few, tokens[at]) and torch.equal(few_logprobs, logprobs[at])
+    assert int((tokens < 0).sum()) == int((~(b["logits"] > -math.inf).any(dim=1)).sum())
